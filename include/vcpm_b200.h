@@ -42,8 +42,9 @@ enum {
     VB_ERR_NOT_IMPLEMENTED = 7
 };
 
-/* Weight types: ggml type ids (GGML_TYPE_F32/F16/Q8_0). */
-enum { VB_TYPE_F32 = 0, VB_TYPE_F16 = 1, VB_TYPE_Q8_0 = 8 };
+/* Weight types: ggml type ids (GGML_TYPE_F32/F16/Q8_0).  VB_TYPE_BF16
+ * (GGML_TYPE_BF16) is a type of activations and cache rows only. */
+enum { VB_TYPE_F32 = 0, VB_TYPE_F16 = 1, VB_TYPE_Q8_0 = 8, VB_TYPE_BF16 = 30 };
 
 /* Q8_0 activation rounding rule.  VB_QRULE_X86 is ggml-CPU's x86 SIMD rule
  * (id = 127/amax, round half to even), the default; VB_QRULE_REF is ggml's
@@ -69,7 +70,8 @@ const char *vb_last_error(const vb_ctx *ctx);
 int vb_sync(vb_ctx *ctx);
 /* Synchronise and report a device-side error code recorded by the
  * tensor-core mat-mul (0 = none; its waits are bounded, a timeout records a
- * code instead of hanging).  Returns VB_ERR_BACKEND when one was recorded. */
+ * code instead of hanging) or by the paged-cache operators (VB_DEV_*, which
+ * are cleared by the report).  Returns VB_ERR_BACKEND when one was recorded. */
 int vb_device_status(vb_ctx *ctx, int *device_error);
 /* Use an external cudaStream_t (passed as void*); NULL restores the
  * context's own stream. */
@@ -536,6 +538,150 @@ int vb_vae_stream_conv_cache_count(vb_vae_stream s);     /* 20 */
 int vb_vae_stream_upconv_cache_count(vb_vae_stream s);   /* 6  */
 int vb_vae_stream_patch_samples(vb_vae_stream s);        /* patch_size * prod(rates) */
 size_t vb_vae_stream_state_bytes(vb_vae_stream s);       /* device bytes of the caches */
+
+/* ------------------------------------------------------------------ */
+/* Paged K/V cache and drafted tokens (no counterpart in the           */
+/* reference, whose cache is one slab per sequence,                    */
+/* src/minicpm4.c:93-122)                                              */
+/* ------------------------------------------------------------------ */
+/* A paged cache: a view of caller-owned device memory.  Row r of sequence s
+ * lies in row r % page_rows of page table[s][r / page_rows]; sequences that
+ * were forked name the same pages until one of them writes.  The table, the
+ * lengths and the counts live on the device and only the calls below change
+ * them, in stream order, without the host: a whole step (extend, store,
+ * attend, keep) can be captured in a vb_graph and replayed.  Calls on one
+ * cache, like all calls of one context, are ordered by the caller when they
+ * go to different streams.
+ * page_rows: a power of two, 16 to 1024; head_dim: a multiple of 8, at most
+ * 256; n_seqs at most 16384; every pointer 16-byte aligned. */
+typedef struct {
+    void *k, *v;          /* [n_layers][n_pages][n_kv_heads][page_rows][head_dim] of `type` */
+    int32_t *table;       /* [n_seqs][max_pages], -1 past a sequence's end */
+    int32_t *length;      /* [n_seqs] rows held */
+    int32_t *refs;        /* [n_pages] table entries that name the page; 0: free */
+    int32_t *status;      /* [4]: first error (VB_PAGES_*), the request that met it */
+    int type;             /* VB_TYPE_BF16 or VB_TYPE_F16 */
+    int n_layers, n_pages, n_kv_heads, page_rows, head_dim, n_seqs, max_pages;
+} vb_pages;
+
+/* Errors of the page calls.  They are found on the device: the call that
+ * meets one changes nothing and records it with the lowest request index it
+ * was found at, and later page calls on the cache change nothing either
+ * until vb_pages_status has read it. */
+enum {
+    VB_PAGES_SEQ = 1,     /* sequence out of range, or in two requests of one call */
+    VB_PAGES_COUNT = 2,   /* negative count, drafted > length, kept > drafted */
+    VB_PAGES_LONG = 3,    /* more than max_pages * page_rows rows */
+    VB_PAGES_FULL = 4,    /* not enough free pages */
+    VB_PAGES_SHARED = 5,  /* keep would move rows of a page that another sequence names */
+    VB_PAGES_PATH = 6,    /* path not rising, or outside the draft */
+    VB_PAGES_TABLE = 7    /* a table entry names no page of the pool */
+};
+
+/* Empties the cache: table -1, lengths, counts and status 0. */
+int vb_pages_init(vb_ctx *ctx, const vb_pages *p);
+/* Makes room for rows[i] more rows of seqs[i] (device int32 [n]; sequences
+ * distinct) and counts them as held: rows length .. length + rows[i] - 1 may
+ * then be stored.  New pages are the lowest-numbered free ones, in request
+ * order.  A partly filled last page that other sequences name is copied
+ * first, in every layer (copy on write); of the requests that share it, the
+ * last one keeps it when nobody else names it. */
+int vb_pages_extend(vb_ctx *ctx, const vb_pages *p, int n, const int32_t *seqs, const int32_t *rows);
+/* dst[i] becomes a copy of src[i]: it names the same pages; no row moves.
+ * What dst[i] held is released.  The dst are distinct and none is a src of
+ * the same call; one src may be forked many times. */
+int vb_pages_fork(vb_ctx *ctx, const vb_pages *p, int n, const int32_t *src, const int32_t *dst);
+/* After drafted tokens were judged: of the last drafted[i] rows of seqs[i],
+ * the rows path[i*ld_path + 0 .. kept[i]-1] (places in the draft, rising:
+ * the accepted path of a tree) move together behind the rows before the
+ * draft, in every layer; the others are dropped and pages past the new end
+ * released.  kept[i] at most ld_path. */
+int vb_pages_keep(vb_ctx *ctx, const vb_pages *p, int n, const int32_t *seqs, const int32_t *drafted,
+                  const int32_t *kept, const int32_t *path, int ld_path);
+/* Drops the rows from length[i] on (none when seqs[i] is shorter) and
+ * releases the pages past the new end; 0 frees the sequence. */
+int vb_pages_truncate(vb_ctx *ctx, const vb_pages *p, int n, const int32_t *seqs, const int32_t *length);
+/* Moves the live pages, in the order of their numbers, to pages 0, 1, 2, ...
+ * of another cache of the same rows (any n_pages that holds them; max_pages
+ * not smaller), which becomes a copy of `from` with its free pages at the
+ * end: to grow a pool, to shrink it, or to pack it.  `to` shares no memory
+ * with `from`; what it held is dropped. */
+int vb_pages_compact(vb_ctx *ctx, const vb_pages *from, const vb_pages *to);
+/* Waits for the stream, reports the recorded error (0 = none) with the
+ * request that met it and clears it, and counts the free pages; each output
+ * may be NULL.  Returns VB_ERR_BACKEND when an error was recorded. */
+int vb_pages_status(vb_ctx *ctx, const vb_pages *p, int *error, int *request, int *free_pages);
+
+/* Device error codes of the two operators below (vb_device_status).  The
+ * token or sequence concerned is skipped: nothing is stored for it, its
+ * output row is zero. */
+enum {
+    VB_DEV_QK_POS = 21,   /* position outside the rotation table */
+    VB_DEV_QK_ROW = 22,   /* sequence or row outside the cache, or no page there */
+    VB_DEV_TREE_SEQ = 31, /* sequence, start or length outside the bounds of the call */
+    VB_DEV_TREE_PAGE = 32 /* a table entry names no page of the pool */
+};
+
+/* (cos, sin) pairs of positions 0 .. n_pos-1 as vb_rope_neox rotates them
+ * (longrope: the LongRoPE short factors, rot_dim 128 only), into host memory
+ * [n_pos][rot_dim]. */
+int vb_rope_table(int rot_dim, float theta, int longrope, int n_pos, float *host);
+
+/* Head norms of queries and keys and the position rotation in one pass over
+ * the rows of a fused projection, with the store of keys and values into a
+ * paged cache.  Per head: y = x * rsqrt(mean(x^2) + eps) * weight (norm 1;
+ * 0 leaves x), then the first rot_dim values are rotated by the position's
+ * table row; statistics and products in 32 bits, each result rounded once.
+ * Values are stored as they come.  One token or many. */
+typedef struct {
+    int type;                       /* of q, k, v, q_out, k_out: VB_TYPE_F32, F16 or BF16 */
+    int n_tokens, n_heads, n_kv_heads, head_dim;   /* head_dim a multiple of 8, at most 256 */
+    int rot_dim;                    /* a multiple of 8, at most head_dim; 0 = head_dim */
+    int adjacent;                   /* pairs (2i, 2i+1); 0: (i, i + rot_dim/2) */
+    int norm;
+    unsigned flags;                 /* VB_OUT_BF16: F32 results rounded to bf16 */
+    float eps;
+    int rope_rows;                  /* positions of the table */
+    int layer;                      /* of the cache */
+    const void *q, *k, *v;          /* row t at + t*ld elements; v only with pages */
+    int64_t ldq, ldk, ldv;          /* 0 = packed */
+    const float *q_weight, *k_weight;   /* device [head_dim] or NULL (ones) */
+    const float *rope;              /* device [rope_rows][rot_dim] (cos, sin) pairs, 16-byte aligned, or NULL: no rotation */
+    const int32_t *pos;             /* device [n_tokens]; unused without rope */
+    void *q_out, *k_out;            /* may alias q and k; k_out may be NULL */
+    int64_t ldq_out, ldk_out;
+    const vb_pages *pages;          /* or NULL: k and v are not stored */
+    const int32_t *seq, *row;       /* device [n_tokens]: where token t is stored; seq -1: nowhere.  No row twice. */
+} vb_qk_args;
+int vb_qk_norm_rope(vb_ctx *ctx, const vb_qk_args *a);
+
+/* Attention of the newest tokens of each sequence over its paged cache
+ * (grouped-query; scores and softmax in 32 bits).  Sequence i of the call has
+ * the tokens start[i] .. start[i+1]-1 of q, whose K/V rows are the last ones
+ * of sequence seqs[i] (stored before the call).  A token sees every row
+ * before them and, of them, those whose bits its mask row has: a tree of
+ * drafted tokens names its ancestors and itself.  Without a mask they are a
+ * chain: token j sees 0 .. j, so one token is a decode step and many are a
+ * prompt.  A token that sees nothing gives zeros; what lies in rows that it
+ * does not see never reaches its result. */
+typedef struct {
+    int type;                       /* of q and out: VB_TYPE_F32 (cache BF16), or the cache's type */
+    int layer;
+    int n;                          /* sequences in the call */
+    int n_tokens;                   /* rows of q and out */
+    int max_tokens;                 /* at least the most tokens of one sequence */
+    int n_heads;                    /* a multiple of the cache's n_kv_heads */
+    int mask_words;                 /* 32-bit words of a mask row */
+    float scale;                    /* 0 = 1/sqrt(head_dim) */
+    const void *q;                  /* [n_tokens][n_heads][head_dim], row stride ldq elements (0 = packed) */
+    int64_t ldq;
+    void *out;                      /* the same shape */
+    int64_t ldo;
+    const int32_t *seqs, *start;    /* device [n], [n+1] */
+    const uint32_t *mask;           /* device [n_tokens][mask_words] or NULL */
+    const vb_pages *pages;
+} vb_tree_args;
+int vb_tree_attention(vb_ctx *ctx, const vb_tree_args *a);
 
 /* Host helpers restated from the reference for its callers. */
 float vb_cfm_sway_t_bf16(int step, int n_steps);   /* src/cfm_solver.c:27-37 */

@@ -194,6 +194,9 @@ extern "C" void vb_destroy(vb_ctx *ctx) {
     for (auto &r : ctx->ropes) cudaFree(r.d_cs);
     if (ctx->ws.ptr) cudaFree(ctx->ws.ptr);
     if (ctx->attn_ws.ptr) cudaFree(ctx->attn_ws.ptr);
+    if (ctx->pages_ws.ptr) cudaFree(ctx->pages_ws.ptr);
+    if (ctx->tree_ws.ptr) cudaFree(ctx->tree_ws.ptr);
+    if (ctx->op_error) cudaFree(ctx->op_error);
     gemm_free(ctx);
     if (ctx->own_stream_handle) cudaStreamDestroy(ctx->own_stream_handle);
     delete ctx;
@@ -208,6 +211,12 @@ extern "C" int vb_device_status(vb_ctx *ctx, int *device_error) {
     int rc = gemm_device_error(ctx, device_error);
     if (rc) return rc;
     if (*device_error) return set_error(ctx, VB_ERR_BACKEND, "mat-mul kernel reported error %d", *device_error);
+    VB_CHECK(ctx, cudaStreamSynchronize(ctx->stream));
+    VB_CHECK(ctx, cudaMemcpy(device_error, ctx->op_error, sizeof(int), cudaMemcpyDeviceToHost));
+    if (*device_error) {
+        VB_CHECK(ctx, cudaMemset(ctx->op_error, 0, sizeof(int)));
+        return set_error(ctx, VB_ERR_BACKEND, "paged-cache operator reported error %d", *device_error);
+    }
     return VB_OK;
 }
 
@@ -358,6 +367,19 @@ extern "C" void vb_cfm_noise(uint64_t seed, int ar_step, float *x, int n) {
         u2 = fmaxf(1e-6f, fminf(u2, 1.0f - 1e-6f));
         x[j] = host_bf16(sqrtf(-2.0f * logf(u1)) * cosf(2.0f * 3.14159265358979323846f * u2));
     }
+}
+
+extern "C" int vb_rope_table(int rot_dim, float theta, int longrope, int n_pos, float *host) {
+    if (!host || rot_dim <= 0 || rot_dim % 2 || n_pos < 0 || !(theta > 0.0f) || (longrope && rot_dim != 128))
+        return VB_ERR_INVALID_ARG;
+    try {
+        std::vector<float> cs;
+        rope_table_host(rot_dim, theta, longrope, n_pos, cs);
+        if (!cs.empty()) memcpy(host, cs.data(), cs.size() * sizeof(float));
+    } catch (...) {
+        return VB_ERR_OOM;
+    }
+    return VB_OK;
 }
 
 extern "C" int vb_round_cache_capacity(int required, int model_max) {

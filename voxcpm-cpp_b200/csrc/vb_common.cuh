@@ -85,6 +85,9 @@ struct vb_ctx {
     int gemm_i8 = 1;                    // Q8_0 on the int8 tensor cores: 1 where faster (the default),
                                         // 2 always (VB_GEMM_I8=2), 0 never (VB_GEMM_I8=0: the fp16 split form)
     void *gemm = nullptr;               // tensor-core path state (vb_gemm.cu)
+    vb::Arena pages_ws;                 // paged cache: lists a plan kernel leaves for the copy kernel
+    vb::Arena tree_ws;                  // drafted-token attention: partial results of split rows
+    int *op_error = nullptr;            // device error word of the paged-cache operators (VB_DEV_*)
     void *attn_noalloc = nullptr;       // device address of vb_attention_noalloc's fixed scratch on this device
     long long dep_wait_limit = 0;       // streaming kernel: cycles of a wait on other CTAs (0 = default)
 };

@@ -37,6 +37,7 @@
 #include "vb_device.cuh"
 #include "vb_kernels.cuh"
 #include "vb_stream.cuh"
+#include "vb_tc.cuh"
 
 namespace vb {
 
@@ -75,79 +76,6 @@ struct GemmArgs {
     float *out_x;
     const float *alpha, *sr_scale, *sr_bias;
 };
-
-__device__ __forceinline__ uint64_t sw128_desc(const void *p) {
-    uint64_t d = (uint64_t)((smem_u32(p) >> 4) & 0x3FFFu);
-    d |= (uint64_t)1 << 16;                 // leading byte offset (unused for swizzled K-major)
-    d |= (uint64_t)(1024 >> 4) << 32;       // stride byte offset: 8 rows x 128 B
-    d |= (uint64_t)1 << 46;                 // descriptor version (sm_100)
-    d |= (uint64_t)2 << 61;                 // 128-byte swizzle
-    return d;
-}
-
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ void umma_f16(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-}
-
-__device__ __forceinline__ void umma_tf32(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-
-// Programmatic dependent launch: kernels of the M >= 16 chain are launched
-// so that they may start while the previous kernel of the stream finishes;
-// this waits until that kernel has completed and its writes are visible
-// (a no-op when the launch was not programmatic).
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the next programmatic launch of the stream begin scheduling its CTAs
-// (they still wait for this grid to complete before touching memory).
-__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// The load and its wait are one asm statement: the destination registers
-// are written asynchronously until tcgen05.wait::ld, and with two
-// statements the compiler may schedule a use of a register between them.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-
-// Bounded mbarrier wait (no abort flag: every role of the CTA reaches the
-// teardown on its own once its waits have ended).
-__device__ __forceinline__ bool gm_wait(uint64_t *bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity))
-        if (clock64() - t0 > WAIT_LIMIT_CYCLES) return false;
-    return true;
-}
 
 __device__ __forceinline__ int64_t gm_out_row(const GemmArgs &a, int m) {
     if (a.seg_plain) return m;
@@ -1195,7 +1123,7 @@ static EncodeTiledFn encode_fn() {
 
 // 2-D tensor map over a row-major [rows][cols] array of `esize`-byte
 // elements, box [box_rows][box_cols].
-static bool make_map(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int esize, int64_t cols, int64_t rows,
+bool make_map(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int esize, int64_t cols, int64_t rows,
                      int box_cols, int box_rows, bool swizzle) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
@@ -1270,24 +1198,6 @@ int init_gemm(vb_ctx *ctx) {
     // no later call allocates them (and every call can be captured)
     if (!gemm_state(ctx)) return set_error(ctx, VB_ERR_OOM, "mat-mul state allocation failed");
     return VB_OK;
-}
-
-// Launch with programmatic stream serialization (the kernel begins with
-// pdl_wait before it reads anything the previous kernel wrote).
-template <typename... KArgs, typename... Args>
-static cudaError_t pdl_launch(vb_ctx *ctx, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                              Args &&...args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
 // Q8_0 weights on the int8 tensor cores (gemm_i8_kernel); K % 128 == 0.

@@ -1,0 +1,628 @@
+// vb_pages.cu -- page operations of a paged K/V cache: extend (with copy on
+// write), fork, keep (the accepted path of a draft), truncate, compact.
+//
+// The bookkeeping lives on the device: a call is a plan (which pages, which
+// rows) and, where rows move, a copy that follows the plan's list.  The plan
+// of a call that allocates or checks across requests runs in one CTA (the
+// free pages are found by one scan of the counts, requests are a few dozen);
+// calls whose requests touch only their own table rows and add to the counts
+// atomically (fork, truncate: integer adds, so the order does not show) run
+// one CTA column per request.  Both kernels of a call are programmatic
+// dependent launches.
+#include "vb_common.cuh"
+#include "vb_kernels.cuh"
+#include "vb_tc.cuh"
+
+#include <algorithm>
+#include <climits>
+
+namespace vb {
+
+constexpr int PG_PLAN = 1024;        // threads of a plan CTA
+constexpr int PG_SCAN = 8;           // counts per thread and scan step
+constexpr int PG_COPY = 256;
+constexpr int PG_MAX_SEQS = 16384;
+
+struct PageJob {                     // rows 0 .. rows-1 of page src, in every layer, to page dst
+    int src, dst, rows, pad;
+};
+
+// Exclusive sum over the CTA's threads; total: the sum of all.  sh: 33 ints.
+__device__ int block_scan(int v, int *sh, int &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) sh[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        int w = lane < (int)(blockDim.x >> 5) ? sh[lane] : 0;
+        const int w0 = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        sh[lane] = w - w0;
+        if (lane == 31) sh[32] = w;
+    }
+    __syncthreads();
+    const int r = sh[warp] + x - v;
+    total = sh[32];
+    __syncthreads();
+    return r;
+}
+
+// First error of a call: lowest request, then lowest code.
+struct PageError {
+    int key;                         // request * 16 + code, INT_MAX: none
+    __device__ void at(int request, int code) { atomicMin(&key, request * 16 + code); }
+};
+
+__device__ void record(const vb_pages &p, int key) {
+    p.status[1] = key >> 4;
+    p.status[0] = key & 15;
+}
+
+// Marks the requests' sequences in a bitmap of shared memory and reports
+// those out of range or met before.
+__device__ void check_seqs(const vb_pages &p, int n, const int32_t *seqs, uint32_t *bits, PageError *err) {
+    for (int i = threadIdx.x; i < (p.n_seqs + 31) / 32; i += blockDim.x) bits[i] = 0;
+    __syncthreads();
+    bool twice = false;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int s = seqs[i];
+        if (s < 0 || s >= p.n_seqs) err->at(i, VB_PAGES_SEQ);
+        else twice |= atomicOr(&bits[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u;
+    }
+    if (!__syncthreads_or(twice)) return;
+    for (int i = threadIdx.x; i < n; i += blockDim.x)     // which request came second
+        for (int j = 0; j < i; j++)
+            if (seqs[j] == seqs[i]) {
+                err->at(i, VB_PAGES_SEQ);
+                break;
+            }
+}
+
+__global__ void __launch_bounds__(PG_PLAN) pages_extend_plan(vb_pages p, int n, const int32_t *seqs,
+                                                             const int32_t *rows, int *ws) {
+    extern __shared__ int sm[];
+    __shared__ int scan[33];
+    __shared__ PageError err;
+    pdl_trigger();
+    pdl_wait();
+    int *last = sm, *first = sm + n;                          // [n] shared partly filled page (or -1), first new page
+    uint32_t *bits = reinterpret_cast<uint32_t *>(sm + 2 * n);
+    PageJob *jobs = reinterpret_cast<PageJob *>(ws + 4);
+    int *freelist = ws + 4 + 4 * n;
+    const int P = p.page_rows;
+    if (threadIdx.x == 0) {
+        err.key = INT_MAX;
+        ws[0] = 0;
+    }
+    if (p.status[0]) return;                                  // every thread reads the same word
+    __syncthreads();
+    check_seqs(p, n, seqs, bits, &err);
+    __syncthreads();
+    if (err.key != INT_MAX) {
+        if (threadIdx.x == 0) record(p, err.key);
+        return;
+    }
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int s = seqs[i], len = p.length[s], r = rows[i];
+        last[i] = -1;
+        if (r < 0) err.at(i, VB_PAGES_COUNT);
+        else if ((int64_t)len + r > (int64_t)p.max_pages * P) err.at(i, VB_PAGES_LONG);
+        else if (r > 0 && len % P) {
+            const int pg = p.table[(int64_t)s * p.max_pages + len / P];
+            if (pg < 0 || pg >= p.n_pages) err.at(i, VB_PAGES_TABLE);
+            else if (p.refs[pg] > 1) last[i] = pg;
+        }
+    }
+    __syncthreads();
+    if (err.key != INT_MAX) {
+        if (threadIdx.x == 0) record(p, err.key);
+        return;
+    }
+    // copy on write: a request leaves the shared page unless every other
+    // holder has left it before (earlier requests of this call)
+    const int per = (n + blockDim.x - 1) / blockDim.x;
+    const int i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
+    int mine = 0;
+    for (int i = i0; i < i1; i++) {
+        const int s = seqs[i], len = p.length[s];
+        int need = (len + rows[i] + P - 1) / P - (len + P - 1) / P;
+        const int pg = last[i];
+        if (pg >= 0) {
+            int left = p.refs[pg];
+            for (int j = 0; j < i && left > 1; j++) left -= last[j] == pg;
+            if (left > 1) need = need + 1 | INT_MIN;          // top bit: the first new page is the copy
+        }
+        first[i] = need;
+        mine += need & INT_MAX;
+    }
+    int total;
+    int at = block_scan(mine, scan, total);
+    // the free pages, lowest numbers first
+    int found = 0;
+    for (int base = 0; base < p.n_pages && found < total; base += blockDim.x * PG_SCAN) {
+        const int q0 = base + threadIdx.x * PG_SCAN;
+        uint32_t is_free = 0;
+#pragma unroll
+        for (int j = 0; j < PG_SCAN; j++)
+            if (q0 + j < p.n_pages && p.refs[q0 + j] == 0) is_free |= 1u << j;
+        int here;
+        int k = found + block_scan(__popc(is_free), scan, here);
+        for (uint32_t b = is_free; b && k < total; b &= b - 1) freelist[k++] = q0 + __ffs(b) - 1;
+        found += here;
+    }
+    __syncthreads();
+    if (found < total) {
+        if (threadIdx.x == 0) {
+            // the request that the pages run out at
+            int sum = 0, i = 0;
+            for (; i < n - 1; i++)
+                if ((sum += first[i] & INT_MAX) > found) break;
+            record(p, i * 16 + VB_PAGES_FULL);
+        }
+        return;
+    }
+    for (int i = i0; i < i1; i++) {
+        const int need = first[i];
+        if (need >= 0) last[i] = -1;                          // keeps its page
+        first[i] = at;
+        at += need & INT_MAX;
+    }
+    __syncthreads();
+    // one warp per request writes its table entries
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < n; i += blockDim.x >> 5) {
+        const int s = seqs[i], len = p.length[s], r = rows[i], cow = last[i] >= 0;
+        const int begin = (len + P - 1) / P - cow, want = (len + r + P - 1) / P;
+        for (int c = begin + lane; c < want; c += 32) {
+            const int pg = freelist[first[i] + c - begin];
+            p.table[(int64_t)s * p.max_pages + c] = pg;
+            p.refs[pg] = 1;
+        }
+        if (lane == 0) {
+            PageJob j = {0, 0, 0, 0};
+            if (cow) {
+                j = {last[i], freelist[first[i]], len % P, 0};
+                atomicSub(&p.refs[last[i]], 1);
+            }
+            jobs[i] = j;
+        }
+        __syncwarp();
+        if (lane == 0) p.length[s] = len + r;
+    }
+    if (threadIdx.x == 0) ws[0] = n;
+}
+
+// Copies the first rows of pages: grid (layer x {k, v}, request).
+__global__ void __launch_bounds__(PG_COPY) pages_copy_rows(vb_pages p, const int *ws) {
+    pdl_trigger();
+    pdl_wait();
+    if ((int)blockIdx.y >= ws[0]) return;
+    const PageJob j = reinterpret_cast<const PageJob *>(ws + 4)[blockIdx.y];
+    if (j.rows == 0) return;
+    const int row16 = p.head_dim / 8, head16 = p.page_rows * row16, n16 = j.rows * row16;   // 16-byte units
+    uint4 *pool = static_cast<uint4 *>((blockIdx.x & 1) ? p.v : p.k) +
+                  (int64_t)(blockIdx.x >> 1) * p.n_pages * p.n_kv_heads * head16;
+    const uint4 *src = pool + (int64_t)j.src * p.n_kv_heads * head16;
+    uint4 *dst = pool + (int64_t)j.dst * p.n_kv_heads * head16;
+    for (int i = threadIdx.x; i < p.n_kv_heads * n16; i += PG_COPY) {
+        const int o = i / n16 * head16 + i % n16;
+        dst[o] = src[o];
+    }
+}
+
+// grid (request, column block): every thread owns table columns of one dst.
+__global__ void __launch_bounds__(256) pages_fork_kernel(vb_pages p, int n, const int32_t *src, const int32_t *dst) {
+    extern __shared__ int sm[];
+    __shared__ PageError err;
+    pdl_trigger();
+    pdl_wait();
+    uint32_t *bits = reinterpret_cast<uint32_t *>(sm);
+    if (threadIdx.x == 0) err.key = INT_MAX;
+    if (p.status[0]) return;
+    __syncthreads();
+    check_seqs(p, n, dst, bits, &err);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int s = src[i];
+        if (s < 0 || s >= p.n_seqs || (bits[s >> 5] >> (s & 31) & 1u)) err.at(i, VB_PAGES_SEQ);
+    }
+    __syncthreads();
+    if (err.key != INT_MAX) {
+        if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) record(p, err.key);
+        return;
+    }
+    const int s = src[blockIdx.x], d = dst[blockIdx.x];
+    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < p.max_pages; c += gridDim.y * blockDim.x) {
+        const int now = p.table[(int64_t)s * p.max_pages + c], old = p.table[(int64_t)d * p.max_pages + c];
+        if (old >= 0 && old < p.n_pages) atomicSub(&p.refs[old], 1);
+        if (now >= 0 && now < p.n_pages) atomicAdd(&p.refs[now], 1);
+        if (now >= 0 || old >= 0) p.table[(int64_t)d * p.max_pages + c] = now;
+    }
+    if (blockIdx.y == 0 && threadIdx.x == 0) p.length[d] = p.length[s];
+}
+
+// grid (request, column block).  cut: the new lengths.
+__global__ void __launch_bounds__(256) pages_truncate_kernel(vb_pages p, int n, const int32_t *seqs,
+                                                             const int32_t *cut) {
+    extern __shared__ int sm[];
+    __shared__ PageError err;
+    pdl_trigger();
+    pdl_wait();
+    uint32_t *bits = reinterpret_cast<uint32_t *>(sm);
+    if (threadIdx.x == 0) err.key = INT_MAX;
+    if (p.status[0]) return;
+    __syncthreads();
+    check_seqs(p, n, seqs, bits, &err);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x)
+        if (cut[i] < 0) err.at(i, VB_PAGES_COUNT);
+    __syncthreads();
+    if (err.key != INT_MAX) {
+        if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) record(p, err.key);
+        return;
+    }
+    const int s = seqs[blockIdx.x], len = cut[blockIdx.x];
+    const int keep = len / p.page_rows + (len % p.page_rows != 0);
+    for (int c = keep + blockIdx.y * blockDim.x + threadIdx.x; c < p.max_pages; c += gridDim.y * blockDim.x) {
+        const int old = p.table[(int64_t)s * p.max_pages + c];
+        if (old < 0) continue;
+        if (old < p.n_pages) atomicSub(&p.refs[old], 1);
+        p.table[(int64_t)s * p.max_pages + c] = -1;
+    }
+    if (blockIdx.y == 0 && threadIdx.x == 0) p.length[s] = min(p.length[s], len);
+}
+
+// moves[i*ld + j]: pool rows (page * page_rows + slot) that row j of request
+// i's path comes from and goes to; -1: stays.
+__global__ void __launch_bounds__(PG_PLAN) pages_keep_plan(vb_pages p, int n, const int32_t *seqs,
+                                                           const int32_t *drafted, const int32_t *kept,
+                                                           const int32_t *path, int ld, int *ws) {
+    extern __shared__ int sm[];
+    __shared__ PageError err;
+    pdl_trigger();
+    pdl_wait();
+    uint32_t *bits = reinterpret_cast<uint32_t *>(sm);
+    int2 *moves = reinterpret_cast<int2 *>(ws + 4);
+    const int P = p.page_rows;
+    if (threadIdx.x == 0) {
+        err.key = INT_MAX;
+        ws[0] = 0;
+    }
+    if (p.status[0]) return;
+    __syncthreads();
+    check_seqs(p, n, seqs, bits, &err);
+    __syncthreads();
+    if (err.key == INT_MAX)
+        for (int i = threadIdx.x; i < n; i += blockDim.x) {
+            const int d = drafted[i], k = kept[i];
+            if (d < 0 || k < 0 || k > d || k > ld || d > p.length[seqs[i]]) err.at(i, VB_PAGES_COUNT);
+        }
+    __syncthreads();
+    if (err.key == INT_MAX)
+        for (int64_t e = threadIdx.x; e < (int64_t)n * ld; e += blockDim.x) {
+            const int i = (int)(e / ld), j = (int)(e % ld);
+            int2 mv = make_int2(-1, -1);
+            if (j < kept[i]) {
+                const int s = seqs[i], at = path[e], base = p.length[s] - drafted[i];
+                const int32_t *row = p.table + (int64_t)s * p.max_pages;
+                if (at < 0 || at >= drafted[i] || (j > 0 && path[e - 1] >= at)) err.at(i, VB_PAGES_PATH);
+                else if (at != j) {
+                    const int ps = row[(base + at) / P], pd = row[(base + j) / P];
+                    if (ps < 0 || ps >= p.n_pages || pd < 0 || pd >= p.n_pages) err.at(i, VB_PAGES_TABLE);
+                    else if (p.refs[pd] != 1) err.at(i, VB_PAGES_SHARED);
+                    mv = make_int2(ps * P + (base + at) % P, pd * P + (base + j) % P);
+                }
+            }
+            moves[e] = mv;
+        }
+    __syncthreads();
+    if (err.key != INT_MAX) {
+        if (threadIdx.x == 0) record(p, err.key);
+        return;
+    }
+    // pages past the new end
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < n; i += blockDim.x >> 5) {
+        const int s = seqs[i], len = p.length[s], now = len - drafted[i] + kept[i];
+        for (int c = (now + P - 1) / P + lane; c < (len + P - 1) / P; c += 32) {
+            const int old = p.table[(int64_t)s * p.max_pages + c];
+            if (old >= 0 && old < p.n_pages) atomicSub(&p.refs[old], 1);
+            p.table[(int64_t)s * p.max_pages + c] = -1;
+        }
+        __syncwarp();
+        if (lane == 0) p.length[s] = now;
+    }
+    if (threadIdx.x == 0) ws[0] = n;
+}
+
+// grid (column blocks, request): a thread owns 16 bytes of every row of one
+// (layer, k or v, head) and walks the path in order.  A row goes to a place
+// at or before its own and later sources lie behind it, so a batch that is
+// loaded before it is stored never reads what it wrote.
+__global__ void __launch_bounds__(PG_COPY) pages_move_rows(vb_pages p, int ld, const int *ws) {
+    constexpr int B = 8;
+    pdl_trigger();
+    pdl_wait();
+    if ((int)blockIdx.y >= ws[0]) return;
+    const int2 *mv = reinterpret_cast<const int2 *>(ws + 4) + (int64_t)blockIdx.y * ld;
+    const int row16 = p.head_dim / 8;
+    const int64_t col = (int64_t)blockIdx.x * PG_COPY + threadIdx.x;
+    if (col >= (int64_t)p.n_layers * 2 * p.n_kv_heads * row16) return;
+    const int c = (int)(col % row16), g = (int)(col / row16 % p.n_kv_heads);
+    const int lay = (int)(col / row16 / p.n_kv_heads);
+    uint4 *pool = static_cast<uint4 *>((lay & 1) ? p.v : p.k) +
+                  (int64_t)(lay >> 1) * p.n_pages * p.n_kv_heads * p.page_rows * row16;
+    auto at = [&](int r) {          // 16-byte unit of pool row r for this thread's head
+        const int pg = r / p.page_rows, sl = r % p.page_rows;
+        return (((int64_t)pg * p.n_kv_heads + g) * p.page_rows + sl) * row16 + c;
+    };
+    for (int j0 = 0; j0 < ld; j0 += B) {
+        uint4 x[B];
+#pragma unroll
+        for (int j = 0; j < B; j++)
+            if (j0 + j < ld && mv[j0 + j].x >= 0) x[j] = pool[at(mv[j0 + j].x)];
+#pragma unroll
+        for (int j = 0; j < B; j++)
+            if (j0 + j < ld && mv[j0 + j].x >= 0) pool[at(mv[j0 + j].y)] = x[j];
+    }
+}
+
+// ws: [0] live pages (0 after an error), [4 ..] the new number of each page,
+// then the old number of each new one.
+__global__ void __launch_bounds__(PG_PLAN) pages_compact_plan(vb_pages p, vb_pages to, int *ws) {
+    __shared__ int scan[33];
+    __shared__ PageError err;
+    pdl_trigger();
+    pdl_wait();
+    int *number = ws + 4, *live = ws + 4 + p.n_pages;
+    if (threadIdx.x == 0) {
+        err.key = INT_MAX;
+        ws[0] = 0;
+        ws[1] = 0;
+    }
+    if (p.status[0]) return;
+    __syncthreads();
+    for (int64_t e = threadIdx.x; e < (int64_t)p.n_seqs; e += blockDim.x)
+        if (p.length[e] < 0 || (int64_t)p.length[e] > (int64_t)p.max_pages * p.page_rows)
+            err.at((int)e, VB_PAGES_LONG);
+    int total = 0;
+    for (int base = 0; base < p.n_pages; base += blockDim.x * PG_SCAN) {
+        const int q0 = base + threadIdx.x * PG_SCAN;
+        uint32_t used = 0;
+#pragma unroll
+        for (int j = 0; j < PG_SCAN; j++)
+            if (q0 + j < p.n_pages && p.refs[q0 + j] > 0) used |= 1u << j;
+        int here;
+        int k = total + block_scan(__popc(used), scan, here);
+#pragma unroll
+        for (int j = 0; j < PG_SCAN; j++)
+            if (q0 + j < p.n_pages) {
+                const bool u = used >> j & 1u;
+                number[q0 + j] = u ? k : -1;
+                if (u) live[k++] = q0 + j;
+            }
+        total += here;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && total > to.n_pages) err.at(0, VB_PAGES_FULL);
+    __syncthreads();
+    if (err.key != INT_MAX) {
+        if (threadIdx.x == 0) record(p, err.key);
+        return;
+    }
+    for (int i = threadIdx.x; i < to.n_pages; i += blockDim.x) to.refs[i] = i < total ? p.refs[live[i]] : 0;
+    for (int i = threadIdx.x; i < p.n_seqs; i += blockDim.x) to.length[i] = p.length[i];
+    if (threadIdx.x < 4) to.status[threadIdx.x] = 0;
+    if (threadIdx.x == 0) {
+        ws[0] = total;
+        ws[1] = 1;
+    }
+}
+
+// Page contents (a unit: the K or V of one page of one layer, contiguous)
+// and the table, over all CTAs.
+__global__ void __launch_bounds__(PG_COPY) pages_compact_copy(vb_pages p, vb_pages to, const int *ws) {
+    constexpr int B = 4;
+    pdl_trigger();
+    pdl_wait();
+    if (!ws[1]) return;
+    const int total = ws[0];
+    const int *number = ws + 4, *live = ws + 4 + p.n_pages;
+    const int64_t page16 = (int64_t)p.n_kv_heads * p.page_rows * (p.head_dim / 8);
+    const int64_t units = (int64_t)total * p.n_layers * 2;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int j = (int)(u % total), lay = (int)(u / total);
+        const uint4 *src = static_cast<const uint4 *>((lay & 1) ? p.v : p.k) +
+                           ((int64_t)(lay >> 1) * p.n_pages + live[j]) * page16;
+        uint4 *dst = static_cast<uint4 *>((lay & 1) ? to.v : to.k) + ((int64_t)(lay >> 1) * to.n_pages + j) * page16;
+        for (int64_t i = threadIdx.x; i < page16; i += B * PG_COPY) {
+            uint4 x[B];
+#pragma unroll
+            for (int b = 0; b < B; b++)
+                if (i + b * PG_COPY < page16) x[b] = src[i + b * PG_COPY];
+#pragma unroll
+            for (int b = 0; b < B; b++)
+                if (i + b * PG_COPY < page16) dst[i + b * PG_COPY] = x[b];
+        }
+    }
+    const int64_t entries = (int64_t)to.n_seqs * to.max_pages;
+    for (int64_t e = (int64_t)blockIdx.x * PG_COPY + threadIdx.x; e < entries; e += (int64_t)gridDim.x * PG_COPY) {
+        const int64_t s = e / to.max_pages, c = e % to.max_pages;
+        const int old = c < p.max_pages ? p.table[s * p.max_pages + c] : -1;
+        to.table[e] = old >= 0 && old < p.n_pages ? number[old] : -1;
+    }
+}
+
+// -------------------------------------------------------------------- host
+int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who) {
+    if (!p || !p->k || !p->v || !p->table || !p->length || !p->refs || !p->status)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "%s: null cache or cache pointer", who);
+    if (p->type != VB_TYPE_BF16 && p->type != VB_TYPE_F16)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "%s: cache rows are BF16 or F16", who);
+    if (p->n_layers <= 0 || p->n_pages <= 0 || p->n_kv_heads <= 0 || p->n_seqs <= 0 || p->max_pages <= 0 ||
+        p->n_seqs > PG_MAX_SEQS)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "%s: cache sizes out of range", who);
+    if (p->page_rows < 16 || p->page_rows > 1024 || (p->page_rows & (p->page_rows - 1)))
+        return set_error(ctx, VB_ERR_INVALID_ARG, "%s: page_rows must be a power of two, 16 to 1024", who);
+    if (p->head_dim < 8 || p->head_dim > 256 || p->head_dim % 8)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "%s: head_dim must be a multiple of 8, at most 256", who);
+    // row numbers of one layer, and rows of one sequence, are 32-bit
+    if ((int64_t)p->n_pages * p->n_kv_heads * p->page_rows > INT_MAX || (int64_t)p->max_pages * p->page_rows > INT_MAX)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "%s: cache too large", who);
+    if (((uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->table | (uintptr_t)p->length | (uintptr_t)p->refs |
+         (uintptr_t)p->status) & 15)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "%s: cache pointers must be 16-byte aligned", who);
+    return VB_OK;
+}
+
+static int check_call(vb_ctx *ctx, const vb_pages *p, int n, const char *who, bool pointers) {
+    int rc = check_pages(ctx, p, who);
+    if (rc) return rc;
+    if (n < 0 || n > p->n_seqs) return set_error(ctx, VB_ERR_INVALID_ARG, "%s: 0 to n_seqs requests", who);
+    if (n > 0 && !pointers) return set_error(ctx, VB_ERR_INVALID_ARG, "%s: null pointer", who);
+    return VB_OK;
+}
+
+static size_t seq_bits(const vb_pages *p) { return (size_t)((p->n_seqs + 31) / 32) * 4; }
+
+int init_pages(vb_ctx *ctx) {
+    VB_CHECK(ctx, cudaMalloc(&ctx->op_error, 256));
+    VB_CHECK(ctx, cudaMemset(ctx->op_error, 0, 256));
+    VB_CHECK(ctx, cudaFuncSetAttribute(pages_extend_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       2 * PG_MAX_SEQS * 4 + PG_MAX_SEQS / 8));
+    return VB_OK;
+}
+
+}  // namespace vb
+
+using namespace vb;
+
+extern "C" int vb_pages_init(vb_ctx *ctx, const vb_pages *p) {
+    if (!ctx) return VB_ERR_INVALID_ARG;
+    int rc = check_pages(ctx, p, "vb_pages_init");
+    if (rc) return rc;
+    VB_CHECK(ctx, cudaMemsetAsync(p->table, 0xff, (size_t)p->n_seqs * p->max_pages * 4, ctx->stream));
+    VB_CHECK(ctx, cudaMemsetAsync(p->length, 0, (size_t)p->n_seqs * 4, ctx->stream));
+    VB_CHECK(ctx, cudaMemsetAsync(p->refs, 0, (size_t)p->n_pages * 4, ctx->stream));
+    VB_CHECK(ctx, cudaMemsetAsync(p->status, 0, 16, ctx->stream));
+    return VB_OK;
+}
+
+extern "C" int vb_pages_extend(vb_ctx *ctx, const vb_pages *p, int n, const int32_t *seqs, const int32_t *rows) {
+    if (!ctx) return VB_ERR_INVALID_ARG;
+    int rc = check_call(ctx, p, n, "vb_pages_extend", seqs && rows);
+    if (rc || n == 0) return rc;
+    rc = arena_reserve(ctx, ctx->pages_ws, 16 + (size_t)n * sizeof(PageJob) + (size_t)p->n_pages * 4);
+    if (rc) return rc;
+    int *ws = static_cast<int *>(ctx->pages_ws.ptr);
+    VB_CHECK(ctx, pdl_launch(ctx, pages_extend_plan, dim3(1), dim3(PG_PLAN), (size_t)2 * n * 4 + seq_bits(p), *p, n,
+                             seqs, rows, ws));
+    VB_LAUNCH_CHECK(ctx, "pages_extend_plan");
+    VB_CHECK(ctx, pdl_launch(ctx, pages_copy_rows, dim3(2 * p->n_layers, n), dim3(PG_COPY), 0, *p,
+                             static_cast<const int *>(ws)));
+    VB_LAUNCH_CHECK(ctx, "pages_copy_rows");
+    return VB_OK;
+}
+
+static dim3 column_grid(const vb_pages *p, int n) {
+    return dim3(n, std::min(16, (p->max_pages + 255) / 256));
+}
+
+extern "C" int vb_pages_fork(vb_ctx *ctx, const vb_pages *p, int n, const int32_t *src, const int32_t *dst) {
+    if (!ctx) return VB_ERR_INVALID_ARG;
+    int rc = check_call(ctx, p, n, "vb_pages_fork", src && dst);
+    if (rc || n == 0) return rc;
+    VB_CHECK(ctx, pdl_launch(ctx, pages_fork_kernel, column_grid(p, n), dim3(256), seq_bits(p), *p, n, src, dst));
+    VB_LAUNCH_CHECK(ctx, "pages_fork");
+    return VB_OK;
+}
+
+extern "C" int vb_pages_truncate(vb_ctx *ctx, const vb_pages *p, int n, const int32_t *seqs, const int32_t *length) {
+    if (!ctx) return VB_ERR_INVALID_ARG;
+    int rc = check_call(ctx, p, n, "vb_pages_truncate", seqs && length);
+    if (rc || n == 0) return rc;
+    VB_CHECK(ctx, pdl_launch(ctx, pages_truncate_kernel, column_grid(p, n), dim3(256), seq_bits(p), *p, n, seqs,
+                             length));
+    VB_LAUNCH_CHECK(ctx, "pages_truncate");
+    return VB_OK;
+}
+
+extern "C" int vb_pages_keep(vb_ctx *ctx, const vb_pages *p, int n, const int32_t *seqs, const int32_t *drafted,
+                             const int32_t *kept, const int32_t *path, int ld_path) {
+    if (!ctx) return VB_ERR_INVALID_ARG;
+    int rc = check_call(ctx, p, n, "vb_pages_keep", seqs && drafted && kept && (path || !ld_path));
+    if (rc) return rc;
+    if (ld_path < 0 || (int64_t)n * ld_path > INT_MAX)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "vb_pages_keep: bad path length");
+    if (n == 0) return VB_OK;
+    rc = arena_reserve(ctx, ctx->pages_ws, 16 + (size_t)n * ld_path * sizeof(int2));
+    if (rc) return rc;
+    int *ws = static_cast<int *>(ctx->pages_ws.ptr);
+    VB_CHECK(ctx, pdl_launch(ctx, pages_keep_plan, dim3(1), dim3(PG_PLAN), seq_bits(p), *p, n, seqs, drafted, kept,
+                             path, ld_path, ws));
+    VB_LAUNCH_CHECK(ctx, "pages_keep_plan");
+    const int64_t cols = (int64_t)p->n_layers * 2 * p->n_kv_heads * (p->head_dim / 8);
+    VB_CHECK(ctx, pdl_launch(ctx, pages_move_rows, dim3((unsigned)((cols + PG_COPY - 1) / PG_COPY), n), dim3(PG_COPY),
+                             0, *p, ld_path, static_cast<const int *>(ws)));
+    VB_LAUNCH_CHECK(ctx, "pages_move_rows");
+    return VB_OK;
+}
+
+extern "C" int vb_pages_compact(vb_ctx *ctx, const vb_pages *p, const vb_pages *to) {
+    if (!ctx) return VB_ERR_INVALID_ARG;
+    int rc = check_pages(ctx, p, "vb_pages_compact");
+    if (rc) return rc;
+    rc = check_pages(ctx, to, "vb_pages_compact");
+    if (rc) return rc;
+    if (p->type != to->type || p->n_layers != to->n_layers || p->n_kv_heads != to->n_kv_heads ||
+        p->page_rows != to->page_rows || p->head_dim != to->head_dim || p->n_seqs != to->n_seqs ||
+        to->max_pages < p->max_pages)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "vb_pages_compact: the caches hold different rows");
+    if (p->k == to->k || p->v == to->v || p->table == to->table || p->length == to->length || p->refs == to->refs ||
+        p->status == to->status)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "vb_pages_compact: the caches share memory");
+    rc = arena_reserve(ctx, ctx->pages_ws, 16 + (size_t)p->n_pages * 8);
+    if (rc) return rc;
+    int *ws = static_cast<int *>(ctx->pages_ws.ptr);
+    VB_CHECK(ctx, pdl_launch(ctx, pages_compact_plan, dim3(1), dim3(PG_PLAN), 0, *p, *to, ws));
+    VB_LAUNCH_CHECK(ctx, "pages_compact_plan");
+    VB_CHECK(ctx, pdl_launch(ctx, pages_compact_copy, dim3(ctx->sm_count * 8), dim3(PG_COPY), 0, *p, *to,
+                             static_cast<const int *>(ws)));
+    VB_LAUNCH_CHECK(ctx, "pages_compact_copy");
+    return VB_OK;
+}
+
+extern "C" int vb_pages_status(vb_ctx *ctx, const vb_pages *p, int *error, int *request, int *free_pages) {
+    if (!ctx) return VB_ERR_INVALID_ARG;
+    int rc = check_pages(ctx, p, "vb_pages_status");
+    if (rc) return rc;
+    int32_t st[4] = {0, 0, 0, 0};
+    VB_CHECK(ctx, cudaMemcpyAsync(st, p->status, sizeof(st), cudaMemcpyDeviceToHost, ctx->stream));
+    VB_CHECK(ctx, cudaStreamSynchronize(ctx->stream));
+    if (free_pages) {
+        try {
+            std::vector<int32_t> refs((size_t)p->n_pages);
+            VB_CHECK(ctx, cudaMemcpyAsync(refs.data(), p->refs, refs.size() * 4, cudaMemcpyDeviceToHost, ctx->stream));
+            VB_CHECK(ctx, cudaStreamSynchronize(ctx->stream));
+            int n = 0;
+            for (int32_t r : refs) n += r == 0;
+            *free_pages = n;
+        } catch (...) {
+            return set_error(ctx, VB_ERR_OOM, "vb_pages_status: out of host memory");
+        }
+    }
+    if (error) *error = st[0];
+    if (request) *request = st[0] ? st[1] : 0;
+    if (!st[0]) return VB_OK;
+    VB_CHECK(ctx, cudaMemsetAsync(p->status, 0, sizeof(st), ctx->stream));
+    return set_error(ctx, VB_ERR_BACKEND, "paged cache: error %d at request %d", st[0], st[1]);
+}

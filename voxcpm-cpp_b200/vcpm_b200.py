@@ -19,9 +19,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libvcpm_b200.so")
 
 VB_OK, VB_ERR_INVALID_ARG, VB_ERR_BACKEND, VB_ERR_OOM, VB_ERR_NOT_IMPLEMENTED = 0, 1, 5, 6, 7
-TYPE_F32, TYPE_F16, TYPE_Q8_0 = 0, 1, 8
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
 QRULE_X86, QRULE_REF = 0, 1
 OUT_BF16 = 1
+PAGES_SEQ, PAGES_COUNT, PAGES_LONG, PAGES_FULL, PAGES_SHARED, PAGES_PATH, PAGES_TABLE = 1, 2, 3, 4, 5, 6, 7
+DEV_QK_POS, DEV_QK_ROW, DEV_TREE_SEQ, DEV_TREE_PAGE = 21, 22, 31, 32
 GEN_LM_HIDDEN, GEN_LAST_LM_HIDDEN, GEN_RESIDUAL_HIDDEN, GEN_PREV_PATCH = 0, 1, 2, 3
 
 _lib = None
@@ -68,6 +70,30 @@ class GenParts(C.Structure):
         "fsq_in_bias", "fsq_out_bias", "fusion_bias", "stop_proj_bias", "stop_head_bias")] + [
         ("feat_dim", C.c_int), ("patch", C.c_int), ("fsq_scale", C.c_float), ("eps", C.c_float),
         ("cfm_steps", C.c_int), ("cfg_value", C.c_float)]
+
+
+class PagesC(C.Structure):
+    """vb_pages."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "table", "length", "refs", "status")] + [
+        (n, C.c_int) for n in ("type", "n_layers", "n_pages", "n_kv_heads", "page_rows", "head_dim", "n_seqs",
+                               "max_pages")]
+
+
+class QKArgsC(C.Structure):
+    """vb_qk_args."""
+    _fields_ = [(n, C.c_int) for n in ("type", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "rot_dim", "adjacent",
+                                       "norm")] + [("flags", C.c_uint), ("eps", C.c_float), ("rope_rows", C.c_int),
+                                                   ("layer", C.c_int)] + [
+        (n, C.c_void_p) for n in ("q", "k", "v")] + [(n, C.c_int64) for n in ("ldq", "ldk", "ldv")] + [
+        (n, C.c_void_p) for n in ("q_weight", "k_weight", "rope", "pos", "q_out", "k_out")] + [
+        ("ldq_out", C.c_int64), ("ldk_out", C.c_int64)] + [(n, C.c_void_p) for n in ("pages", "seq", "row")]
+
+
+class TreeArgsC(C.Structure):
+    """vb_tree_args."""
+    _fields_ = [(n, C.c_int) for n in ("type", "layer", "n", "n_tokens", "max_tokens", "n_heads", "mask_words")] + [
+        ("scale", C.c_float), ("q", C.c_void_p), ("ldq", C.c_int64), ("out", C.c_void_p), ("ldo", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("seqs", "start", "mask", "pages")]
 
 
 # exported name -> (restype, argtypes)
@@ -160,6 +186,16 @@ SIGNATURES = {
     "vb_vae_stream_upconv_cache_count": (_I, [_P]),
     "vb_vae_stream_patch_samples": (_I, [_P]),
     "vb_vae_stream_state_bytes": (_SZ, [_P]),
+    "vb_pages_init": (_I, [_P, _P]),
+    "vb_pages_extend": (_I, [_P, _P, _I, _P, _P]),
+    "vb_pages_fork": (_I, [_P, _P, _I, _P, _P]),
+    "vb_pages_keep": (_I, [_P, _P, _I, _P, _P, _P, _P, _I]),
+    "vb_pages_truncate": (_I, [_P, _P, _I, _P, _P]),
+    "vb_pages_compact": (_I, [_P, _P, _P]),
+    "vb_pages_status": (_I, [_P, _P, C.POINTER(_I), C.POINTER(_I), C.POINTER(_I)]),
+    "vb_rope_table": (_I, [_I, _F, _I, _I, _P]),
+    "vb_qk_norm_rope": (_I, [_P, _P]),
+    "vb_tree_attention": (_I, [_P, _P]),
     "vb_cfm_sway_t_bf16": (_F, [_I, _I]),
     "vb_cfm_zero_star_steps": (_I, [_I]),
     "vb_cfm_noise": (None, [C.c_uint64, _I, _P, _I]),
@@ -338,6 +374,182 @@ class Context:
     def kv_write(self, k, v, kc, vc, n_rows, T, n_kv, head_dim, dst_row):
         self.check(self.L.vb_kv_write(self.h, _addr(k), _addr(v), _addr(kc), _addr(vc), n_rows, T, n_kv, head_dim,
                                       _addr(dst_row)))
+
+    # ------------------------------------- paged cache and drafted tokens
+    def pages_init(self, p):
+        self.check(self.L.vb_pages_init(self.h, p.ref))
+
+    def pages_extend(self, p, seqs, rows):
+        """Room for rows[i] more rows of seqs[i] (device int32 tensors)."""
+        self.check(self.L.vb_pages_extend(self.h, p.ref, _count(seqs, rows), seqs.data_ptr(), rows.data_ptr()))
+
+    def pages_fork(self, p, src, dst):
+        """dst[i] becomes a copy of src[i] that shares its pages."""
+        self.check(self.L.vb_pages_fork(self.h, p.ref, _count(src, dst), src.data_ptr(), dst.data_ptr()))
+
+    def pages_keep(self, p, seqs, drafted, kept, path):
+        """Of the last drafted[i] rows of seqs[i] keep those at
+        path[i][:kept[i]] (int32 [n][most])."""
+        n = _count(seqs, drafted, kept)
+        if path.dim() != 2 or path.shape[0] != n or str(path.dtype) != "torch.int32" or not path.is_contiguous():
+            raise ValueError("path: contiguous int32 [n][most]")
+        self.check(self.L.vb_pages_keep(self.h, p.ref, n, seqs.data_ptr(), drafted.data_ptr(), kept.data_ptr(),
+                                        path.data_ptr(), path.shape[1]))
+
+    def pages_truncate(self, p, seqs, length):
+        """Drops the rows from length[i] on; 0 frees the sequence."""
+        self.check(self.L.vb_pages_truncate(self.h, p.ref, _count(seqs, length), seqs.data_ptr(), length.data_ptr()))
+
+    def pages_compact(self, p, to):
+        """Moves p's live pages to the front of another cache's pool."""
+        self.check(self.L.vb_pages_compact(self.h, p.ref, to.ref))
+
+    def pages_status(self, p):
+        """(rc, error, request, free pages): synchronises and clears the error."""
+        e, r, f = C.c_int(0), C.c_int(0), C.c_int(0)
+        rc = self.L.vb_pages_status(self.h, p.ref, C.byref(e), C.byref(r), C.byref(f))
+        if rc not in (VB_OK, VB_ERR_BACKEND) or (rc and not e.value):
+            self.check(rc)
+        return rc, e.value, r.value, f.value
+
+    def qk_norm_rope(self, args):
+        self.check(self.L.vb_qk_norm_rope(self.h, args.ref))
+
+    def tree_attention(self, args):
+        self.check(self.L.vb_tree_attention(self.h, args.ref))
+
+
+def _count(*arrays):
+    """Length of device int32 vectors that belong together."""
+    n = arrays[0].shape[0]
+    for a in arrays:
+        if a.dim() != 1 or a.shape[0] != n or str(a.dtype) != "torch.int32" or not (n < 2 or a.is_contiguous()):
+            raise ValueError("contiguous int32 vectors of one length are wanted")
+    return n
+
+
+def _type_of(t):
+    code = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}.get(str(t.dtype))
+    if code is None:
+        raise TypeError(f"float32, float16 or bfloat16 is wanted, not {t.dtype}")
+    return code
+
+
+def _rows(t, width, what):
+    """(address, row stride) of a [rows][width] tensor whose rows are dense."""
+    if t.dim() != 2 or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: [tokens][{width}] with dense rows is wanted")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+def _vector(t, n, what):
+    if t.shape != (n,) or str(t.dtype) != "torch.int32" or not (n < 2 or t.is_contiguous()):
+        raise ValueError(f"{what}: contiguous int32 [{n}] is wanted")
+    return t.data_ptr()
+
+
+class Pages:
+    """A paged K/V cache over the caller's CUDA tensors (vb_pages): k, v
+    [layers][pages][kv heads][page rows][head dim] in bfloat16 or float16,
+    table int32 [sequences][most pages], length int32 [sequences], refs int32
+    [pages], status int32 [4]."""
+
+    def __init__(self, k, v, table, length, refs, status):
+        if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("k and v: [layers][pages][kv heads][page rows][head dim] of one type")
+        layers, pages, kv, rows, hd = k.shape
+        if table.dim() != 2 or length.shape != table.shape[:1] or refs.shape != (pages,) or status.shape != (4,):
+            raise ValueError("table [sequences][pages], length [sequences], refs [pages], status [4]")
+        for t in (k, v, table, length, refs, status):
+            if not t.is_contiguous():
+                raise ValueError("the cache's tensors are contiguous")
+        for t in (table, length, refs, status):
+            if str(t.dtype) != "torch.int32":
+                raise ValueError("table, length, refs and status are int32")
+        self.k, self.v, self.table, self.length, self.refs, self.status = k, v, table, length, refs, status
+        self.c = PagesC(k.data_ptr(), v.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(),
+                        status.data_ptr(), _type_of(k), layers, pages, kv, rows, hd, table.shape[0], table.shape[1])
+        self.ref = C.byref(self.c)
+
+    @classmethod
+    def empty(cls, ctx, layers, pages, kv_heads, page_rows, head_dim, seqs, max_pages, dtype=None):
+        """An empty cache in new tensors."""
+        import torch
+        shape = (layers, pages, kv_heads, page_rows, head_dim)
+        dev = f"cuda:{ctx.device}"
+        new = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
+        k, v = (torch.zeros(shape, dtype=dtype or torch.bfloat16, device=dev) for _ in range(2))
+        p = cls(k, v, new(seqs, max_pages), new(seqs), new(pages), new(4))
+        p.table.fill_(-1)
+        torch.cuda.synchronize()
+        return p
+
+
+class QKArgs:
+    """Arguments of Context.qk_norm_rope (vb_qk_args), made once for a set of
+    buffers.  q, k, v: [tokens][heads * head_dim] with dense rows (slices of a
+    fused projection's rows are fine); q_out, k_out like q, k."""
+
+    def __init__(self, q, k, v, *, heads, kv_heads, head_dim, q_out, k_out=None, rope=None, pos=None, q_weight=None,
+                 k_weight=None, norm=False, eps=1e-5, rot_dim=0, adjacent=False, flags=0, pages=None, layer=0, seq=None,
+                 row=None):
+        n = q.shape[0]
+        qd, kd = heads * head_dim, kv_heads * head_dim
+        c = QKArgsC(type=_type_of(q), n_tokens=n, n_heads=heads, n_kv_heads=kv_heads, head_dim=head_dim,
+                    rot_dim=rot_dim, adjacent=int(adjacent), norm=int(norm), flags=flags, eps=eps, layer=layer)
+        for name, t, width in (("q", q, qd), ("k", k, kd), ("v", v, kd), ("q_out", q_out, qd), ("k_out", k_out, kd)):
+            if t is None:
+                continue
+            if t.dtype != q.dtype or t.shape[0] != n:
+                raise ValueError(f"{name}: {n} rows of q's type are wanted")
+            at, ld = _rows(t, width, name)
+            setattr(c, name, at)
+            setattr(c, "ld" + name, ld)
+        for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if t is not None:
+                if t.shape != (head_dim,) or _type_of(t) != TYPE_F32 or not t.is_contiguous():
+                    raise ValueError(f"{name}: contiguous float32 [{head_dim}] is wanted")
+                setattr(c, name, t.data_ptr())
+        if rope is not None:
+            if rope.dim() != 2 or rope.shape[1] != (rot_dim or head_dim) or _type_of(rope) != TYPE_F32 \
+                    or not rope.is_contiguous():
+                raise ValueError("rope: contiguous float32 [positions][rot_dim] is wanted")
+            c.rope, c.rope_rows, c.pos = rope.data_ptr(), rope.shape[0], _vector(pos, n, "pos")
+        if pages is not None:
+            c.pages, c.seq, c.row = C.addressof(pages.c), _vector(seq, n, "seq"), _vector(row, n, "row")
+        self.c, self.ref = c, C.byref(c)
+        self._keep = (q, k, v, q_out, k_out, rope, pos, q_weight, k_weight, pages, seq, row)
+
+
+class TreeArgs:
+    """Arguments of Context.tree_attention (vb_tree_args), made once for a set
+    of buffers.  q, out: [tokens][heads * head_dim]; seqs int32 [n], start
+    int32 [n + 1]; mask int32 [tokens][words] or None (a chain)."""
+
+    def __init__(self, q, pages, layer, seqs, start, out, *, heads, max_tokens, mask=None, scale=0.0):
+        n, t = seqs.shape[0], q.shape[0]
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out: like q")
+        c = TreeArgsC(type=_type_of(q), layer=layer, n=n, n_tokens=t, max_tokens=max_tokens, n_heads=heads,
+                      scale=scale)
+        c.q, c.ldq = _rows(q, heads * pages.c.head_dim, "q")
+        c.out, c.ldo = _rows(out, heads * pages.c.head_dim, "out")
+        c.seqs, c.start, c.pages = _vector(seqs, n, "seqs"), _vector(start, n + 1, "start"), C.addressof(pages.c)
+        if mask is not None:
+            if mask.dim() != 2 or mask.shape[0] != t or str(mask.dtype) != "torch.int32" or not mask.is_contiguous():
+                raise ValueError("mask: contiguous int32 [tokens][words]")
+            c.mask, c.mask_words = mask.data_ptr(), mask.shape[1]
+        self.c, self.ref = c, C.byref(c)
+        self._keep = (q, pages, seqs, start, out, mask)
+
+
+def rope_table(rot_dim, theta, longrope, n_pos):
+    """(cos, sin) pairs of positions 0..n_pos-1 (float32 [n_pos][rot_dim])."""
+    t = np.empty((n_pos, rot_dim), np.float32)
+    rc = lib().vb_rope_table(rot_dim, theta, int(longrope), n_pos, t.ctypes.data)
+    if rc != VB_OK:
+        raise VBError(rc, "vb_rope_table: bad argument")
+    return t
 
 
 class Program:
