@@ -614,12 +614,14 @@ int vb_pages_status(vb_ctx *ctx, const vb_pages *p, int *error, int *request, in
 
 /* Device error codes of the two operators below (vb_device_status).  The
  * token or sequence concerned is skipped: nothing is stored for it, its
- * output row is zero. */
+ * output rows are zero (a sequence whose start is out of bounds has none;
+ * after VB_DEV_TREE_PAGE its rows are of no use). */
 enum {
     VB_DEV_QK_POS = 21,   /* position outside the rotation table */
     VB_DEV_QK_ROW = 22,   /* sequence or row outside the cache, or no page there */
     VB_DEV_TREE_SEQ = 31, /* sequence, start or length outside the bounds of the call */
-    VB_DEV_TREE_PAGE = 32 /* a table entry names no page of the pool */
+    VB_DEV_TREE_PAGE = 32, /* a table entry names no page of the pool */
+    VB_DEV_TREE_WAIT = 33 /* a wait inside the kernel ran out (its waits are bounded) */
 };
 
 /* (cos, sin) pairs of positions 0 .. n_pos-1 as vb_rope_neox rotates them

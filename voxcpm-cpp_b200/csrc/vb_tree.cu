@@ -2,94 +2,874 @@
 //
 // For token j of sequence i and query head h of K/V head g:
 //   o = sum_r p_r v_r / sum_r p_r,  p_r = exp(scale * q.k_r - max)
-// over the rows before the draft and the draft rows that j's mask names.
+// over the rows before the draft and the draft rows that j's mask names
+// (without a mask: rows up to its own).  A row that sees nothing gives 0.
 //
-// One warp owns one (token, head): a lane holds head dimensions lane,
-// lane + 32, ..., scores are warp sums, and the maximum and sum run along.
+// The rows of the score matrix are the (token, query head) pairs of one K/V
+// head: T * group rows share every K/V row that is read.  One pass over the
+// cache with the running maximum and sum of the softmax; its tiles go
+// through a TMA ring in shared memory, the products through the tensor
+// cores.
+//
+// Work split: an item is (sequence, K/V head, block of MT rows), a unit one
+// 64-row tile of an item's cache.  All units of a call form one line that is
+// cut evenly over the CTAs (one per SM), whatever the sequences' lengths, by
+// arithmetic that every CTA repeats from the device's own lengths.  A CTA's
+// first and last item may be shared with its neighbours: it leaves their
+// (max, sum, weighted sum) in its two slots of a workspace and
+// tree_combine_kernel adds the slots of an item in CTA order, so results do
+// not depend on timing.
 #include "vb_common.cuh"
 #include "vb_kernels.cuh"
 #include "vb_tc.cuh"
 
+#include <algorithm>
+
 namespace vb {
 
-constexpr int TR_WARPS = 8;
+constexpr int TR_KT = 64;            // cache rows per tile
+constexpr int TR_MAX_STAGES = 8;
+constexpr int TR_THREADS = 384;      // warps 0..7 compute, warp 8 loads
+// Registers: the launch gives 168 a thread; the loading warpgroup goes down
+// to 56 and the two computing ones up to 224 (2 * 224 + 56 = 3 * 168), which
+// their sums need.
+constexpr int TR_SMEM = 226 * 1024;  // dynamic shared memory
+
+enum { TR_F32 = 0, TR_BF16 = 1, TR_F16 = 2 };
 
 struct TreeArgs {
     vb_tree_args a;
     vb_pages p;
-    float scale;
+    float scale_log2;                // scale * log2(e): the softmax runs in powers of two
+    int group;                       // query heads per K/V head
+    int mt;                          // rows per block
+    int max_blocks;                  // blocks of the longest draft
+    int stages;
+    int vec;                         // 4-value accesses of q, 2-value ones of out
     int *err;
+    float *part;                     // [2 * CTAs][mt][head_dim + 2]
+    int2 *desc;                      // [n][n_kv][max_blocks] CTAs of an item
 };
 
-template <typename T>
-__device__ __forceinline__ float to_f(T v) { return (float)v; }
+// Sequence i of the call.  T = 0: no rows of q (or none that can be named);
+// bad: its tokens get zeros.
+struct TreeSeq {
+    int t0, T, s, len, base, bad;
+};
 
-template <typename Q, typename C>
-__global__ void __launch_bounds__(TR_WARPS * 32) tree_attention_kernel(const __grid_constant__ TreeArgs g) {
-    pdl_trigger();
-    pdl_wait();
-    constexpr int U = 8;
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &g, int i) {
+    TreeSeq q;
     const vb_tree_args &a = g.a;
-    const vb_pages &p = g.p;
-    const int lane = threadIdx.x & 31;
-    const int64_t item = (int64_t)blockIdx.x * TR_WARPS + (threadIdx.x >> 5);
-    if (item >= (int64_t)a.n * a.max_tokens * a.n_heads) return;
-    const int h = (int)(item % a.n_heads), j = (int)(item / a.n_heads % a.max_tokens);
-    const int i = (int)(item / a.n_heads / a.max_tokens);
-    const int t0 = a.start[i], T = a.start[i + 1] - t0, s = a.seqs[i];
-    const int hd = p.head_dim;
-    if (t0 < 0 || T < 0 || T > a.max_tokens || t0 > a.n_tokens - T) {
-        if (lane == 0) atomicCAS(g.err, 0, VB_DEV_TREE_SEQ);
-        return;
+    q.t0 = a.start[i];
+    const int t1 = a.start[i + 1];
+    q.s = a.seqs[i];
+    q.T = t1 - q.t0;
+    q.bad = 0;
+    if (q.t0 < 0 || t1 < q.t0 || t1 > a.n_tokens || q.T > a.max_tokens) {
+        q.T = 0;
+        q.bad = 1;
+        q.len = q.base = 0;
+        return q;
     }
-    if (j >= T) return;
-    const int len = s >= 0 && s < p.n_seqs ? p.length[s] : -1;
-    Q *out = static_cast<Q *>(const_cast<void *>(a.out)) + (int64_t)(t0 + j) * a.ldo + (int64_t)h * hd;
-    const int base = len - T;
-    if (base < 0 || (int64_t)len > (int64_t)p.max_pages * p.page_rows || (a.mask && T > 32 * a.mask_words)) {
-        if (lane == 0) atomicCAS(g.err, 0, VB_DEV_TREE_SEQ);
-        for (int d = lane; d < hd; d += 32) out[d] = Q(0.0f);
-        return;
+    q.len = q.s >= 0 && q.s < g.p.n_seqs ? g.p.length[q.s] : -1;
+    q.base = q.len - q.T;
+    if (q.base < 0 || (int64_t)q.len > (int64_t)g.p.max_pages * g.p.page_rows ||
+        (a.mask && q.T > 32 * (int64_t)a.mask_words)) {
+        q.bad = 1;
+        q.len = q.base = 0;
     }
-    const Q *q = static_cast<const Q *>(a.q) + (int64_t)(t0 + j) * a.ldq + (int64_t)h * hd;
-    const uint32_t *mask = a.mask ? a.mask + (int64_t)(t0 + j) * a.mask_words : nullptr;
-    float qv[U], o[U], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        qv[u] = lane + 32 * u < hd ? to_f(q[lane + 32 * u]) : 0.0f;
-        o[u] = 0.0f;
-    }
-    const int kvh = h / (a.n_heads / p.n_kv_heads);
-    const int last = mask ? len : base + j + 1;
-    for (int r = 0; r < last; r++) {
-        if (mask && r >= base && !(mask[(r - base) >> 5] >> ((r - base) & 31) & 1u)) continue;
-        const int page = p.table[(int64_t)s * p.max_pages + r / p.page_rows];
-        if (page < 0 || page >= p.n_pages) {
-            if (lane == 0) atomicCAS(g.err, 0, VB_DEV_TREE_PAGE);
-            continue;
-        }
-        const int64_t at = ((((int64_t)a.layer * p.n_pages + page) * p.n_kv_heads + kvh) * p.page_rows +
-                            r % p.page_rows) * hd;
-        const C *k = static_cast<const C *>(p.k) + at, *v = static_cast<const C *>(p.v) + at;
-        float sc = 0.0f;
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (lane + 32 * u < hd) sc = fmaf(qv[u], to_f(k[lane + 32 * u]), sc);
-        sc = warp_sum(sc) * g.scale;
-        const float mn = fmaxf(m, sc), ms = mn == -INFINITY ? 0.0f : mn;
-        const float al = expf(m - ms), e = expf(sc - ms);
-        m = mn;
-        l = fmaf(l, al, e);
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (lane + 32 * u < hd) o[u] = fmaf(o[u], al, e * to_f(v[lane + 32 * u]));
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++)
-        if (lane + 32 * u < hd) out[lane + 32 * u] = Q(l > 0.0f || l != l ? o[u] / l : 0.0f);
+    return q;
 }
 
+__device__ __forceinline__ int tree_blocks(const TreeArgs &g, const TreeSeq &q) {
+    return (int)(((int64_t)q.T * g.group + g.mt - 1) / g.mt);
+}
+
+// Rows of the cache that block b of a sequence reads, and its units (at
+// least one, so that every output row is written).
+__device__ __forceinline__ int tree_visible(const TreeArgs &g, const TreeSeq &q, int b) {
+    if (q.bad) return 0;
+    if (g.a.mask) return q.len;
+    return q.base + (int)min((int64_t)q.T, (((int64_t)b + 1) * g.mt + g.group - 1) / g.group);
+}
+
+__device__ __forceinline__ int tree_units(int visible) { return max(1, (visible + TR_KT - 1) / TR_KT); }
+
+__device__ int64_t tree_seq_units(const TreeArgs &g, const TreeSeq &q) {
+    const int nb = tree_blocks(g, q);
+    if (g.a.mask || q.bad) return (int64_t)nb * tree_units(tree_visible(g, q, 0)) * g.p.n_kv_heads;
+    int64_t u = 0;
+    for (int b = 0; b < nb; b++) u += tree_units(tree_visible(g, q, b));
+    return u * g.p.n_kv_heads;
+}
+
+// A place in the line of units: the item (i, kv head, block) and the tile.
+struct TreeWalk {
+    TreeSeq q;
+    int i, g, b, nb, visible, units, tile;
+    int64_t left;                    // units of this CTA from here on
+};
+
+__device__ __forceinline__ void tree_item(const TreeArgs &g, TreeWalk &w) {
+    w.visible = tree_visible(g, w.q, w.b);
+    w.units = tree_units(w.visible);
+}
+
+__device__ __forceinline__ void tree_next(const TreeArgs &g, TreeWalk &w) {
+    w.tile = 0;
+    if (++w.b == w.nb) {
+        w.b = 0;
+        if (++w.g == g.p.n_kv_heads) {
+            w.g = 0;
+            do w.q = tree_seq(g, ++w.i);
+            while (w.q.T == 0);
+            w.nb = tree_blocks(g, w.q);
+        }
+    }
+    tree_item(g, w);
+}
+
+// ------------------------------------------------------------ mma helpers
+template <int TYPE>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (TYPE == TR_F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (TYPE == TR_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <int TYPE>
+__device__ __forceinline__ float unpack(uint16_t h) {
+    if constexpr (TYPE == TR_F16) return h2f(h);
+    else return bf16_to_f(h);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Byte offset of 16-byte chunk c of row r in a [rows][128 B] tile with the
+// 128-byte swizzle that TMA writes.
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// A bounded barrier wait; the first that runs out records the error and
+// lets every later wait of the CTA return at once.
+__device__ __forceinline__ void tree_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *err) {
+    if (mbar_try_wait(bar, parity)) return;
+    if (*abort) return;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort) return;
+        if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
+            *abort = 1;
+            atomicCAS(err, 0, VB_DEV_TREE_WAIT);
+            return;
+        }
+    }
+}
+
+// TYPE: the types; HDP: head_dim rounded up to 64, 128 or 256; R: 16-row
+// pieces per warp; WM: row groups of warps.  8 / WM warps share a row group
+// and split a tile's rows 16 each (with WM = 1 two sets of four take tiles
+// in turn) and merge at the item's end.
+template <int TYPE, int HDP, int R, int WM>
+__global__ void __launch_bounds__(TR_THREADS, 1)
+    tree_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                          const __grid_constant__ TreeArgs g) {
+    constexpr int MT = 16 * R * WM;
+    constexpr int KW = 8 / WM;                       // warps of a row group
+    constexpr int SETS = WM == 1 ? 2 : 1;
+    constexpr int QT = TYPE == TR_F32 ? 3 : 1;       // 16-bit terms of a query value: 3 bf16 hold an fp32 exactly
+    constexpr int CB = HDP / 64;                     // 128-byte column blocks
+    constexpr int NT = HDP / 8;                      // output tiles of 8 columns
+    constexpr uint32_t TILE = TR_KT * 128;           // bytes of a column block
+    constexpr uint32_t STAGE = 2 * CB * TILE;
+    constexpr int QPITCH = HDP * 2 + 16;             // bytes; rows 16 bytes apart modulo 128: no bank conflicts
+    constexpr int MPITCH = HDP + 4;                  // floats
+
+    extern __shared__ uint8_t raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    float *merge = reinterpret_cast<float *>(ring + (size_t)g.stages * STAGE);      // [4][16][MPITCH]
+    uint8_t *qs = reinterpret_cast<uint8_t *>(merge + 4 * 16 * MPITCH);             // [QT][MT][QPITCH]
+    float2 *ml = reinterpret_cast<float2 *>(qs + QT * MT * QPITCH);                 // [8][16 * R]
+    __shared__ uint64_t full[TR_MAX_STAGES], empty[TR_MAX_STAGES];
+    __shared__ int64_t scan[TR_THREADS / 32];
+    __shared__ int abort_flag, s_seq;
+    __shared__ int64_t s_off;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < TR_MAX_STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], WM == 1 ? 4 : 8);
+        }
+        mbar_fence_init();
+        abort_flag = 0;
+        s_seq = -1;
+    }
+    pdl_trigger();
+    pdl_wait();
+
+    // ---- this CTA's part of the line of units
+    const int n = g.a.n;
+    const int per = (n + TR_THREADS - 1) / TR_THREADS;
+    const int i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
+    int64_t mine = 0;
+    for (int i = i0; i < i1; i++) {
+        const TreeSeq q = tree_seq(g, i);
+        if (q.bad && blockIdx.x == 0) atomicCAS(g.err, 0, VB_DEV_TREE_SEQ);
+        mine += tree_seq_units(g, q);
+    }
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+    }
+    if (lane == 31) scan[warp] = before;
+    before -= mine;
+    __syncthreads();
+    int64_t total = 0;
+    for (int w = 0; w < TR_THREADS / 32; w++) {
+        if (w < warp) before += scan[w];
+        total += scan[w];
+    }
+    const int64_t ctas = min((int64_t)gridDim.x, total);          // that get a unit
+    const int64_t u0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : total;
+    const int64_t u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : total;
+    if (u0 >= before && u0 < before + mine) {
+        int64_t at = before;
+        for (int i = i0; i < i1; i++) {
+            const int64_t u = tree_seq_units(g, tree_seq(g, i));
+            if (u0 < at + u) {
+                s_seq = i;
+                s_off = u0 - at;
+                break;
+            }
+            at += u;
+        }
+    }
+    __syncthreads();
+    if (u0 >= u1) return;
+
+    TreeWalk w;
+    w.i = s_seq;
+    w.q = tree_seq(g, w.i);
+    w.nb = tree_blocks(g, w.q);
+    w.left = u1 - u0;
+    {
+        const int64_t head_units = tree_seq_units(g, w.q) / g.p.n_kv_heads;
+        w.g = (int)(s_off / head_units);
+        int64_t off = s_off % head_units;
+        w.b = 0;
+        tree_item(g, w);
+        while (off >= w.units) {
+            off -= w.units;
+            w.b++;
+            tree_item(g, w);
+        }
+        w.tile = (int)off;
+    }
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp > 8) return;
+        // ------------------------------------------------------------ loads
+        const int P = g.p.page_rows, box = min(P, TR_KT), boxes = TR_KT / box;
+        int it = 0;
+        while (w.left > 0) {
+            const int n_tiles = (int)min((int64_t)(w.units - w.tile), w.left);
+            const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
+            int pages = 0;                              // lane's page of the current 32 boxes
+            for (int x = 0; x < n_tiles; x++, it++) {
+                const int r0 = (w.tile + x) * TR_KT;
+                const int have = min(TR_KT, w.visible - r0);              // rows of the tile that count
+                const int nbox = have <= 0 ? 0 : (have + box - 1) / box;
+                const int k0 = x * boxes % 32;                            // first lane of this tile's boxes
+                if (k0 == 0) {
+                    const int r = r0 + lane * box;
+                    pages = 0;
+                    if (r < w.visible) {
+                        pages = row[r / P];
+                        if (pages < 0 || pages >= g.p.n_pages) {
+                            atomicCAS(g.err, 0, VB_DEV_TREE_PAGE);
+                            pages = 0;
+                        }
+                    }
+                }
+                const int s = it % g.stages;
+                tree_wait(&empty[s], ((uint32_t)(it / g.stages) & 1u) ^ 1u, &abort_flag, g.err);
+                const int nload = abort_flag ? 0 : nbox;
+                uint8_t *st = ring + (size_t)s * STAGE;
+                if (lane == 0) {
+                    if (nload) mbar_arrive_expect_tx(&full[s], (uint32_t)nload * box * 128 * 2 * CB);
+                    else mbar_arrive(&full[s]);
+                }
+                __syncwarp();
+                const int k = lane - k0;
+                if (k >= 0 && k < nload) {
+                    const int y = (pages * g.p.n_kv_heads + w.g) * P + (r0 + k * box) % P;
+#pragma unroll
+                    for (int c = 0; c < CB; c++) {
+                        tma_load_2d(st + c * TILE + k * box * 128, &tk, 64 * c, y, &full[s]);
+                        tma_load_2d(st + (CB + c) * TILE + k * box * 128, &tv, 64 * c, y, &full[s]);
+                    }
+                }
+            }
+            w.left -= n_tiles;
+            if (w.left > 0) tree_next(g, w);
+        }
+        // every copy has landed before the CTA can end
+        for (int s = 0; s < g.stages; s++) {
+            const int fills = it / g.stages + (it % g.stages > s ? 1 : 0);
+            if (fills) gm_wait(&full[s], (uint32_t)(fills - 1) & 1u);
+        }
+        return;
+    }
+
+    // ---------------------------------------------------------------- compute
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int wm = WM == 1 ? 0 : warp / KW, kw = warp % KW, set = SETS == 2 ? warp >> 2 : 0;
+    const int slice = (warp & 3) * 16;                 // this warp's 16 rows of a tile
+    const int hd = g.p.head_dim;
+    const int quad = lane >> 2, ql = lane & 3;
+    int it = 0;
+    bool first_item = true;
+    while (w.left > 0) {
+        const int n_tiles = (int)min((int64_t)(w.units - w.tile), w.left);
+        const bool whole = w.tile == 0 && n_tiles == w.units;
+        const int rows = min(MT, w.q.T * g.group - w.b * MT);           // rows of the block that exist
+        // queries of the block, in 16-bit terms
+        for (int e = threadIdx.x; e < MT * (HDP / 4); e += 256) {
+            const int m = e / (HDP / 4), d = e % (HDP / 4) * 4;
+            float x[4] = {};
+            if (m < rows && d < hd) {
+                const int row = w.b * MT + m, j = row / g.group;
+                const int64_t at = (int64_t)(w.q.t0 + j) * g.a.ldq + (int64_t)(w.g * g.group + row % g.group) * hd + d;
+                if constexpr (TYPE == TR_F32) {
+                    const float *src = static_cast<const float *>(g.a.q) + at;
+                    if (g.vec) *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(src);
+                    else
+                        for (int c = 0; c < 4; c++) x[c] = src[c];
+                } else {
+                    const uint16_t *src = static_cast<const uint16_t *>(g.a.q) + at;
+                    uint16_t h[4];
+                    if (g.vec) *reinterpret_cast<uint2 *>(h) = *reinterpret_cast<const uint2 *>(src);
+                    else
+                        for (int c = 0; c < 4; c++) h[c] = src[c];
+                    *reinterpret_cast<uint2 *>(qs + m * QPITCH + d * 2) = *reinterpret_cast<uint2 *>(h);
+                }
+            } else if constexpr (TYPE != TR_F32) {
+                *reinterpret_cast<uint2 *>(qs + m * QPITCH + d * 2) = make_uint2(0, 0);
+            }
+            if constexpr (TYPE == TR_F32) {
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    uint32_t h[2] = {pack2<TYPE>(x[0], x[1]), pack2<TYPE>(x[2], x[3])};
+                    *reinterpret_cast<uint2 *>(qs + (t * MT + m) * QPITCH + d * 2) = make_uint2(h[0], h[1]);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[c] -= bf16_to_f((uint16_t)(h[c >> 1] >> (16 * (c & 1))));
+                }
+            }
+        }
+        consumer_sync(256);
+
+        float o[R][NT][4], m[R][2], l[R][2];
+        int tok[R][2];                                  // token of the thread's rows, -1: no such row
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                m[r][h] = -INFINITY;
+                l[r][h] = 0.0f;
+                const int mr = wm * 16 * R + 16 * r + quad + 8 * h;
+                tok[r][h] = mr < rows ? (w.b * MT + mr) / g.group : -1;
+#pragma unroll
+                for (int t = 0; t < NT; t++) o[r][t][2 * h] = o[r][t][2 * h + 1] = 0.0f;
+            }
+        const uint32_t q_at = smem_u32(qs) +
+                              (uint32_t)((wm * 16 * R + (lane & 7) + ((lane >> 3) & 1) * 8) * QPITCH + (lane >> 4) * 16);
+        for (int x = 0; x < n_tiles; x++, it++) {
+            if (SETS == 2 && (it & 1) != set) continue;
+            const int s = it % g.stages;
+            tree_wait(&full[s], (uint32_t)(it / g.stages) & 1u, &abort_flag, g.err);
+            const uint32_t kt = smem_u32(ring + (size_t)s * STAGE), vt = kt + CB * TILE;
+            // scores: 16 rows x 16 cache rows
+            float c[R][2][4];
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) c[r][t][0] = c[r][t][1] = c[r][t][2] = c[r][t][3] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < HDP / 16; ks++) {
+                uint32_t kb[4];
+                ldsm4(kb, kt + (ks / 4) * TILE +
+                              sw128(slice + (lane & 7) + (lane >> 4) * 8, (ks % 4) * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int t = QT - 1; t >= 0; t--) {
+                        uint32_t qa[4];
+                        ldsm4(qa, q_at + (uint32_t)((t * MT + 16 * r) * QPITCH + ks * 32));
+                        mma16816<TYPE>(c[r][0], qa, kb[0], kb[1]);
+                        mma16816<TYPE>(c[r][1], qa, kb[2], kb[3]);
+                    }
+            }
+            const int r0 = (w.tile + x) * TR_KT + slice;       // cache row of the warp's first column
+            const bool edge = r0 + 16 > w.q.base;              // not every row is seen by every token
+            bool careful = false;
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) c[r][t][e] *= g.scale_log2;
+            uint32_t seen[R] = {};                             // bit t*4+e
+            if (edge) {
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int j = tok[r][e >> 1], d = r0 + 8 * t + 2 * ql + (e & 1) - w.q.base;
+                            bool see = j >= 0 && d + w.q.base < w.visible;
+                            if (see && d >= 0)
+                                see = g.a.mask ? g.a.mask[(int64_t)(w.q.t0 + j) * g.a.mask_words + (d >> 5)] >> (d & 31) & 1u
+                                               : d <= j;
+                            if (!see) c[r][t][e] = -INFINITY;
+                            else seen[r] |= 1u << (t * 4 + e);
+                        }
+                // rows past the end may hold anything: they become zeros.
+                // A draft row that is not finite must not meet the zero
+                // weights of the tokens that do not see it: those tiles take
+                // the products one by one below.
+                uint8_t *vg = ring + (size_t)s * STAGE + CB * TILE;
+                for (int e = lane; e < 16 * CB * 8; e += 32) {
+                    const int rr = e / (CB * 8), cc = e % (CB * 8);
+                    uint4 *p = reinterpret_cast<uint4 *>(vg + (cc >> 3) * TILE + sw128(slice + rr, cc & 7));
+                    if (r0 + rr >= w.visible) *p = make_uint4(0, 0, 0, 0);
+                    else if (r0 + rr >= w.q.base) {
+                        const uint4 v = *p;
+                        const uint32_t inf = TYPE == TR_F16 ? 0x7c007c00u : 0x7f807f80u;
+                        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t z = vv[k] & inf;
+                            careful |= (z & 0xffffu) == (inf & 0xffffu) || (z >> 16) == (inf >> 16);
+                        }
+                    }
+                }
+                careful = __any_sync(0xffffffffu, careful);
+                __syncwarp();
+            }
+            // running maximum and sum
+            float al[R][2];
+            bool moved = false;
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float v = fmaxf(fmaxf(c[r][0][2 * h], c[r][0][2 * h + 1]), fmaxf(c[r][1][2 * h], c[r][1][2 * h + 1]));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+                    const float mn = fmaxf(m[r][h], v), ms = mn == -INFINITY ? 0.0f : mn;
+                    al[r][h] = ex2(m[r][h] - ms);
+                    moved |= mn != m[r][h];
+                    m[r][h] = mn;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float &p = c[r][t][2 * h + e];
+                            p = ex2(p - ms);
+                            sum += p;
+                        }
+                    l[r][h] = fmaf(l[r][h], al[r][h], sum);
+                }
+            moved = __any_sync(0xffffffffu, moved);
+            if (TYPE != TR_F32 || careful) {
+                if (moved) {
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[r][t][e] *= al[r][e >> 1];
+                }
+            }
+            if (careful) {
+                const uint8_t *vg = ring + (size_t)s * STAGE + CB * TILE;
+                for (int kr = 0; kr < 16; kr++) {
+                    // the weights of cache row kr sit in lane kr/2 % 4 of each quad
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        const int from = (lane & ~3) | (kr >> 1 & 3);
+                        float p[2];
+                        bool see[2];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float x0 = kr & 1 ? c[r][0][2 * h + 1] : c[r][0][2 * h];
+                            const float x1 = kr & 1 ? c[r][1][2 * h + 1] : c[r][1][2 * h];
+                            p[h] = __shfl_sync(0xffffffffu, kr < 8 ? x0 : x1, from);
+                            const uint32_t sb = __shfl_sync(0xffffffffu, seen[r], from);
+                            see[h] = sb >> ((kr >> 3) * 4 + 2 * h + (kr & 1)) & 1u;
+                        }
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            const uint32_t v2 = *reinterpret_cast<const uint32_t *>(
+                                vg + (t >> 3) * TILE + sw128(slice + kr, t & 7) + 4 * ql);
+                            const float v0 = unpack<TYPE>((uint16_t)v2), v1 = unpack<TYPE>((uint16_t)(v2 >> 16));
+#pragma unroll
+                            for (int h = 0; h < 2; h++)
+                                if (see[h]) {
+                                    o[r][t][2 * h] = fmaf(p[h], v0, o[r][t][2 * h]);
+                                    o[r][t][2 * h + 1] = fmaf(p[h], v1, o[r][t][2 * h + 1]);
+                                }
+                        }
+                    }
+                }
+            } else {
+                uint32_t pa[R][4], pb[R][4];
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float x0 = c[r][k >> 1][2 * (k & 1)], x1 = c[r][k >> 1][2 * (k & 1) + 1];
+                        pa[r][k] = pack2<TYPE>(x0, x1);
+                        if constexpr (TYPE == TR_F32)
+                            pb[r][k] = pack2<TYPE>(x0 - bf16_to_f((uint16_t)pa[r][k]), x1 - bf16_to_f((uint16_t)(pa[r][k] >> 16)));
+                    }
+#pragma unroll
+                for (int t = 0; t < NT; t += 2) {
+                    uint32_t vb[4];
+                    ldsm4_t(vb, vt + (t >> 3) * TILE +
+                                    sw128(slice + (lane & 7) + ((lane >> 3) & 1) * 8, (t & 7) + (lane >> 4)));
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        if constexpr (TYPE == TR_F32) {
+                            // a tile's products start from zero and join the sum in
+                            // one rounded fp32 step: the tensor cores' own long sums
+                            // lose more
+                            float d0[4] = {}, d1[4] = {};
+                            mma16816<TYPE>(d0, pb[r], vb[0], vb[1]);
+                            mma16816<TYPE>(d1, pb[r], vb[2], vb[3]);
+                            mma16816<TYPE>(d0, pa[r], vb[0], vb[1]);
+                            mma16816<TYPE>(d1, pa[r], vb[2], vb[3]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                o[r][t][e] = fmaf(o[r][t][e], al[r][e >> 1], d0[e]);
+                                o[r][t + 1][e] = fmaf(o[r][t + 1][e], al[r][e >> 1], d1[e]);
+                            }
+                        } else {
+                            mma16816<TYPE>(o[r][t], pa[r], vb[0], vb[1]);
+                            mma16816<TYPE>(o[r][t + 1], pa[r], vb[2], vb[3]);
+                        }
+                    }
+                }
+            }
+            if (edge) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // zeros written before the next copy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+
+        // ---- merge the row group's warps
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float &x = l[r][h];
+                x += __shfl_xor_sync(0xffffffffu, x, 1);
+                x += __shfl_xor_sync(0xffffffffu, x, 2);
+                if (ql == 0) ml[warp * 16 * R + 16 * r + quad + 8 * h] = make_float2(m[r][h], x);
+            }
+        consumer_sync(256);
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float2 other[KW];
+                float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KW; k++) {
+                    other[k] = ml[(wm * KW + k) * 16 * R + 16 * r + quad + 8 * h];
+                    top = fmaxf(top, other[k].x);
+                }
+                const float ms = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int k = 0; k < KW; k++) sum = fmaf(other[k].y, ex2(other[k].x - ms), sum);
+                const float f = ex2(m[r][h] - ms);
+                m[r][h] = top;
+                l[r][h] = sum;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    o[r][t][2 * h] *= f;
+                    o[r][t][2 * h + 1] *= f;
+                }
+            }
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int half = KW / 2; half >= 1; half >>= 1) {
+                float *slot = merge + (size_t)((wm * (KW / 2) + kw % half) * 16) * MPITCH;
+                if (kw >= half && kw < 2 * half) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            *reinterpret_cast<float2 *>(slot + (quad + 8 * h) * MPITCH + 8 * t + 2 * ql) =
+                                make_float2(o[r][t][2 * h], o[r][t][2 * h + 1]);
+                }
+                consumer_sync(256);
+                if (kw < half) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float2 v = *reinterpret_cast<const float2 *>(slot + (quad + 8 * h) * MPITCH + 8 * t + 2 * ql);
+                            o[r][t][2 * h] += v.x;
+                            o[r][t][2 * h + 1] += v.y;
+                        }
+                }
+                consumer_sync(256);
+            }
+        if (kw == 0) {
+            float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * MT * (hd + 2);
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int mr = wm * 16 * R + 16 * r + quad + 8 * h;
+                    if (mr >= rows) continue;
+                    if (whole) {
+                        const int row = w.b * MT + mr;
+                        const int64_t at = (int64_t)(w.q.t0 + row / g.group) * g.a.ldo +
+                                           (int64_t)(w.g * g.group + row % g.group) * hd;
+                        const float inv = l[r][h] > 0.0f || l[r][h] != l[r][h] ? 1.0f / l[r][h] : 0.0f;
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            if (8 * t >= hd) break;
+                            const float y0 = o[r][t][2 * h] * inv, y1 = o[r][t][2 * h + 1] * inv;
+                            const int64_t e = at + 8 * t + 2 * ql;
+                            if constexpr (TYPE == TR_F32) {
+                                float *dst = static_cast<float *>(g.a.out) + e;
+                                if (g.vec) *reinterpret_cast<float2 *>(dst) = make_float2(y0, y1);
+                                else dst[0] = y0, dst[1] = y1;
+                            } else {
+                                uint16_t *dst = static_cast<uint16_t *>(g.a.out) + e;
+                                const uint32_t y = pack2<TYPE>(y0, y1);
+                                if (g.vec) *reinterpret_cast<uint32_t *>(dst) = y;
+                                else dst[0] = (uint16_t)y, dst[1] = (uint16_t)(y >> 16);
+                            }
+                        }
+                    } else {
+                        float *dst = part + (size_t)mr * (hd + 2);
+                        if (ql == 0) *reinterpret_cast<float2 *>(dst) = make_float2(m[r][h], l[r][h]);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            if (8 * t >= hd) break;
+                            *reinterpret_cast<float2 *>(dst + 2 + 8 * t + 2 * ql) =
+                                make_float2(o[r][t][2 * h], o[r][t][2 * h + 1]);
+                        }
+                    }
+                }
+        }
+        // the CTA that holds an item's first unit says which CTAs hold the rest
+        if (threadIdx.x == 0 && w.tile == 0) {
+            const int64_t at = u1 - w.left;                        // the item's first unit
+            const int64_t end = at + w.units - 1;
+            const int last = (int)(((end + 1) * ctas - 1) / total);
+            g.desc[((int64_t)w.i * g.p.n_kv_heads + w.g) * g.max_blocks + w.b] =
+                make_int2((int)blockIdx.x * 2 + (first_item ? 0 : 1), last);
+        }
+        first_item = false;
+        w.left -= n_tiles;
+        if (w.left > 0) tree_next(g, w);
+    }
+}
+
+// Joins the parts of items that several CTAs shared: one CTA per (item, row),
+// its warps taking the parts in turn.
+constexpr int TC_WARPS = 4;
+template <int TYPE>
+__global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeArgs g) {
+    __shared__ float so[TC_WARPS][256], sm[TC_WARPS], sl[TC_WARPS];
+    pdl_trigger();
+    pdl_wait();
+    const int64_t item = blockIdx.x;
+    const int mr = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = g.p.head_dim;
+    const int b = (int)(item % g.max_blocks), kv = (int)(item / g.max_blocks % g.p.n_kv_heads);
+    const TreeSeq q = tree_seq(g, (int)(item / g.max_blocks / g.p.n_kv_heads));
+    if ((int64_t)b * g.mt + mr >= (int64_t)q.T * g.group) return;
+    const int2 d = g.desc[item];
+    const int c0 = d.x >> 1, c1 = d.y;
+    if (c0 == c1) return;
+    float m = -INFINITY, l = 0.0f, o[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) o[u] = 0.0f;
+    for (int c = c0 + warp; c <= c1; c += TC_WARPS) {
+        const int slot = c == c0 ? d.x : 2 * c;
+        const float *part = g.part + ((size_t)slot * g.mt + mr) * (hd + 2);
+        const float2 x = *reinterpret_cast<const float2 *>(part);
+        const float mn = fmaxf(m, x.x), ms = mn == -INFINITY ? 0.0f : mn;
+        const float f = ex2(m - ms), e = ex2(x.x - ms);
+        m = mn;
+        l = l * f + x.y * e;
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (lane + 32 * u < hd) o[u] = o[u] * f + part[2 + lane + 32 * u] * e;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++) so[warp][lane + 32 * u] = o[u];
+    if (lane == 0) {
+        sm[warp] = m;
+        sl[warp] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY, sum = 0.0f, f[TC_WARPS];
+#pragma unroll
+    for (int k = 0; k < TC_WARPS; k++) top = fmaxf(top, sm[k]);
+    const float ms = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < TC_WARPS; k++) {
+        f[k] = ex2(sm[k] - ms);
+        sum = fmaf(sl[k], f[k], sum);
+    }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const int row = b * g.mt + mr;
+    const int64_t at = (int64_t)(q.t0 + row / g.group) * g.a.ldo + (int64_t)(kv * g.group + row % g.group) * hd;
+    for (int c = threadIdx.x; c < hd; c += TC_WARPS * 32) {
+        float y = 0.0f;
+#pragma unroll
+        for (int k = 0; k < TC_WARPS; k++) y = fmaf(so[k][c], f[k], y);
+        y *= inv;
+        if constexpr (TYPE == TR_F32) static_cast<float *>(g.a.out)[at + c] = y;
+        else if constexpr (TYPE == TR_F16) static_cast<__half *>(g.a.out)[at + c] = __float2half_rn(y);
+        else static_cast<__nv_bfloat16 *>(g.a.out)[at + c] = __float2bfloat16_rn(y);
+    }
+}
+
+// -------------------------------------------------------------------- host
 int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who);
+
+typedef void (*TreeKernel)(CUtensorMap, CUtensorMap, TreeArgs);
+
+template <int TYPE, int HDP, int R, int WM>
+static int tree_fit(TreeArgs &g, size_t &smem) {
+    constexpr int MT = 16 * R * WM, QT = TYPE == TR_F32 ? 3 : 1;
+    constexpr size_t stage = (size_t)2 * TR_KT * HDP * 2;
+    constexpr size_t rest = (size_t)4 * 16 * (HDP + 4) * 4 + (size_t)QT * MT * (HDP * 2 + 16) + (size_t)8 * 16 * R * 8 + 1024;
+    static_assert(rest + 2 * stage <= TR_SMEM, "two stages must fit");
+    g.mt = MT;
+    g.stages = (int)std::min<size_t>(TR_MAX_STAGES, (TR_SMEM - rest) / stage);
+    smem = g.stages * stage + rest;
+    return MT;
+}
+
+template <int TYPE, int HDP, int R, int WM>
+static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
+    size_t smem;
+    tree_fit<TYPE, HDP, R, WM>(g, smem);
+    const vb_pages &p = g.p;
+    const int grid = ctx->sm_count;
+    g.max_blocks = (int)(((int64_t)g.a.max_tokens * g.group + g.mt - 1) / g.mt);
+    const int64_t items = (int64_t)g.a.n * p.n_kv_heads * g.max_blocks;
+    if (items > INT32_MAX) return set_error(ctx, VB_ERR_INVALID_ARG, "vb_tree_attention: too many rows");
+    const size_t parts = (size_t)2 * grid * g.mt * (p.head_dim + 2) * sizeof(float);
+    int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)items * sizeof(int2));
+    if (rc) return rc;
+    g.part = static_cast<float *>(ctx->tree_ws.ptr);
+    g.desc = reinterpret_cast<int2 *>(static_cast<char *>(ctx->tree_ws.ptr) + parts);
+    CUtensorMap tk, tv;
+    const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;
+    const CUtensorMapDataType dt = p.type == VB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int box = std::min(p.page_rows, TR_KT);
+    if (!make_map(&tk, static_cast<char *>(p.k) + layer, dt, 2, p.head_dim, rows, 64, box, true) ||
+        !make_map(&tv, static_cast<char *>(p.v) + layer, dt, 2, p.head_dim, rows, 64, box, true))
+        return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the cache refused");
+    VB_CHECK(ctx, pdl_launch(ctx, tree_attention_kernel<TYPE, HDP, R, WM>, dim3(grid), dim3(TR_THREADS), smem, tk, tv, g));
+    VB_LAUNCH_CHECK(ctx, "tree_attention");
+    VB_CHECK(ctx, pdl_launch(ctx, tree_combine_kernel<TYPE>, dim3((unsigned)items, g.mt), dim3(TC_WARPS * 32), 0, g));
+    VB_LAUNCH_CHECK(ctx, "tree_combine");
+    return VB_OK;
+}
+
+// Rows per block: the fewest of 16, 32 and 64 that hold a sequence's rows
+// (heads above 128: 32 at most, as their sums fill the registers, and 16 for
+// fp32 queries, whose terms would leave no room for two stages).
+template <int TYPE, int HDP>
+static int launch_rows(vb_ctx *ctx, TreeArgs &g) {
+    const int64_t rows = (int64_t)g.a.max_tokens * g.group;
+    if (rows <= 16) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);
+    if constexpr (HDP == 256 && TYPE == TR_F32) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);
+    else if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 1, 2>(ctx, g);
+    else {
+        if (rows <= 32) return launch_tree<TYPE, HDP, 2, 1>(ctx, g);
+        return launch_tree<TYPE, HDP, 2, 2>(ctx, g);
+    }
+}
+
+template <int TYPE>
+static int launch_heads(vb_ctx *ctx, TreeArgs &g) {
+    const int hd = g.p.head_dim;
+    return hd <= 64 ? launch_rows<TYPE, 64>(ctx, g) : hd <= 128 ? launch_rows<TYPE, 128>(ctx, g) : launch_rows<TYPE, 256>(ctx, g);
+}
+
+template <int TYPE, int HDP, int R, int WM>
+static cudaError_t allow_smem() {
+    return cudaFuncSetAttribute(tree_attention_kernel<TYPE, HDP, R, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
+}
+
+template <int TYPE>
+static cudaError_t allow_smem_type() {
+    cudaError_t e = cudaSuccess;
+    auto keep = [&](cudaError_t x) { e = e == cudaSuccess ? x : e; };
+    keep(allow_smem<TYPE, 64, 1, 1>());
+    keep(allow_smem<TYPE, 64, 2, 1>());
+    keep(allow_smem<TYPE, 64, 2, 2>());
+    keep(allow_smem<TYPE, 128, 1, 1>());
+    keep(allow_smem<TYPE, 128, 2, 1>());
+    keep(allow_smem<TYPE, 128, 2, 2>());
+    keep(allow_smem<TYPE, 256, 1, 1>());
+    if constexpr (TYPE != TR_F32) keep(allow_smem<TYPE, 256, 1, 2>());
+    return e;
+}
+
+int init_tree(vb_ctx *ctx) {
+    VB_CHECK(ctx, allow_smem_type<TR_F32>());
+    VB_CHECK(ctx, allow_smem_type<TR_BF16>());
+    VB_CHECK(ctx, allow_smem_type<TR_F16>());
+    return VB_OK;
+}
 
 }  // namespace vb
 
@@ -110,23 +890,23 @@ extern "C" int vb_tree_attention(vb_ctx *ctx, const vb_tree_args *in) {
     if (a.layer < 0 || a.layer >= g.p.n_layers) return bad("layer out of range");
     if (a.n < 0 || a.n_tokens < 0 || a.max_tokens < 0 || a.n_heads <= 0) return bad("bad sizes");
     if (a.n_heads % g.p.n_kv_heads) return bad("n_heads must be a multiple of the cache's n_kv_heads");
+    g.group = a.n_heads / g.p.n_kv_heads;
     const int64_t qd = (int64_t)a.n_heads * g.p.head_dim;
     if (!a.ldq) a.ldq = qd;
     if (!a.ldo) a.ldo = qd;
     if (a.ldq < qd || a.ldo < qd) return bad("row stride below the row");
     if (!(a.scale >= 0.0f)) return bad("negative scale");
-    g.scale = a.scale == 0.0f ? 1.0f / sqrtf((float)g.p.head_dim) : a.scale;
+    g.scale_log2 = (float)((a.scale == 0.0f ? 1.0 / sqrt((double)g.p.head_dim) : (double)a.scale) * 1.4426950408889634);
     if (a.mask && a.mask_words <= 0) return bad("mask without words");
+    if ((int64_t)a.max_tokens * g.group > INT32_MAX / 2) return bad("too many rows");
     if (a.n == 0 || a.n_tokens == 0 || a.max_tokens == 0) return VB_OK;
     if (!a.q || !a.out || !a.seqs || !a.start) return bad("null pointer");
-    const int64_t items = (int64_t)a.n * a.max_tokens * a.n_heads;
-    if (items / TR_WARPS >= INT32_MAX) return bad("too many rows");
+    const uintptr_t es = a.type == VB_TYPE_F32 ? 4 : 2;
+    if (((uintptr_t)a.q | (uintptr_t)a.out) % es || ((uintptr_t)a.seqs | (uintptr_t)a.start | (uintptr_t)a.mask) % 4)
+        return bad("misaligned pointer");
+    g.vec = ((uintptr_t)a.q | (uintptr_t)a.out) % (4 * es) == 0 && (a.ldq | a.ldo) % 4 == 0;
     g.err = ctx->op_error;
-    const dim3 grid((unsigned)((items + TR_WARPS - 1) / TR_WARPS)), block(TR_WARPS * 32);
-    cudaError_t e = a.type == VB_TYPE_F32 ? pdl_launch(ctx, tree_attention_kernel<float, __nv_bfloat16>, grid, block, 0, g)
-                    : a.type == VB_TYPE_F16 ? pdl_launch(ctx, tree_attention_kernel<__half, __half>, grid, block, 0, g)
-                                            : pdl_launch(ctx, tree_attention_kernel<__nv_bfloat16, __nv_bfloat16>, grid, block, 0, g);
-    VB_CHECK(ctx, e);
-    VB_LAUNCH_CHECK(ctx, "tree_attention");
-    return VB_OK;
+    return a.type == VB_TYPE_F32   ? launch_heads<TR_F32>(ctx, g)
+           : a.type == VB_TYPE_F16 ? launch_heads<TR_F16>(ctx, g)
+                                   : launch_heads<TR_BF16>(ctx, g);
 }
