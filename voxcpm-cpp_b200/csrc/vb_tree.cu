@@ -21,7 +21,7 @@
 // not depend on timing.
 #include "vb_common.cuh"
 #include "vb_kernels.cuh"
-#include "vb_tc.cuh"
+#include "vb_tree.cuh"
 
 #include <algorithm>
 
@@ -34,100 +34,6 @@ constexpr int TR_THREADS = 384;      // warps 0..7 compute, warp 8 loads
 // to 56 and the two computing ones up to 224 (2 * 224 + 56 = 3 * 168), which
 // their sums need.
 constexpr int TR_SMEM = 226 * 1024;  // dynamic shared memory
-
-enum { TR_F32 = 0, TR_BF16 = 1, TR_F16 = 2 };
-
-struct TreeArgs {
-    vb_tree_args a;
-    vb_pages p;
-    float scale_log2;                // scale * log2(e): the softmax runs in powers of two
-    int group;                       // query heads per K/V head
-    int mt;                          // rows per block
-    int max_blocks;                  // blocks of the longest draft
-    int stages;
-    int vec;                         // 4-value accesses of q, 2-value ones of out
-    int *err;
-    float *part;                     // [2 * CTAs][mt][head_dim + 2]
-    int2 *desc;                      // [n][n_kv][max_blocks] CTAs of an item
-};
-
-// Sequence i of the call.  T = 0: no rows of q (or none that can be named);
-// bad: its tokens get zeros.
-struct TreeSeq {
-    int t0, T, s, len, base, bad;
-};
-
-__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &g, int i) {
-    TreeSeq q;
-    const vb_tree_args &a = g.a;
-    q.t0 = a.start[i];
-    const int t1 = a.start[i + 1];
-    q.s = a.seqs[i];
-    q.T = t1 - q.t0;
-    q.bad = 0;
-    if (q.t0 < 0 || t1 < q.t0 || t1 > a.n_tokens || q.T > a.max_tokens) {
-        q.T = 0;
-        q.bad = 1;
-        q.len = q.base = 0;
-        return q;
-    }
-    q.len = q.s >= 0 && q.s < g.p.n_seqs ? g.p.length[q.s] : -1;
-    q.base = q.len - q.T;
-    if (q.base < 0 || (int64_t)q.len > (int64_t)g.p.max_pages * g.p.page_rows ||
-        (a.mask && q.T > 32 * (int64_t)a.mask_words)) {
-        q.bad = 1;
-        q.len = q.base = 0;
-    }
-    return q;
-}
-
-__device__ __forceinline__ int tree_blocks(const TreeArgs &g, const TreeSeq &q) {
-    return (int)(((int64_t)q.T * g.group + g.mt - 1) / g.mt);
-}
-
-// Rows of the cache that block b of a sequence reads, and its units (at
-// least one, so that every output row is written).
-__device__ __forceinline__ int tree_visible(const TreeArgs &g, const TreeSeq &q, int b) {
-    if (q.bad) return 0;
-    if (g.a.mask) return q.len;
-    return q.base + (int)min((int64_t)q.T, (((int64_t)b + 1) * g.mt + g.group - 1) / g.group);
-}
-
-__device__ __forceinline__ int tree_units(int visible) { return max(1, (visible + TR_KT - 1) / TR_KT); }
-
-__device__ int64_t tree_seq_units(const TreeArgs &g, const TreeSeq &q) {
-    const int nb = tree_blocks(g, q);
-    if (g.a.mask || q.bad) return (int64_t)nb * tree_units(tree_visible(g, q, 0)) * g.p.n_kv_heads;
-    int64_t u = 0;
-    for (int b = 0; b < nb; b++) u += tree_units(tree_visible(g, q, b));
-    return u * g.p.n_kv_heads;
-}
-
-// A place in the line of units: the item (i, kv head, block) and the tile.
-struct TreeWalk {
-    TreeSeq q;
-    int i, g, b, nb, visible, units, tile;
-    int64_t left;                    // units of this CTA from here on
-};
-
-__device__ __forceinline__ void tree_item(const TreeArgs &g, TreeWalk &w) {
-    w.visible = tree_visible(g, w.q, w.b);
-    w.units = tree_units(w.visible);
-}
-
-__device__ __forceinline__ void tree_next(const TreeArgs &g, TreeWalk &w) {
-    w.tile = 0;
-    if (++w.b == w.nb) {
-        w.b = 0;
-        if (++w.g == g.p.n_kv_heads) {
-            w.g = 0;
-            do w.q = tree_seq(g, ++w.i);
-            while (w.q.T == 0);
-            w.nb = tree_blocks(g, w.q);
-        }
-    }
-    tree_item(g, w);
-}
 
 // ------------------------------------------------------------ mma helpers
 template <int TYPE>
@@ -156,46 +62,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "memory");
 }
 
-template <int TYPE>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    uint32_t r;
-    if constexpr (TYPE == TR_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-template <int TYPE>
-__device__ __forceinline__ float unpack(uint16_t h) {
-    if constexpr (TYPE == TR_F16) return h2f(h);
-    else return bf16_to_f(h);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Byte offset of 16-byte chunk c of row r in a [rows][128 B] tile with the
-// 128-byte swizzle that TMA writes.
-__device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
-
-// A bounded barrier wait; the first that runs out records the error and
-// lets every later wait of the CTA return at once.
-__device__ __forceinline__ void tree_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *err) {
-    if (mbar_try_wait(bar, parity)) return;
-    if (*abort) return;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*abort) return;
-        if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
-            *abort = 1;
-            atomicCAS(err, 0, VB_DEV_TREE_WAIT);
-            return;
-        }
-    }
-}
-
 // TYPE: the types; HDP: head_dim rounded up to 64, 128 or 256; R: 16-row
 // pieces per warp; WM: row groups of warps.  8 / WM warps share a row group
 // and split a tile's rows 16 each (with WM = 1 two sets of four take tiles
@@ -221,9 +87,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     uint8_t *qs = reinterpret_cast<uint8_t *>(merge + 4 * 16 * MPITCH);             // [QT][MT][QPITCH]
     float2 *ml = reinterpret_cast<float2 *>(qs + QT * MT * QPITCH);                 // [8][16 * R]
     __shared__ uint64_t full[TR_MAX_STAGES], empty[TR_MAX_STAGES];
-    __shared__ int64_t scan[TR_THREADS / 32];
-    __shared__ int abort_flag, s_seq;
-    __shared__ int64_t s_off;
+    __shared__ TreeCut cut;
+    __shared__ int abort_flag, not_finite;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -233,71 +98,15 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         }
         mbar_fence_init();
         abort_flag = 0;
-        s_seq = -1;
+        not_finite = 0;
     }
     pdl_trigger();
     pdl_wait();
 
-    // ---- this CTA's part of the line of units
-    const int n = g.a.n;
-    const int per = (n + TR_THREADS - 1) / TR_THREADS;
-    const int i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
-    int64_t mine = 0;
-    for (int i = i0; i < i1; i++) {
-        const TreeSeq q = tree_seq(g, i);
-        if (q.bad && blockIdx.x == 0) atomicCAS(g.err, 0, VB_DEV_TREE_SEQ);
-        mine += tree_seq_units(g, q);
-    }
-    int64_t before = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += y;
-    }
-    if (lane == 31) scan[warp] = before;
-    before -= mine;
-    __syncthreads();
-    int64_t total = 0;
-    for (int w = 0; w < TR_THREADS / 32; w++) {
-        if (w < warp) before += scan[w];
-        total += scan[w];
-    }
-    const int64_t ctas = min((int64_t)gridDim.x, total);          // that get a unit
-    const int64_t u0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : total;
-    const int64_t u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : total;
-    if (u0 >= before && u0 < before + mine) {
-        int64_t at = before;
-        for (int i = i0; i < i1; i++) {
-            const int64_t u = tree_seq_units(g, tree_seq(g, i));
-            if (u0 < at + u) {
-                s_seq = i;
-                s_off = u0 - at;
-                break;
-            }
-            at += u;
-        }
-    }
-    __syncthreads();
-    if (u0 >= u1) return;
-
     TreeWalk w;
-    w.i = s_seq;
-    w.q = tree_seq(g, w.i);
-    w.nb = tree_blocks(g, w.q);
-    w.left = u1 - u0;
-    {
-        const int64_t head_units = tree_seq_units(g, w.q) / g.p.n_kv_heads;
-        w.g = (int)(s_off / head_units);
-        int64_t off = s_off % head_units;
-        w.b = 0;
-        tree_item(g, w);
-        while (off >= w.units) {
-            off -= w.units;
-            w.b++;
-            tree_item(g, w);
-        }
-        w.tile = (int)off;
-    }
+    int64_t u1, total, ctas;
+    tree_cut<TR_THREADS>(g, cut, w, u1, total, ctas);
+    if (w.left <= 0) return;
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -423,36 +232,61 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             tree_wait(&full[s], (uint32_t)(it / g.stages) & 1u, &abort_flag, g.err);
             const uint32_t kt = smem_u32(ring + (size_t)s * STAGE), vt = kt + CB * TILE;
             // scores: 16 rows x 16 cache rows
-            float c[R][2][4];
+            float c[R][2][4], lo[R][2][4];
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int t = 0; t < 2; t++) c[r][t][0] = c[r][t][1] = c[r][t][2] = c[r][t][3] = 0.0f;
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) c[r][t][e] = lo[r][t][e] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < HDP / 16; ks++) {
+                // fp32: the leading term of each step starts from zero and joins
+                // the sum in a rounded fp32 add, the small terms run along in `lo`
                 uint32_t kb[4];
                 ldsm4(kb, kt + (ks / 4) * TILE +
                               sw128(slice + (lane & 7) + (lane >> 4) * 8, (ks % 4) * 2 + ((lane >> 3) & 1)));
 #pragma unroll
-                for (int r = 0; r < R; r++)
+                for (int r = 0; r < R; r++) {
+                    uint32_t qa[4];
 #pragma unroll
-                    for (int t = QT - 1; t >= 0; t--) {
-                        uint32_t qa[4];
+                    for (int t = QT - 1; t > 0; t--) {
                         ldsm4(qa, q_at + (uint32_t)((t * MT + 16 * r) * QPITCH + ks * 32));
+                        mma16816<TYPE>(lo[r][0], qa, kb[0], kb[1]);
+                        mma16816<TYPE>(lo[r][1], qa, kb[2], kb[3]);
+                    }
+                    ldsm4(qa, q_at + (uint32_t)(16 * r * QPITCH + ks * 32));
+                    if constexpr (TYPE == TR_F32) {
+                        float d0[4] = {}, d1[4] = {};
+                        mma16816<TYPE>(d0, qa, kb[0], kb[1]);
+                        mma16816<TYPE>(d1, qa, kb[2], kb[3]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            c[r][0][e] += d0[e];
+                            c[r][1][e] += d1[e];
+                        }
+                    } else {
                         mma16816<TYPE>(c[r][0], qa, kb[0], kb[1]);
                         mma16816<TYPE>(c[r][1], qa, kb[2], kb[3]);
                     }
+                }
+            }
+            if constexpr (TYPE == TR_F32) {
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) c[r][t][e] += lo[r][t][e];
             }
             const int r0 = (w.tile + x) * TR_KT + slice;       // cache row of the warp's first column
             const bool edge = r0 + 16 > w.q.base;              // not every row is seen by every token
-            bool careful = false;
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) c[r][t][e] *= g.scale_log2;
-            uint32_t seen[R] = {};                             // bit t*4+e
             if (edge) {
 #pragma unroll
                 for (int r = 0; r < R; r++)
@@ -461,34 +295,25 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int j = tok[r][e >> 1], d = r0 + 8 * t + 2 * ql + (e & 1) - w.q.base;
-                            bool see = j >= 0 && d + w.q.base < w.visible;
-                            if (see && d >= 0)
-                                see = g.a.mask ? g.a.mask[(int64_t)(w.q.t0 + j) * g.a.mask_words + (d >> 5)] >> (d & 31) & 1u
-                                               : d <= j;
-                            if (!see) c[r][t][e] = -INFINITY;
-                            else seen[r] |= 1u << (t * 4 + e);
+                            if (j < 0 || d + w.q.base >= w.visible || (d >= 0 && !tree_sees(g, w.q, j, d)))
+                                c[r][t][e] = -INFINITY;
                         }
-                // rows past the end may hold anything: they become zeros.
-                // A draft row that is not finite must not meet the zero
-                // weights of the tokens that do not see it: those tiles take
-                // the products one by one below.
+                // rows past the end may hold anything: they become zeros, as
+                // do draft values that are not finite
                 uint8_t *vg = ring + (size_t)s * STAGE + CB * TILE;
+                bool found = false;
                 for (int e = lane; e < 16 * CB * 8; e += 32) {
                     const int rr = e / (CB * 8), cc = e % (CB * 8);
                     uint4 *p = reinterpret_cast<uint4 *>(vg + (cc >> 3) * TILE + sw128(slice + rr, cc & 7));
                     if (r0 + rr >= w.visible) *p = make_uint4(0, 0, 0, 0);
                     else if (r0 + rr >= w.q.base) {
-                        const uint4 v = *p;
-                        const uint32_t inf = TYPE == TR_F16 ? 0x7c007c00u : 0x7f807f80u;
-                        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint32_t z = vv[k] & inf;
-                            careful |= (z & 0xffffu) == (inf & 0xffffu) || (z >> 16) == (inf >> 16);
-                        }
+                        bool here = false;
+                        const uint4 v = tree_finite<TYPE>(*p, here);
+                        if (here) *p = v;
+                        found |= here;
                     }
                 }
-                careful = __any_sync(0xffffffffu, careful);
+                if (found) not_finite = 1;
                 __syncwarp();
             }
             // running maximum and sum
@@ -516,9 +341,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         }
                     l[r][h] = fmaf(l[r][h], al[r][h], sum);
                 }
-            moved = __any_sync(0xffffffffu, moved);
-            if (TYPE != TR_F32 || careful) {
-                if (moved) {
+            if constexpr (TYPE != TR_F32) {
+                if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                     for (int r = 0; r < R; r++)
 #pragma unroll
@@ -527,38 +351,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                             for (int e = 0; e < 4; e++) o[r][t][e] *= al[r][e >> 1];
                 }
             }
-            if (careful) {
-                const uint8_t *vg = ring + (size_t)s * STAGE + CB * TILE;
-                for (int kr = 0; kr < 16; kr++) {
-                    // the weights of cache row kr sit in lane kr/2 % 4 of each quad
-#pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        const int from = (lane & ~3) | (kr >> 1 & 3);
-                        float p[2];
-                        bool see[2];
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const float x0 = kr & 1 ? c[r][0][2 * h + 1] : c[r][0][2 * h];
-                            const float x1 = kr & 1 ? c[r][1][2 * h + 1] : c[r][1][2 * h];
-                            p[h] = __shfl_sync(0xffffffffu, kr < 8 ? x0 : x1, from);
-                            const uint32_t sb = __shfl_sync(0xffffffffu, seen[r], from);
-                            see[h] = sb >> ((kr >> 3) * 4 + 2 * h + (kr & 1)) & 1u;
-                        }
-#pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            const uint32_t v2 = *reinterpret_cast<const uint32_t *>(
-                                vg + (t >> 3) * TILE + sw128(slice + kr, t & 7) + 4 * ql);
-                            const float v0 = unpack<TYPE>((uint16_t)v2), v1 = unpack<TYPE>((uint16_t)(v2 >> 16));
-#pragma unroll
-                            for (int h = 0; h < 2; h++)
-                                if (see[h]) {
-                                    o[r][t][2 * h] = fmaf(p[h], v0, o[r][t][2 * h]);
-                                    o[r][t][2 * h + 1] = fmaf(p[h], v1, o[r][t][2 * h + 1]);
-                                }
-                        }
-                    }
-                }
-            } else {
+            {
                 uint32_t pa[R][4], pb[R][4];
 #pragma unroll
                 for (int r = 0; r < R; r++)
@@ -613,6 +406,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 if (ql == 0) ml[warp * 16 * R + 16 * r + quad + 8 * h] = make_float2(m[r][h], x);
             }
         consumer_sync(256);
+        const bool mend = not_finite != 0;
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
@@ -662,6 +456,23 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 }
                 consumer_sync(256);
             }
+        if (threadIdx.x == 0) not_finite = 0;          // every warp has read it, and none sets it before the next barrier
+        if (mend && kw == 0) {
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (tok[r][h] >= 0)
+                        for (int t = 0; t < hd / 8; t++)
+                            for (int e = 0; e < 2; e++) {
+                                const float add = tree_not_finite<TYPE>(&g, &w.q, w.g, tok[r][h], w.tile * TR_KT,
+                                                                        min(w.visible, (w.tile + n_tiles) * TR_KT),
+                                                                        8 * t + 2 * ql + e);
+#pragma unroll
+                                for (int u = 0; u < NT; u++)
+                                    if (u == t) o[r][u][2 * h + e] += add;
+                            }
+        }
         if (kw == 0) {
             float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * MT * (hd + 2);
 #pragma unroll
@@ -703,14 +514,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     }
                 }
         }
-        // the CTA that holds an item's first unit says which CTAs hold the rest
-        if (threadIdx.x == 0 && w.tile == 0) {
-            const int64_t at = u1 - w.left;                        // the item's first unit
-            const int64_t end = at + w.units - 1;
-            const int last = (int)(((end + 1) * ctas - 1) / total);
-            g.desc[((int64_t)w.i * g.p.n_kv_heads + w.g) * g.max_blocks + w.b] =
-                make_int2((int)blockIdx.x * 2 + (first_item ? 0 : 1), last);
-        }
+        if (threadIdx.x == 0 && w.tile == 0) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
         first_item = false;
         w.left -= n_tiles;
         if (w.left > 0) tree_next(g, w);
@@ -795,20 +599,37 @@ static int tree_fit(TreeArgs &g, size_t &smem) {
     return MT;
 }
 
+// The parts and the description of every item of a call.
+int tree_workspace(vb_ctx *ctx, TreeArgs &g) {
+    g.max_blocks = (int)(((int64_t)g.a.max_tokens * g.group + g.mt - 1) / g.mt);
+    const int64_t items = (int64_t)g.a.n * g.p.n_kv_heads * g.max_blocks;
+    if (items > INT32_MAX) return set_error(ctx, VB_ERR_INVALID_ARG, "vb_tree_attention: too many rows");
+    const size_t parts = (size_t)2 * ctx->sm_count * g.mt * (g.p.head_dim + 2) * sizeof(float);
+    int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)items * sizeof(int2));
+    if (rc) return rc;
+    g.part = static_cast<float *>(ctx->tree_ws.ptr);
+    g.desc = reinterpret_cast<int2 *>(static_cast<char *>(ctx->tree_ws.ptr) + parts);
+    return VB_OK;
+}
+
+int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g) {
+    const int64_t items = (int64_t)g.a.n * g.p.n_kv_heads * g.max_blocks;
+    auto kernel = g.a.type == VB_TYPE_F32   ? tree_combine_kernel<TR_F32>
+                  : g.a.type == VB_TYPE_F16 ? tree_combine_kernel<TR_F16>
+                                            : tree_combine_kernel<TR_BF16>;
+    VB_CHECK(ctx, pdl_launch(ctx, kernel, dim3((unsigned)items, g.mt), dim3(TC_WARPS * 32), 0, g));
+    VB_LAUNCH_CHECK(ctx, "tree_combine");
+    return VB_OK;
+}
+
 template <int TYPE, int HDP, int R, int WM>
 static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     size_t smem;
     tree_fit<TYPE, HDP, R, WM>(g, smem);
     const vb_pages &p = g.p;
-    const int grid = ctx->sm_count;
-    g.max_blocks = (int)(((int64_t)g.a.max_tokens * g.group + g.mt - 1) / g.mt);
-    const int64_t items = (int64_t)g.a.n * p.n_kv_heads * g.max_blocks;
-    if (items > INT32_MAX) return set_error(ctx, VB_ERR_INVALID_ARG, "vb_tree_attention: too many rows");
-    const size_t parts = (size_t)2 * grid * g.mt * (p.head_dim + 2) * sizeof(float);
-    int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)items * sizeof(int2));
+    g.kt = TR_KT;
+    int rc = tree_workspace(ctx, g);
     if (rc) return rc;
-    g.part = static_cast<float *>(ctx->tree_ws.ptr);
-    g.desc = reinterpret_cast<int2 *>(static_cast<char *>(ctx->tree_ws.ptr) + parts);
     CUtensorMap tk, tv;
     const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;
     const CUtensorMapDataType dt = p.type == VB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -816,25 +637,30 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     if (!make_map(&tk, static_cast<char *>(p.k) + layer, dt, 2, p.head_dim, rows, 64, box, true) ||
         !make_map(&tv, static_cast<char *>(p.v) + layer, dt, 2, p.head_dim, rows, 64, box, true))
         return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the cache refused");
-    VB_CHECK(ctx, pdl_launch(ctx, tree_attention_kernel<TYPE, HDP, R, WM>, dim3(grid), dim3(TR_THREADS), smem, tk, tv, g));
+    VB_CHECK(ctx, pdl_launch(ctx, tree_attention_kernel<TYPE, HDP, R, WM>, dim3(ctx->sm_count), dim3(TR_THREADS), smem, tk,
+                             tv, g));
     VB_LAUNCH_CHECK(ctx, "tree_attention");
-    VB_CHECK(ctx, pdl_launch(ctx, tree_combine_kernel<TYPE>, dim3((unsigned)items, g.mt), dim3(TC_WARPS * 32), 0, g));
-    VB_LAUNCH_CHECK(ctx, "tree_combine");
-    return VB_OK;
+    return launch_tree_combine(ctx, g);
 }
 
-// Rows per block: the fewest of 16, 32 and 64 that hold a sequence's rows
-// (heads above 128: 32 at most, as their sums fill the registers, and 16 for
-// fp32 queries, whose terms would leave no room for two stages).
+// Which kernel and how many rows per block.  16-bit queries of more than 16
+// rows go to the tcgen05 kernel (vb_tree_tc.cu), whose tile of 128 rows costs
+// the tensor cores less than reading the cache costs the memory, however few
+// of its rows exist.  What is left: up to 16 rows, where padding to 128 only
+// delays the first result; heads above 128 values, whose sums and scores do
+// not fit its tensor memory; and fp32 queries, whose sums the tcgen05
+// accumulators hold less exactly.
 template <int TYPE, int HDP>
 static int launch_rows(vb_ctx *ctx, TreeArgs &g) {
     const int64_t rows = (int64_t)g.a.max_tokens * g.group;
     if (rows <= 16) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);
-    if constexpr (HDP == 256 && TYPE == TR_F32) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);
-    else if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 1, 2>(ctx, g);
-    else {
-        if (rows <= 32) return launch_tree<TYPE, HDP, 2, 1>(ctx, g);
-        return launch_tree<TYPE, HDP, 2, 2>(ctx, g);
+    if constexpr (TYPE == TR_F32) {
+        if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);      // more rows leave no room for two stages
+        else if (rows <= 32) return launch_tree<TYPE, HDP, 2, 1>(ctx, g);
+        else return launch_tree<TYPE, HDP, 2, 2>(ctx, g);
+    } else {
+        if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 1, 2>(ctx, g);      // more would not fit the registers
+        else return launch_tree_tc(ctx, g);
     }
 }
 
@@ -849,26 +675,23 @@ static cudaError_t allow_smem() {
     return cudaFuncSetAttribute(tree_attention_kernel<TYPE, HDP, R, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
 }
 
-template <int TYPE>
-static cudaError_t allow_smem_type() {
-    cudaError_t e = cudaSuccess;
-    auto keep = [&](cudaError_t x) { e = e == cudaSuccess ? x : e; };
-    keep(allow_smem<TYPE, 64, 1, 1>());
-    keep(allow_smem<TYPE, 64, 2, 1>());
-    keep(allow_smem<TYPE, 64, 2, 2>());
-    keep(allow_smem<TYPE, 128, 1, 1>());
-    keep(allow_smem<TYPE, 128, 2, 1>());
-    keep(allow_smem<TYPE, 128, 2, 2>());
-    keep(allow_smem<TYPE, 256, 1, 1>());
-    if constexpr (TYPE != TR_F32) keep(allow_smem<TYPE, 256, 1, 2>());
-    return e;
-}
-
 int init_tree(vb_ctx *ctx) {
-    VB_CHECK(ctx, allow_smem_type<TR_F32>());
-    VB_CHECK(ctx, allow_smem_type<TR_BF16>());
-    VB_CHECK(ctx, allow_smem_type<TR_F16>());
-    return VB_OK;
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 2, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 2, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 2, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 2, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 64, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 128, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 64, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 128, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1, 2>()));
+    return init_tree_tc(ctx);
 }
 
 }  // namespace vb
@@ -904,7 +727,7 @@ extern "C" int vb_tree_attention(vb_ctx *ctx, const vb_tree_args *in) {
     const uintptr_t es = a.type == VB_TYPE_F32 ? 4 : 2;
     if (((uintptr_t)a.q | (uintptr_t)a.out) % es || ((uintptr_t)a.seqs | (uintptr_t)a.start | (uintptr_t)a.mask) % 4)
         return bad("misaligned pointer");
-    g.vec = ((uintptr_t)a.q | (uintptr_t)a.out) % (4 * es) == 0 && (a.ldq | a.ldo) % 4 == 0;
+    g.vec = ((uintptr_t)a.q | (uintptr_t)a.out) % 16 == 0 && (a.ldq | a.ldo) % (16 / (int64_t)es) == 0;
     g.err = ctx->op_error;
     return a.type == VB_TYPE_F32   ? launch_heads<TR_F32>(ctx, g)
            : a.type == VB_TYPE_F16 ? launch_heads<TR_F16>(ctx, g)

@@ -1,0 +1,564 @@
+// vb_tree_tc.cu -- drafted-token attention on the tcgen05 tensor cores, for
+// 16-bit queries of more than 16 rows (tokens x query heads of a K/V head).
+//
+// Both products run as kind::f16 MMAs of 128 score rows: S = Q K^T from
+// shared memory into tensor memory, where the softmax threads (one per row)
+// read it and leave the weights P as 16-bit values in its place; O += P V
+// takes P from tensor memory and V as it lies in the cache (rows along the
+// contraction) from shared memory.
+//
+// Two streams of four softmax warps keep the tensor cores busy while the
+// other stream takes its exponentials:
+//   PAIR  (more than 128 rows): the streams are two row tiles that share
+//         every K and V tile, 256 rows per block;
+//   else: the streams take the cache tiles of one row tile in turn and are
+//         added at the end.
+// The sums follow a running maximum that moves only when a score exceeds it
+// by 2^8 (the weights stay far inside the 16-bit formats), so O is rarely
+// rescaled in tensor memory.
+//
+// Warps 0..7 softmax (warpgroup = stream), 8 loads (TMA, one box per page),
+// 9 issues the MMAs, 10 and 11 complete the warpgroup.
+#include "vb_kernels.cuh"
+#include "vb_tree.cuh"
+
+#include <algorithm>
+
+namespace vb {
+
+constexpr int TT_KT = 128;
+constexpr int TT_THREADS = 384;
+constexpr int TT_SLOTS = 12;
+constexpr int TT_SMEM = 225 * 1024;
+constexpr float TT_SLACK = 8.0f;     // log2 of how far a score may exceed the running maximum
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// A tile of [rows][64 values] column blocks 16 KB apart whose rows run along
+// the contraction: 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t addr) {
+    uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(16384 >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// Load and wait in one statement (the registers are written asynchronously).
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The ring holds K and V tiles in the order in which the MMAs use them:
+// PAIR K0 V0 K1 V1 ..., else K0 K1 V0 K2 V1 ... V(n-1).
+template <bool PAIR>
+__device__ __forceinline__ void ring_entry(int e, int n, int &tile, bool &is_v) {
+    if (PAIR) {
+        tile = e >> 1;
+        is_v = e & 1;
+    } else if (e & 1) {
+        is_v = (e + 1) / 2 >= n;
+        tile = is_v ? n - 1 : (e + 1) / 2;
+    } else {
+        is_v = e > 0;
+        tile = is_v ? e / 2 - 1 : 0;
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ int ring_k(int j) { return PAIR ? 2 * j : j == 0 ? 0 : 2 * j - 1; }
+template <bool PAIR>
+__device__ __forceinline__ int ring_v(int j, int n) { return PAIR ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1); }
+
+template <int TYPE, int HDP, bool PAIR>
+__global__ void __launch_bounds__(TT_THREADS, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                   const __grid_constant__ TreeArgs g) {
+    constexpr int CB = HDP / 64;
+    constexpr uint32_t BLOCK = TT_KT * 128;          // bytes of a 64-value column block of 128 rows
+    constexpr uint32_t SLOT = CB * BLOCK;
+    constexpr int MT = PAIR ? 256 : 128;
+
+    extern __shared__ uint8_t raw[];
+    uint8_t *qs = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *ring = qs + (PAIR ? 2 : 1) * SLOT;
+    float2 (*ml)[128] = reinterpret_cast<float2 (*)[128]>(ring + (size_t)g.stages * SLOT);   // !PAIR: (max, sum) of both streams
+    __shared__ uint64_t full[TT_SLOTS], empty[TT_SLOTS], q_full, s_full[2], p_full[2], pv_done[2];
+    __shared__ TreeCut cut;
+    __shared__ uint32_t s_tmem;
+    __shared__ int abort_flag, not_finite[2];        // item number in which a draft value was not finite, by its parity
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < TT_SLOTS; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&q_full, 8);
+        for (int t = 0; t < 2; t++) {
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 4);
+            mbar_init(&pv_done[t], 1);
+            not_finite[t] = -1;
+        }
+        mbar_fence_init();
+        abort_flag = 0;
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    pdl_trigger();
+    pdl_wait();
+    TreeWalk w;
+    int64_t u1, total, ctas;
+    tree_cut<TT_THREADS>(g, cut, w, u1, total, ctas);
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + HDP};
+    const int n_slots = g.stages;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8) {
+            // -------------------------------------------------------- loads
+            const int P = g.p.page_rows, box = min(P, TT_KT);
+            int pos = 0;
+            while (w.left > 0) {
+                const int n = (int)min((int64_t)(w.units - w.tile), w.left);
+                const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
+                // a lane's row within its box's page, and that page
+                auto page_of = [&](int e, int &y, int &nbox, bool &is_v) {
+                    int tile;
+                    ring_entry<PAIR>(e, n, tile, is_v);
+                    const int r0 = (w.tile + tile) * TT_KT, have = min(TT_KT, w.visible - r0);
+                    nbox = have <= 0 ? 0 : (have + box - 1) / box;
+                    y = 0;
+                    if (lane < nbox) {
+                        const int r = r0 + lane * box;
+                        int page = row[r / P];
+                        if (page < 0 || page >= g.p.n_pages) {
+                            atomicCAS(g.err, 0, VB_DEV_TREE_PAGE);
+                            page = 0;
+                        }
+                        y = (page * g.p.n_kv_heads + w.g) * P + r % P;
+                    }
+                };
+                int y, nbox;
+                bool is_v;
+                page_of(0, y, nbox, is_v);
+                for (int e = 0; e < 2 * n; e++, pos++) {
+                    int y1 = 0, nbox1 = 0;
+                    bool is_v1 = false;
+                    if (e + 1 < 2 * n) page_of(e + 1, y1, nbox1, is_v1);
+                    const int s = pos % n_slots;
+                    tree_wait(&empty[s], ((uint32_t)(pos / n_slots) & 1u) ^ 1u, &abort_flag, g.err);
+                    __syncwarp();
+                    // (every lane takes the same answer)
+                    const int load = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag ? 0 : nbox, 0);
+                    if (lane == 0) {
+                        if (load) mbar_arrive_expect_tx(&full[s], (uint32_t)load * box * 128 * CB);
+                        else mbar_arrive(&full[s]);
+                    }
+                    __syncwarp();
+                    if (lane < load) {
+                        uint8_t *dst = ring + (size_t)s * SLOT + lane * box * 128;
+#pragma unroll
+                        for (int c = 0; c < CB; c++) tma_load_2d(dst + c * BLOCK, is_v ? &tv : &tk, 64 * c, y, &full[s]);
+                    }
+                    y = y1;
+                    nbox = nbox1;
+                    is_v = is_v1;
+                }
+                w.left -= n;
+                if (w.left > 0) tree_next(g, w);
+            }
+            // every copy has landed before the CTA can end
+            for (int s = 0; s < n_slots; s++) {
+                const int fills = pos / n_slots + (pos % n_slots > s ? 1 : 0);
+                if (fills) gm_wait(&full[s], (uint32_t)(fills - 1) & 1u);
+            }
+        } else if (warp == 9 && lane == 0) {
+            // --------------------------------------------------------- MMAs
+            const int hd = g.p.head_dim, k_steps = (hd + 15) / 16;
+            const uint32_t fmt = TYPE == TR_F16 ? 0u : 1u;
+            const uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
+            const uint32_t id_s = common | ((uint32_t)(TT_KT >> 3) << 17);
+            const uint32_t id_o = common | (1u << 16) | ((uint32_t)(k_steps * 16 >> 3) << 17);     // V: rows along k
+            int pos = 0, item = 0;
+            int done[2] = {0, 0};                     // tiles whose P was taken, per stream
+            auto wait_ring = [&](int at) {
+                tree_wait(&full[at % n_slots], (uint32_t)(at / n_slots) & 1u, &abort_flag, g.err);
+                tc_fence_after();
+            };
+            auto scores = [&](int t, int at) {
+                const uint8_t *k = ring + (size_t)(at % n_slots) * SLOT, *q = qs + (PAIR ? t * SLOT : 0);
+                for (int i = 0; i < k_steps; i++)
+                    umma_f16(t_s[t], sw128_desc(q + (i >> 2) * BLOCK + (i & 3) * 32),
+                             sw128_desc(k + (i >> 2) * BLOCK + (i & 3) * 32), id_s, i > 0);
+                umma_commit(&s_full[t]);
+            };
+            auto values = [&](int t, int at, bool first) {
+                tree_wait(&p_full[t], (uint32_t)done[t]++ & 1u, &abort_flag, g.err);
+                tc_fence_after();
+                const uint32_t v = smem_u32(ring + (size_t)(at % n_slots) * SLOT);
+#pragma unroll
+                for (int i = 0; i < TT_KT / 16; i++)
+                    umma_f16_ts(t_o[t], t_s[t] + 8 * i, sw128_desc_mn(v + i * 2048), id_o, !(first && i == 0));
+                umma_commit(&pv_done[t]);
+            };
+            while (w.left > 0) {
+                const int n = (int)min((int64_t)(w.units - w.tile), w.left);
+                tree_wait(&q_full, (uint32_t)item & 1u, &abort_flag, g.err);
+                tc_fence_after();
+                for (int j = 0; j < (PAIR ? 1 : min(2, n)); j++) {
+                    const int at = pos + ring_k<PAIR>(j);
+                    wait_ring(at);
+                    scores(j, at);
+                    if (PAIR) scores(1, at);
+                    umma_commit(&empty[at % n_slots]);
+                }
+                for (int j = 0; j < n; j++) {
+                    const int at = pos + ring_v<PAIR>(j, n), next = pos + ring_k<PAIR>(j + (PAIR ? 1 : 2));
+                    const bool more = j + (PAIR ? 1 : 2) < n;
+                    wait_ring(at);
+                    if (PAIR) {
+                        values(0, at, j == 0);
+                        if (more) {
+                            wait_ring(next);
+                            scores(0, next);
+                        }
+                        values(1, at, j == 0);
+                        umma_commit(&empty[at % n_slots]);
+                        if (more) {
+                            scores(1, next);
+                            umma_commit(&empty[next % n_slots]);
+                        }
+                    } else {
+                        values(j & 1, at, j < 2);
+                        umma_commit(&empty[at % n_slots]);
+                        if (more) {
+                            wait_ring(next);
+                            scores(j & 1, next);
+                            umma_commit(&empty[next % n_slots]);
+                        }
+                    }
+                }
+                pos += 2 * n;
+                item++;
+                w.left -= n;
+                if (w.left > 0) tree_next(g, w);
+            }
+        }
+    } else {
+        // -------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int t = warp >> 2, tid = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // TMEM lane of the warp's first row
+        const int hd = g.p.head_dim;
+        int pos = 0, item = 0, seen = 0;                             // seen: tiles of this stream so far
+        bool first_item = true;
+        while (w.left > 0) {
+            const int n = (int)min((int64_t)(w.units - w.tile), w.left);
+            const int rows = (int)min((int64_t)MT, (int64_t)w.q.T * g.group - (int64_t)w.b * MT);
+            // the queries of this stream's row tile (of half of the one tile)
+            {
+                uint8_t *qt = qs + (PAIR ? t * SLOT : 0);
+                for (int e = PAIR ? tid : (int)threadIdx.x; e < 128 * (HDP / 8); e += PAIR ? 128 : 256) {
+                    const int r = e / (HDP / 8), c = e % (HDP / 8), m = (PAIR ? 128 * t : 0) + r;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (m < rows && 8 * c < hd) {
+                        const int64_t row = (int64_t)w.b * MT + m;
+                        const uint16_t *src = static_cast<const uint16_t *>(g.a.q) + (w.q.t0 + row / g.group) * g.a.ldq +
+                                              (w.g * g.group + row % g.group) * hd + 8 * c;
+                        if (g.vec) x = *reinterpret_cast<const uint4 *>(src);
+                        else
+                            x = make_uint4(src[0] | (uint32_t)src[1] << 16, src[2] | (uint32_t)src[3] << 16,
+                                           src[4] | (uint32_t)src[5] << 16, src[6] | (uint32_t)src[7] << 16);
+                    }
+                    *reinterpret_cast<uint4 *>(qt + (c >> 3) * BLOCK + sw128(r, c & 7)) = x;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full);
+            }
+            const int mrow = (PAIR ? 128 * t : 0) + 32 * (warp & 3) + lane;      // this thread's row of the block
+            const bool alive = mrow - lane < rows;                               // the warp has rows
+            const int j = mrow < rows ? (int)(((int64_t)w.b * MT + mrow) / g.group) : -1;
+            float m = -INFINITY, l = 0.0f;
+            const int mine = PAIR ? n : (n + 1 - t) / 2;                         // tiles of this stream
+            for (int x = 0; x < mine; x++, seen++) {
+                const int jt = PAIR ? x : 2 * x + t;
+                const int r0 = (w.tile + jt) * TT_KT;
+                const bool edge = r0 + TT_KT > w.q.base;
+                if (edge && (t == 0 || !PAIR)) {
+                    // V rows past the end may hold anything: they become zeros,
+                    // as do draft values that are not finite
+                    const int at = pos + ring_v<PAIR>(jt, n);
+                    tree_wait(&full[at % n_slots], (uint32_t)(at / n_slots) & 1u, &abort_flag, g.err);
+                    uint8_t *v = ring + (size_t)(at % n_slots) * SLOT;
+                    bool found = false;
+                    const int from = max(0, w.q.base - r0);
+                    for (int e = from * CB * 8 + tid; e < TT_KT * CB * 8; e += 128) {
+                        const int r = e / (CB * 8), c = e % (CB * 8);
+                        uint4 *p = reinterpret_cast<uint4 *>(v + (c >> 3) * BLOCK + sw128(r, c & 7));
+                        if (r0 + r >= w.visible) *p = make_uint4(0, 0, 0, 0);
+                        else {
+                            bool here = false;
+                            const uint4 y = tree_finite<TYPE>(*p, here);
+                            if (here) *p = y;
+                            found |= here;
+                        }
+                    }
+                    if (found) not_finite[item & 1] = item;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                tree_wait(&s_full[t], (uint32_t)seen & 1u, &abort_flag, g.err);
+                tc_fence_after();
+                if (alive) {
+                    float s[4][32];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) tmem_ld32(t_s[t] + lanes + 32 * k, s[k]);
+                    if (edge) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int d = r0 + 32 * k - w.q.base;                // draft place of the first column
+                            int lim = w.visible - (r0 + 32 * k);
+                            uint32_t bits = 0xffffffffu;
+                            if (!g.a.mask) lim = min(lim, d < 0 && j >= 0 ? max(0, j + 1 - d) : j + 1 - d);
+                            else if (d > -32 && j >= 0) {
+                                const uint32_t *row = g.a.mask + (int64_t)(w.q.t0 + j) * g.a.mask_words;
+                                if (d < 0) bits = (row[0] << -d) | ((1u << -d) - 1u);
+                                else {
+                                    const int k0 = d >> 5;
+                                    const uint32_t lo = k0 < g.a.mask_words ? row[k0] : 0u;
+                                    const uint32_t hi = k0 + 1 < g.a.mask_words ? row[k0 + 1] : 0u;
+                                    bits = __funnelshift_r(lo, hi, d & 31);
+                                }
+                            }
+                            if (j < 0 || lim <= 0) bits = 0u;
+                            else if (lim < 32) bits &= (1u << lim) - 1u;
+#pragma unroll
+                            for (int c = 0; c < 32; c++)
+                                if (!(bits >> c & 1u)) s[k][c] = -INFINITY;
+                        }
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        top[k] = s[k][0];
+#pragma unroll
+                        for (int c = 1; c < 31; c += 2) top[k] = fmaxf(top[k], fmaxf(s[k][c], s[k][c + 1]));
+                        top[k] = fmaxf(top[k], s[k][31]);
+                    }
+                    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * g.scale_log2;
+                    const bool move = now > m + TT_SLACK || (m == -INFINITY && now > m);
+                    if (x == 0) m = now;
+                    else if (__any_sync(0xffffffffu, move)) {
+                        const float f = move ? ex2(m - now) : 1.0f;
+                        if (move) m = now;
+                        l *= f;
+                        tree_wait(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < HDP / 32; k++) {
+                            float o[32];
+                            uint32_t y[32];
+                            tmem_ld32(t_o[t] + lanes + 32 * k, o);
+#pragma unroll
+                            for (int c = 0; c < 32; c++) y[c] = __float_as_uint(o[c] * f);
+                            tmem_st32(t_o[t] + lanes + 32 * k, y);
+                        }
+                    }
+                    const float off = m == -INFINITY ? 0.0f : m;
+                    float sum[4] = {};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t y[32];
+#pragma unroll
+                        for (int c = 0; c < 32; c++) {
+                            const float p0 = ex2(fmaf(s[2 * h + (c >> 4)][2 * (c & 15)], g.scale_log2, -off));
+                            const float p1 = ex2(fmaf(s[2 * h + (c >> 4)][2 * (c & 15) + 1], g.scale_log2, -off));
+                            sum[2 * h] += p0;
+                            sum[2 * h + 1] += p1;
+                            y[c] = pack2<TYPE>(p0, p1);
+                        }
+                        tmem_st32(t_s[t] + lanes + 32 * h, y);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+            }
+            if (mine > 0) tree_wait(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
+
+            // ---- the block's result, or this CTA's part of it
+            const bool whole = w.tile == 0 && n == w.units;
+            float f0 = 1.0f, f1 = 0.0f;
+            if (!PAIR) {
+                ml[t][tid] = make_float2(m, l);
+                tc_fence_before();
+                consumer_sync(256);
+                const float2 a = ml[0][tid], b = ml[1][tid];
+                m = fmaxf(a.x, b.x);
+                const float off = m == -INFINITY ? 0.0f : m;
+                f0 = ex2(a.x - off);
+                f1 = ex2(b.x - off);
+                l = a.y * f0 + b.y * f1;
+            }
+            tc_fence_after();
+            const bool mend = *(volatile int *)&not_finite[item & 1] == item;
+            if (alive) {
+                const int64_t row = (int64_t)w.b * MT + mrow;
+                const int head = w.g * g.group + (int)(row % g.group);
+                const float inv = whole ? (l > 0.0f || l != l ? 1.0f / l : 0.0f) : 1.0f;
+                float *part = g.part + ((size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * MT + mrow) * (hd + 2);
+                uint16_t *out = static_cast<uint16_t *>(g.a.out) + (w.q.t0 + row / g.group) * g.a.ldo + (int64_t)head * hd;
+                if (!whole && j >= 0 && (PAIR || t == 0)) *reinterpret_cast<float2 *>(part) = make_float2(m, l);
+                // PAIR: all columns of the thread's row; else half of them, of both streams
+#pragma unroll
+                for (int k = 0; k < (PAIR ? HDP / 32 : HDP / 64); k++) {
+                    const int c0 = 32 * (PAIR ? k : t * (HDP / 64) + k);
+                    float o[32];
+                    tmem_ld32(t_o[PAIR ? t : 0] + lanes + c0, o);
+                    if (!PAIR) {
+                        float o1[32];
+                        if (n > 1) tmem_ld32(t_o[1] + lanes + c0, o1);
+#pragma unroll
+                        for (int c = 0; c < 32; c++) o[c] = n > 1 ? o[c] * f0 + o1[c] * f1 : o[c] * f0;
+                    }
+                    if (mend && j >= 0)
+#pragma unroll
+                        for (int c = 0; c < 32; c++)
+                            if (c0 + c < hd)
+                                o[c] += tree_not_finite<TYPE>(&g, &w.q, w.g, j, w.tile * TT_KT,
+                                                              min(w.visible, (w.tile + n) * TT_KT), c0 + c);
+                    if (j < 0) continue;
+                    if (!whole) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2)
+                            if (c0 + c < hd) *reinterpret_cast<float2 *>(part + 2 + c0 + c) = make_float2(o[c], o[c + 1]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8) {
+                            if (c0 + c >= hd) continue;
+                            const uint4 y = make_uint4(pack2<TYPE>(o[c] * inv, o[c + 1] * inv), pack2<TYPE>(o[c + 2] * inv, o[c + 3] * inv),
+                                                       pack2<TYPE>(o[c + 4] * inv, o[c + 5] * inv), pack2<TYPE>(o[c + 6] * inv, o[c + 7] * inv));
+                            uint16_t *dst = out + c0 + c;
+                            if (g.vec) *reinterpret_cast<uint4 *>(dst) = y;
+                            else {
+                                const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                                for (int i = 0; i < 8; i++) dst[i] = (uint16_t)(z[i >> 1] >> (16 * (i & 1)));
+                            }
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            if (!PAIR) consumer_sync(256);           // both streams' sums are read: the next item may overwrite them
+            if (threadIdx.x == 0 && w.tile == 0) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
+            first_item = false;
+            pos += 2 * n;
+            item++;
+            w.left -= n;
+            if (w.left > 0) tree_next(g, w);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// -------------------------------------------------------------------- host
+template <int TYPE, int HDP, bool PAIR>
+static int launch_tc(vb_ctx *ctx, TreeArgs &g) {
+    constexpr size_t slot = (size_t)HDP / 64 * TT_KT * 128, q = (PAIR ? 2 : 1) * slot;
+    const vb_pages &p = g.p;
+    g.mt = PAIR ? 256 : 128;
+    g.kt = TT_KT;
+    const size_t rest = 1024 + q + (PAIR ? 0 : 2 * 128 * sizeof(float2));
+    g.stages = (int)std::min<size_t>(TT_SLOTS, (TT_SMEM - rest) / slot);
+    const size_t smem = rest + g.stages * slot;
+    int rc = tree_workspace(ctx, g);
+    if (rc) return rc;
+    CUtensorMap tk, tv;
+    const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;
+    const CUtensorMapDataType dt = p.type == VB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int box = std::min(p.page_rows, TT_KT);
+    if (!make_map(&tk, static_cast<char *>(p.k) + layer, dt, 2, p.head_dim, rows, 64, box, true) ||
+        !make_map(&tv, static_cast<char *>(p.v) + layer, dt, 2, p.head_dim, rows, 64, box, true))
+        return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the cache refused");
+    VB_CHECK(ctx, pdl_launch(ctx, tree_tc_kernel<TYPE, HDP, PAIR>, dim3(ctx->sm_count), dim3(TT_THREADS), smem, tk, tv, g));
+    VB_LAUNCH_CHECK(ctx, "tree_tc");
+    return launch_tree_combine(ctx, g);
+}
+
+template <int TYPE, int HDP>
+static int launch_tc_rows(vb_ctx *ctx, TreeArgs &g) {
+    return (int64_t)g.a.max_tokens * g.group > 128 ? launch_tc<TYPE, HDP, true>(ctx, g) : launch_tc<TYPE, HDP, false>(ctx, g);
+}
+
+int launch_tree_tc(vb_ctx *ctx, TreeArgs &g) {
+    if (g.a.type == VB_TYPE_F16)
+        return g.p.head_dim <= 64 ? launch_tc_rows<TR_F16, 64>(ctx, g) : launch_tc_rows<TR_F16, 128>(ctx, g);
+    return g.p.head_dim <= 64 ? launch_tc_rows<TR_BF16, 64>(ctx, g) : launch_tc_rows<TR_BF16, 128>(ctx, g);
+}
+
+template <int TYPE, int HDP, bool PAIR>
+static cudaError_t allow_tc() {
+    return cudaFuncSetAttribute(tree_tc_kernel<TYPE, HDP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TT_SMEM);
+}
+
+int init_tree_tc(vb_ctx *ctx) {
+    VB_CHECK(ctx, (allow_tc<TR_BF16, 64, false>()));
+    VB_CHECK(ctx, (allow_tc<TR_BF16, 64, true>()));
+    VB_CHECK(ctx, (allow_tc<TR_BF16, 128, false>()));
+    VB_CHECK(ctx, (allow_tc<TR_BF16, 128, true>()));
+    VB_CHECK(ctx, (allow_tc<TR_F16, 64, false>()));
+    VB_CHECK(ctx, (allow_tc<TR_F16, 64, true>()));
+    VB_CHECK(ctx, (allow_tc<TR_F16, 128, false>()));
+    VB_CHECK(ctx, (allow_tc<TR_F16, 128, true>()));
+    return VB_OK;
+}
+
+}  // namespace vb
