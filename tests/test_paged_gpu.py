@@ -525,6 +525,16 @@ def test_tree_attention(ctx, type, lens, drafted, nh, nkv, hd, P, mask):
     check_tree(ctx, tree_case(ctx, type, lens, drafted, nh, nkv, hd, P, mask))
 
 
+@pytest.mark.parametrize("type", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens,drafted,P", [([30000], [2], 64), ([9000, 20000], [1, 1], 16), ([25000, 100], [40, 3], 32)])
+def test_tree_many_tiles_for_each_cta(ctx, type, lens, drafted, P):
+    """Calls one after another, each CTA working through many tiles of the ring."""
+    t = tree_case(ctx, type, lens, drafted, 8, 1, 128, P, seed=8)
+    for _ in range(8):
+        ctx.tree_attention(t["args"])
+    check_tree(ctx, t)
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 def test_tree_strided_rows_and_wide_masks(ctx, type):
     check_tree(ctx, tree_case(ctx, type, [90, 64], [30, 20], 4, 2, 128, 16, extra_words=3, pad=8))

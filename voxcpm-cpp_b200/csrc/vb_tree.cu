@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     }
                 }
                 const int s = it % g.stages;
-                tree_wait(&empty[s], ((uint32_t)(it / g.stages) & 1u) ^ 1u, &abort_flag, g.err);
-                const int nload = abort_flag ? 0 : nbox;
+                tree_wait_warp(&empty[s], ((uint32_t)(it / g.stages) & 1u) ^ 1u, &abort_flag, g.err);
+                const int nload = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag ? 0 : nbox, 0);
                 uint8_t *st = ring + (size_t)s * STAGE;
                 if (lane == 0) {
                     if (nload) mbar_arrive_expect_tx(&full[s], (uint32_t)nload * box * 128 * 2 * CB);
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         for (int x = 0; x < n_tiles; x++, it++) {
             if (SETS == 2 && (it & 1) != set) continue;
             const int s = it % g.stages;
-            tree_wait(&full[s], (uint32_t)(it / g.stages) & 1u, &abort_flag, g.err);
+            tree_wait_warp(&full[s], (uint32_t)(it / g.stages) & 1u, &abort_flag, g.err);
             const uint32_t kt = smem_u32(ring + (size_t)s * STAGE), vt = kt + CB * TILE;
             // scores: 16 rows x 16 cache rows
             float c[R][2][4], lo[R][2][4];
@@ -515,6 +515,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 }
         }
         if (threadIdx.x == 0 && w.tile == 0) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
+        __syncwarp();
         first_item = false;
         w.left -= n_tiles;
         if (w.left > 0) tree_next(g, w);

@@ -231,6 +231,13 @@ __device__ __forceinline__ void tree_wait(uint64_t *bar, uint32_t parity, volati
     }
 }
 
+// The same by all lanes of a warp, which go on together: what follows
+// (ldmatrix, mma, tcgen05.ld) takes part of its operands from every lane.
+__device__ __forceinline__ void tree_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort, int *err) {
+    tree_wait(bar, parity, abort, err);
+    __syncwarp();
+}
+
 // Values of the draft that are not finite are taken out of the tiles (a zero
 // weight times infinity would reach tokens that do not see them).  This adds
 // up those that token j does see among cache rows lo .. hi-1 in column c:

@@ -186,8 +186,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     bool is_v1 = false;
                     if (e + 1 < 2 * n) page_of(e + 1, y1, nbox1, is_v1);
                     const int s = pos % n_slots;
-                    tree_wait(&empty[s], ((uint32_t)(pos / n_slots) & 1u) ^ 1u, &abort_flag, g.err);
-                    __syncwarp();
+                    tree_wait_warp(&empty[s], ((uint32_t)(pos / n_slots) & 1u) ^ 1u, &abort_flag, g.err);
                     // (every lane takes the same answer)
                     const int load = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag ? 0 : nbox, 0);
                     if (lane == 0) {
@@ -283,6 +282,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 w.left -= n;
                 if (w.left > 0) tree_next(g, w);
             }
+            // the last commit has reached its barrier before the CTA can end
+            if (pos) tree_wait(&empty[(pos - 1) % n_slots], (uint32_t)((pos - 1) / n_slots) & 1u, &abort_flag, g.err);
         }
     } else {
         // -------------------------------------------------------- softmax
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     // V rows past the end may hold anything: they become zeros,
                     // as do draft values that are not finite
                     const int at = pos + ring_v<PAIR>(jt, n);
-                    tree_wait(&full[at % n_slots], (uint32_t)(at / n_slots) & 1u, &abort_flag, g.err);
+                    tree_wait_warp(&full[at % n_slots], (uint32_t)(at / n_slots) & 1u, &abort_flag, g.err);
                     uint8_t *v = ring + (size_t)(at % n_slots) * SLOT;
                     bool found = false;
                     const int from = max(0, w.q.base - r0);
@@ -345,9 +346,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                         }
                     }
                     if (found) not_finite[item & 1] = item;
+                    __syncwarp();
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                tree_wait(&s_full[t], (uint32_t)seen & 1u, &abort_flag, g.err);
+                tree_wait_warp(&s_full[t], (uint32_t)seen & 1u, &abort_flag, g.err);
                 tc_fence_after();
                 if (alive) {
                     float s[4][32];
@@ -392,7 +394,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                         const float f = move ? ex2(m - now) : 1.0f;
                         if (move) m = now;
                         l *= f;
-                        tree_wait(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
+                        tree_wait_warp(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
                         tc_fence_after();
 #pragma unroll
                         for (int k = 0; k < HDP / 32; k++) {
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
             }
-            if (mine > 0) tree_wait(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
+            if (mine > 0) tree_wait_warp(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
 
             // ---- the block's result, or this CTA's part of it
             const bool whole = w.tile == 0 && n == w.units;
@@ -494,6 +496,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             tc_fence_before();
             if (!PAIR) consumer_sync(256);           // both streams' sums are read: the next item may overwrite them
             if (threadIdx.x == 0 && w.tile == 0) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
+            __syncwarp();
             first_item = false;
             pos += 2 * n;
             item++;
