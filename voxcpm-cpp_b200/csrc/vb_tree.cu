@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         for (int e = 0; e < 4; e++) c[r][t][e] += lo[r][t][e];
             }
             const int r0 = (w.tile + x) * TR_KT + slice;       // cache row of the warp's first column
-            const bool edge = r0 + 16 > w.q.base;              // not every row is seen by every token
+            const bool edge = r0 + 16 > w.clear;               // not every row is seen by every token
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     const int rr = e / (CB * 8), cc = e % (CB * 8);
                     uint4 *p = reinterpret_cast<uint4 *>(vg + (cc >> 3) * TILE + sw128(slice + rr, cc & 7));
                     if (r0 + rr >= w.visible) *p = make_uint4(0, 0, 0, 0);
-                    else if (r0 + rr >= w.q.base) {
+                    else if (r0 + rr >= w.clear) {
                         bool here = false;
                         const uint4 v = tree_finite<TYPE>(*p, here);
                         if (here) *p = v;
@@ -352,15 +352,18 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 }
             }
             {
-                uint32_t pa[R][4], pb[R][4];
+                uint32_t pa[R][4], pb[R][4], pc[R][4];      // fp32: a weight in three bf16 terms
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const float x0 = c[r][k >> 1][2 * (k & 1)], x1 = c[r][k >> 1][2 * (k & 1) + 1];
                         pa[r][k] = pack2<TYPE>(x0, x1);
-                        if constexpr (TYPE == TR_F32)
-                            pb[r][k] = pack2<TYPE>(x0 - bf16_to_f((uint16_t)pa[r][k]), x1 - bf16_to_f((uint16_t)(pa[r][k] >> 16)));
+                        if constexpr (TYPE == TR_F32) {
+                            const float y0 = x0 - bf16_to_f((uint16_t)pa[r][k]), y1 = x1 - bf16_to_f((uint16_t)(pa[r][k] >> 16));
+                            pb[r][k] = pack2<TYPE>(y0, y1);
+                            pc[r][k] = pack2<TYPE>(y0 - bf16_to_f((uint16_t)pb[r][k]), y1 - bf16_to_f((uint16_t)(pb[r][k] >> 16)));
+                        }
                     }
 #pragma unroll
                 for (int t = 0; t < NT; t += 2) {
@@ -374,6 +377,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                             // one rounded fp32 step: the tensor cores' own long sums
                             // lose more
                             float d0[4] = {}, d1[4] = {};
+                            mma16816<TYPE>(d0, pc[r], vb[0], vb[1]);
+                            mma16816<TYPE>(d1, pc[r], vb[2], vb[3]);
                             mma16816<TYPE>(d0, pb[r], vb[0], vb[1]);
                             mma16816<TYPE>(d1, pb[r], vb[2], vb[3]);
                             mma16816<TYPE>(d0, pa[r], vb[0], vb[1]);
@@ -457,24 +462,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 consumer_sync(256);
             }
         if (threadIdx.x == 0) not_finite = 0;          // every warp has read it, and none sets it before the next barrier
-        if (mend && kw == 0) {
-#pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (tok[r][h] >= 0)
-                        for (int t = 0; t < hd / 8; t++)
-                            for (int e = 0; e < 2; e++) {
-                                const float add = tree_not_finite<TYPE>(&g, &w.q, w.g, tok[r][h], w.tile * TR_KT,
-                                                                        min(w.visible, (w.tile + n_tiles) * TR_KT),
-                                                                        8 * t + 2 * ql + e);
-#pragma unroll
-                                for (int u = 0; u < NT; u++)
-                                    if (u == t) o[r][u][2 * h + e] += add;
-                            }
-        }
         if (kw == 0) {
             float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * MT * (hd + 2);
+            const int lo = max(w.clear, w.tile * TR_KT), hi = min(w.visible, (w.tile + n_tiles) * TR_KT);
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
@@ -502,19 +492,29 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                                 else dst[0] = (uint16_t)y, dst[1] = (uint16_t)(y >> 16);
                             }
                         }
+                        __syncwarp(__activemask());
+                        if (mend && ql == 0)
+                            tree_not_finite<TYPE>(&g, w.q.t0, w.q.s, w.q.base, w.g, tok[r][h], lo, hi, 0, hd,
+                                                  static_cast<uint8_t *>(g.a.out) + at * (TYPE == TR_F32 ? 4 : 2), 1,
+                                                  TYPE == TR_F32);
                     } else {
-                        float *dst = part + (size_t)mr * (hd + 2);
-                        if (ql == 0) *reinterpret_cast<float2 *>(dst) = make_float2(m[r][h], l[r][h]);
+                        if (ql == 0) {
+                            part[hd * MT + mr] = m[r][h];
+                            part[(hd + 1) * MT + mr] = l[r][h];
+                        }
 #pragma unroll
                         for (int t = 0; t < NT; t++) {
                             if (8 * t >= hd) break;
-                            *reinterpret_cast<float2 *>(dst + 2 + 8 * t + 2 * ql) =
-                                make_float2(o[r][t][2 * h], o[r][t][2 * h + 1]);
+                            part[(8 * t + 2 * ql) * MT + mr] = o[r][t][2 * h];
+                            part[(8 * t + 2 * ql + 1) * MT + mr] = o[r][t][2 * h + 1];
                         }
+                        __syncwarp(__activemask());
+                        if (mend && ql == 0)
+                            tree_not_finite<TYPE>(&g, w.q.t0, w.q.s, w.q.base, w.g, tok[r][h], lo, hi, 0, hd, part + mr, MT, 1);
                     }
                 }
         }
-        if (threadIdx.x == 0 && w.tile == 0) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
+        if (threadIdx.x == 0 && w.tile == 0 && n_tiles < w.units) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
         __syncwarp();
         first_item = false;
         w.left -= n_tiles;
@@ -522,65 +522,65 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     }
 }
 
-// Joins the parts of items that several CTAs shared: one CTA per (item, row),
-// its warps taking the parts in turn.
+// Joins the parts of items that several CTAs shared.  grid (CTA whose last
+// item goes on, 32 rows, 32 columns): a lane holds 32 columns of a row, the
+// warps take the parts in turn and are added in shared memory.
 constexpr int TC_WARPS = 4;
 template <int TYPE>
 __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeArgs g) {
-    __shared__ float so[TC_WARPS][256], sm[TC_WARPS], sl[TC_WARPS];
+    __shared__ float so[TC_WARPS][32][33], sm[TC_WARPS][32], sl[TC_WARPS][32];
     pdl_trigger();
     pdl_wait();
-    const int64_t item = blockIdx.x;
-    const int mr = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = g.p.head_dim;
-    const int b = (int)(item % g.max_blocks), kv = (int)(item / g.max_blocks % g.p.n_kv_heads);
-    const TreeSeq q = tree_seq(g, (int)(item / g.max_blocks / g.p.n_kv_heads));
-    if ((int64_t)b * g.mt + mr >= (int64_t)q.T * g.group) return;
-    const int2 d = g.desc[item];
-    const int c0 = d.x >> 1, c1 = d.y;
-    if (c0 == c1) return;
-    float m = -INFINITY, l = 0.0f, o[8];
+    const TreeShare d = g.share[blockIdx.x];
+    if (d.last < 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = g.p.head_dim;
+    const int mr = blockIdx.y * 32 + lane, col = blockIdx.z * 32;
+    const TreeSeq q = tree_seq(g, d.i);
+    const int rows = min(g.mt, q.T * g.group - d.b * g.mt);
+    if ((int)blockIdx.y * 32 >= rows) return;
+    const int at = min(mr, rows - 1), cols = min(32, hd - col);         // a multiple of 8
+    float m = -INFINITY, l = 0.0f, o[32];
 #pragma unroll
-    for (int u = 0; u < 8; u++) o[u] = 0.0f;
-    for (int c = c0 + warp; c <= c1; c += TC_WARPS) {
-        const int slot = c == c0 ? d.x : 2 * c;
-        const float *part = g.part + ((size_t)slot * g.mt + mr) * (hd + 2);
-        const float2 x = *reinterpret_cast<const float2 *>(part);
-        const float mn = fmaxf(m, x.x), ms = mn == -INFINITY ? 0.0f : mn;
-        const float f = ex2(m - ms), e = ex2(x.x - ms);
+    for (int c = 0; c < 32; c++) o[c] = 0.0f;
+    for (int k = blockIdx.x + warp; k <= d.last; k += TC_WARPS) {
+        const float *part = g.part + (size_t)(k == (int)blockIdx.x ? d.slot : 2 * k) * (hd + 2) * g.mt + at;
+        const float om = part[(size_t)hd * g.mt], ol = part[(size_t)(hd + 1) * g.mt];
+        float v[32];
+#pragma unroll
+        for (int c = 0; c < 32; c++) v[c] = c < cols ? part[(size_t)(col + c) * g.mt] : 0.0f;
+        const float mn = fmaxf(m, om), ms = mn == -INFINITY ? 0.0f : mn;
+        const float f = ex2(m - ms), e = ex2(om - ms);
         m = mn;
-        l = l * f + x.y * e;
+        l = l * f + ol * e;
 #pragma unroll
-        for (int u = 0; u < 8; u++)
-            if (lane + 32 * u < hd) o[u] = o[u] * f + part[2 + lane + 32 * u] * e;
+        for (int c = 0; c < 32; c++) o[c] = o[c] * f + v[c] * e;
     }
 #pragma unroll
-    for (int u = 0; u < 8; u++) so[warp][lane + 32 * u] = o[u];
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
-    }
+    for (int c = 0; c < 32; c++) so[warp][c][lane] = o[c];
+    sm[warp][lane] = m;
+    sl[warp][lane] = l;
     __syncthreads();
-    float top = -INFINITY, sum = 0.0f, f[TC_WARPS];
+    float top = -INFINITY, sum = 0.0f, f[TC_WARPS], y[8];
 #pragma unroll
-    for (int k = 0; k < TC_WARPS; k++) top = fmaxf(top, sm[k]);
+    for (int k = 0; k < TC_WARPS; k++) top = fmaxf(top, sm[k][lane]);
     const float ms = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int k = 0; k < TC_WARPS; k++) {
-        f[k] = ex2(sm[k] - ms);
-        sum = fmaf(sl[k], f[k], sum);
+        f[k] = ex2(sm[k][lane] - ms);
+        sum = fmaf(sl[k][lane], f[k], sum);
     }
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    const int row = b * g.mt + mr;
-    const int64_t at = (int64_t)(q.t0 + row / g.group) * g.a.ldo + (int64_t)(kv * g.group + row % g.group) * hd;
-    for (int c = threadIdx.x; c < hd; c += TC_WARPS * 32) {
-        float y = 0.0f;
+    if (mr >= rows || 8 * warp >= cols) return;
 #pragma unroll
-        for (int k = 0; k < TC_WARPS; k++) y = fmaf(so[k][c], f[k], y);
-        y *= inv;
-        if constexpr (TYPE == TR_F32) static_cast<float *>(g.a.out)[at + c] = y;
-        else if constexpr (TYPE == TR_F16) static_cast<__half *>(g.a.out)[at + c] = __float2half_rn(y);
-        else static_cast<__nv_bfloat16 *>(g.a.out)[at + c] = __float2bfloat16_rn(y);
+    for (int c = 0; c < 8; c++) {
+        float x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < TC_WARPS; k++) x = fmaf(so[k][8 * warp + c][lane], f[k], x);
+        y[c] = x * inv;
     }
+    const int row = d.b * g.mt + mr;
+    const int64_t dst = (int64_t)(q.t0 + row / g.group) * g.a.ldo + (d.g * g.group + row % g.group) * hd + col + 8 * warp;
+    tree_store8<TYPE>(g, dst, y);
 }
 
 // -------------------------------------------------------------------- host
@@ -600,25 +600,23 @@ static int tree_fit(TreeArgs &g, size_t &smem) {
     return MT;
 }
 
-// The parts and the description of every item of a call.
+// Two parts for each CTA, and what its last item is.
 int tree_workspace(vb_ctx *ctx, TreeArgs &g) {
-    g.max_blocks = (int)(((int64_t)g.a.max_tokens * g.group + g.mt - 1) / g.mt);
-    const int64_t items = (int64_t)g.a.n * g.p.n_kv_heads * g.max_blocks;
-    if (items > INT32_MAX) return set_error(ctx, VB_ERR_INVALID_ARG, "vb_tree_attention: too many rows");
     const size_t parts = (size_t)2 * ctx->sm_count * g.mt * (g.p.head_dim + 2) * sizeof(float);
-    int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)items * sizeof(int2));
+    int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)ctx->sm_count * sizeof(TreeShare));
     if (rc) return rc;
     g.part = static_cast<float *>(ctx->tree_ws.ptr);
-    g.desc = reinterpret_cast<int2 *>(static_cast<char *>(ctx->tree_ws.ptr) + parts);
+    g.share = reinterpret_cast<TreeShare *>(static_cast<char *>(ctx->tree_ws.ptr) + parts);
     return VB_OK;
 }
 
 int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g) {
-    const int64_t items = (int64_t)g.a.n * g.p.n_kv_heads * g.max_blocks;
     auto kernel = g.a.type == VB_TYPE_F32   ? tree_combine_kernel<TR_F32>
                   : g.a.type == VB_TYPE_F16 ? tree_combine_kernel<TR_F16>
                                             : tree_combine_kernel<TR_BF16>;
-    VB_CHECK(ctx, pdl_launch(ctx, kernel, dim3((unsigned)items, g.mt), dim3(TC_WARPS * 32), 0, g));
+    const int64_t rows = std::min<int64_t>(g.mt, (int64_t)g.a.max_tokens * g.group);
+    VB_CHECK(ctx, pdl_launch(ctx, kernel, dim3(ctx->sm_count, (unsigned)((rows + 31) / 32), (g.p.head_dim + 31) / 32),
+                             dim3(TC_WARPS * 32), 0, g));
     VB_LAUNCH_CHECK(ctx, "tree_combine");
     return VB_OK;
 }

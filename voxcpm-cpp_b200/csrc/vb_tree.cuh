@@ -16,13 +16,12 @@ struct TreeArgs {
     float scale_log2;                // scale * log2(e): the softmax runs in powers of two
     int group;                       // query heads per K/V head
     int mt;                          // rows per block
-    int max_blocks;                  // blocks of the longest draft
     int kt;                          // cache rows per tile
     int stages;
     int vec;                         // 16-byte accesses of q and out
     int *err;
-    float *part;                     // [2 * CTAs][mt][head_dim + 2]
-    int2 *desc;                      // [n][n_kv][max_blocks] CTAs of an item
+    float *part;                     // [2 * CTAs][head_dim + 2][mt]: sums, then the maximum and the sum of the weights
+    struct TreeShare *share;         // [CTAs]
 };
 
 // Sequence i of the call.  T = 0: no rows of q (or none that can be named);
@@ -56,7 +55,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &g, int i) {
 }
 
 __device__ __forceinline__ int tree_blocks(const TreeArgs &g, const TreeSeq &q) {
-    return (int)(((int64_t)q.T * g.group + g.mt - 1) / g.mt);
+    return (q.T * g.group + g.mt - 1) / g.mt;
 }
 
 // Rows of the cache that block b of a sequence reads, and its units (at
@@ -64,7 +63,12 @@ __device__ __forceinline__ int tree_blocks(const TreeArgs &g, const TreeSeq &q) 
 __device__ __forceinline__ int tree_visible(const TreeArgs &g, const TreeSeq &q, int b) {
     if (q.bad) return 0;
     if (g.a.mask) return q.len;
-    return q.base + (int)min((int64_t)q.T, (((int64_t)b + 1) * g.mt + g.group - 1) / g.group);
+    return q.base + min(q.T, ((b + 1) * g.mt + g.group - 1) / g.group);
+}
+
+// Of those, the rows that every token of the block sees.
+__device__ __forceinline__ int tree_clear(const TreeArgs &g, const TreeSeq &q, int b) {
+    return g.a.mask || q.bad ? q.base : q.base + b * g.mt / g.group + 1;
 }
 
 __device__ __forceinline__ int tree_units(const TreeArgs &g, int visible) { return max(1, (visible + g.kt - 1) / g.kt); }
@@ -80,12 +84,13 @@ __device__ __forceinline__ int64_t tree_seq_units(const TreeArgs &g, const TreeS
 // A place in the line of units: the item (i, kv head, block) and the tile.
 struct TreeWalk {
     TreeSeq q;
-    int i, g, b, nb, visible, units, tile;
+    int i, g, b, nb, visible, clear, units, tile;
     int64_t left;                    // units of this CTA from here on
 };
 
 __device__ __forceinline__ void tree_item(const TreeArgs &g, TreeWalk &w) {
     w.visible = tree_visible(g, w.q, w.b);
+    w.clear = tree_clear(g, w.q, w.b);
     w.units = tree_units(g, w.visible);
 }
 
@@ -154,6 +159,7 @@ __device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWal
             at += u;
         }
     }
+    if (threadIdx.x == 0) g.share[blockIdx.x].last = -1;
     __syncthreads();
     w.left = u1 - u0;
     if (w.left <= 0) return;
@@ -178,12 +184,16 @@ __device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWal
     w.tile = (int)off;
 }
 
-// The CTA that holds an item's first unit (`at`) says which hold the rest.
+// An item that goes on in the next CTAs: described by the CTA that holds its
+// first unit (`at`), as its last item.
+struct TreeShare {
+    int i, g, b, slot, last, pad[3];        // last: the CTA of its last unit; -1: no such item
+};
+
 __device__ __forceinline__ void tree_describe(const TreeArgs &g, const TreeWalk &w, int64_t at, int64_t total,
                                               int64_t ctas, bool first_item) {
     const int64_t end = at + w.units - 1;
-    g.desc[((int64_t)w.i * g.p.n_kv_heads + w.g) * g.max_blocks + w.b] =
-        make_int2((int)blockIdx.x * 2 + (first_item ? 0 : 1), (int)(((end + 1) * ctas - 1) / total));
+    g.share[blockIdx.x] = {w.i, w.g, w.b, (int)blockIdx.x * 2 + (first_item ? 0 : 1), (int)(((end + 1) * ctas - 1) / total), {}};
 }
 
 // Whether token j of the sequence sees draft row d (0 <= d < T).
@@ -238,23 +248,34 @@ __device__ __forceinline__ void tree_wait_warp(uint64_t *bar, uint32_t parity, v
     __syncwarp();
 }
 
-// Values of the draft that are not finite are taken out of the tiles (a zero
-// weight times infinity would reach tokens that do not see them).  This adds
-// up those that token j does see among cache rows lo .. hi-1 in column c:
-// zero, or the infinity or NaN that its result is.
+// Values of draft rows that are not finite are taken out of the tiles that
+// not every token sees (a zero weight times infinity would reach those that
+// do not).  This puts them back: in result columns c0 .. c1-1 of token j, dst
+// (`stride` apart) becomes the sum of those that the token does see among
+// cache rows lo .. hi-1 (not before the draft), where it sees any.  P: how a
+// result is stored.  Rare, and kept out of the kernels' code for that.
 template <int TYPE>
-__device__ __noinline__ float tree_not_finite(const TreeArgs *g, const TreeSeq *q, int kv, int j, int lo, int hi, int c) {
-    float sum = 0.0f;
-    for (int r = max(lo, q->base); r < hi; r++) {
-        if (!tree_sees(*g, *q, j, r - q->base)) continue;
-        int page = g->p.table[(int64_t)q->s * g->p.max_pages + r / g->p.page_rows];
-        if (page < 0 || page >= g->p.n_pages) page = 0;
-        const int64_t at = ((((int64_t)g->a.layer * g->p.n_pages + page) * g->p.n_kv_heads + kv) * g->p.page_rows +
-                            r % g->p.page_rows) * g->p.head_dim + c;
-        const float v = unpack<TYPE>(static_cast<const uint16_t *>(g->p.v)[at]);
-        if (!isfinite(v)) sum += v;
+__device__ __noinline__ void tree_not_finite(const TreeArgs *g, int t0, int s, int base, int kv, int j, int lo, int hi, int c0,
+                                             int c1, void *dst, int64_t stride, int as_float) {
+    for (int c = c0; c < c1; c++) {
+        float sum = 0.0f;
+        bool any = false;
+        for (int r = lo; r < hi; r++) {
+            const int d = r - base;
+            if (!(g->a.mask ? g->a.mask[(int64_t)(t0 + j) * g->a.mask_words + (d >> 5)] >> (d & 31) & 1u : d <= j)) continue;
+            int page = g->p.table[(int64_t)s * g->p.max_pages + r / g->p.page_rows];
+            if (page < 0 || page >= g->p.n_pages) page = 0;
+            const int64_t at = ((((int64_t)g->a.layer * g->p.n_pages + page) * g->p.n_kv_heads + kv) * g->p.page_rows +
+                                r % g->p.page_rows) * g->p.head_dim + c;
+            const float v = unpack<TYPE>(static_cast<const uint16_t *>(g->p.v)[at]);
+            if (isfinite(v)) continue;
+            sum += v;
+            any = true;
+        }
+        if (!any) continue;
+        if (as_float) static_cast<float *>(dst)[c * stride] = sum;
+        else static_cast<uint16_t *>(dst)[c * stride] = (uint16_t)pack2<TYPE>(sum, 0.0f);
     }
-    return sum;
 }
 
 // 16 bytes of V with the values that are not finite set to zero; found: there were some.
@@ -274,6 +295,31 @@ __device__ __forceinline__ uint4 tree_finite(uint4 v, bool &found) {
         }
     }
     return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
+// Eight results of a row, at element `at` of the output.
+template <int TYPE>
+__device__ __forceinline__ void tree_store8(const TreeArgs &g, int64_t at, const float (&y)[8]) {
+    if constexpr (TYPE == TR_F32) {
+        float *dst = static_cast<float *>(g.a.out) + at;
+        if (g.vec) {
+            reinterpret_cast<float4 *>(dst)[0] = make_float4(y[0], y[1], y[2], y[3]);
+            reinterpret_cast<float4 *>(dst)[1] = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; c++) dst[c] = y[c];
+        }
+    } else {
+        uint16_t *dst = static_cast<uint16_t *>(g.a.out) + at;
+        uint32_t z[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) z[c] = pack2<TYPE>(y[2 * c], y[2 * c + 1]);
+        if (g.vec) *reinterpret_cast<uint4 *>(dst) = make_uint4(z[0], z[1], z[2], z[3]);
+        else {
+#pragma unroll
+            for (int c = 0; c < 8; c++) dst[c] = (uint16_t)(z[c >> 1] >> (16 * (c & 1)));
+        }
+    }
 }
 
 int launch_tree_tc(vb_ctx *ctx, TreeArgs &g);

@@ -81,6 +81,63 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// A load whose wait comes later: until then nothing may touch the registers,
+// so the wait takes them all as its operands.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// Pairs of fp32 values in one 64-bit register.
+__device__ __forceinline__ uint64_t pack_b32x2(uint32_t a, uint32_t b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) { return pack_b32x2(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void unpack_f32x2(uint64_t d, float &a, float &b) {
+    uint32_t x, y;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(d));
+    a = __uint_as_float(x);
+    b = __uint_as_float(y);
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 // The ring holds K and V tiles in the order in which the MMAs use them:
 // PAIR K0 V0 K1 V1 ..., else K0 K1 V0 K2 V1 ... V(n-1).
 template <bool PAIR>
@@ -149,11 +206,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
     tree_cut<TT_THREADS>(g, cut, w, u1, total, ctas);
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + HDP};
+    // tensor memory: scores (then weights) of stream t at column 128 t, sums at 256 + HDP t
     const int n_slots = g.stages;
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8) {
             // -------------------------------------------------------- loads
             const int P = g.p.page_rows, box = min(P, TT_KT);
@@ -213,68 +269,54 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             }
         } else if (warp == 9 && lane == 0) {
             // --------------------------------------------------------- MMAs
-            const int hd = g.p.head_dim, k_steps = (hd + 15) / 16;
             const uint32_t fmt = TYPE == TR_F16 ? 0u : 1u;
-            const uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
-            const uint32_t id_s = common | ((uint32_t)(TT_KT >> 3) << 17);
-            const uint32_t id_o = common | (1u << 16) | ((uint32_t)(k_steps * 16 >> 3) << 17);     // V: rows along k
+            constexpr uint32_t N_S = (uint32_t)(TT_KT >> 3) << 17, N_O = (uint32_t)(HDP >> 3) << 17;
+            const uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24) | N_S;
+            const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24) | N_O | (1u << 16);   // V: rows along k
+            const uint64_t d_q = sw128_desc(qs), d_k = sw128_desc(ring), d_v = sw128_desc_mn(smem_u32(ring));
             int pos = 0, item = 0;
-            int done[2] = {0, 0};                     // tiles whose P was taken, per stream
+            uint32_t phase = 0;                       // parity of p_full, a bit per stream
             auto wait_ring = [&](int at) {
                 tree_wait(&full[at % n_slots], (uint32_t)(at / n_slots) & 1u, &abort_flag, g.err);
                 tc_fence_after();
             };
-            auto scores = [&](int t, int at) {
-                const uint8_t *k = ring + (size_t)(at % n_slots) * SLOT, *q = qs + (PAIR ? t * SLOT : 0);
-                for (int i = 0; i < k_steps; i++)
-                    umma_f16(t_s[t], sw128_desc(q + (i >> 2) * BLOCK + (i & 3) * 32),
-                             sw128_desc(k + (i >> 2) * BLOCK + (i & 3) * 32), id_s, i > 0);
-                umma_commit(&s_full[t]);
-            };
-            auto values = [&](int t, int at, bool first) {
-                tree_wait(&p_full[t], (uint32_t)done[t]++ & 1u, &abort_flag, g.err);
-                tc_fence_after();
-                const uint32_t v = smem_u32(ring + (size_t)(at % n_slots) * SLOT);
-#pragma unroll
-                for (int i = 0; i < TT_KT / 16; i++)
-                    umma_f16_ts(t_o[t], t_s[t] + 8 * i, sw128_desc_mn(v + i * 2048), id_o, !(first && i == 0));
-                umma_commit(&pv_done[t]);
-            };
+            // One place of the pipeline: the values of tile j, then the scores of
+            // the tile that stream t takes next.
             while (w.left > 0) {
                 const int n = (int)min((int64_t)(w.units - w.tile), w.left);
                 tree_wait(&q_full, (uint32_t)item & 1u, &abort_flag, g.err);
                 tc_fence_after();
-                for (int j = 0; j < (PAIR ? 1 : min(2, n)); j++) {
-                    const int at = pos + ring_k<PAIR>(j);
-                    wait_ring(at);
-                    scores(j, at);
-                    if (PAIR) scores(1, at);
-                    umma_commit(&empty[at % n_slots]);
-                }
-                for (int j = 0; j < n; j++) {
-                    const int at = pos + ring_v<PAIR>(j, n), next = pos + ring_k<PAIR>(j + (PAIR ? 1 : 2));
-                    const bool more = j + (PAIR ? 1 : 2) < n;
-                    wait_ring(at);
-                    if (PAIR) {
-                        values(0, at, j == 0);
-                        if (more) {
-                            wait_ring(next);
-                            scores(0, next);
+                constexpr int AHEAD = PAIR ? 1 : 2;
+#pragma unroll 1
+                for (int x = -2; x < (PAIR ? 2 * n : n); x++) {
+                    const int j = PAIR ? x >> 1 : x, t = x & 1, next = j + AHEAD;
+                    if (j >= 0) {
+                        const int at = pos + ring_v<PAIR>(j, n), slot = at % n_slots;
+                        if (!PAIR || t == 0) wait_ring(at);
+                        tree_wait(&p_full[t], phase >> t & 1u, &abort_flag, g.err);
+                        phase ^= 1u << t;
+                        tc_fence_after();
+                        const uint64_t v = d_v + (uint64_t)(slot * (SLOT >> 4));
+                        const uint32_t p = tmem + 128 * t, o = tmem + 256 + HDP * t;
+                        const uint32_t more = PAIR ? j > 0 : j > 1;
+#pragma unroll
+                        for (int i = 0; i < TT_KT / 16; i++)
+                            umma_f16_ts(o, p + 8 * i, v + (uint64_t)(i * (2048 >> 4)), id_o, i ? 1u : more);
+                        umma_commit(&pv_done[t]);
+                        if (!PAIR || t == 1) umma_commit(&empty[slot]);
+                    }
+                    if (next >= 0 && next < n) {
+                        const int at = pos + ring_k<PAIR>(next), slot = at % n_slots;
+                        if (!PAIR || t == 0) wait_ring(at);
+                        const uint64_t k = d_k + (uint64_t)(slot * (SLOT >> 4)), q = d_q + (uint64_t)(PAIR ? t * (SLOT >> 4) : 0);
+                        const uint32_t sc = tmem + 128 * t;
+#pragma unroll
+                        for (int i = 0; i < HDP / 16; i++) {
+                            const uint64_t off = (i >> 2) * (BLOCK >> 4) + (i & 3) * 2;
+                            umma_f16(sc, q + off, k + off, id_s, i ? 1u : 0u);
                         }
-                        values(1, at, j == 0);
-                        umma_commit(&empty[at % n_slots]);
-                        if (more) {
-                            scores(1, next);
-                            umma_commit(&empty[next % n_slots]);
-                        }
-                    } else {
-                        values(j & 1, at, j < 2);
-                        umma_commit(&empty[at % n_slots]);
-                        if (more) {
-                            wait_ring(next);
-                            scores(j & 1, next);
-                            umma_commit(&empty[next % n_slots]);
-                        }
+                        umma_commit(&s_full[t]);
+                        if (!PAIR || t == 1) umma_commit(&empty[slot]);
                     }
                 }
                 pos += 2 * n;
@@ -287,7 +329,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
         }
     } else {
         // -------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = warp >> 2, tid = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // TMEM lane of the warp's first row
         const int hd = g.p.head_dim;
@@ -295,7 +336,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
         bool first_item = true;
         while (w.left > 0) {
             const int n = (int)min((int64_t)(w.units - w.tile), w.left);
-            const int rows = (int)min((int64_t)MT, (int64_t)w.q.T * g.group - (int64_t)w.b * MT);
+            const int rows = min(MT, w.q.T * g.group - w.b * MT);
             // the queries of this stream's row tile (of half of the one tile)
             {
                 uint8_t *qt = qs + (PAIR ? t * SLOT : 0);
@@ -303,7 +344,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     const int r = e / (HDP / 8), c = e % (HDP / 8), m = (PAIR ? 128 * t : 0) + r;
                     uint4 x = make_uint4(0, 0, 0, 0);
                     if (m < rows && 8 * c < hd) {
-                        const int64_t row = (int64_t)w.b * MT + m;
+                        const int row = w.b * MT + m;
                         const uint16_t *src = static_cast<const uint16_t *>(g.a.q) + (w.q.t0 + row / g.group) * g.a.ldq +
                                               (w.g * g.group + row % g.group) * hd + 8 * c;
                         if (g.vec) x = *reinterpret_cast<const uint4 *>(src);
@@ -319,13 +360,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             }
             const int mrow = (PAIR ? 128 * t : 0) + 32 * (warp & 3) + lane;      // this thread's row of the block
             const bool alive = mrow - lane < rows;                               // the warp has rows
-            const int j = mrow < rows ? (int)(((int64_t)w.b * MT + mrow) / g.group) : -1;
+            const int j = mrow < rows ? (w.b * MT + mrow) / g.group : -1;
             float m = -INFINITY, l = 0.0f;
             const int mine = PAIR ? n : (n + 1 - t) / 2;                         // tiles of this stream
             for (int x = 0; x < mine; x++, seen++) {
                 const int jt = PAIR ? x : 2 * x + t;
                 const int r0 = (w.tile + jt) * TT_KT;
-                const bool edge = r0 + TT_KT > w.q.base;
+                const bool edge = r0 + TT_KT > w.clear;          // not every row is seen by every token
                 if (edge && (t == 0 || !PAIR)) {
                     // V rows past the end may hold anything: they become zeros,
                     // as do draft values that are not finite
@@ -333,7 +374,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     tree_wait_warp(&full[at % n_slots], (uint32_t)(at / n_slots) & 1u, &abort_flag, g.err);
                     uint8_t *v = ring + (size_t)(at % n_slots) * SLOT;
                     bool found = false;
-                    const int from = max(0, w.q.base - r0);
+                    const int from = max(0, w.clear - r0);
                     for (int e = from * CB * 8 + tid; e < TT_KT * CB * 8; e += 128) {
                         const int r = e / (CB * 8), c = e % (CB * 8);
                         uint4 *p = reinterpret_cast<uint4 *>(v + (c >> 3) * BLOCK + sw128(r, c & 7));
@@ -352,16 +393,16 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 tree_wait_warp(&s_full[t], (uint32_t)seen & 1u, &abort_flag, g.err);
                 tc_fence_after();
                 if (alive) {
-                    float s[4][32];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) tmem_ld32(t_s[t] + lanes + 32 * k, s[k]);
+                    const uint32_t sc = tmem + 128 * t + lanes;
+                    // columns that this row does not see, 32 to a word
+                    uint32_t gone[4] = {};
                     if (edge) {
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const int d = r0 + 32 * k - w.q.base;                // draft place of the first column
                             int lim = w.visible - (r0 + 32 * k);
                             uint32_t bits = 0xffffffffu;
-                            if (!g.a.mask) lim = min(lim, d < 0 && j >= 0 ? max(0, j + 1 - d) : j + 1 - d);
+                            if (!g.a.mask) lim = min(lim, j + 1 - d);
                             else if (d > -32 && j >= 0) {
                                 const uint32_t *row = g.a.mask + (int64_t)(w.q.t0 + j) * g.a.mask_words;
                                 if (d < 0) bits = (row[0] << -d) | ((1u << -d) - 1u);
@@ -374,20 +415,39 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                             }
                             if (j < 0 || lim <= 0) bits = 0u;
                             else if (lim < 32) bits &= (1u << lim) - 1u;
-#pragma unroll
-                            for (int c = 0; c < 32; c++)
-                                if (!(bits >> c & 1u)) s[k][c] = -INFINITY;
+                            gone[k] = ~bits;
                         }
                     }
-                    float top[4];
+                    // two passes over the row in pieces of 32, the next piece on
+                    // its way from tensor memory while one is worked on: the
+                    // maximum, then the weights
+                    uint32_t a[32], b[32];
+                    float top = -INFINITY;
+                    auto piece_max = [&](uint32_t (&x)[32], uint32_t out) {
+                        if (edge)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        top[k] = s[k][0];
+                            for (int c = 0; c < 32; c++)
+                                if (out >> c & 1u) x[c] = 0xff800000u;
+                        float u = top, v = __uint_as_float(x[0]);
 #pragma unroll
-                        for (int c = 1; c < 31; c += 2) top[k] = fmaxf(top[k], fmaxf(s[k][c], s[k][c + 1]));
-                        top[k] = fmaxf(top[k], s[k][31]);
+                        for (int c = 1; c < 31; c += 2) {
+                            float &z = (c >> 1) & 1 ? v : u;
+                            z = fmaxf(z, fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 1])));
+                        }
+                        top = fmaxf(fmaxf(u, v), __uint_as_float(x[31]));
+                    };
+                    tmem_ld32_start(sc, a);
+                    tmem_ld32_wait(a);
+#pragma unroll 1
+                    for (int k = 0; k < 4; k += 2) {
+                        tmem_ld32_start(sc + 32 * k + 32, b);
+                        piece_max(a, k ? gone[2] : gone[0]);
+                        tmem_ld32_wait(b);
+                        tmem_ld32_start(sc + (k ? 0 : 64), a);          // after the last: the first again, for the weights
+                        piece_max(b, k ? gone[3] : gone[1]);
+                        tmem_ld32_wait(a);
                     }
-                    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * g.scale_log2;
+                    const float now = top * g.scale_log2;
                     const bool move = now > m + TT_SLACK || (m == -INFINITY && now > m);
                     if (x == 0) m = now;
                     else if (__any_sync(0xffffffffu, move)) {
@@ -396,32 +456,48 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                         l *= f;
                         tree_wait_warp(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
                         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (int k = 0; k < HDP / 32; k++) {
                             float o[32];
                             uint32_t y[32];
-                            tmem_ld32(t_o[t] + lanes + 32 * k, o);
+                            tmem_ld32(tmem + 256 + HDP * t + lanes + 32 * k, o);
 #pragma unroll
                             for (int c = 0; c < 32; c++) y[c] = __float_as_uint(o[c] * f);
-                            tmem_st32(t_o[t] + lanes + 32 * k, y);
+                            tmem_st32(tmem + 256 + HDP * t + lanes + 32 * k, y);
                         }
                     }
-                    const float off = m == -INFINITY ? 0.0f : m;
-                    float sum[4] = {};
+                    const float off = m == -INFINITY ? 0.0f : -m;
+                    const uint64_t off2 = pack_f32x2(off, off), scale2 = pack_f32x2(g.scale_log2, g.scale_log2);
+                    uint64_t sum2 = 0;
+                    auto piece_exp = [&](uint32_t (&x)[32], uint32_t out, uint32_t dst) {
+                        if (edge)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t y[32];
+                            for (int c = 0; c < 32; c++)
+                                if (out >> c & 1u) x[c] = 0xff800000u;
+                        uint32_t y[16];
 #pragma unroll
-                        for (int c = 0; c < 32; c++) {
-                            const float p0 = ex2(fmaf(s[2 * h + (c >> 4)][2 * (c & 15)], g.scale_log2, -off));
-                            const float p1 = ex2(fmaf(s[2 * h + (c >> 4)][2 * (c & 15) + 1], g.scale_log2, -off));
-                            sum[2 * h] += p0;
-                            sum[2 * h + 1] += p1;
+                        for (int c = 0; c < 16; c++) {
+                            float p0, p1;
+                            unpack_f32x2(fma_f32x2(pack_b32x2(x[2 * c], x[2 * c + 1]), scale2, off2), p0, p1);
+                            p0 = ex2(p0);
+                            p1 = ex2(p1);
+                            sum2 = add_f32x2(sum2, pack_f32x2(p0, p1));
                             y[c] = pack2<TYPE>(p0, p1);
                         }
-                        tmem_st32(t_s[t] + lanes + 32 * h, y);
+                        tmem_st16(dst, y);
+                    };
+#pragma unroll 1
+                    for (int k = 0; k < 4; k += 2) {
+                        tmem_ld32_start(sc + 32 * k + 32, b);
+                        piece_exp(a, k ? gone[2] : gone[0], sc + 16 * k);
+                        tmem_ld32_wait(b);
+                        tmem_ld32_start(sc + 64, a);                    // (not used after the last)
+                        piece_exp(b, k ? gone[3] : gone[1], sc + 16 * k + 16);
+                        tmem_ld32_wait(a);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    float s0, s1;
+                    unpack_f32x2(sum2, s0, s1);
+                    l += s0 + s1;
                     tmem_st_wait();
                 }
                 tc_fence_before();
@@ -447,55 +523,54 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             tc_fence_after();
             const bool mend = *(volatile int *)&not_finite[item & 1] == item;
             if (alive) {
-                const int64_t row = (int64_t)w.b * MT + mrow;
-                const int head = w.g * g.group + (int)(row % g.group);
+                const int row = w.b * MT + mrow;
+                const int64_t out = (int64_t)(w.q.t0 + row / g.group) * g.a.ldo + (w.g * g.group + row % g.group) * hd;
                 const float inv = whole ? (l > 0.0f || l != l ? 1.0f / l : 0.0f) : 1.0f;
-                float *part = g.part + ((size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * MT + mrow) * (hd + 2);
-                uint16_t *out = static_cast<uint16_t *>(g.a.out) + (w.q.t0 + row / g.group) * g.a.ldo + (int64_t)head * hd;
-                if (!whole && j >= 0 && (PAIR || t == 0)) *reinterpret_cast<float2 *>(part) = make_float2(m, l);
+                float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * (hd + 2) * MT + mrow;
+                if (!whole && (PAIR || t == 0)) {
+                    part[(size_t)hd * MT] = m;
+                    part[(size_t)(hd + 1) * MT] = l;
+                }
                 // PAIR: all columns of the thread's row; else half of them, of both streams
-#pragma unroll
-                for (int k = 0; k < (PAIR ? HDP / 32 : HDP / 64); k++) {
-                    const int c0 = 32 * (PAIR ? k : t * (HDP / 64) + k);
+                const int c_lo = PAIR ? 0 : t * (HDP / 2), c_hi = min(hd, PAIR ? HDP : c_lo + HDP / 2);
+                f0 *= inv;
+                f1 *= inv;
+#pragma unroll 1
+                for (int c0 = c_lo; c0 < c_hi; c0 += 32) {
                     float o[32];
-                    tmem_ld32(t_o[PAIR ? t : 0] + lanes + c0, o);
-                    if (!PAIR) {
+                    tmem_ld32(tmem + 256 + (PAIR ? HDP * t : 0) + lanes + c0, o);
+                    if (!PAIR && n > 1) {
                         float o1[32];
-                        if (n > 1) tmem_ld32(t_o[1] + lanes + c0, o1);
+                        tmem_ld32(tmem + 256 + HDP + lanes + c0, o1);
 #pragma unroll
-                        for (int c = 0; c < 32; c++) o[c] = n > 1 ? o[c] * f0 + o1[c] * f1 : o[c] * f0;
+                        for (int c = 0; c < 32; c++) o[c] = o[c] * f0 + o1[c] * f1;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; c++) o[c] *= f0;
                     }
-                    if (mend && j >= 0)
-#pragma unroll
-                        for (int c = 0; c < 32; c++)
-                            if (c0 + c < hd)
-                                o[c] += tree_not_finite<TYPE>(&g, &w.q, w.g, j, w.tile * TT_KT,
-                                                              min(w.visible, (w.tile + n) * TT_KT), c0 + c);
                     if (j < 0) continue;
                     if (!whole) {
 #pragma unroll
-                        for (int c = 0; c < 32; c += 2)
-                            if (c0 + c < hd) *reinterpret_cast<float2 *>(part + 2 + c0 + c) = make_float2(o[c], o[c + 1]);
+                        for (int c = 0; c < 32; c++)
+                            if (c0 + c < hd) part[(size_t)(c0 + c) * MT] = o[c];
                     } else {
 #pragma unroll
                         for (int c = 0; c < 32; c += 8) {
-                            if (c0 + c >= hd) continue;
-                            const uint4 y = make_uint4(pack2<TYPE>(o[c] * inv, o[c + 1] * inv), pack2<TYPE>(o[c + 2] * inv, o[c + 3] * inv),
-                                                       pack2<TYPE>(o[c + 4] * inv, o[c + 5] * inv), pack2<TYPE>(o[c + 6] * inv, o[c + 7] * inv));
-                            uint16_t *dst = out + c0 + c;
-                            if (g.vec) *reinterpret_cast<uint4 *>(dst) = y;
-                            else {
-                                const uint32_t z[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                                for (int i = 0; i < 8; i++) dst[i] = (uint16_t)(z[i >> 1] >> (16 * (i & 1)));
-                            }
+                            const float y[8] = {o[c], o[c + 1], o[c + 2], o[c + 3], o[c + 4], o[c + 5], o[c + 6], o[c + 7]};
+                            if (c0 + c < hd) tree_store8<TYPE>(g, out + c0 + c, y);
                         }
                     }
                 }
+                if (mend && j >= 0) {
+                    const int lo = max(w.clear, w.tile * TT_KT), hi = min(w.visible, (w.tile + n) * TT_KT);
+                    void *dst = whole ? static_cast<void *>(static_cast<uint16_t *>(g.a.out) + out) : part;
+                    tree_not_finite<TYPE>(&g, w.q.t0, w.q.s, w.q.base, w.g, j, lo, hi, c_lo, c_hi, dst, whole ? 1 : MT, !whole);
+                }
             }
+            __syncwarp();
             tc_fence_before();
             if (!PAIR) consumer_sync(256);           // both streams' sums are read: the next item may overwrite them
-            if (threadIdx.x == 0 && w.tile == 0) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
+            if (threadIdx.x == 0 && w.tile == 0 && !whole) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
             __syncwarp();
             first_item = false;
             pos += 2 * n;
