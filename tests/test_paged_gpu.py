@@ -520,6 +520,9 @@ def check_tree(ctx, t):
     ([333], [100], 16, 2, 128, 1024, "tree"),
     ([2500], [3], 16, 2, 128, 32, "tree"),
     ([600, 2000, 100], [70, 16, 17], 16, 1, 64, 16, "tree"),       # 16 heads on one
+    ([100, 37], [3, 2], 72, 1, 64, 16, "tree"),                    # more heads on one than a block has rows
+    ([90, 200, 16], [2, 1, 16], 300, 1, 32, 16, "any"),
+    ([1000], [37], 24, 2, 128, 32, "chain"),                       # blocks of whole tokens, not of a power of two
 ])
 def test_tree_attention(ctx, type, lens, drafted, nh, nkv, hd, P, mask):
     check_tree(ctx, tree_case(ctx, type, lens, drafted, nh, nkv, hd, P, mask))
@@ -533,6 +536,17 @@ def test_tree_many_tiles_for_each_cta(ctx, type, lens, drafted, P):
     for _ in range(8):
         ctx.tree_attention(t["args"])
     check_tree(ctx, t)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_tree_many_sequences_and_long_chains(ctx, type):
+    rng = np.random.default_rng(1)
+    lens = rng.integers(0, 60, 900)
+    check_tree(ctx, tree_case(ctx, type, lens.tolist(), [int(min(x, d)) for x, d in zip(lens, rng.integers(0, 9, 900))], 2, 1, 8, 16, seed=1))
+    # more blocks of tokens than threads in a CTA, in the middle of other sequences
+    check_tree(ctx, tree_case(ctx, type, [40, 3300, 9], [4, 3250, 9], 8, 1, 8, 16, "chain", seed=2))
+    if type == "bf16":
+        check_tree(ctx, tree_case(ctx, type, [3100], [3100], 256, 1, 8, 64, "chain", seed=3))
 
 
 @pytest.mark.parametrize("type", ["f32", "bf16"])

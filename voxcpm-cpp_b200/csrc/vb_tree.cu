@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     pdl_wait();
 
     TreeWalk w;
-    int64_t u1, total, ctas;
-    tree_cut<TR_THREADS>(g, cut, w, u1, total, ctas);
+    TreeLine line;
+    tree_cut<TR_THREADS>(g, cut, w, line);
     if (w.left <= 0) return;
 
     if (warp >= 8) {
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         const int P = g.p.page_rows, box = min(P, TR_KT), boxes = TR_KT / box;
         int it = 0;
         while (w.left > 0) {
-            const int n_tiles = (int)min((int64_t)(w.units - w.tile), w.left);
+            const int n_tiles = min(w.units - w.tile, w.left);
             const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
             int pages = 0;                              // lane's page of the current 32 boxes
             for (int x = 0; x < n_tiles; x++, it++) {
@@ -173,39 +173,49 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     int it = 0;
     bool first_item = true;
     while (w.left > 0) {
-        const int n_tiles = (int)min((int64_t)(w.units - w.tile), w.left);
+        const int n_tiles = min(w.units - w.tile, w.left);
         const bool whole = w.tile == 0 && n_tiles == w.units;
-        const int rows = min(MT, w.q.T * g.group - w.b * MT);           // rows of the block that exist
+        const int rows = w.rows;                                        // rows of the block that exist
         // queries of the block, in 16-bit terms
-        for (int e = threadIdx.x; e < MT * (HDP / 4); e += 256) {
-            const int m = e / (HDP / 4), d = e % (HDP / 4) * 4;
-            float x[4] = {};
-            if (m < rows && d < hd) {
-                const int row = w.b * MT + m, j = row / g.group;
-                const int64_t at = (int64_t)(w.q.t0 + j) * g.a.ldq + (int64_t)(w.g * g.group + row % g.group) * hd + d;
-                if constexpr (TYPE == TR_F32) {
-                    const float *src = static_cast<const float *>(g.a.q) + at;
-                    if (g.vec) *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(src);
-                    else
-                        for (int c = 0; c < 4; c++) x[c] = src[c];
-                } else {
-                    const uint16_t *src = static_cast<const uint16_t *>(g.a.q) + at;
-                    uint16_t h[4];
-                    if (g.vec) *reinterpret_cast<uint2 *>(h) = *reinterpret_cast<const uint2 *>(src);
-                    else
-                        for (int c = 0; c < 4; c++) h[c] = src[c];
-                    *reinterpret_cast<uint2 *>(qs + m * QPITCH + d * 2) = *reinterpret_cast<uint2 *>(h);
+        constexpr int N_Q = (MT * (HDP / 4) + 255) / 256;          // four values each
+#pragma unroll
+        for (int i0 = 0; i0 < N_Q; i0 += 4) {
+            float x[4][4];
+            uint2 y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = threadIdx.x + 256 * (i0 + i), m = e / (HDP / 4), d = e % (HDP / 4) * 4;
+                x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+                y[i] = make_uint2(0, 0);
+                if (i0 + i < N_Q && m < rows && d < hd) {
+                    const int64_t at = tree_row(g, w.q.t0, w.tok, w.heads, w.head, m, g.a.ldq) + d;
+                    if constexpr (TYPE == TR_F32) {
+                        const float *src = static_cast<const float *>(g.a.q) + at;
+                        if (g.vec) *reinterpret_cast<float4 *>(x[i]) = *reinterpret_cast<const float4 *>(src);
+                        else
+#pragma unroll
+                            for (int c = 0; c < 4; c++) x[i][c] = src[c];
+                    } else {
+                        const uint16_t *src = static_cast<const uint16_t *>(g.a.q) + at;
+                        if (g.vec) y[i] = *reinterpret_cast<const uint2 *>(src);
+                        else y[i] = make_uint2(src[0] | (uint32_t)src[1] << 16, src[2] | (uint32_t)src[3] << 16);
+                    }
                 }
-            } else if constexpr (TYPE != TR_F32) {
-                *reinterpret_cast<uint2 *>(qs + m * QPITCH + d * 2) = make_uint2(0, 0);
             }
-            if constexpr (TYPE == TR_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = threadIdx.x + 256 * (i0 + i), m = e / (HDP / 4), d = e % (HDP / 4) * 4;
+                if (i0 + i >= N_Q || m >= MT) continue;
 #pragma unroll
                 for (int t = 0; t < QT; t++) {
-                    uint32_t h[2] = {pack2<TYPE>(x[0], x[1]), pack2<TYPE>(x[2], x[3])};
-                    *reinterpret_cast<uint2 *>(qs + (t * MT + m) * QPITCH + d * 2) = make_uint2(h[0], h[1]);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) x[c] -= bf16_to_f((uint16_t)(h[c >> 1] >> (16 * (c & 1))));
+                    if constexpr (TYPE == TR_F32) {
+                        y[i] = make_uint2(pack2<TYPE>(x[i][0], x[i][1]), pack2<TYPE>(x[i][2], x[i][3]));
+                        x[i][0] -= bf16_to_f((uint16_t)y[i].x);
+                        x[i][1] -= bf16_to_f((uint16_t)(y[i].x >> 16));
+                        x[i][2] -= bf16_to_f((uint16_t)y[i].y);
+                        x[i][3] -= bf16_to_f((uint16_t)(y[i].y >> 16));
+                    }
+                    *reinterpret_cast<uint2 *>(qs + (t * MT + m) * QPITCH + d * 2) = y[i];
                 }
             }
         }
@@ -220,7 +230,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 m[r][h] = -INFINITY;
                 l[r][h] = 0.0f;
                 const int mr = wm * 16 * R + 16 * r + quad + 8 * h;
-                tok[r][h] = mr < rows ? (w.b * MT + mr) / g.group : -1;
+                tok[r][h] = mr < rows ? w.tok + mr / w.heads : -1;
 #pragma unroll
                 for (int t = 0; t < NT; t++) o[r][t][2 * h] = o[r][t][2 * h + 1] = 0.0f;
             }
@@ -472,9 +482,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     const int mr = wm * 16 * R + 16 * r + quad + 8 * h;
                     if (mr >= rows) continue;
                     if (whole) {
-                        const int row = w.b * MT + mr;
-                        const int64_t at = (int64_t)(w.q.t0 + row / g.group) * g.a.ldo +
-                                           (int64_t)(w.g * g.group + row % g.group) * hd;
+                        const int64_t at = tree_row(g, w.q.t0, w.tok, w.heads, w.head, mr, g.a.ldo);
                         const float inv = l[r][h] > 0.0f || l[r][h] != l[r][h] ? 1.0f / l[r][h] : 0.0f;
 #pragma unroll
                         for (int t = 0; t < NT; t++) {
@@ -514,7 +522,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     }
                 }
         }
-        if (threadIdx.x == 0 && w.tile == 0 && n_tiles < w.units) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
+        if (threadIdx.x == 0 && w.tile == 0 && n_tiles < w.units) tree_describe(g, w, line, first_item);
         __syncwarp();
         first_item = false;
         w.left -= n_tiles;
@@ -535,8 +543,7 @@ __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const __gri
     if (d.last < 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = g.p.head_dim;
     const int mr = blockIdx.y * 32 + lane, col = blockIdx.z * 32;
-    const TreeSeq q = tree_seq(g, d.i);
-    const int rows = min(g.mt, q.T * g.group - d.b * g.mt);
+    const int rows = d.rows;
     if ((int)blockIdx.y * 32 >= rows) return;
     const int at = min(mr, rows - 1), cols = min(32, hd - col);         // a multiple of 8
     float m = -INFINITY, l = 0.0f, o[32];
@@ -578,9 +585,7 @@ __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const __gri
         for (int k = 0; k < TC_WARPS; k++) x = fmaf(so[k][8 * warp + c][lane], f[k], x);
         y[c] = x * inv;
     }
-    const int row = d.b * g.mt + mr;
-    const int64_t dst = (int64_t)(q.t0 + row / g.group) * g.a.ldo + (d.g * g.group + row % g.group) * hd + col + 8 * warp;
-    tree_store8<TYPE>(g, dst, y);
+    tree_store8<TYPE>(g, tree_row(g, d.t0, d.tok, d.heads, d.head, mr, g.a.ldo) + col + 8 * warp, y);
 }
 
 // -------------------------------------------------------------------- host
@@ -589,19 +594,27 @@ int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who);
 typedef void (*TreeKernel)(CUtensorMap, CUtensorMap, TreeArgs);
 
 template <int TYPE, int HDP, int R, int WM>
-static int tree_fit(TreeArgs &g, size_t &smem) {
+static void tree_fit(TreeArgs &g, size_t &smem) {
     constexpr int MT = 16 * R * WM, QT = TYPE == TR_F32 ? 3 : 1;
     constexpr size_t stage = (size_t)2 * TR_KT * HDP * 2;
     constexpr size_t rest = (size_t)4 * 16 * (HDP + 4) * 4 + (size_t)QT * MT * (HDP * 2 + 16) + (size_t)8 * 16 * R * 8 + 1024;
     static_assert(rest + 2 * stage <= TR_SMEM, "two stages must fit");
-    g.mt = MT;
     g.stages = (int)std::min<size_t>(TR_MAX_STAGES, (TR_SMEM - rest) / stage);
     smem = g.stages * stage + rest;
-    return MT;
 }
 
-// Two parts for each CTA, and what its last item is.
-int tree_workspace(vb_ctx *ctx, TreeArgs &g) {
+// How blocks of mt rows and tiles of kt cache rows cut a call, and its
+// workspace: two parts for each CTA, and what its last item is.
+int tree_prepare(vb_ctx *ctx, TreeArgs &g, int mt, int kt) {
+    g.mt = mt;
+    g.tb = std::max(1, mt / g.group);
+    g.chunks = (g.group + mt - 1) / mt;
+    g.kt_log2 = 0;
+    while ((1 << g.kt_log2) < kt) g.kt_log2++;
+    const int64_t blocks = (int64_t)((g.a.max_tokens + g.tb - 1) / g.tb) * g.chunks;
+    const int64_t tiles = ((int64_t)g.p.max_pages * g.p.page_rows + kt - 1) / kt;
+    if ((double)g.a.n * g.p.n_kv_heads * (double)blocks * (double)tiles >= 2147483647.0)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "vb_tree_attention: too many rows for one call");
     const size_t parts = (size_t)2 * ctx->sm_count * g.mt * (g.p.head_dim + 2) * sizeof(float);
     int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)ctx->sm_count * sizeof(TreeShare));
     if (rc) return rc;
@@ -626,8 +639,7 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     size_t smem;
     tree_fit<TYPE, HDP, R, WM>(g, smem);
     const vb_pages &p = g.p;
-    g.kt = TR_KT;
-    int rc = tree_workspace(ctx, g);
+    int rc = tree_prepare(ctx, g, 16 * R * WM, TR_KT);
     if (rc) return rc;
     CUtensorMap tk, tv;
     const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;

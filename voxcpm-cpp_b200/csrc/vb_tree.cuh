@@ -15,8 +15,10 @@ struct TreeArgs {
     vb_pages p;
     float scale_log2;                // scale * log2(e): the softmax runs in powers of two
     int group;                       // query heads per K/V head
-    int mt;                          // rows per block
-    int kt;                          // cache rows per tile
+    int mt;                          // most rows of a block
+    int tb;                          // tokens of a block
+    int chunks;                      // blocks that share a token's heads (1 unless group > mt)
+    int kt_log2;                     // cache rows per tile, a power of two
     int stages;
     int vec;                         // 16-byte accesses of q and out
     int *err;
@@ -54,104 +56,145 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &g, int i) {
     return q;
 }
 
-__device__ __forceinline__ int tree_blocks(const TreeArgs &g, const TreeSeq &q) {
-    return (q.T * g.group + g.mt - 1) / g.mt;
+// A block: tb tokens with the heads of one K/V head (or, where those are more
+// than mt, one token with a chunk of mt heads).  Its rows are its (token,
+// head) pairs, tokens first.  Units of a block: the tiles of the cache rows
+// that its last token sees, at least one, so that every output row is
+// written.  The host refuses calls whose units could pass 2^31.
+__device__ __forceinline__ int tree_units(const TreeArgs &g, int visible) {
+    return max(1, (visible + (1 << g.kt_log2) - 1) >> g.kt_log2);
 }
 
-// Rows of the cache that block b of a sequence reads, and its units (at
-// least one, so that every output row is written).
-__device__ __forceinline__ int tree_visible(const TreeArgs &g, const TreeSeq &q, int b) {
-    if (q.bad) return 0;
-    if (g.a.mask) return q.len;
-    return q.base + min(q.T, ((b + 1) * g.mt + g.group - 1) / g.group);
+// sum of floor((a k + b) / 2^s) over k = 0 .. n-1, a and b not negative.
+static __device__ __noinline__ uint32_t tree_floor_sum(uint32_t n, int s, uint32_t a, uint32_t b) {
+    uint64_t sum = 0, m = (uint64_t)1 << s, aa = a, bb = b, nn = n;
+    while (nn) {                                      // Euclid on (a, m)
+        sum += (uint64_t)(uint32_t)(aa / m) * (nn * (nn - 1) / 2) + (bb / m) * nn;
+        aa %= m;
+        bb %= m;
+        const uint64_t y = aa * nn + bb;
+        if (y < m) break;
+        nn = y / m;
+        bb = y % m;
+        const uint64_t t = m;
+        m = aa;
+        aa = t;
+    }
+    return (uint32_t)sum;
 }
 
-// Of those, the rows that every token of the block sees.
-__device__ __forceinline__ int tree_clear(const TreeArgs &g, const TreeSeq &q, int b) {
-    return g.a.mask || q.bad ? q.base : q.base + b * g.mt / g.group + 1;
+// Units of the first k token blocks (one chunk, one K/V head).
+__device__ __forceinline__ int tree_units_before(const TreeArgs &g, const TreeSeq &q, int k) {
+    if (g.a.mask || q.bad) return k * tree_units(g, q.len);
+    const int kt = 1 << g.kt_log2, whole = min(k, q.T / g.tb);       // blocks of tb tokens
+    int u = g.tb >= kt || k <= 4 ? 0 : (int)tree_floor_sum(whole, g.kt_log2, g.tb, q.base + g.tb + kt - 1);
+    if (g.tb >= kt || k <= 4)
+        for (int j = 0; j < whole; j++) u += tree_units(g, q.base + (j + 1) * g.tb);
+    return u + (k > whole ? tree_units(g, q.len) : 0);
 }
 
-__device__ __forceinline__ int tree_units(const TreeArgs &g, int visible) { return max(1, (visible + g.kt - 1) / g.kt); }
-
-__device__ __forceinline__ int64_t tree_seq_units(const TreeArgs &g, const TreeSeq &q) {
-    const int nb = tree_blocks(g, q);
-    if (g.a.mask || q.bad) return (int64_t)nb * tree_units(g, tree_visible(g, q, 0)) * g.p.n_kv_heads;
-    int64_t u = 0;
-    for (int b = 0; b < nb; b++) u += tree_units(g, tree_visible(g, q, b));
-    return u * g.p.n_kv_heads;
-}
+__device__ __forceinline__ int tree_token_blocks(const TreeArgs &g, const TreeSeq &q) { return (q.T + g.tb - 1) / g.tb; }
 
 // A place in the line of units: the item (i, kv head, block) and the tile.
 struct TreeWalk {
     TreeSeq q;
-    int i, g, b, nb, visible, clear, units, tile;
-    int64_t left;                    // units of this CTA from here on
+    int i, g, b, chunk;              // block b of tokens
+    int tile, left;                  // left: units of this CTA from here on
+    // the item's
+    int visible, clear, units;       // rows that its last token sees; that every token sees; tiles
+    int tok, heads, head;            // first token, heads of the block, the first of them
+    int rows;
 };
 
 __device__ __forceinline__ void tree_item(const TreeArgs &g, TreeWalk &w) {
-    w.visible = tree_visible(g, w.q, w.b);
-    w.clear = tree_clear(g, w.q, w.b);
+    w.tok = w.b * g.tb;
+    const int tokens = min(g.tb, w.q.T - w.tok), h0 = w.chunk * g.mt;
+    w.heads = min(g.mt, g.group - h0);
+    w.head = w.g * g.group + h0;
+    w.rows = tokens * w.heads;
+    const bool chain = !g.a.mask && !w.q.bad;
+    w.visible = chain ? w.q.base + w.tok + tokens : w.q.len;
+    w.clear = chain ? w.q.base + w.tok + 1 : w.q.base;
     w.units = tree_units(g, w.visible);
 }
 
 __device__ __forceinline__ void tree_next(const TreeArgs &g, TreeWalk &w) {
     w.tile = 0;
-    if (++w.b == w.nb) {
-        w.b = 0;
-        if (++w.g == g.p.n_kv_heads) {
-            w.g = 0;
-            do w.q = tree_seq(g, ++w.i);
-            while (w.q.T == 0);
-            w.nb = tree_blocks(g, w.q);
+    if (++w.chunk == g.chunks) {
+        w.chunk = 0;
+        if (++w.b * g.tb >= w.q.T) {
+            w.b = 0;
+            if (++w.g == g.p.n_kv_heads) {
+                w.g = 0;
+                do w.q = tree_seq(g, ++w.i);
+                while (w.q.T == 0);
+            }
         }
     }
     tree_item(g, w);
 }
 
-// The part of the line of units that this CTA works on, found by all its
-// threads together (THREADS of them): the first place in w, whose `left` is 0
-// when there is none.  `total` and `ctas` describe the whole cut: CTA c has
-// the units c * total / ctas up to (c + 1) * total / ctas.
+// The cut of the line: `ctas` CTAs get total / ctas units each, the first
+// total % ctas one more.
+struct TreeLine {
+    int total, ctas, each, more;
+    __device__ __forceinline__ int first(int c) const { return c * each + min(c, more); }
+    __device__ __forceinline__ int owner(int u) const {
+        const int head = more * (each + 1);
+        return u < head ? u / (each + 1) : more + (u - head) / each;
+    }
+};
+
+// The part of the line that this CTA works on, found by all its threads
+// together (THREADS of them): the first place in w, whose `left` is 0 when
+// there is none.
 struct TreeCut {
-    int64_t scan[32], off;
-    int seq;
+    TreeSeq q;
+    int scan[32], seq, off, b, rest;
 };
 
 template <int THREADS>
-__device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWalk &w, int64_t &u1, int64_t &total,
-                                         int64_t &ctas) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n = g.a.n;
+__device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWalk &w, TreeLine &line) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = g.a.n, heads = g.p.n_kv_heads * g.chunks;
     const int per = (n + THREADS - 1) / THREADS;
     const int i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
-    int64_t mine = 0;
+    int mine = 0;
+    TreeSeq q;
     for (int i = i0; i < i1; i++) {
-        const TreeSeq q = tree_seq(g, i);
+        q = tree_seq(g, i);
         if (q.bad && blockIdx.x == 0) atomicCAS(g.err, 0, VB_DEV_TREE_SEQ);
-        mine += tree_seq_units(g, q);
+        mine += heads * tree_units_before(g, q, tree_token_blocks(g, q));
     }
-    int64_t before = mine;
+    int before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, before, o);
+        const int y = __shfl_up_sync(0xffffffffu, before, o);
         if (lane >= o) before += y;
     }
     if (lane == 31) sh.scan[warp] = before;
     before -= mine;
+    if (threadIdx.x == 0) g.share[blockIdx.x].last = -1;
     __syncthreads();
-    total = 0;
+    line.total = 0;
+#pragma unroll
     for (int k = 0; k < THREADS / 32; k++) {
-        if (k < warp) before += sh.scan[k];
-        total += sh.scan[k];
+        const int x = sh.scan[k];
+        if (k < warp) before += x;
+        line.total += x;
     }
-    ctas = min((int64_t)gridDim.x, total);
-    const int64_t u0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : total;
-    u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : total;
+    w.left = 0;
+    line.ctas = min((int)gridDim.x, line.total);
+    if (line.ctas == 0) return;
+    line.each = line.total / line.ctas;
+    line.more = line.total - line.each * line.ctas;
+    const int u0 = line.first(min((int)blockIdx.x, line.ctas)), u1 = line.first(min((int)blockIdx.x + 1, line.ctas));
     if (u0 >= before && u0 < before + mine) {
-        int64_t at = before;
-        for (int i = i0; i < i1; i++) {
-            const int64_t u = tree_seq_units(g, tree_seq(g, i));
+        int at = before;
+        for (int i = i0;; i++) {
+            if (per > 1) q = tree_seq(g, i);
+            const int u = per > 1 ? heads * tree_units_before(g, q, tree_token_blocks(g, q)) : mine;
             if (u0 < at + u) {
+                sh.q = q;
                 sh.seq = i;
                 sh.off = u0 - at;
                 break;
@@ -159,41 +202,61 @@ __device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWal
             at += u;
         }
     }
-    if (threadIdx.x == 0) g.share[blockIdx.x].last = -1;
     __syncthreads();
+    if (u1 <= u0) return;
     w.left = u1 - u0;
-    if (w.left <= 0) return;
     w.i = sh.seq;
-    w.q = tree_seq(g, w.i);
-    w.nb = tree_blocks(g, w.q);
-    const int64_t head_units = tree_seq_units(g, w.q) / g.p.n_kv_heads;
-    w.g = (int)(sh.off / head_units);
-    int64_t off = sh.off % head_units;
-    w.b = 0;
-    tree_item(g, w);
-    if (g.a.mask || w.q.bad) {                          // blocks of equal length
-        w.b = (int)(off / w.units);
-        off %= w.units;
+    w.q = sh.q;
+    const int nb = tree_token_blocks(g, w.q), each = tree_units_before(g, w.q, nb) * g.chunks;
+    w.g = sh.off / each;
+    int off = sh.off - w.g * each;
+    if (g.a.mask || w.q.bad || nb == 1) {               // blocks of equal length
+        const int u = tree_units(g, w.q.len) * g.chunks;
+        w.b = off / u;
+        off -= w.b * u;
     } else {
-        while (off >= w.units) {
-            off -= w.units;
-            w.b++;
-            tree_item(g, w);
+        // every thread looks at a few of the blocks
+        const int step = (nb + THREADS - 1) / THREADS, k0 = min(nb, (int)threadIdx.x * step), k1 = min(nb, k0 + step);
+        int at = tree_units_before(g, w.q, k0) * g.chunks;
+        for (int k = k0; k < k1; k++) {
+            const int u = tree_units(g, w.q.base + min(w.q.T, (k + 1) * g.tb)) * g.chunks;
+            if (off >= at && off < at + u) {
+                sh.b = k;
+                sh.rest = off - at;
+            }
+            at += u;
         }
+        __syncthreads();
+        w.b = sh.b;
+        off = sh.rest;
     }
-    w.tile = (int)off;
+    w.chunk = 0;
+    tree_item(g, w);
+    if (g.chunks > 1) {
+        w.chunk = off / w.units;
+        off -= w.chunk * w.units;
+        tree_item(g, w);
+    }
+    w.tile = off;
 }
 
 // An item that goes on in the next CTAs: described by the CTA that holds its
 // first unit (`at`), as its last item.
 struct TreeShare {
-    int i, g, b, slot, last, pad[3];        // last: the CTA of its last unit; -1: no such item
+    int slot, last;                  // last: the CTA of its last unit; -1: no such item
+    int t0, tok, heads, head, rows, pad;
 };
 
-__device__ __forceinline__ void tree_describe(const TreeArgs &g, const TreeWalk &w, int64_t at, int64_t total,
-                                              int64_t ctas, bool first_item) {
-    const int64_t end = at + w.units - 1;
-    g.share[blockIdx.x] = {w.i, w.g, w.b, (int)blockIdx.x * 2 + (first_item ? 0 : 1), (int)(((end + 1) * ctas - 1) / total), {}};
+__device__ __forceinline__ void tree_describe(const TreeArgs &g, const TreeWalk &w, const TreeLine &line, bool first_item) {
+    const int at = line.first(blockIdx.x + 1) - w.left;             // the item's first unit
+    g.share[blockIdx.x] = {(int)blockIdx.x * 2 + (first_item ? 0 : 1), line.owner(at + w.units - 1), w.q.t0, w.tok, w.heads, w.head,
+                           w.rows, 0};
+}
+
+// Where row r of a block lies in q (ld: its row stride) or out.
+__device__ __forceinline__ int64_t tree_row(const TreeArgs &g, int t0, int tok, int heads, int head, int r, int64_t ld) {
+    const int t = r / heads;
+    return (int64_t)(t0 + tok + t) * ld + (int64_t)(head + r - t * heads) * g.p.head_dim;
 }
 
 // Whether token j of the sequence sees draft row d (0 <= d < T).
@@ -324,7 +387,7 @@ __device__ __forceinline__ void tree_store8(const TreeArgs &g, int64_t at, const
 
 int launch_tree_tc(vb_ctx *ctx, TreeArgs &g);
 int init_tree_tc(vb_ctx *ctx);
-int tree_workspace(vb_ctx *ctx, TreeArgs &g);
+int tree_prepare(vb_ctx *ctx, TreeArgs &g, int mt, int kt);
 int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g);
 
 }  // namespace vb

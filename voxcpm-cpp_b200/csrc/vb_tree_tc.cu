@@ -32,11 +32,36 @@ constexpr int TT_SLOTS = 12;
 constexpr int TT_SMEM = 225 * 1024;
 constexpr float TT_SLACK = 8.0f;     // log2 of how far a score may exceed the running maximum
 
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// One lane of the (converged) warp.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
+}
+
+// MMAs and commits issued where `one` is set, so that the code around them
+// is the same for the whole warp.
+__device__ __forceinline__ void umma_f16_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p, e;\n setp.ne.b32 e, %0, 0;\n setp.ne.b32 p, %5, 0;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%1], %2, %3, %4, p;\n}\n" ::"r"(one),
+        "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p, e;\n setp.ne.b32 e, %0, 0;\n setp.ne.b32 p, %5, 0;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], %3, %4, p;\n}\n" ::"r"(one),
+        "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_commit_one(uint32_t one, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.b32 e, %0, 0;\n"
+        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}\n" ::"r"(one),
+        "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -202,8 +227,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
     pdl_trigger();
     pdl_wait();
     TreeWalk w;
-    int64_t u1, total, ctas;
-    tree_cut<TT_THREADS>(g, cut, w, u1, total, ctas);
+    TreeLine line;
+    tree_cut<TT_THREADS>(g, cut, w, line);
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     // tensor memory: scores (then weights) of stream t at column 128 t, sums at 256 + HDP t
@@ -215,7 +240,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             const int P = g.p.page_rows, box = min(P, TT_KT);
             int pos = 0;
             while (w.left > 0) {
-                const int n = (int)min((int64_t)(w.units - w.tile), w.left);
+                const int n = min(w.units - w.tile, w.left);
                 const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
                 // a lane's row within its box's page, and that page
                 auto page_of = [&](int e, int &y, int &nbox, bool &is_v) {
@@ -267,65 +292,75 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 const int fills = pos / n_slots + (pos % n_slots > s ? 1 : 0);
                 if (fills) gm_wait(&full[s], (uint32_t)(fills - 1) & 1u);
             }
-        } else if (warp == 9 && lane == 0) {
+        } else if (warp == 9) {
             // --------------------------------------------------------- MMAs
             const uint32_t fmt = TYPE == TR_F16 ? 0u : 1u;
             constexpr uint32_t N_S = (uint32_t)(TT_KT >> 3) << 17, N_O = (uint32_t)(HDP >> 3) << 17;
             const uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24) | N_S;
             const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24) | N_O | (1u << 16);   // V: rows along k
             const uint64_t d_q = sw128_desc(qs), d_k = sw128_desc(ring), d_v = sw128_desc_mn(smem_u32(ring));
-            int pos = 0, item = 0;
-            uint32_t phase = 0;                       // parity of p_full, a bit per stream
-            auto wait_ring = [&](int at) {
-                tree_wait(&full[at % n_slots], (uint32_t)(at / n_slots) & 1u, &abort_flag, g.err);
+            // The whole warp goes through the steps, one lane of it issues.
+            const uint32_t one = elect_one();
+            int item = 0, slot = 0;                   // slot: the ring's next tile, in the order of use
+            uint32_t ring_phase = 0, phase = 0;       // phase: parity of p_full, a bit per stream
+            auto take = [&]() {
+                tree_wait_warp(&full[slot], ring_phase, &abort_flag, g.err);
                 tc_fence_after();
+                const int s = slot;
+                if (++slot == n_slots) {
+                    slot = 0;
+                    ring_phase ^= 1u;
+                }
+                return s;
             };
-            // One place of the pipeline: the values of tile j, then the scores of
-            // the tile that stream t takes next.
+            int last = -1;
+            uint32_t last_phase = 0;
             while (w.left > 0) {
-                const int n = (int)min((int64_t)(w.units - w.tile), w.left);
-                tree_wait(&q_full, (uint32_t)item & 1u, &abort_flag, g.err);
+                const int n = __shfl_sync(0xffffffffu, min(w.units - w.tile, w.left), 0);
+                tree_wait_warp(&q_full, (uint32_t)item & 1u, &abort_flag, g.err);
                 tc_fence_after();
-                constexpr int AHEAD = PAIR ? 1 : 2;
+                // One place of the pipeline: the values of tile j, then the scores of
+                // the tile that stream t takes next.
+                int v_slot = 0, k_slot = 0;
 #pragma unroll 1
                 for (int x = -2; x < (PAIR ? 2 * n : n); x++) {
-                    const int j = PAIR ? x >> 1 : x, t = x & 1, next = j + AHEAD;
+                    const int j = PAIR ? x >> 1 : x, t = x & 1, next = j + (PAIR ? 1 : 2);
                     if (j >= 0) {
-                        const int at = pos + ring_v<PAIR>(j, n), slot = at % n_slots;
-                        if (!PAIR || t == 0) wait_ring(at);
-                        tree_wait(&p_full[t], phase >> t & 1u, &abort_flag, g.err);
-                        phase ^= 1u << t;
-                        tc_fence_after();
-                        const uint64_t v = d_v + (uint64_t)(slot * (SLOT >> 4));
+                        if (!PAIR || t == 0) {
+                            last_phase = ring_phase;
+                            last = v_slot = take();
+                        }
+                        const uint64_t v = d_v + (uint64_t)((uint32_t)v_slot * (SLOT >> 4));
                         const uint32_t p = tmem + 128 * t, o = tmem + 256 + HDP * t;
                         const uint32_t more = PAIR ? j > 0 : j > 1;
+                        tree_wait_warp(&p_full[t], phase >> t & 1u, &abort_flag, g.err);
+                        phase ^= 1u << t;
+                        tc_fence_after();
 #pragma unroll
                         for (int i = 0; i < TT_KT / 16; i++)
-                            umma_f16_ts(o, p + 8 * i, v + (uint64_t)(i * (2048 >> 4)), id_o, i ? 1u : more);
-                        umma_commit(&pv_done[t]);
-                        if (!PAIR || t == 1) umma_commit(&empty[slot]);
+                            umma_f16_ts(one, o, p + 8 * i, v + (uint64_t)(i * (2048 >> 4)), id_o, i ? 1u : more);
+                        umma_commit_one(one, &pv_done[t]);
+                        if (!PAIR || t == 1) umma_commit_one(one, &empty[v_slot]);
                     }
                     if (next >= 0 && next < n) {
-                        const int at = pos + ring_k<PAIR>(next), slot = at % n_slots;
-                        if (!PAIR || t == 0) wait_ring(at);
-                        const uint64_t k = d_k + (uint64_t)(slot * (SLOT >> 4)), q = d_q + (uint64_t)(PAIR ? t * (SLOT >> 4) : 0);
+                        if (!PAIR || t == 0) k_slot = take();
+                        const uint64_t k = d_k + (uint64_t)((uint32_t)k_slot * (SLOT >> 4)), q = d_q + (uint64_t)(PAIR ? t * (SLOT >> 4) : 0);
                         const uint32_t sc = tmem + 128 * t;
 #pragma unroll
                         for (int i = 0; i < HDP / 16; i++) {
                             const uint64_t off = (i >> 2) * (BLOCK >> 4) + (i & 3) * 2;
-                            umma_f16(sc, q + off, k + off, id_s, i ? 1u : 0u);
+                            umma_f16_ss(one, sc, q + off, k + off, id_s, i ? 1u : 0u);
                         }
-                        umma_commit(&s_full[t]);
-                        if (!PAIR || t == 1) umma_commit(&empty[slot]);
+                        umma_commit_one(one, &s_full[t]);
+                        if (!PAIR || t == 1) umma_commit_one(one, &empty[k_slot]);
                     }
                 }
-                pos += 2 * n;
                 item++;
                 w.left -= n;
                 if (w.left > 0) tree_next(g, w);
             }
             // the last commit has reached its barrier before the CTA can end
-            if (pos) tree_wait(&empty[(pos - 1) % n_slots], (uint32_t)((pos - 1) / n_slots) & 1u, &abort_flag, g.err);
+            if (last >= 0) tree_wait_warp(&empty[last], last_phase, &abort_flag, g.err);
         }
     } else {
         // -------------------------------------------------------- softmax
@@ -335,32 +370,37 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
         int pos = 0, item = 0, seen = 0;                             // seen: tiles of this stream so far
         bool first_item = true;
         while (w.left > 0) {
-            const int n = (int)min((int64_t)(w.units - w.tile), w.left);
-            const int rows = min(MT, w.q.T * g.group - w.b * MT);
+            const int n = min(w.units - w.tile, w.left);
+            const int rows = w.rows;
             // the queries of this stream's row tile (of half of the one tile)
             {
                 uint8_t *qt = qs + (PAIR ? t * SLOT : 0);
-                for (int e = PAIR ? tid : (int)threadIdx.x; e < 128 * (HDP / 8); e += PAIR ? 128 : 256) {
-                    const int r = e / (HDP / 8), c = e % (HDP / 8), m = (PAIR ? 128 * t : 0) + r;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (m < rows && 8 * c < hd) {
-                        const int row = w.b * MT + m;
-                        const uint16_t *src = static_cast<const uint16_t *>(g.a.q) + (w.q.t0 + row / g.group) * g.a.ldq +
-                                              (w.g * g.group + row % g.group) * hd + 8 * c;
-                        if (g.vec) x = *reinterpret_cast<const uint4 *>(src);
+                // a thread takes a row (PAIR) or half a row, its loads in flight together
+                constexpr int N_C = HDP / 8 / (PAIR ? 1 : 2);          // 16-byte chunks
+                const int r = PAIR ? tid : (int)threadIdx.x >> 1, m = (PAIR ? 128 * t : 0) + r, c0 = PAIR ? 0 : (threadIdx.x & 1) * N_C;
+                const uint16_t *src = static_cast<const uint16_t *>(g.a.q) + (m < rows ? tree_row(g, w.q.t0, w.tok, w.heads, w.head, m, g.a.ldq) : 0);
+                uint4 x[N_C];
+#pragma unroll
+                for (int i = 0; i < N_C; i++) {
+                    const uint16_t *p = src + 8 * (c0 + i);
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (m < rows && 8 * (c0 + i) < hd) {
+                        if (g.vec) x[i] = *reinterpret_cast<const uint4 *>(p);
                         else
-                            x = make_uint4(src[0] | (uint32_t)src[1] << 16, src[2] | (uint32_t)src[3] << 16,
-                                           src[4] | (uint32_t)src[5] << 16, src[6] | (uint32_t)src[7] << 16);
+                            x[i] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16,
+                                              p[6] | (uint32_t)p[7] << 16);
                     }
-                    *reinterpret_cast<uint4 *>(qt + (c >> 3) * BLOCK + sw128(r, c & 7)) = x;
                 }
+#pragma unroll
+                for (int i = 0; i < N_C; i++)
+                    *reinterpret_cast<uint4 *>(qt + ((c0 + i) >> 3) * BLOCK + sw128(r, (c0 + i) & 7)) = x[i];
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
             }
             const int mrow = (PAIR ? 128 * t : 0) + 32 * (warp & 3) + lane;      // this thread's row of the block
             const bool alive = mrow - lane < rows;                               // the warp has rows
-            const int j = mrow < rows ? (w.b * MT + mrow) / g.group : -1;
+            const int j = mrow < rows ? w.tok + mrow / w.heads : -1;
             float m = -INFINITY, l = 0.0f;
             const int mine = PAIR ? n : (n + 1 - t) / 2;                         // tiles of this stream
             for (int x = 0; x < mine; x++, seen++) {
@@ -523,8 +563,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             tc_fence_after();
             const bool mend = *(volatile int *)&not_finite[item & 1] == item;
             if (alive) {
-                const int row = w.b * MT + mrow;
-                const int64_t out = (int64_t)(w.q.t0 + row / g.group) * g.a.ldo + (w.g * g.group + row % g.group) * hd;
+                const int64_t out = tree_row(g, w.q.t0, w.tok, w.heads, w.head, mrow, g.a.ldo);
                 const float inv = whole ? (l > 0.0f || l != l ? 1.0f / l : 0.0f) : 1.0f;
                 float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * (hd + 2) * MT + mrow;
                 if (!whole && (PAIR || t == 0)) {
@@ -570,7 +609,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             __syncwarp();
             tc_fence_before();
             if (!PAIR) consumer_sync(256);           // both streams' sums are read: the next item may overwrite them
-            if (threadIdx.x == 0 && w.tile == 0 && !whole) tree_describe(g, w, u1 - w.left, total, ctas, first_item);
+            if (threadIdx.x == 0 && w.tile == 0 && !whole) tree_describe(g, w, line, first_item);
             __syncwarp();
             first_item = false;
             pos += 2 * n;
@@ -592,12 +631,10 @@ template <int TYPE, int HDP, bool PAIR>
 static int launch_tc(vb_ctx *ctx, TreeArgs &g) {
     constexpr size_t slot = (size_t)HDP / 64 * TT_KT * 128, q = (PAIR ? 2 : 1) * slot;
     const vb_pages &p = g.p;
-    g.mt = PAIR ? 256 : 128;
-    g.kt = TT_KT;
     const size_t rest = 1024 + q + (PAIR ? 0 : 2 * 128 * sizeof(float2));
     g.stages = (int)std::min<size_t>(TT_SLOTS, (TT_SMEM - rest) / slot);
     const size_t smem = rest + g.stages * slot;
-    int rc = tree_workspace(ctx, g);
+    int rc = tree_prepare(ctx, g, PAIR ? 256 : 128, TT_KT);
     if (rc) return rc;
     CUtensorMap tk, tv;
     const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;
