@@ -1136,6 +1136,20 @@ bool make_map(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int esiz
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// 3-D tensor map: [planes][rows][cols], `row` and `plane` bytes apart, box
+// [box_planes][box_rows][box_cols], 128-byte swizzle.
+bool make_map_3d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int64_t cols, int64_t rows, int64_t planes,
+                 int64_t row, int64_t plane, int box_cols, int box_rows, int box_planes) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    cuuint64_t strides[2] = {(cuuint64_t)row, (cuuint64_t)plane};
+    cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, (cuuint32_t)box_planes};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(m, dt, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct ActMaps {                // TMA descriptors of one activation buffer shape
     const void *bh = nullptr, *bl = nullptr;
     int K = 0, M = 0, BN = 0;

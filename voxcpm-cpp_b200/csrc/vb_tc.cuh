@@ -17,6 +17,9 @@ namespace vb {
 bool make_map(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int esize, int64_t cols, int64_t rows,
               int box_cols, int box_rows, bool swizzle);
 
+bool make_map_3d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int64_t cols, int64_t rows, int64_t planes,
+                 int64_t row, int64_t plane, int box_cols, int box_rows, int box_planes);
+
 __device__ __forceinline__ uint64_t sw128_desc(const void *p) {
     uint64_t d = (uint64_t)((smem_u32(p) >> 4) & 0x3FFFu);
     d |= (uint64_t)1 << 16;                 // leading byte offset (unused for swizzled K-major)
@@ -31,6 +34,14 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, i
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
             smem_u32(dst)),
         "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
 

@@ -29,6 +29,7 @@ namespace vb {
 
 constexpr int TR_KT = 64;            // cache rows per tile
 constexpr int TR_MAX_STAGES = 8;
+constexpr int TR_OVER = 2;           // an item's start and end cost about as much as two of its tiles
 constexpr int TR_THREADS = 384;      // warps 0..7 compute, warp 8 loads
 // Registers: the launch gives 168 a thread; the loading warpgroup goes down
 // to 56 and the two computing ones up to 224 (2 * 224 + 56 = 3 * 168), which
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         const int P = g.p.page_rows, box = min(P, TR_KT), boxes = TR_KT / box;
         int it = 0;
         while (w.left > 0) {
-            const int n_tiles = min(w.units - w.tile, w.left);
+            const int n_tiles = tree_take(g, w);
             const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
             int pages = 0;                              // lane's page of the current 32 boxes
             for (int x = 0; x < n_tiles; x++, it++) {
@@ -153,7 +154,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     }
                 }
             }
-            w.left -= n_tiles;
             if (w.left > 0) tree_next(g, w);
         }
         // every copy has landed before the CTA can end
@@ -173,9 +173,13 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     int it = 0;
     bool first_item = true;
     while (w.left > 0) {
-        const int n_tiles = min(w.units - w.tile, w.left);
-        const bool whole = w.tile == 0 && n_tiles == w.units;
-        const int rows = w.rows;                                        // rows of the block that exist
+        const int n_tiles = tree_take(g, w);
+        if (n_tiles == 0) {
+            if (w.left > 0) tree_next(g, w);
+            continue;
+        }
+        const bool whole = n_tiles == w.units;
+        const int rows = w.tokens * w.heads;                            // rows of the block that exist
         // queries of the block, in 16-bit terms
         constexpr int N_Q = (MT * (HDP / 4) + 255) / 256;          // four values each
 #pragma unroll
@@ -188,7 +192,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
                 y[i] = make_uint2(0, 0);
                 if (i0 + i < N_Q && m < rows && d < hd) {
-                    const int64_t at = tree_row(g, w.q.t0, w.tok, w.heads, w.head, m, g.a.ldq) + d;
+                    const int64_t at = tree_row(g, w.q.t0, w.tok, w.heads, w.head, 0, m, g.a.ldq) + d;
                     if constexpr (TYPE == TR_F32) {
                         const float *src = static_cast<const float *>(g.a.q) + at;
                         if (g.vec) *reinterpret_cast<float4 *>(x[i]) = *reinterpret_cast<const float4 *>(src);
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     const int mr = wm * 16 * R + 16 * r + quad + 8 * h;
                     if (mr >= rows) continue;
                     if (whole) {
-                        const int64_t at = tree_row(g, w.q.t0, w.tok, w.heads, w.head, mr, g.a.ldo);
+                        const int64_t at = tree_row(g, w.q.t0, w.tok, w.heads, w.head, 0, mr, g.a.ldo);
                         const float inv = l[r][h] > 0.0f || l[r][h] != l[r][h] ? 1.0f / l[r][h] : 0.0f;
 #pragma unroll
                         for (int t = 0; t < NT; t++) {
@@ -522,70 +526,93 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     }
                 }
         }
-        if (threadIdx.x == 0 && w.tile == 0 && n_tiles < w.units) tree_describe(g, w, line, first_item);
+        if (threadIdx.x == 0) tree_describe(g, w, line, n_tiles, first_item);
         __syncwarp();
         first_item = false;
-        w.left -= n_tiles;
         if (w.left > 0) tree_next(g, w);
     }
 }
 
-// Joins the parts of items that several CTAs shared.  grid (CTA whose last
-// item goes on, 32 rows, 32 columns): a lane holds 32 columns of a row, the
-// warps take the parts in turn and are added in shared memory.
-constexpr int TC_WARPS = 4;
+// Joins the parts of items that several CTAs shared.  A task is 32 rows by
+// 16 columns of an item; a lane holds a row of it.  grid (entry of `share`,
+// tasks): where an item has many parts the warps of a CTA take them in turn
+// and are added in shared memory, else each warp has a task of its own.
+constexpr int TC_WARPS = 8;
+constexpr int TC_COLS = 16;
+constexpr int TC_FEW = 4;            // parts
 template <int TYPE>
 __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeArgs g) {
-    __shared__ float so[TC_WARPS][32][33], sm[TC_WARPS][32], sl[TC_WARPS][32];
+    __shared__ float so[TC_WARPS][TC_COLS][32], sm[TC_WARPS][32], sl[TC_WARPS][32];
     pdl_trigger();
     pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = g.p.head_dim;
+    if (g.by_item) {                                 // the entry was written if the item exists
+        const int c = blockIdx.x % g.item_blocks, i = blockIdx.x / g.item_blocks / g.p.n_kv_heads;
+        if (c / g.chunks * g.tb >= tree_seq(g, i).T) return;
+    }
     const TreeShare d = g.share[blockIdx.x];
     if (d.last < 0) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = g.p.head_dim;
-    const int mr = blockIdx.y * 32 + lane, col = blockIdx.z * 32;
-    const int rows = d.rows;
-    if ((int)blockIdx.y * 32 >= rows) return;
-    const int at = min(mr, rows - 1), cols = min(32, hd - col);         // a multiple of 8
-    float m = -INFINITY, l = 0.0f, o[32];
+    const bool few = d.last - d.first < TC_FEW;
+    const int row_tasks = (g.mt + 31) / 32, tasks = row_tasks * ((hd + TC_COLS - 1) / TC_COLS);
+    for (int task = few ? blockIdx.y * TC_WARPS + warp : blockIdx.y; task < tasks; task += gridDim.y * (few ? TC_WARPS : 1)) {
+        const int mr = task % row_tasks * 32 + lane, col = task / row_tasks * TC_COLS;
+        const int t = mr / g.tile_rows, tr = mr - t * g.tile_rows;
+        const bool real = mr < g.mt && tree_token(g, d.tokens, d.heads, t, tr) >= 0;
+        // (for the whole CTA alike: a task's rows are the same in every warp)
+        if (!__any_sync(0xffffffffu, real)) continue;
+        const int at = real ? mr : 0, cols = min(TC_COLS, hd - col);
+        float m = -INFINITY, l = 0.0f, o[TC_COLS];
 #pragma unroll
-    for (int c = 0; c < 32; c++) o[c] = 0.0f;
-    for (int k = blockIdx.x + warp; k <= d.last; k += TC_WARPS) {
-        const float *part = g.part + (size_t)(k == (int)blockIdx.x ? d.slot : 2 * k) * (hd + 2) * g.mt + at;
-        const float om = part[(size_t)hd * g.mt], ol = part[(size_t)(hd + 1) * g.mt];
-        float v[32];
+        for (int c = 0; c < TC_COLS; c++) o[c] = 0.0f;
+#pragma unroll 2
+        for (int k = d.first + (few ? 0 : warp); k <= d.last; k += few ? 1 : TC_WARPS) {
+            const float *part = g.part + (size_t)(k == d.first ? d.slot : 2 * k) * (hd + 2) * g.mt + at;
+            const float om = part[(size_t)hd * g.mt], ol = part[(size_t)(hd + 1) * g.mt];
+            float v[TC_COLS];
 #pragma unroll
-        for (int c = 0; c < 32; c++) v[c] = c < cols ? part[(size_t)(col + c) * g.mt] : 0.0f;
-        const float mn = fmaxf(m, om), ms = mn == -INFINITY ? 0.0f : mn;
-        const float f = ex2(m - ms), e = ex2(om - ms);
-        m = mn;
-        l = l * f + ol * e;
+            for (int c = 0; c < TC_COLS; c++) v[c] = c < cols ? part[(size_t)(col + c) * g.mt] : 0.0f;
+            const float mn = fmaxf(m, om), ms = mn == -INFINITY ? 0.0f : mn;
+            const float f = ex2(m - ms), e = ex2(om - ms);
+            m = mn;
+            l = l * f + ol * e;
 #pragma unroll
-        for (int c = 0; c < 32; c++) o[c] = o[c] * f + v[c] * e;
+            for (int c = 0; c < TC_COLS; c++) o[c] = o[c] * f + v[c] * e;
+        }
+        const int64_t dst = tree_row(g, d.t0, d.tok, d.heads, d.head, t, tr, g.a.ldo) + col;
+        if (few) {
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int c = 0; c < TC_COLS; c += 8) {
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) y[k] = o[c + k] * inv;
+                if (real && c < cols) tree_store8<TYPE>(g, dst + c, y);
+            }
+            continue;
+        }
+        __syncthreads();                              // the task before has been read
+#pragma unroll
+        for (int c = 0; c < TC_COLS; c++) so[warp][c][lane] = o[c];
+        sm[warp][lane] = m;
+        sl[warp][lane] = l;
+        __syncthreads();
+        if (8 * warp >= cols) continue;               // warps 0 and 1 write eight columns each
+        float top = -INFINITY, sum = 0.0f, f[TC_WARPS], y[8] = {};
+#pragma unroll
+        for (int k = 0; k < TC_WARPS; k++) top = fmaxf(top, sm[k][lane]);
+        const float ms = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int k = 0; k < TC_WARPS; k++) {
+            f[k] = ex2(sm[k][lane] - ms);
+            sum = fmaf(sl[k][lane], f[k], sum);
+#pragma unroll
+            for (int c = 0; c < 8; c++) y[c] = fmaf(so[k][8 * warp + c][lane], f[k], y[c]);
+        }
+        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; c++) y[c] *= inv;
+        if (real) tree_store8<TYPE>(g, dst + 8 * warp, y);
     }
-#pragma unroll
-    for (int c = 0; c < 32; c++) so[warp][c][lane] = o[c];
-    sm[warp][lane] = m;
-    sl[warp][lane] = l;
-    __syncthreads();
-    float top = -INFINITY, sum = 0.0f, f[TC_WARPS], y[8];
-#pragma unroll
-    for (int k = 0; k < TC_WARPS; k++) top = fmaxf(top, sm[k][lane]);
-    const float ms = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int k = 0; k < TC_WARPS; k++) {
-        f[k] = ex2(sm[k][lane] - ms);
-        sum = fmaf(sl[k][lane], f[k], sum);
-    }
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    if (mr >= rows || 8 * warp >= cols) return;
-#pragma unroll
-    for (int c = 0; c < 8; c++) {
-        float x = 0.0f;
-#pragma unroll
-        for (int k = 0; k < TC_WARPS; k++) x = fmaf(so[k][8 * warp + c][lane], f[k], x);
-        y[c] = x * inv;
-    }
-    tree_store8<TYPE>(g, tree_row(g, d.t0, d.tok, d.heads, d.head, mr, g.a.ldo) + col + 8 * warp, y);
 }
 
 // -------------------------------------------------------------------- host
@@ -603,18 +630,23 @@ static void tree_fit(TreeArgs &g, size_t &smem) {
     smem = g.stages * stage + rest;
 }
 
-// How blocks of mt rows and tiles of kt cache rows cut a call, and its
-// workspace: two parts for each CTA, and what its last item is.
-int tree_prepare(vb_ctx *ctx, TreeArgs &g, int mt, int kt) {
-    g.mt = mt;
-    g.tb = std::max(1, mt / g.group);
-    g.chunks = (g.group + mt - 1) / mt;
+// How blocks of row tiles and tiles of kt cache rows cut a call, and its
+// workspace: two parts for each CTA, and where the items' parts are.
+int tree_prepare(vb_ctx *ctx, TreeArgs &g, int tile_rows, int tiles, int kt, int over) {
+    g.tile_rows = tile_rows;
+    g.tile_tokens = std::max(1, tile_rows / g.group);
+    g.tb = tiles * g.tile_tokens;
+    g.mt = tiles * tile_rows;
+    g.chunks = (g.group + tile_rows - 1) / tile_rows;
+    g.over = over;
     g.kt_log2 = 0;
     while ((1 << g.kt_log2) < kt) g.kt_log2++;
-    const int64_t blocks = (int64_t)((g.a.max_tokens + g.tb - 1) / g.tb) * g.chunks;
-    const int64_t tiles = ((int64_t)g.p.max_pages * g.p.page_rows + kt - 1) / kt;
-    if ((double)g.a.n * g.p.n_kv_heads * (double)blocks * (double)tiles >= 2147483647.0)
+    const int64_t blocks = (int64_t)((g.a.max_tokens + g.tb - 1) / g.tb) * g.chunks, items = blocks * g.a.n * g.p.n_kv_heads;
+    const int64_t most = ((int64_t)g.p.max_pages * g.p.page_rows + kt - 1) / kt + over;
+    if ((double)items * (double)most >= 2147483647.0)
         return set_error(ctx, VB_ERR_INVALID_ARG, "vb_tree_attention: too many rows for one call");
+    g.by_item = items < ctx->sm_count;
+    g.item_blocks = (int)blocks;
     const size_t parts = (size_t)2 * ctx->sm_count * g.mt * (g.p.head_dim + 2) * sizeof(float);
     int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)ctx->sm_count * sizeof(TreeShare));
     if (rc) return rc;
@@ -627,9 +659,11 @@ int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g) {
     auto kernel = g.a.type == VB_TYPE_F32   ? tree_combine_kernel<TR_F32>
                   : g.a.type == VB_TYPE_F16 ? tree_combine_kernel<TR_F16>
                                             : tree_combine_kernel<TR_BF16>;
-    const int64_t rows = std::min<int64_t>(g.mt, (int64_t)g.a.max_tokens * g.group);
-    VB_CHECK(ctx, pdl_launch(ctx, kernel, dim3(ctx->sm_count, (unsigned)((rows + 31) / 32), (g.p.head_dim + 31) / 32),
-                             dim3(TC_WARPS * 32), 0, g));
+    const int tasks = (g.mt + 31) / 32 * ((g.p.head_dim + TC_COLS - 1) / TC_COLS);
+    // few items are shared by many CTAs each; with more items than CTAs one is shared by two, mostly
+    const dim3 grid = g.by_item ? dim3(g.a.n * g.p.n_kv_heads * g.item_blocks, tasks)
+                                : dim3(ctx->sm_count, (tasks + TC_WARPS - 1) / TC_WARPS);
+    VB_CHECK(ctx, pdl_launch(ctx, kernel, grid, dim3(TC_WARPS * 32), 0, g));
     VB_LAUNCH_CHECK(ctx, "tree_combine");
     return VB_OK;
 }
@@ -639,7 +673,7 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     size_t smem;
     tree_fit<TYPE, HDP, R, WM>(g, smem);
     const vb_pages &p = g.p;
-    int rc = tree_prepare(ctx, g, 16 * R * WM, TR_KT);
+    int rc = tree_prepare(ctx, g, 16 * R * WM, 1, TR_KT, TR_OVER);
     if (rc) return rc;
     CUtensorMap tk, tv;
     const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;

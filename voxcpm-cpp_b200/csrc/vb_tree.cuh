@@ -15,15 +15,21 @@ struct TreeArgs {
     vb_pages p;
     float scale_log2;                // scale * log2(e): the softmax runs in powers of two
     int group;                       // query heads per K/V head
-    int mt;                          // most rows of a block
-    int tb;                          // tokens of a block
-    int chunks;                      // blocks that share a token's heads (1 unless group > mt)
+    int tile_rows;                   // rows of a row tile
+    int tile_tokens;                 // tokens of a row tile
+    int tb;                          // tokens of a block, of one or two row tiles
+    int mt;                          // rows of a block's parts: tile_rows for each row tile
+    int chunks;                      // blocks that share a token's heads (1 unless group > tile_rows)
     int kt_log2;                     // cache rows per tile, a power of two
+    int over;                        // what an item costs beside its tiles, in tiles
+    int by_item;                     // `share` goes by item, not by CTA
+    int item_blocks;                 // most blocks of a sequence, for that
     int stages;
     int vec;                         // 16-byte accesses of q and out
+    int q_tma;                       // tcgen05 kernel: TMA loads the queries
     int *err;
     float *part;                     // [2 * CTAs][head_dim + 2][mt]: sums, then the maximum and the sum of the weights
-    struct TreeShare *share;         // [CTAs]
+    struct TreeShare *share;         // [CTAs], or [n][n_kv][item_blocks]
 };
 
 // Sequence i of the call.  T = 0: no rows of q (or none that can be named);
@@ -57,10 +63,11 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &g, int i) {
 }
 
 // A block: tb tokens with the heads of one K/V head (or, where those are more
-// than mt, one token with a chunk of mt heads).  Its rows are its (token,
-// head) pairs, tokens first.  Units of a block: the tiles of the cache rows
-// that its last token sees, at least one, so that every output row is
-// written.  The host refuses calls whose units could pass 2^31.
+// than tile_rows, with a chunk of tile_rows of them).  Row r of its row tile
+// t is token t * tile_tokens + r / heads, head r % heads.  Tiles of a block:
+// those of the cache rows that its last token sees, at least one, so that
+// every output row is written.  In the line of units it counts `over` units
+// more, before them.  The host refuses calls whose units could pass 2^31.
 __device__ __forceinline__ int tree_units(const TreeArgs &g, int visible) {
     return max(1, (visible + (1 << g.kt_log2) - 1) >> g.kt_log2);
 }
@@ -85,9 +92,10 @@ static __device__ __noinline__ uint32_t tree_floor_sum(uint32_t n, int s, uint32
 
 // Units of the first k token blocks (one chunk, one K/V head).
 __device__ __forceinline__ int tree_units_before(const TreeArgs &g, const TreeSeq &q, int k) {
-    if (g.a.mask || q.bad) return k * tree_units(g, q.len);
+    if (g.a.mask || q.bad) return k * (g.over + tree_units(g, q.len));
     const int kt = 1 << g.kt_log2, whole = min(k, q.T / g.tb);       // blocks of tb tokens
-    int u = g.tb >= kt || k <= 4 ? 0 : (int)tree_floor_sum(whole, g.kt_log2, g.tb, q.base + g.tb + kt - 1);
+    int u = k * g.over;
+    u += g.tb >= kt || k <= 4 ? 0 : (int)tree_floor_sum(whole, g.kt_log2, g.tb, q.base + g.tb + kt - 1);
     if (g.tb >= kt || k <= 4)
         for (int j = 0; j < whole; j++) u += tree_units(g, q.base + (j + 1) * g.tb);
     return u + (k > whole ? tree_units(g, q.len) : 0);
@@ -95,31 +103,41 @@ __device__ __forceinline__ int tree_units_before(const TreeArgs &g, const TreeSe
 
 __device__ __forceinline__ int tree_token_blocks(const TreeArgs &g, const TreeSeq &q) { return (q.T + g.tb - 1) / g.tb; }
 
-// A place in the line of units: the item (i, kv head, block) and the tile.
+// A place in the line of units.
 struct TreeWalk {
     TreeSeq q;
-    int i, g, b, chunk;              // block b of tokens
-    int tile, left;                  // left: units of this CTA from here on
-    // the item's
+    int i, g, b, chunk;              // the item: sequence, K/V head, block, chunk of heads
+    int at, pos, left;               // the item's first unit, the place in it, units of this CTA from here on
     int visible, clear, units;       // rows that its last token sees; that every token sees; tiles
-    int tok, heads, head;            // first token, heads of the block, the first of them
-    int rows;
+    int tok, tokens, heads, head;    // first token and their number, heads and the first of them
+    int tile;                        // first tile of this CTA's part
 };
 
 __device__ __forceinline__ void tree_item(const TreeArgs &g, TreeWalk &w) {
     w.tok = w.b * g.tb;
-    const int tokens = min(g.tb, w.q.T - w.tok), h0 = w.chunk * g.mt;
-    w.heads = min(g.mt, g.group - h0);
+    w.tokens = min(g.tb, w.q.T - w.tok);
+    const int h0 = w.chunk * g.tile_rows;
+    w.heads = min(g.tile_rows, g.group - h0);
     w.head = w.g * g.group + h0;
-    w.rows = tokens * w.heads;
     const bool chain = !g.a.mask && !w.q.bad;
-    w.visible = chain ? w.q.base + w.tok + tokens : w.q.len;
+    w.visible = chain ? w.q.base + w.tok + w.tokens : w.q.len;
     w.clear = chain ? w.q.base + w.tok + 1 : w.q.base;
     w.units = tree_units(g, w.visible);
 }
 
+// Takes this CTA's part of the item: its tiles from w.tile on, their number
+// (none when only the item's extra units fell to this CTA).
+__device__ __forceinline__ int tree_take(const TreeArgs &g, TreeWalk &w) {
+    const int n = min(g.over + w.units - w.pos, w.left);
+    w.tile = max(0, w.pos - g.over);
+    w.pos += n;
+    w.left -= n;
+    return max(0, w.pos - g.over) - w.tile;
+}
+
 __device__ __forceinline__ void tree_next(const TreeArgs &g, TreeWalk &w) {
-    w.tile = 0;
+    w.pos = 0;
+    w.at += g.over + w.units;
     if (++w.chunk == g.chunks) {
         w.chunk = 0;
         if (++w.b * g.tb >= w.q.T) {
@@ -173,7 +191,7 @@ __device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWal
     }
     if (lane == 31) sh.scan[warp] = before;
     before -= mine;
-    if (threadIdx.x == 0) g.share[blockIdx.x].last = -1;
+    if (!g.by_item && threadIdx.x == 0) g.share[blockIdx.x].last = -1;
     __syncthreads();
     line.total = 0;
 #pragma unroll
@@ -211,7 +229,7 @@ __device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWal
     w.g = sh.off / each;
     int off = sh.off - w.g * each;
     if (g.a.mask || w.q.bad || nb == 1) {               // blocks of equal length
-        const int u = tree_units(g, w.q.len) * g.chunks;
+        const int u = (g.over + tree_units(g, w.q.len)) * g.chunks;
         w.b = off / u;
         off -= w.b * u;
     } else {
@@ -219,7 +237,7 @@ __device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWal
         const int step = (nb + THREADS - 1) / THREADS, k0 = min(nb, (int)threadIdx.x * step), k1 = min(nb, k0 + step);
         int at = tree_units_before(g, w.q, k0) * g.chunks;
         for (int k = k0; k < k1; k++) {
-            const int u = tree_units(g, w.q.base + min(w.q.T, (k + 1) * g.tb)) * g.chunks;
+            const int u = (g.over + tree_units(g, w.q.base + min(w.q.T, (k + 1) * g.tb))) * g.chunks;
             if (off >= at && off < at + u) {
                 sh.b = k;
                 sh.rest = off - at;
@@ -233,30 +251,40 @@ __device__ __forceinline__ void tree_cut(const TreeArgs &g, TreeCut &sh, TreeWal
     w.chunk = 0;
     tree_item(g, w);
     if (g.chunks > 1) {
-        w.chunk = off / w.units;
-        off -= w.chunk * w.units;
+        w.chunk = off / (g.over + w.units);
+        off -= w.chunk * (g.over + w.units);
         tree_item(g, w);
     }
-    w.tile = off;
+    w.pos = off;
+    w.at = u0 - off;
 }
 
-// An item that goes on in the next CTAs: described by the CTA that holds its
-// first unit (`at`), as its last item.
+// Where an item's parts are, described by the CTA that holds its first tile:
+// for every item, where there are fewer than CTAs, else for a CTA's last item
+// when that goes on in the next ones.
 struct TreeShare {
-    int slot, last;                  // last: the CTA of its last unit; -1: no such item
-    int t0, tok, heads, head, rows, pad;
+    int slot, last;                  // its first part's slot, the CTA of its last tile; -1: nothing to join
+    int first;                       // the CTA of its first
+    int t0, tok, tokens, heads, head;
 };
 
-__device__ __forceinline__ void tree_describe(const TreeArgs &g, const TreeWalk &w, const TreeLine &line, bool first_item) {
-    const int at = line.first(blockIdx.x + 1) - w.left;             // the item's first unit
-    g.share[blockIdx.x] = {(int)blockIdx.x * 2 + (first_item ? 0 : 1), line.owner(at + w.units - 1), w.q.t0, w.tok, w.heads, w.head,
-                           w.rows, 0};
+__device__ __forceinline__ void tree_describe(const TreeArgs &g, const TreeWalk &w, const TreeLine &line, int n, bool first_item) {
+    if (w.tile != 0 || (n == w.units && !g.by_item)) return;
+    const int at = g.by_item ? (w.i * g.p.n_kv_heads + w.g) * g.item_blocks + w.b * g.chunks + w.chunk : (int)blockIdx.x;
+    g.share[at] = {(int)blockIdx.x * 2 + (first_item ? 0 : 1), n == w.units ? -1 : line.owner(w.at + g.over + w.units - 1),
+                   (int)blockIdx.x, w.q.t0, w.tok, w.tokens, w.heads, w.head};
 }
 
-// Where row r of a block lies in q (ld: its row stride) or out.
-__device__ __forceinline__ int64_t tree_row(const TreeArgs &g, int t0, int tok, int heads, int head, int r, int64_t ld) {
-    const int t = r / heads;
-    return (int64_t)(t0 + tok + t) * ld + (int64_t)(head + r - t * heads) * g.p.head_dim;
+// Row r of row tile t of a block: its token in the block (-1: no such row)
+// and where the row lies in q (ld: its row stride) or out.
+__device__ __forceinline__ int tree_token(const TreeArgs &g, int tokens, int heads, int t, int r) {
+    const int k = r / heads;
+    return k < g.tile_tokens && t * g.tile_tokens + k < tokens ? t * g.tile_tokens + k : -1;
+}
+
+__device__ __forceinline__ int64_t tree_row(const TreeArgs &g, int t0, int tok, int heads, int head, int t, int r, int64_t ld) {
+    const int k = r / heads;
+    return (int64_t)(t0 + tok + t * g.tile_tokens + k) * ld + (int64_t)(head + r - k * heads) * g.p.head_dim;
 }
 
 // Whether token j of the sequence sees draft row d (0 <= d < T).
@@ -387,7 +415,7 @@ __device__ __forceinline__ void tree_store8(const TreeArgs &g, int64_t at, const
 
 int launch_tree_tc(vb_ctx *ctx, TreeArgs &g);
 int init_tree_tc(vb_ctx *ctx);
-int tree_prepare(vb_ctx *ctx, TreeArgs &g, int mt, int kt);
+int tree_prepare(vb_ctx *ctx, TreeArgs &g, int tile_rows, int tiles, int kt, int over);
 int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g);
 
 }  // namespace vb

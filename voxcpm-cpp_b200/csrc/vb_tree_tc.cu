@@ -29,7 +29,9 @@ namespace vb {
 constexpr int TT_KT = 128;
 constexpr int TT_THREADS = 384;
 constexpr int TT_SLOTS = 12;
+constexpr int TT_OVER = 2;           // an item's start and end cost about as much as two of its tiles
 constexpr int TT_SMEM = 225 * 1024;
+constexpr int TT_POLY = 5;           // of 16 pairs of weights, those that the multiply-add pipe takes
 constexpr float TT_SLACK = 8.0f;     // log2 of how far a score may exceed the running maximum
 
 // One lane of the (converged) warp.
@@ -163,6 +165,34 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
     return d;
 }
 
+// max(a, b, c), NaN where there is one.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^x of two values on the multiply-add pipe instead of the special-function
+// unit: x = i + f with i its nearest integer (adding 1.5 * 2^23 leaves i in
+// the low bits), 2^f by the cubic of least relative error on [-1/2, 1/2]
+// (7.5e-5, a sixth of fp16's rounding), i added to the exponent.  Values
+// below -126 count as -126; NaN is not kept.
+__device__ __forceinline__ void exp2_pair(uint64_t x2, float &p0, float &p1) {
+    float x0, x1, i0, i1;
+    unpack_f32x2(x2, x0, x1);
+    x2 = pack_f32x2(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+    const uint64_t magic = pack_f32x2(12582912.0f, 12582912.0f);
+    const uint64_t t = add_f32x2(x2, magic);
+    const uint64_t f = add_f32x2(x2, fma_f32x2(t, pack_f32x2(-1.0f, -1.0f), magic));
+    uint64_t p = fma_f32x2(f, pack_f32x2(0.05517167f, 0.05517167f), pack_f32x2(0.24261113f, 0.24261113f));
+    p = fma_f32x2(p, f, pack_f32x2(0.69326097f, 0.69326097f));
+    p = fma_f32x2(p, f, pack_f32x2(0.99992806f, 0.99992806f));
+    unpack_f32x2(p, p0, p1);
+    unpack_f32x2(t, i0, i1);
+    p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(i0) << 23));
+    p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(i1) << 23));
+}
+
 // The ring holds K and V tiles in the order in which the MMAs use them:
 // PAIR K0 V0 K1 V1 ..., else K0 K1 V0 K2 V1 ... V(n-1).
 template <bool PAIR>
@@ -186,7 +216,7 @@ __device__ __forceinline__ int ring_v(int j, int n) { return PAIR ? 2 * j + 1 : 
 template <int TYPE, int HDP, bool PAIR>
 __global__ void __launch_bounds__(TT_THREADS, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                   const __grid_constant__ TreeArgs g) {
+                   const __grid_constant__ CUtensorMap tq, const __grid_constant__ TreeArgs g) {
     constexpr int CB = HDP / 64;
     constexpr uint32_t BLOCK = TT_KT * 128;          // bytes of a 64-value column block of 128 rows
     constexpr uint32_t SLOT = CB * BLOCK;
@@ -196,7 +226,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
     uint8_t *qs = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = qs + (PAIR ? 2 : 1) * SLOT;
     float2 (*ml)[128] = reinterpret_cast<float2 (*)[128]>(ring + (size_t)g.stages * SLOT);   // !PAIR: (max, sum) of both streams
-    __shared__ uint64_t full[TT_SLOTS], empty[TT_SLOTS], q_full, s_full[2], p_full[2], pv_done[2];
+    __shared__ uint64_t full[TT_SLOTS], empty[TT_SLOTS], q_full, q_empty, s_full[2], p_full[2], pv_done[2];
     __shared__ TreeCut cut;
     __shared__ uint32_t s_tmem;
     __shared__ int abort_flag, not_finite[2];        // item number in which a draft value was not finite, by its parity
@@ -207,7 +237,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(&q_full, 8);
+        mbar_init(&q_full, g.q_tma ? 1 : 8);
+        mbar_init(&q_empty, 1);
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
@@ -235,12 +266,33 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
     const int n_slots = g.stages;
 
     if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
         if (warp == 8) {
             // -------------------------------------------------------- loads
             const int P = g.p.page_rows, box = min(P, TT_KT);
-            int pos = 0;
+            int pos = 0, item = 0;
             while (w.left > 0) {
-                const int n = min(w.units - w.tile, w.left);
+                const int n = tree_take(g, w);
+                if (n == 0) {
+                    if (w.left > 0) tree_next(g, w);
+                    continue;
+                }
+                if (g.q_tma) {
+                    // the queries, once the scores of the item before are done
+                    if (item) tree_wait_warp(&q_empty, (uint32_t)(item - 1) & 1u, &abort_flag, g.err);
+                    const int tiles = PAIR && w.tokens > g.tile_tokens ? 2 : 1;
+                    const bool go = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag, 0) == 0;
+                    if (lane == 0) {
+                        if (go) mbar_arrive_expect_tx(&q_full, (uint32_t)(tiles * CB * 128) * (uint32_t)(w.heads * g.tile_tokens));
+                        else mbar_arrive(&q_full);
+                    }
+                    __syncwarp();
+                    if (go && lane < tiles * CB) {
+                        const int t = lane / CB, c = lane % CB;
+                        tma_load_3d(qs + t * SLOT + c * BLOCK, &tq, 64 * c, w.head, w.q.t0 + w.tok + t * g.tile_tokens, &q_full);
+                    }
+                }
+                item++;
                 const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
                 // a lane's row within its box's page, and that page
                 auto page_of = [&](int e, int &y, int &nbox, bool &is_v) {
@@ -284,10 +336,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     nbox = nbox1;
                     is_v = is_v1;
                 }
-                w.left -= n;
                 if (w.left > 0) tree_next(g, w);
             }
             // every copy has landed before the CTA can end
+            if (g.q_tma && item) gm_wait(&q_full, (uint32_t)(item - 1) & 1u);
             for (int s = 0; s < n_slots; s++) {
                 const int fills = pos / n_slots + (pos % n_slots > s ? 1 : 0);
                 if (fills) gm_wait(&full[s], (uint32_t)(fills - 1) & 1u);
@@ -316,7 +368,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             int last = -1;
             uint32_t last_phase = 0;
             while (w.left > 0) {
-                const int n = __shfl_sync(0xffffffffu, min(w.units - w.tile, w.left), 0);
+                const int n = __shfl_sync(0xffffffffu, tree_take(g, w), 0);
+                if (n == 0) {
+                    if (w.left > 0) tree_next(g, w);
+                    continue;
+                }
                 tree_wait_warp(&q_full, (uint32_t)item & 1u, &abort_flag, g.err);
                 tc_fence_after();
                 // One place of the pipeline: the values of tile j, then the scores of
@@ -353,10 +409,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                         }
                         umma_commit_one(one, &s_full[t]);
                         if (!PAIR || t == 1) umma_commit_one(one, &empty[k_slot]);
+                        if (next == n - 1 && (!PAIR || t == 1)) umma_commit_one(one, &q_empty);
                     }
                 }
                 item++;
-                w.left -= n;
                 if (w.left > 0) tree_next(g, w);
             }
             // the last commit has reached its barrier before the CTA can end
@@ -364,31 +420,42 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
         }
     } else {
         // -------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");        // 2 * 176 + 152 = 3 * 168, the launch's share
         const int t = warp >> 2, tid = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // TMEM lane of the warp's first row
         const int hd = g.p.head_dim;
         int pos = 0, item = 0, seen = 0;                             // seen: tiles of this stream so far
         bool first_item = true;
         while (w.left > 0) {
-            const int n = min(w.units - w.tile, w.left);
-            const int rows = w.rows;
-            // the queries of this stream's row tile (of half of the one tile)
-            {
+            const int n = tree_take(g, w);
+            if (n == 0) {
+                if (w.left > 0) tree_next(g, w);
+                continue;
+            }
+            // where TMA cannot: the queries of this stream's row tile (of half of the one tile)
+            if (!g.q_tma) {
                 uint8_t *qt = qs + (PAIR ? t * SLOT : 0);
                 // a thread takes a row (PAIR) or half a row, its loads in flight together
                 constexpr int N_C = HDP / 8 / (PAIR ? 1 : 2);          // 16-byte chunks
-                const int r = PAIR ? tid : (int)threadIdx.x >> 1, m = (PAIR ? 128 * t : 0) + r, c0 = PAIR ? 0 : (threadIdx.x & 1) * N_C;
-                const uint16_t *src = static_cast<const uint16_t *>(g.a.q) + (m < rows ? tree_row(g, w.q.t0, w.tok, w.heads, w.head, m, g.a.ldq) : 0);
+                const int r = PAIR ? tid : (int)threadIdx.x >> 1, c0 = PAIR ? 0 : (threadIdx.x & 1) * N_C;
+                const bool real = tree_token(g, w.tokens, w.heads, PAIR ? t : 0, r) >= 0;
+                const uint16_t *src = static_cast<const uint16_t *>(g.a.q) +
+                                      (real ? tree_row(g, w.q.t0, w.tok, w.heads, w.head, PAIR ? t : 0, r, g.a.ldq) : 0);
+                const int n_c = real ? (hd - 8 * c0) / 8 : 0;              // chunks that exist
                 uint4 x[N_C];
+                if (g.vec) {
 #pragma unroll
-                for (int i = 0; i < N_C; i++) {
-                    const uint16_t *p = src + 8 * (c0 + i);
-                    x[i] = make_uint4(0, 0, 0, 0);
-                    if (m < rows && 8 * (c0 + i) < hd) {
-                        if (g.vec) x[i] = *reinterpret_cast<const uint4 *>(p);
-                        else
-                            x[i] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16,
-                                              p[6] | (uint32_t)p[7] << 16);
+                    for (int i = 0; i < N_C; i++)
+                        x[i] = i < n_c ? *reinterpret_cast<const uint4 *>(src + 8 * (c0 + i)) : make_uint4(0, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N_C; i++) {
+                        uint32_t y[4] = {};
+                        if (i < n_c)
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                y[k] = src[8 * (c0 + i) + 2 * k] | (uint32_t)src[8 * (c0 + i) + 2 * k + 1] << 16;
+                        x[i] = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
 #pragma unroll
@@ -398,9 +465,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
             }
-            const int mrow = (PAIR ? 128 * t : 0) + 32 * (warp & 3) + lane;      // this thread's row of the block
-            const bool alive = mrow - lane < rows;                               // the warp has rows
-            const int j = mrow < rows ? w.tok + mrow / w.heads : -1;
+            const int mrow = 32 * (warp & 3) + lane;                             // this thread's row of the row tile
+            const int in_block = tree_token(g, w.tokens, w.heads, PAIR ? t : 0, mrow);
+            const bool alive = __any_sync(0xffffffffu, in_block >= 0);           // the warp has rows
+            const int j = in_block >= 0 ? w.tok + in_block : -1;
             float m = -INFINITY, l = 0.0f;
             const int mine = PAIR ? n : (n + 1 - t) / 2;                         // tiles of this stream
             for (int x = 0; x < mine; x++, seen++) {
@@ -458,10 +526,54 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                             gone[k] = ~bits;
                         }
                     }
-                    // two passes over the row in pieces of 32, the next piece on
-                    // its way from tensor memory while one is worked on: the
-                    // maximum, then the weights
+                    // One pass over the row in pieces of 32, the next on its way from
+                    // tensor memory: the weights against the running maximum as it
+                    // stands, and the row's own maximum beside them.  They count if
+                    // that maximum is no further than 2^TT_SLACK above and there was
+                    // no NaN; else two passes, the maximum first.  (The weights wait
+                    // in registers: in tensor memory they would take the scores' place.)
                     uint32_t a[32], b[32];
+                    bool done = !edge && x > 0;
+                    if (done) {
+                        const uint64_t off2 = pack_f32x2(-m, -m), scale2 = pack_f32x2(g.scale_log2, g.scale_log2);
+                        uint32_t y[2][32];
+                        uint64_t sum2 = 0;
+                        float t0 = -INFINITY, t1 = -INFINITY;
+                        tmem_ld32_start(sc, a);
+                        tmem_ld32_wait(a);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            uint32_t (&now)[32] = k & 1 ? b : a;
+                            if (k < 3) tmem_ld32_start(sc + 32 * (k + 1), k & 1 ? a : b);
+#pragma unroll
+                            for (int c = 0; c < 16; c++) {
+                                float &z = c & 1 ? t1 : t0;
+                                z = max3_nan(z, __uint_as_float(now[2 * c]), __uint_as_float(now[2 * c + 1]));
+                                const uint64_t v = fma_f32x2(pack_b32x2(now[2 * c], now[2 * c + 1]), scale2, off2);
+                                float p0, p1;
+                                if (c % 16 < TT_POLY) exp2_pair(v, p0, p1);
+                                else {
+                                    unpack_f32x2(v, p0, p1);
+                                    p0 = ex2(p0);
+                                    p1 = ex2(p1);
+                                }
+                                sum2 = add_f32x2(sum2, pack_f32x2(p0, p1));
+                                y[k >> 1][16 * (k & 1) + c] = pack2<TYPE>(p0, p1);
+                            }
+                            if (k < 3) tmem_ld32_wait(k & 1 ? a : b);
+                        }
+                        const float top = max3_nan(t0, t1, t1) * g.scale_log2;
+                        done = !__any_sync(0xffffffffu, !(top <= m + TT_SLACK) || m == -INFINITY);
+                        if (done) {
+                            tmem_st32(sc, y[0]);
+                            tmem_st32(sc + 32, y[1]);
+                            float s0, s1;
+                            unpack_f32x2(sum2, s0, s1);
+                            l += s0 + s1;
+                            tmem_st_wait();
+                        }
+                    }
+                    if (!done) {
                     float top = -INFINITY;
                     auto piece_max = [&](uint32_t (&x)[32], uint32_t out) {
                         if (edge)
@@ -539,6 +651,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     unpack_f32x2(sum2, s0, s1);
                     l += s0 + s1;
                     tmem_st_wait();
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -547,7 +660,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             if (mine > 0) tree_wait_warp(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
 
             // ---- the block's result, or this CTA's part of it
-            const bool whole = w.tile == 0 && n == w.units;
+            const bool whole = n == w.units;
             float f0 = 1.0f, f1 = 0.0f;
             if (!PAIR) {
                 ml[t][tid] = make_float2(m, l);
@@ -563,9 +676,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             tc_fence_after();
             const bool mend = *(volatile int *)&not_finite[item & 1] == item;
             if (alive) {
-                const int64_t out = tree_row(g, w.q.t0, w.tok, w.heads, w.head, mrow, g.a.ldo);
+                const int64_t out = tree_row(g, w.q.t0, w.tok, w.heads, w.head, PAIR ? t : 0, mrow, g.a.ldo);
                 const float inv = whole ? (l > 0.0f || l != l ? 1.0f / l : 0.0f) : 1.0f;
-                float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * (hd + 2) * MT + mrow;
+                float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * (hd + 2) * MT + (PAIR ? 128 * t : 0) + mrow;
                 if (!whole && (PAIR || t == 0)) {
                     part[(size_t)hd * MT] = m;
                     part[(size_t)(hd + 1) * MT] = l;
@@ -609,12 +722,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             __syncwarp();
             tc_fence_before();
             if (!PAIR) consumer_sync(256);           // both streams' sums are read: the next item may overwrite them
-            if (threadIdx.x == 0 && w.tile == 0 && !whole) tree_describe(g, w, line, first_item);
+            if (threadIdx.x == 0) tree_describe(g, w, line, n, first_item);
             __syncwarp();
             first_item = false;
             pos += 2 * n;
             item++;
-            w.left -= n;
             if (w.left > 0) tree_next(g, w);
         }
     }
@@ -634,23 +746,29 @@ static int launch_tc(vb_ctx *ctx, TreeArgs &g) {
     const size_t rest = 1024 + q + (PAIR ? 0 : 2 * 128 * sizeof(float2));
     g.stages = (int)std::min<size_t>(TT_SLOTS, (TT_SMEM - rest) / slot);
     const size_t smem = rest + g.stages * slot;
-    int rc = tree_prepare(ctx, g, PAIR ? 256 : 128, TT_KT);
+    int rc = tree_prepare(ctx, g, 128, PAIR ? 2 : 1, TT_KT, TT_OVER);
     if (rc) return rc;
-    CUtensorMap tk, tv;
+    CUtensorMap tk, tv, tq;
     const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;
     const CUtensorMapDataType dt = p.type == VB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const int box = std::min(p.page_rows, TT_KT);
     if (!make_map(&tk, static_cast<char *>(p.k) + layer, dt, 2, p.head_dim, rows, 64, box, true) ||
         !make_map(&tv, static_cast<char *>(p.v) + layer, dt, 2, p.head_dim, rows, 64, box, true))
         return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the cache refused");
-    VB_CHECK(ctx, pdl_launch(ctx, tree_tc_kernel<TYPE, HDP, PAIR>, dim3(ctx->sm_count), dim3(TT_THREADS), smem, tk, tv, g));
+    // queries whose rows TMA can gather: a box is the heads of tile_tokens tokens
+    g.q_tma = g.vec && g.chunks == 1;
+    if (!g.q_tma) tq = tk;
+    else if (!make_map_3d(&tq, g.a.q, dt, p.head_dim, g.a.n_heads, g.a.n_tokens, (int64_t)p.head_dim * 2, g.a.ldq * 2, 64, g.group,
+                          g.tile_tokens))
+        return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the queries refused");
+    VB_CHECK(ctx, pdl_launch(ctx, tree_tc_kernel<TYPE, HDP, PAIR>, dim3(ctx->sm_count), dim3(TT_THREADS), smem, tk, tv, tq, g));
     VB_LAUNCH_CHECK(ctx, "tree_tc");
     return launch_tree_combine(ctx, g);
 }
 
 template <int TYPE, int HDP>
 static int launch_tc_rows(vb_ctx *ctx, TreeArgs &g) {
-    return (int64_t)g.a.max_tokens * g.group > 128 ? launch_tc<TYPE, HDP, true>(ctx, g) : launch_tc<TYPE, HDP, false>(ctx, g);
+    return g.a.max_tokens > std::max(1, 128 / g.group) ? launch_tc<TYPE, HDP, true>(ctx, g) : launch_tc<TYPE, HDP, false>(ctx, g);
 }
 
 int launch_tree_tc(vb_ctx *ctx, TreeArgs &g) {
