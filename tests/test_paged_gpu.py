@@ -538,6 +538,16 @@ def test_tree_many_tiles_for_each_cta(ctx, type, lens, drafted, P):
     check_tree(ctx, t)
 
 
+@pytest.mark.parametrize("type", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("drafted", [1, 8, 40])
+def test_tree_rings_go_round(ctx, type, drafted):
+    """Every CTA goes many times round its ring of tiles, faster than they come."""
+    t = tree_case(ctx, type, [200000], [drafted], 2 if drafted > 1 else 1, 1, 128, 64, seed=9, layers=1)
+    for _ in range(12):
+        ctx.tree_attention(t["args"])
+    check_tree(ctx, t)
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 def test_tree_many_sequences_and_long_chains(ctx, type):
     rng = np.random.default_rng(1)

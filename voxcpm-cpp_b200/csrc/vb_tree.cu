@@ -627,6 +627,11 @@ static void tree_fit(TreeArgs &g, size_t &smem) {
     constexpr size_t rest = (size_t)4 * 16 * (HDP + 4) * 4 + (size_t)QT * MT * (HDP * 2 + 16) + (size_t)8 * 16 * R * 8 + 1024;
     static_assert(rest + 2 * stage <= TR_SMEM, "two stages must fit");
     g.stages = (int)std::min<size_t>(TR_MAX_STAGES, (TR_SMEM - rest) / stage);
+    // two sets of warps take tiles in turn: an even ring gives each its own
+    // stages.  (A set that met a stage of the other's could wait for its
+    // second fill while the first is still on its way, and a parity wait
+    // takes that for the phase before, which is over.)
+    if (WM == 1) g.stages &= ~1;
     smem = g.stages * stage + rest;
 }
 

@@ -475,7 +475,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 const int jt = PAIR ? x : 2 * x + t;
                 const int r0 = (w.tile + jt) * TT_KT;
                 const bool edge = r0 + TT_KT > w.clear;          // not every row is seen by every token
+                tree_wait_warp(&s_full[t], (uint32_t)seen & 1u, &abort_flag, g.err);
+                tc_fence_after();
                 if (edge && (t == 0 || !PAIR)) {
+                    // (after the scores: the ring's tiles up to their K have landed, so
+                    // this slot's fill before V is over and the parity names V's)
                     // V rows past the end may hold anything: they become zeros,
                     // as do draft values that are not finite
                     const int at = pos + ring_v<PAIR>(jt, n);
@@ -498,8 +502,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     __syncwarp();
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                tree_wait_warp(&s_full[t], (uint32_t)seen & 1u, &abort_flag, g.err);
-                tc_fence_after();
                 if (alive) {
                     const uint32_t sc = tmem + 128 * t + lanes;
                     // columns that this row does not see, 32 to a word
