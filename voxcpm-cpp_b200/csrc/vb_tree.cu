@@ -534,84 +534,118 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 }
 
 // Joins the parts of items that several CTAs shared.  A task is 32 rows by
-// 16 columns of an item; a lane holds a row of it.  grid (entry of `share`,
-// tasks): where an item has many parts the warps of a CTA take them in turn
-// and are added in shared memory, else each warp has a task of its own.
-constexpr int TC_WARPS = 8;
+// 16 columns of an item; a lane holds a row of it and adds up parts, several
+// of them on their way at once.
 constexpr int TC_COLS = 16;
-constexpr int TC_FEW = 4;            // parts
-template <int TYPE>
-__global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeArgs g) {
-    __shared__ float so[TC_WARPS][TC_COLS][32], sm[TC_WARPS][32], sl[TC_WARPS][32];
+
+struct TreeTask {
+    int row, t, tr, col, cols;
+    bool real;
+};
+
+__device__ __forceinline__ TreeTask tree_task(const TreeArgs &g, const TreeShare &d, int task) {
+    const int lane = threadIdx.x & 31, row_tasks = (g.mt + 31) / 32;
+    TreeTask k;
+    const int r = task % row_tasks * 32 + lane;
+    k.col = task / row_tasks * TC_COLS;
+    k.cols = min(TC_COLS, g.p.head_dim - k.col);
+    k.t = r / g.tile_rows;
+    k.tr = r - k.t * g.tile_rows;
+    k.real = r < g.mt && tree_token(g, d.tokens, d.heads, k.t, k.tr) >= 0;
+    k.row = k.real ? r : 0;
+    return k;
+}
+
+// Parts of CTAs first, first + step, ... of the item.
+template <int AHEAD>
+__device__ __forceinline__ void tree_join(const TreeArgs &g, const TreeShare &d, const TreeTask &k, int first, int step, float &m, float &l,
+                                          float (&o)[TC_COLS]) {
+    const int hd = g.p.head_dim;
+    for (int c0 = first; c0 <= d.last; c0 += AHEAD * step) {
+        float om[AHEAD], ol[AHEAD], v[AHEAD][TC_COLS];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int c = c0 + a * step;
+            const float *part = g.part + (size_t)(c == d.first ? d.slot : 2 * c) * (hd + 2) * g.mt + k.row;
+            const bool there = c <= d.last;
+            om[a] = there ? part[(size_t)hd * g.mt] : -INFINITY;
+            ol[a] = there ? part[(size_t)(hd + 1) * g.mt] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < TC_COLS; i++) v[a][i] = there && i < k.cols ? part[(size_t)(k.col + i) * g.mt] : 0.0f;
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const float mn = fmaxf(m, om[a]), ms = mn == -INFINITY ? 0.0f : mn;
+            const float f = ex2(m - ms), e = ex2(om[a] - ms);
+            m = mn;
+            l = l * f + ol[a] * e;
+#pragma unroll
+            for (int i = 0; i < TC_COLS; i++) o[i] = o[i] * f + v[a][i] * e;
+        }
+    }
+}
+
+// Few items, each shared by many CTAs: grid (item, task), the warps take the
+// parts in turn and are added in shared memory in their order.
+template <int TYPE, int TC_MANY>
+__global__ void __launch_bounds__(TC_MANY * 32) tree_join_many(const __grid_constant__ TreeArgs g) {
+    __shared__ float so[TC_MANY][TC_COLS][32], sm[TC_MANY][32], sl[TC_MANY][32];
     pdl_trigger();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = g.p.head_dim;
-    if (g.by_item) {                                 // the entry was written if the item exists
-        const int c = blockIdx.x % g.item_blocks, i = blockIdx.x / g.item_blocks / g.p.n_kv_heads;
-        if (c / g.chunks * g.tb >= tree_seq(g, i).T) return;
+    // the entry was written if the item exists
+    const int b = blockIdx.x % g.item_blocks / g.chunks, i = blockIdx.x / g.item_blocks / g.p.n_kv_heads;
+    const TreeShare d = g.share[blockIdx.x];
+    if (b * g.tb >= tree_seq(g, i).T || d.last < 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const TreeTask k = tree_task(g, d, blockIdx.y);
+    if (!__any_sync(0xffffffffu, k.real)) return;     // for the whole CTA alike: the rows are the same in every warp
+    float m = -INFINITY, l = 0.0f, o[TC_COLS] = {};
+    tree_join<3>(g, d, k, d.first + warp, TC_MANY, m, l, o);
+#pragma unroll
+    for (int c = 0; c < TC_COLS; c++) so[warp][c][lane] = o[c];
+    sm[warp][lane] = m;
+    sl[warp][lane] = l;
+    __syncthreads();
+    if (8 * warp >= k.cols) return;                   // two warps write eight columns each
+    float top = -INFINITY, sum = 0.0f, f[TC_MANY], y[8] = {};
+#pragma unroll
+    for (int w = 0; w < TC_MANY; w++) top = fmaxf(top, sm[w][lane]);
+    const float ms = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < TC_MANY; w++) {
+        f[w] = ex2(sm[w][lane] - ms);
+        sum = fmaf(sl[w][lane], f[w], sum);
+#pragma unroll
+        for (int c = 0; c < 8; c++) y[c] = fmaf(so[w][8 * warp + c][lane], f[w], y[c]);
     }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int c = 0; c < 8; c++) y[c] *= inv;
+    if (k.real) tree_store8<TYPE>(g, tree_row(g, d.t0, d.tok, d.heads, d.head, k.t, k.tr, g.a.ldo) + k.col + 8 * warp, y);
+}
+
+// More items, of two or three parts, seldom more:
+// grid (CTA whose last item goes on, tasks / 4), a task for each warp.
+constexpr int TC_FEW = 4;            // warps
+template <int TYPE>
+__global__ void __launch_bounds__(TC_FEW * 32) tree_join_few(const __grid_constant__ TreeArgs g) {
+    pdl_trigger();
+    pdl_wait();
     const TreeShare d = g.share[blockIdx.x];
     if (d.last < 0) return;
-    const bool few = d.last - d.first < TC_FEW;
-    const int row_tasks = (g.mt + 31) / 32, tasks = row_tasks * ((hd + TC_COLS - 1) / TC_COLS);
-    for (int task = few ? blockIdx.y * TC_WARPS + warp : blockIdx.y; task < tasks; task += gridDim.y * (few ? TC_WARPS : 1)) {
-        const int mr = task % row_tasks * 32 + lane, col = task / row_tasks * TC_COLS;
-        const int t = mr / g.tile_rows, tr = mr - t * g.tile_rows;
-        const bool real = mr < g.mt && tree_token(g, d.tokens, d.heads, t, tr) >= 0;
-        // (for the whole CTA alike: a task's rows are the same in every warp)
-        if (!__any_sync(0xffffffffu, real)) continue;
-        const int at = real ? mr : 0, cols = min(TC_COLS, hd - col);
-        float m = -INFINITY, l = 0.0f, o[TC_COLS];
+    const int task = blockIdx.y * TC_FEW + (threadIdx.x >> 5);
+    const TreeTask k = tree_task(g, d, task);
+    if (k.cols <= 0 || !k.real) return;
+    float m = -INFINITY, l = 0.0f, o[TC_COLS] = {};
+    tree_join<2>(g, d, k, d.first, 1, m, l, o);
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const int64_t dst = tree_row(g, d.t0, d.tok, d.heads, d.head, k.t, k.tr, g.a.ldo) + k.col;
 #pragma unroll
-        for (int c = 0; c < TC_COLS; c++) o[c] = 0.0f;
-#pragma unroll 2
-        for (int k = d.first + (few ? 0 : warp); k <= d.last; k += few ? 1 : TC_WARPS) {
-            const float *part = g.part + (size_t)(k == d.first ? d.slot : 2 * k) * (hd + 2) * g.mt + at;
-            const float om = part[(size_t)hd * g.mt], ol = part[(size_t)(hd + 1) * g.mt];
-            float v[TC_COLS];
+    for (int c = 0; c < TC_COLS; c += 8) {
+        float y[8];
 #pragma unroll
-            for (int c = 0; c < TC_COLS; c++) v[c] = c < cols ? part[(size_t)(col + c) * g.mt] : 0.0f;
-            const float mn = fmaxf(m, om), ms = mn == -INFINITY ? 0.0f : mn;
-            const float f = ex2(m - ms), e = ex2(om - ms);
-            m = mn;
-            l = l * f + ol * e;
-#pragma unroll
-            for (int c = 0; c < TC_COLS; c++) o[c] = o[c] * f + v[c] * e;
-        }
-        const int64_t dst = tree_row(g, d.t0, d.tok, d.heads, d.head, t, tr, g.a.ldo) + col;
-        if (few) {
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-#pragma unroll
-            for (int c = 0; c < TC_COLS; c += 8) {
-                float y[8];
-#pragma unroll
-                for (int k = 0; k < 8; k++) y[k] = o[c + k] * inv;
-                if (real && c < cols) tree_store8<TYPE>(g, dst + c, y);
-            }
-            continue;
-        }
-        __syncthreads();                              // the task before has been read
-#pragma unroll
-        for (int c = 0; c < TC_COLS; c++) so[warp][c][lane] = o[c];
-        sm[warp][lane] = m;
-        sl[warp][lane] = l;
-        __syncthreads();
-        if (8 * warp >= cols) continue;               // warps 0 and 1 write eight columns each
-        float top = -INFINITY, sum = 0.0f, f[TC_WARPS], y[8] = {};
-#pragma unroll
-        for (int k = 0; k < TC_WARPS; k++) top = fmaxf(top, sm[k][lane]);
-        const float ms = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int k = 0; k < TC_WARPS; k++) {
-            f[k] = ex2(sm[k][lane] - ms);
-            sum = fmaf(sl[k][lane], f[k], sum);
-#pragma unroll
-            for (int c = 0; c < 8; c++) y[c] = fmaf(so[k][8 * warp + c][lane], f[k], y[c]);
-        }
-        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-#pragma unroll
-        for (int c = 0; c < 8; c++) y[c] *= inv;
-        if (real) tree_store8<TYPE>(g, dst + 8 * warp, y);
+        for (int i = 0; i < 8; i++) y[i] = o[c + i] * inv;
+        if (c < k.cols) tree_store8<TYPE>(g, dst + c, y);
     }
 }
 
@@ -650,7 +684,7 @@ int tree_prepare(vb_ctx *ctx, TreeArgs &g, int tile_rows, int tiles, int kt, int
     const int64_t most = ((int64_t)g.p.max_pages * g.p.page_rows + kt - 1) / kt + over;
     if ((double)items * (double)most >= 2147483647.0)
         return set_error(ctx, VB_ERR_INVALID_ARG, "vb_tree_attention: too many rows for one call");
-    g.by_item = items < ctx->sm_count;
+    g.by_item = items * 4 <= ctx->sm_count;      // four parts each, or more
     g.item_blocks = (int)blocks;
     const size_t parts = (size_t)2 * ctx->sm_count * g.mt * (g.p.head_dim + 2) * sizeof(float);
     int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)ctx->sm_count * sizeof(TreeShare));
@@ -660,16 +694,23 @@ int tree_prepare(vb_ctx *ctx, TreeArgs &g, int tile_rows, int tiles, int kt, int
     return VB_OK;
 }
 
-int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g) {
-    auto kernel = g.a.type == VB_TYPE_F32   ? tree_combine_kernel<TR_F32>
-                  : g.a.type == VB_TYPE_F16 ? tree_combine_kernel<TR_F16>
-                                            : tree_combine_kernel<TR_BF16>;
+template <int TYPE>
+static cudaError_t launch_join(vb_ctx *ctx, const TreeArgs &g) {
     const int tasks = (g.mt + 31) / 32 * ((g.p.head_dim + TC_COLS - 1) / TC_COLS);
-    // few items are shared by many CTAs each; with more items than CTAs one is shared by two, mostly
-    const dim3 grid = g.by_item ? dim3(g.a.n * g.p.n_kv_heads * g.item_blocks, tasks)
-                                : dim3(ctx->sm_count, (tasks + TC_WARPS - 1) / TC_WARPS);
-    VB_CHECK(ctx, pdl_launch(ctx, kernel, grid, dim3(TC_WARPS * 32), 0, g));
-    VB_LAUNCH_CHECK(ctx, "tree_combine");
+    if (g.by_item) {
+        const int items = g.a.n * g.p.n_kv_heads * g.item_blocks;
+        if (items * 16 <= ctx->sm_count)
+            return pdl_launch(ctx, tree_join_many<TYPE, 16>, dim3(items, tasks), dim3(16 * 32), 0, g);
+        return pdl_launch(ctx, tree_join_many<TYPE, 4>, dim3(items, tasks), dim3(4 * 32), 0, g);
+    }
+    return pdl_launch(ctx, tree_join_few<TYPE>, dim3(ctx->sm_count, (tasks + TC_FEW - 1) / TC_FEW), dim3(TC_FEW * 32), 0, g);
+}
+
+int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g) {
+    VB_CHECK(ctx, g.a.type == VB_TYPE_F32   ? launch_join<TR_F32>(ctx, g)
+                  : g.a.type == VB_TYPE_F16 ? launch_join<TR_F16>(ctx, g)
+                                            : launch_join<TR_BF16>(ctx, g));
+    VB_LAUNCH_CHECK(ctx, "tree_join");
     return VB_OK;
 }
 

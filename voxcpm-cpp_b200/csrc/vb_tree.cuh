@@ -95,9 +95,19 @@ __device__ __forceinline__ int tree_units_before(const TreeArgs &g, const TreeSe
     if (g.a.mask || q.bad) return k * (g.over + tree_units(g, q.len));
     const int kt = 1 << g.kt_log2, whole = min(k, q.T / g.tb);       // blocks of tb tokens
     int u = k * g.over;
-    u += g.tb >= kt || k <= 4 ? 0 : (int)tree_floor_sum(whole, g.kt_log2, g.tb, q.base + g.tb + kt - 1);
-    if (g.tb >= kt || k <= 4)
+    if (k <= 4 || g.tb >= kt) {
         for (int j = 0; j < whole; j++) u += tree_units(g, q.base + (j + 1) * g.tb);
+    } else if ((g.tb & (g.tb - 1)) == 0) {
+        // tb divides kt: sum of floor((j + c) / r), r = kt / tb
+        const int r_log2 = g.kt_log2 - (31 - __clz(g.tb)), c = (q.base + g.tb + kt - 1) / g.tb;
+        auto sum = [&](int64_t x) {                   // of floor(i / r) for i < x
+            const int64_t m = x >> r_log2;
+            return (m * (m - 1) / 2 << r_log2) + m * (x - (m << r_log2));
+        };
+        u += (int)(sum((int64_t)whole + c) - sum(c));
+    } else {
+        u += (int)tree_floor_sum(whole, g.kt_log2, g.tb, q.base + g.tb + kt - 1);
+    }
     return u + (k > whole ? tree_units(g, q.len) : 0);
 }
 

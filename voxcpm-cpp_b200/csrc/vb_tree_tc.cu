@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             mbar_init(&empty[s], 1);
         }
         mbar_init(&q_full, g.q_tma ? 1 : 8);
-        mbar_init(&q_empty, 1);
+        mbar_init(&q_empty, 2);
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
@@ -357,16 +357,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             uint32_t ring_phase = 0, phase = 0;       // phase: parity of p_full, a bit per stream
             auto take = [&]() {
                 tree_wait_warp(&full[slot], ring_phase, &abort_flag, g.err);
-                tc_fence_after();
                 const int s = slot;
                 if (++slot == n_slots) {
                     slot = 0;
                     ring_phase ^= 1u;
                 }
-                return s;
+                return (uint32_t)s * (SLOT >> 4);
             };
-            int last = -1;
-            uint32_t last_phase = 0;
             while (w.left > 0) {
                 const int n = __shfl_sync(0xffffffffu, tree_take(g, w), 0);
                 if (n == 0) {
@@ -374,49 +371,46 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     continue;
                 }
                 tree_wait_warp(&q_full, (uint32_t)item & 1u, &abort_flag, g.err);
-                tc_fence_after();
-                // One place of the pipeline: the values of tile j, then the scores of
-                // the tile that stream t takes next.
-                int v_slot = 0, k_slot = 0;
+                // One place of the pipeline: the values of tile j, the scores of the
+                // tile that stream t takes next, and one commit for both (a commit
+                // holds up the MMAs behind it, and scores that have come say that the
+                // values before them are done: no other commit is needed).
+                uint32_t v_slot = 0, k_slot = 0;
 #pragma unroll 1
                 for (int x = -2; x < (PAIR ? 2 * n : n); x++) {
                     const int j = PAIR ? x >> 1 : x, t = x & 1, next = j + (PAIR ? 1 : 2);
+                    const bool scores = next >= 0 && next < n;
+                    if (!PAIR || t == 0) {
+                        if (j >= 0) v_slot = take();
+                        if (scores) k_slot = take();
+                    }
                     if (j >= 0) {
-                        if (!PAIR || t == 0) {
-                            last_phase = ring_phase;
-                            last = v_slot = take();
-                        }
-                        const uint64_t v = d_v + (uint64_t)((uint32_t)v_slot * (SLOT >> 4));
-                        const uint32_t p = tmem + 128 * t, o = tmem + 256 + HDP * t;
-                        const uint32_t more = PAIR ? j > 0 : j > 1;
                         tree_wait_warp(&p_full[t], phase >> t & 1u, &abort_flag, g.err);
                         phase ^= 1u << t;
-                        tc_fence_after();
+                    }
+                    tc_fence_after();
+                    if (j >= 0) {
+                        const uint64_t v = d_v + v_slot;
+                        const uint32_t p = tmem + 128 * t, o = tmem + 256 + HDP * t;
+                        const uint32_t more = PAIR ? j > 0 : j > 1;
 #pragma unroll
                         for (int i = 0; i < TT_KT / 16; i++)
                             umma_f16_ts(one, o, p + 8 * i, v + (uint64_t)(i * (2048 >> 4)), id_o, i ? 1u : more);
-                        umma_commit_one(one, &pv_done[t]);
-                        if (!PAIR || t == 1) umma_commit_one(one, &empty[v_slot]);
                     }
-                    if (next >= 0 && next < n) {
-                        if (!PAIR || t == 0) k_slot = take();
-                        const uint64_t k = d_k + (uint64_t)((uint32_t)k_slot * (SLOT >> 4)), q = d_q + (uint64_t)(PAIR ? t * (SLOT >> 4) : 0);
+                    if (scores) {
+                        const uint64_t k = d_k + k_slot, q = d_q + (uint64_t)(PAIR ? t * (SLOT >> 4) : 0);
                         const uint32_t sc = tmem + 128 * t;
 #pragma unroll
                         for (int i = 0; i < HDP / 16; i++) {
                             const uint64_t off = (i >> 2) * (BLOCK >> 4) + (i & 3) * 2;
                             umma_f16_ss(one, sc, q + off, k + off, id_s, i ? 1u : 0u);
                         }
-                        umma_commit_one(one, &s_full[t]);
-                        if (!PAIR || t == 1) umma_commit_one(one, &empty[k_slot]);
-                        if (next == n - 1 && (!PAIR || t == 1)) umma_commit_one(one, &q_empty);
                     }
+                    if (scores || j >= 0) umma_commit_one(one, scores ? &s_full[t] : &pv_done[t]);
                 }
                 item++;
                 if (w.left > 0) tree_next(g, w);
             }
-            // the last commit has reached its barrier before the CTA can end
-            if (last >= 0) tree_wait_warp(&empty[last], last_phase, &abort_flag, g.err);
         }
     } else {
         // -------------------------------------------------------- softmax
@@ -424,7 +418,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
         const int t = warp >> 2, tid = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // TMEM lane of the warp's first row
         const int hd = g.p.head_dim;
-        int pos = 0, item = 0, seen = 0;                             // seen: tiles of this stream so far
+        const bool lead = (warp & 3) == 0 && lane == 0;
+        int pos = 0, item = 0, seen = 0, ends = 0;                   // tiles and items of this stream so far
         bool first_item = true;
         while (w.left > 0) {
             const int n = tree_take(g, w);
@@ -477,6 +472,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 const bool edge = r0 + TT_KT > w.clear;          // not every row is seen by every token
                 tree_wait_warp(&s_full[t], (uint32_t)seen & 1u, &abort_flag, g.err);
                 tc_fence_after();
+                // what the scores' MMAs and those before them read is free again
+                if (lead) {
+                    if (t == 1 || !PAIR) {
+                        mbar_arrive(&empty[(pos + ring_k<PAIR>(jt)) % n_slots]);
+                        if (x > 0) mbar_arrive(&empty[(pos + ring_v<PAIR>(jt - (PAIR ? 1 : 2), n)) % n_slots]);
+                    }
+                    if (g.q_tma && x == mine - 1) mbar_arrive(&q_empty);
+                }
                 if (edge && (t == 0 || !PAIR)) {
                     // (after the scores: the ring's tiles up to their K have landed, so
                     // this slot's fill before V is over and the parity names V's)
@@ -608,8 +611,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                         const float f = move ? ex2(m - now) : 1.0f;
                         if (move) m = now;
                         l *= f;
-                        tree_wait_warp(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
-                        tc_fence_after();
+                        // (the scores have come, so the values before them are done)
 #pragma unroll 1
                         for (int k = 0; k < HDP / 32; k++) {
                             float o[32];
@@ -659,7 +661,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
             }
-            if (mine > 0) tree_wait_warp(&pv_done[t], (uint32_t)(seen - 1) & 1u, &abort_flag, g.err);
+            if (mine > 0) {
+                tree_wait_warp(&pv_done[t], (uint32_t)ends & 1u, &abort_flag, g.err);
+                ends++;
+                if (lead && (t == 1 || !PAIR)) mbar_arrive(&empty[(pos + ring_v<PAIR>(PAIR ? n - 1 : 2 * mine - 2 + t, n)) % n_slots]);
+            } else if (lead && g.q_tma) {
+                mbar_arrive(&q_empty);
+            }
 
             // ---- the block's result, or this CTA's part of it
             const bool whole = n == w.units;
