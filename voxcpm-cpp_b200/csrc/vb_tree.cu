@@ -111,48 +111,46 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp > 8) return;
         // ------------------------------------------------------------ loads
-        const int P = g.p.page_rows, box = min(P, TR_KT), boxes = TR_KT / box;
+        // Four warps issue a tile's copies (a box per page, column block and
+        // K or V; with pages of 16 rows 16 of them, more than one warp can
+        // issue in the time of a tile).  Every warp waits for every stage, so
+        // that none meets a barrier two fills ahead.
+        const int P = g.p.page_rows, box = min(P, TR_KT), me = warp - 8;
         int it = 0;
         while (w.left > 0) {
             const int n_tiles = tree_take(g, w);
             const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
-            int pages = 0;                              // lane's page of the current 32 boxes
-            for (int x = 0; x < n_tiles; x++, it++) {
-                const int r0 = (w.tile + x) * TR_KT;
-                const int have = min(TR_KT, w.visible - r0);              // rows of the tile that count
-                const int nbox = have <= 0 ? 0 : (have + box - 1) / box;
-                const int k0 = x * boxes % 32;                            // first lane of this tile's boxes
-                if (k0 == 0) {
-                    const int r = r0 + lane * box;
-                    pages = 0;
-                    if (r < w.visible) {
-                        pages = row[r / P];
-                        if (pages < 0 || pages >= g.p.n_pages) {
-                            atomicCAS(g.err, 0, VB_DEV_TREE_PAGE);
-                            pages = 0;
-                        }
-                    }
+            // unit u of a tile: K or V, box u / 2 / CB, column block u / 2 % CB
+            const int u = 4 * lane + me, k = u / 2 / CB, c = u / 2 % CB;
+            auto place = [&](int x) {                   // row of the pool that the lane's box starts at
+                const int r = (w.tile + x) * TR_KT + k * box;
+                if (r >= w.visible || k * box >= TR_KT) return 0;
+                int page = row[r / P];
+                if (page < 0 || page >= g.p.n_pages) {
+                    atomicCAS(g.err, 0, VB_DEV_TREE_PAGE);
+                    page = 0;
                 }
+                return (page * g.p.n_kv_heads + w.g) * P + r % P;
+            };
+            int y = n_tiles > 0 ? place(0) : 0;
+            for (int x = 0; x < n_tiles; x++, it++) {
+                const int y1 = x + 1 < n_tiles ? place(x + 1) : 0;
+                const int have = min(TR_KT, w.visible - (w.tile + x) * TR_KT);        // rows of the tile that count
+                const int nbox = have <= 0 ? 0 : (have + box - 1) / box;
                 const int s = it % g.stages;
                 tree_wait_warp(&empty[s], ((uint32_t)(it / g.stages) & 1u) ^ 1u, &abort_flag, g.err);
-                const int nload = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag ? 0 : nbox, 0);
-                uint8_t *st = ring + (size_t)s * STAGE;
-                if (lane == 0) {
-                    if (nload) mbar_arrive_expect_tx(&full[s], (uint32_t)nload * box * 128 * 2 * CB);
+                // after a wait that ran out no barrier is touched any more
+                const bool go = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag, 0) == 0;
+                if (go && me == 0 && lane == 0) {
+                    if (nbox) mbar_arrive_expect_tx(&full[s], (uint32_t)nbox * box * 128 * 2 * CB);
                     else mbar_arrive(&full[s]);
                 }
+                if (go && k < nbox)
+                    tma_load_2d(ring + (size_t)s * STAGE + ((u & 1) * CB + c) * TILE + k * box * 128, u & 1 ? &tv : &tk, 64 * c, y,
+                                &full[s]);
                 __syncwarp();
-                const int k = lane - k0;
-                if (k >= 0 && k < nload) {
-                    const int y = (pages * g.p.n_kv_heads + w.g) * P + (r0 + k * box) % P;
-#pragma unroll
-                    for (int c = 0; c < CB; c++) {
-                        tma_load_2d(st + c * TILE + k * box * 128, &tk, 64 * c, y, &full[s]);
-                        tma_load_2d(st + (CB + c) * TILE + k * box * 128, &tv, 64 * c, y, &full[s]);
-                    }
-                }
+                y = y1;
             }
             if (w.left > 0) tree_next(g, w);
         }

@@ -267,70 +267,73 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
-        if (warp == 8) {
+        if (warp != 9) {
             // -------------------------------------------------------- loads
-            const int P = g.p.page_rows, box = min(P, TT_KT);
-            int pos = 0, item = 0;
+            // Three warps issue a tile's copies (a box per page and column
+            // block: 16 of them with pages of 16 rows, more than one warp can
+            // issue in the time of a tile).  Every warp waits for every slot, so
+            // that none meets a barrier two fills ahead.
+            const int P = g.p.page_rows, box = min(P, TT_KT), me = warp == 8 ? 0 : warp - 9;
+            const int u = 3 * lane + me, k = u / CB, c = u % CB;         // box and column block of the lane's copy
+            int slot = 0, item = 0;
+            uint32_t phase = 1;
+            bool filled = false;                                         // the ring has gone round
+            // after a wait that ran out no barrier is touched any more
+            auto going = [&]() { return __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag, 0) == 0; };
             while (w.left > 0) {
                 const int n = tree_take(g, w);
                 if (n == 0) {
                     if (w.left > 0) tree_next(g, w);
                     continue;
                 }
-                if (g.q_tma) {
+                if (g.q_tma && me == 0) {
                     // the queries, once the scores of the item before are done
                     if (item) tree_wait_warp(&q_empty, (uint32_t)(item - 1) & 1u, &abort_flag, g.err);
                     const int tiles = PAIR && w.tokens > g.tile_tokens ? 2 : 1;
-                    const bool go = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag, 0) == 0;
-                    if (lane == 0) {
-                        if (go) mbar_arrive_expect_tx(&q_full, (uint32_t)(tiles * CB * 128) * (uint32_t)(w.heads * g.tile_tokens));
-                        else mbar_arrive(&q_full);
-                    }
+                    const bool go = going();
+                    if (go && lane == 0) mbar_arrive_expect_tx(&q_full, (uint32_t)(tiles * CB * 128) * (uint32_t)(w.heads * g.tile_tokens));
                     __syncwarp();
                     if (go && lane < tiles * CB) {
-                        const int t = lane / CB, c = lane % CB;
-                        tma_load_3d(qs + t * SLOT + c * BLOCK, &tq, 64 * c, w.head, w.q.t0 + w.tok + t * g.tile_tokens, &q_full);
+                        const int t = lane / CB, cq = lane % CB;
+                        tma_load_3d(qs + t * SLOT + cq * BLOCK, &tq, 64 * cq, w.head, w.q.t0 + w.tok + t * g.tile_tokens, &q_full);
                     }
                 }
                 item++;
                 const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
-                // a lane's row within its box's page, and that page
-                auto page_of = [&](int e, int &y, int &nbox, bool &is_v) {
+                auto place = [&](int e, int &nbox, bool &is_v) {         // row of the pool that the lane's box starts at
                     int tile;
                     ring_entry<PAIR>(e, n, tile, is_v);
                     const int r0 = (w.tile + tile) * TT_KT, have = min(TT_KT, w.visible - r0);
                     nbox = have <= 0 ? 0 : (have + box - 1) / box;
-                    y = 0;
-                    if (lane < nbox) {
-                        const int r = r0 + lane * box;
-                        int page = row[r / P];
-                        if (page < 0 || page >= g.p.n_pages) {
-                            atomicCAS(g.err, 0, VB_DEV_TREE_PAGE);
-                            page = 0;
-                        }
-                        y = (page * g.p.n_kv_heads + w.g) * P + r % P;
+                    if (k >= nbox) return 0;
+                    const int r = r0 + k * box;
+                    int page = row[r / P];
+                    if (page < 0 || page >= g.p.n_pages) {
+                        atomicCAS(g.err, 0, VB_DEV_TREE_PAGE);
+                        page = 0;
                     }
+                    return (page * g.p.n_kv_heads + w.g) * P + r % P;
                 };
-                int y, nbox;
+                int nbox;
                 bool is_v;
-                page_of(0, y, nbox, is_v);
-                for (int e = 0; e < 2 * n; e++, pos++) {
-                    int y1 = 0, nbox1 = 0;
+                int y = place(0, nbox, is_v);
+                for (int e = 0; e < 2 * n; e++) {
+                    int nbox1 = 0;
                     bool is_v1 = false;
-                    if (e + 1 < 2 * n) page_of(e + 1, y1, nbox1, is_v1);
-                    const int s = pos % n_slots;
-                    tree_wait_warp(&empty[s], ((uint32_t)(pos / n_slots) & 1u) ^ 1u, &abort_flag, g.err);
-                    // (every lane takes the same answer)
-                    const int load = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag ? 0 : nbox, 0);
-                    if (lane == 0) {
-                        if (load) mbar_arrive_expect_tx(&full[s], (uint32_t)load * box * 128 * CB);
-                        else mbar_arrive(&full[s]);
+                    const int y1 = e + 1 < 2 * n ? place(e + 1, nbox1, is_v1) : 0;
+                    tree_wait_warp(&empty[slot], phase, &abort_flag, g.err);
+                    const bool go = going();
+                    if (go && me == 0 && lane == 0) {
+                        if (nbox) mbar_arrive_expect_tx(&full[slot], (uint32_t)nbox * box * 128 * CB);
+                        else mbar_arrive(&full[slot]);
                     }
+                    if (go && k < nbox)
+                        tma_load_2d(ring + (size_t)slot * SLOT + c * BLOCK + k * box * 128, is_v ? &tv : &tk, 64 * c, y, &full[slot]);
                     __syncwarp();
-                    if (lane < load) {
-                        uint8_t *dst = ring + (size_t)s * SLOT + lane * box * 128;
-#pragma unroll
-                        for (int c = 0; c < CB; c++) tma_load_2d(dst + c * BLOCK, is_v ? &tv : &tk, 64 * c, y, &full[s]);
+                    if (++slot == n_slots) {
+                        slot = 0;
+                        phase ^= 1u;
+                        filled = true;
                     }
                     y = y1;
                     nbox = nbox1;
@@ -338,12 +341,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                 }
                 if (w.left > 0) tree_next(g, w);
             }
-            // every copy has landed before the CTA can end
+            // every copy has landed before the CTA can end: the last fill of each
+            // slot, in this round of the ring (phase is the parity waited for in
+            // it, the opposite of its fills') or the one before
+            for (int s = 0; s < n_slots; s++)
+                if (s < slot) gm_wait(&full[s], phase ^ 1u);
+                else if (filled) gm_wait(&full[s], phase);
             if (g.q_tma && item) gm_wait(&q_full, (uint32_t)(item - 1) & 1u);
-            for (int s = 0; s < n_slots; s++) {
-                const int fills = pos / n_slots + (pos % n_slots > s ? 1 : 0);
-                if (fills) gm_wait(&full[s], (uint32_t)(fills - 1) & 1u);
-            }
         } else if (warp == 9) {
             // --------------------------------------------------------- MMAs
             const uint32_t fmt = TYPE == TR_F16 ? 0u : 1u;
