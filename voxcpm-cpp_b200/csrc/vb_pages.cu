@@ -1,14 +1,17 @@
 // vb_pages.cu -- page operations of a paged K/V cache: extend (with copy on
 // write), fork, keep (the accepted path of a draft), truncate, compact.
 //
-// The bookkeeping lives on the device: a call is a plan (which pages, which
-// rows) and, where rows move, a copy that follows the plan's list.  The plan
-// of a call that allocates or checks across requests runs in one CTA (the
-// free pages are found by one scan of the counts, requests are a few dozen);
-// calls whose requests touch only their own table rows and add to the counts
-// atomically (fork, truncate: integer adds, so the order does not show) run
-// one CTA column per request.  Both kernels of a call are programmatic
-// dependent launches.
+// The bookkeeping lives on the device.  Where rows move (extend, keep,
+// compact) a call is a plan, one CTA that checks the requests, works out pages
+// and rows and writes the new state, and a copy by all SMs that follows the
+// plan's list; both are programmatic dependent launches.  A plan is four
+// dependent rounds of loads and a few barriers, so it runs in few threads with
+// everything that does not depend on an earlier round loaded in the first.
+// (One launch for both, every CTA planning for itself and the last one to
+// finish writing the state, took longer: 35 us against 22 for a step of 64
+// sequences that extends, keeps and truncates.)  Fork and truncate touch only
+// their own requests' table rows and add to the counts atomically (integer
+// adds, so the order does not show): a column of CTAs per request.
 #include "vb_common.cuh"
 #include "vb_kernels.cuh"
 #include "vb_tc.cuh"
@@ -18,42 +21,36 @@
 
 namespace vb {
 
-constexpr int PG_PLAN = 1024;        // threads of a plan CTA
-constexpr int PG_SCAN = 8;           // counts per thread and scan step
+constexpr int PG_PLAN = 1024;        // threads of compact's plan
+constexpr int PG_STEP = 256;         // threads of extend's plan: few, as barriers are part of what it costs
+constexpr int PG_KEEP = 512;         // threads of keep's plan
+constexpr int PG_SCAN = 16;          // counts per thread and scan step
 constexpr int PG_COPY = 256;
 constexpr int PG_MAX_SEQS = 16384;
 
-struct PageJob {                     // rows 0 .. rows-1 of page src, in every layer, to page dst
-    int src, dst, rows, pad;
-};
-
-// Exclusive sum over the CTA's threads; total: the sum of all.  sh: 33 ints.
-__device__ int block_scan(int v, int *sh, int &total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+// Exclusive sum over the CTA's threads; total: the sum of all.  sh: two rows
+// of 32, used in turn (`turn` counts the calls), so one barrier is enough.
+template <typename T>
+__device__ T block_scan(T v, T (*sh)[32], int turn, T &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    T x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    if (lane == 31) sh[warp] = x;
+    T *row = sh[turn & 1];
+    if (lane == 31) row[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        int w = lane < (int)(blockDim.x >> 5) ? sh[lane] : 0;
-        const int w0 = w;
+    T w = lane < warps ? row[lane] : T(0);
+    const T own = __shfl_sync(0xffffffffu, w, warp);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
-        }
-        sh[lane] = w - w0;
-        if (lane == 31) sh[32] = w;
+    for (int o = 1; o < 32; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
     }
-    __syncthreads();
-    const int r = sh[warp] + x - v;
-    total = sh[32];
-    __syncthreads();
-    return r;
+    total = __shfl_sync(0xffffffffu, w, 31);
+    return __shfl_sync(0xffffffffu, w, warp) - own + x - v;
 }
 
 // First error of a call: lowest request, then lowest code.
@@ -67,6 +64,16 @@ __device__ void record(const vb_pages &p, int key) {
     p.status[0] = key & 15;
 }
 
+// Which requests came second for a sequence.
+__device__ void which_twice(int n, const int32_t *seqs, PageError *err) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x)
+        for (int j = 0; j < i; j++)
+            if (seqs[j] == seqs[i]) {
+                err->at(i, VB_PAGES_SEQ);
+                break;
+            }
+}
+
 // Marks the requests' sequences in a bitmap of shared memory and reports
 // those out of range or met before.
 __device__ void check_seqs(const vb_pages &p, int n, const int32_t *seqs, uint32_t *bits, PageError *err) {
@@ -78,42 +85,79 @@ __device__ void check_seqs(const vb_pages &p, int n, const int32_t *seqs, uint32
         if (s < 0 || s >= p.n_seqs) err->at(i, VB_PAGES_SEQ);
         else twice |= atomicOr(&bits[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u;
     }
-    if (!__syncthreads_or(twice)) return;
-    for (int i = threadIdx.x; i < n; i += blockDim.x)     // which request came second
-        for (int j = 0; j < i; j++)
-            if (seqs[j] == seqs[i]) {
-                err->at(i, VB_PAGES_SEQ);
-                break;
-            }
+    if (__syncthreads_or(twice)) which_twice(n, seqs, err);
 }
 
-__global__ void __launch_bounds__(PG_PLAN) pages_extend_plan(vb_pages p, int n, const int32_t *seqs,
-                                                             const int32_t *rows, int *ws) {
+struct PageJob {                     // rows 0 .. rows-1 of page src, in every layer, to page dst
+    int src, dst, rows, pad;
+};
+
+// Which of this thread's PG_SCAN pages from `base` on are free.
+__device__ __forceinline__ uint32_t free_bits(const vb_pages &p, int base) {
+    const int q0 = base + threadIdx.x * PG_SCAN;
+    uint32_t bits = 0;
+    if (q0 + PG_SCAN <= p.n_pages) {
+#pragma unroll
+        for (int j = 0; j < PG_SCAN; j += 4) {
+            const int4 r = *reinterpret_cast<const int4 *>(p.refs + q0 + j);
+            bits |= (uint32_t)(r.x == 0) << j | (uint32_t)(r.y == 0) << (j + 1) | (uint32_t)(r.z == 0) << (j + 2) |
+                    (uint32_t)(r.w == 0) << (j + 3);
+        }
+    } else {
+        for (int j = 0; j < PG_SCAN; j++)
+            if (q0 + j < p.n_pages && p.refs[q0 + j] == 0) bits |= 1u << j;
+    }
+    return bits;
+}
+
+// Calls take(rank, page) for the first `total` free pages, lowest numbers
+// first, and returns how many there are (up to at least total).  here: the
+// free_bits of the first step.
+template <typename Take>
+__device__ int free_pages(const vb_pages &p, int total, uint32_t here, int (*scan)[32], int &turn, Take take) {
+    int found = 0;
+    for (int base = 0; base < p.n_pages && found < total; base += blockDim.x * PG_SCAN) {
+        if (base) here = free_bits(p, base);
+        int step;
+        int k = found + block_scan(__popc(here), scan, turn++, step);
+        const int q0 = base + threadIdx.x * PG_SCAN;
+        for (uint32_t b = here; b && k < total; b &= b - 1) take(k++, q0 + __ffs(b) - 1);
+        found += step;
+    }
+    return found;
+}
+
+// ws: [0] number of jobs, [4 ..] jobs.
+__global__ void __launch_bounds__(PG_STEP) pages_extend_plan(vb_pages p, int n, const int32_t *seqs, const int32_t *rows,
+                                                             int *ws) {
     extern __shared__ int sm[];
-    __shared__ int scan[33];
+    __shared__ int scan[2][32];
+    __shared__ long long scan2[2][32];
     __shared__ PageError err;
+    // per request: the partly filled page that it shares and leaves (-1: none),
+    // the rank of its first new page, its length
+    int *last = sm, *first = sm + n, *length = sm + 2 * n;
+    uint32_t *bits = reinterpret_cast<uint32_t *>(sm + 3 * n);
+    PageJob *jobs = reinterpret_cast<PageJob *>(ws + 4);
+    const int P = p.page_rows;
+    if (threadIdx.x == 0) err.key = INT_MAX;
+    for (int i = threadIdx.x; i < (p.n_seqs + 31) / 32; i += blockDim.x) bits[i] = 0;
     pdl_trigger();
     pdl_wait();
-    int *last = sm, *first = sm + n;                          // [n] shared partly filled page (or -1), first new page
-    uint32_t *bits = reinterpret_cast<uint32_t *>(sm + 2 * n);
-    PageJob *jobs = reinterpret_cast<PageJob *>(ws + 4);
-    int *freelist = ws + 4 + 4 * n;
-    const int P = p.page_rows;
-    if (threadIdx.x == 0) {
-        err.key = INT_MAX;
-        ws[0] = 0;
-    }
-    if (p.status[0]) return;                                  // every thread reads the same word
+    const bool held = p.status[0] != 0;                       // an error waits to be read: nothing changes
+    const uint32_t free0 = free_bits(p, 0);
     __syncthreads();
-    check_seqs(p, n, seqs, bits, &err);
-    __syncthreads();
-    if (err.key != INT_MAX) {
-        if (threadIdx.x == 0) record(p, err.key);
-        return;
-    }
+    bool twice = false;
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const int s = seqs[i], len = p.length[s], r = rows[i];
+        const int s = seqs[i], r = rows[i];
         last[i] = -1;
+        if (s < 0 || s >= p.n_seqs) {
+            err.at(i, VB_PAGES_SEQ);
+            continue;
+        }
+        const int len = p.length[s];
+        twice |= atomicOr(&bits[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u;
+        length[i] = len;
         if (r < 0) err.at(i, VB_PAGES_COUNT);
         else if ((int64_t)len + r > (int64_t)p.max_pages * P) err.at(i, VB_PAGES_LONG);
         else if (r > 0 && len % P) {
@@ -122,100 +166,105 @@ __global__ void __launch_bounds__(PG_PLAN) pages_extend_plan(vb_pages p, int n, 
             else if (p.refs[pg] > 1) last[i] = pg;
         }
     }
-    __syncthreads();
-    if (err.key != INT_MAX) {
-        if (threadIdx.x == 0) record(p, err.key);
+    if (__syncthreads_or(twice)) {
+        which_twice(n, seqs, &err);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) ws[0] = 0;
+    if (err.key != INT_MAX || held) {
+        if (threadIdx.x == 0 && !held) record(p, err.key);
         return;
     }
     // copy on write: a request leaves the shared page unless every other
     // holder has left it before (earlier requests of this call)
     const int per = (n + blockDim.x - 1) / blockDim.x;
     const int i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
-    int mine = 0;
+    int mine = 0, leave = 0;
     for (int i = i0; i < i1; i++) {
-        const int s = seqs[i], len = p.length[s];
+        const int len = length[i];
         int need = (len + rows[i] + P - 1) / P - (len + P - 1) / P;
         const int pg = last[i];
         if (pg >= 0) {
             int left = p.refs[pg];
             for (int j = 0; j < i && left > 1; j++) left -= last[j] == pg;
-            if (left > 1) need = need + 1 | INT_MIN;          // top bit: the first new page is the copy
+            if (left > 1) {
+                need = (need + 1) | INT_MIN;                  // top bit: the first new page is the copy
+                leave++;
+            }
         }
         first[i] = need;
         mine += need & INT_MAX;
     }
-    int total;
-    int at = block_scan(mine, scan, total);
-    // the free pages, lowest numbers first
-    int found = 0;
-    for (int base = 0; base < p.n_pages && found < total; base += blockDim.x * PG_SCAN) {
-        const int q0 = base + threadIdx.x * PG_SCAN;
-        uint32_t is_free = 0;
-#pragma unroll
-        for (int j = 0; j < PG_SCAN; j++)
-            if (q0 + j < p.n_pages && p.refs[q0 + j] == 0) is_free |= 1u << j;
-        int here;
-        int k = found + block_scan(__popc(is_free), scan, here);
-        for (uint32_t b = is_free; b && k < total; b &= b - 1) freelist[k++] = q0 + __ffs(b) - 1;
-        found += here;
-    }
-    __syncthreads();
-    if (found < total) {
-        if (threadIdx.x == 0) {
-            // the request that the pages run out at
-            int sum = 0, i = 0;
-            for (; i < n - 1; i++)
-                if ((sum += first[i] & INT_MAX) > found) break;
-            record(p, i * 16 + VB_PAGES_FULL);
-        }
-        return;
-    }
+    long long sums;
+    const long long before = block_scan((long long)leave << 32 | mine, scan2, 0, sums);
+    const int total = (int)sums, n_leave = (int)(sums >> 32);
+    int at = (int)before, k = (int)(before >> 32), turn = 0;
     for (int i = i0; i < i1; i++) {
         const int need = first[i];
         if (need >= 0) last[i] = -1;                          // keeps its page
+        else {
+            jobs[k] = {last[i], 0, length[i] % P, 0};
+            last[i] = k++;                                    // from here on: its job
+        }
         first[i] = at;
         at += need & INT_MAX;
     }
     __syncthreads();
-    // one warp per request writes its table entries
-    const int lane = threadIdx.x & 31;
-    for (int i = threadIdx.x >> 5; i < n; i += blockDim.x >> 5) {
-        const int s = seqs[i], len = p.length[s], r = rows[i], cow = last[i] >= 0;
-        const int begin = (len + P - 1) / P - cow, want = (len + r + P - 1) / P;
-        for (int c = begin + lane; c < want; c += 32) {
-            const int pg = freelist[first[i] + c - begin];
-            p.table[(int64_t)s * p.max_pages + c] = pg;
-            p.refs[pg] = 1;
+    // Two passes over the counts, as nothing may change before it is known
+    // that there are pages enough; more than one step only when the pool's
+    // first pages are taken.
+    const int found = free_pages(p, total, free0, scan, turn, [](int, int) {});
+    if (found < total) {
+        if (threadIdx.x == 0) {                               // the request that the pages run out at
+            int i = 0;
+            while (i < n - 1 && first[i + 1] <= found) i++;
+            record(p, i * 16 + VB_PAGES_FULL);
         }
-        if (lane == 0) {
-            PageJob j = {0, 0, 0, 0};
-            if (cow) {
-                j = {last[i], freelist[first[i]], len % P, 0};
-                atomicSub(&p.refs[last[i]], 1);
-            }
-            jobs[i] = j;
-        }
-        __syncwarp();
-        if (lane == 0) p.length[s] = len + r;
+        return;
     }
-    if (threadIdx.x == 0) ws[0] = n;
+    free_pages(p, total, free0, scan, turn, [&](int rank, int page) {
+        int lo = 0, hi = n - 1;                               // the request whose page of this rank it is
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (first[mid] <= rank) lo = mid;
+            else hi = mid - 1;
+        }
+        const int begin = (length[lo] + P - 1) / P - (last[lo] >= 0);
+        p.table[(int64_t)seqs[lo] * p.max_pages + begin + rank - first[lo]] = page;
+        p.refs[page] = 1;
+        if (last[lo] >= 0 && rank == first[lo]) jobs[last[lo]].dst = page;
+    });
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        if (last[i] >= 0) atomicSub(&p.refs[jobs[last[i]].src], 1);
+        p.length[seqs[i]] = length[i] + rows[i];
+    }
+    if (threadIdx.x == 0) ws[0] = n_leave;
 }
 
-// Copies the first rows of pages: grid (layer x {k, v}, request).
+// Copies the first rows of pages; a warp takes one (job, layer, k or v, head).
 __global__ void __launch_bounds__(PG_COPY) pages_copy_rows(vb_pages p, const int *ws) {
+    constexpr int B = 8;
     pdl_trigger();
     pdl_wait();
-    if ((int)blockIdx.y >= ws[0]) return;
-    const PageJob j = reinterpret_cast<const PageJob *>(ws + 4)[blockIdx.y];
-    if (j.rows == 0) return;
-    const int row16 = p.head_dim / 8, head16 = p.page_rows * row16, n16 = j.rows * row16;   // 16-byte units
-    uint4 *pool = static_cast<uint4 *>((blockIdx.x & 1) ? p.v : p.k) +
-                  (int64_t)(blockIdx.x >> 1) * p.n_pages * p.n_kv_heads * head16;
-    const uint4 *src = pool + (int64_t)j.src * p.n_kv_heads * head16;
-    uint4 *dst = pool + (int64_t)j.dst * p.n_kv_heads * head16;
-    for (int i = threadIdx.x; i < p.n_kv_heads * n16; i += PG_COPY) {
-        const int o = i / n16 * head16 + i % n16;
-        dst[o] = src[o];
+    const PageJob *jobs = reinterpret_cast<const PageJob *>(ws + 4);
+    const int row16 = p.head_dim / 8, head16 = p.page_rows * row16, lane = threadIdx.x & 31;       // 16-byte units
+    const int64_t tasks = (int64_t)ws[0] * p.n_layers * 2 * p.n_kv_heads;
+    for (int64_t t = (int64_t)blockIdx.x * (PG_COPY / 32) + (threadIdx.x >> 5); t < tasks; t += gridDim.x * (PG_COPY / 32)) {
+        const int h = (int)(t % p.n_kv_heads), lay = (int)(t / p.n_kv_heads % (2 * p.n_layers));
+        const PageJob j = jobs[t / p.n_kv_heads / (2 * p.n_layers)];
+        uint4 *pool = static_cast<uint4 *>((lay & 1) ? p.v : p.k) + ((int64_t)(lay >> 1) * p.n_pages * p.n_kv_heads + h) * head16;
+        const uint4 *src = pool + (int64_t)j.src * p.n_kv_heads * head16;
+        uint4 *dst = pool + (int64_t)j.dst * p.n_kv_heads * head16;
+        const int n16 = j.rows * row16;
+        for (int c = lane; c < n16; c += 32 * B) {
+            uint4 x[B];
+#pragma unroll
+            for (int i = 0; i < B; i++)
+                if (c + 32 * i < n16) x[i] = src[c + 32 * i];
+#pragma unroll
+            for (int i = 0; i < B; i++)
+                if (c + 32 * i < n16) dst[c + 32 * i] = x[i];
+        }
     }
 }
 
@@ -281,52 +330,57 @@ __global__ void __launch_bounds__(256) pages_truncate_kernel(vb_pages p, int n, 
     if (blockIdx.y == 0 && threadIdx.x == 0) p.length[s] = min(p.length[s], len);
 }
 
-// moves[i*ld + j]: pool rows (page * page_rows + slot) that row j of request
-// i's path comes from and goes to; -1: stays.
-__global__ void __launch_bounds__(PG_PLAN) pages_keep_plan(vb_pages p, int n, const int32_t *seqs,
-                                                           const int32_t *drafted, const int32_t *kept,
-                                                           const int32_t *path, int ld, int *ws) {
+// ws: [0] requests (0 after an error), [4 ..] moves: [i*ld + j] the pool rows
+// (page * page_rows + slot) that row j of request i's path comes from and goes
+// to; -1: stays.
+__global__ void __launch_bounds__(PG_KEEP) pages_keep_plan(vb_pages p, int n, const int32_t *seqs, const int32_t *drafted,
+                                                           const int32_t *kept, const int32_t *path, int ld, int *ws) {
     extern __shared__ int sm[];
     __shared__ PageError err;
-    pdl_trigger();
-    pdl_wait();
     uint32_t *bits = reinterpret_cast<uint32_t *>(sm);
     int2 *moves = reinterpret_cast<int2 *>(ws + 4);
     const int P = p.page_rows;
-    if (threadIdx.x == 0) {
-        err.key = INT_MAX;
-        ws[0] = 0;
+    if (threadIdx.x == 0) err.key = INT_MAX;
+    for (int i = threadIdx.x; i < (p.n_seqs + 31) / 32; i += blockDim.x) bits[i] = 0;
+    pdl_trigger();
+    pdl_wait();
+    const bool held = p.status[0] != 0;
+    __syncthreads();
+    bool twice = false;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int s = seqs[i], d = drafted[i], k = kept[i];
+        if (s < 0 || s >= p.n_seqs) {
+            err.at(i, VB_PAGES_SEQ);
+            continue;
+        }
+        twice |= atomicOr(&bits[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u;
+        if (d < 0 || k < 0 || k > d || k > ld || d > p.length[s]) err.at(i, VB_PAGES_COUNT);
     }
-    if (p.status[0]) return;
-    __syncthreads();
-    check_seqs(p, n, seqs, bits, &err);
-    __syncthreads();
-    if (err.key == INT_MAX)
-        for (int i = threadIdx.x; i < n; i += blockDim.x) {
-            const int d = drafted[i], k = kept[i];
-            if (d < 0 || k < 0 || k > d || k > ld || d > p.length[seqs[i]]) err.at(i, VB_PAGES_COUNT);
+    // the paths, of requests that are in order themselves; by the other warps
+    // first, while those above wait for their lengths
+    const int busy = min((n + 31) & ~31, PG_KEEP / 2);
+    for (int e = (threadIdx.x + PG_KEEP - busy) % PG_KEEP; e < n * ld; e += PG_KEEP) {
+        const int i = e / ld, j = e - i * ld, s = seqs[i], d = drafted[i], at = path[e], prev = j ? path[e - 1] : -1;
+        moves[e] = make_int2(-1, -1);
+        if (j >= kept[i] || s < 0 || s >= p.n_seqs) continue;
+        const int base = p.length[s] - d;
+        if (d < 0 || kept[i] > d || base < 0) continue;
+        const int32_t *row = p.table + (int64_t)s * p.max_pages;
+        if (at < 0 || at >= d || prev >= at) err.at(i, VB_PAGES_PATH);
+        else if (at != j) {
+            const int ps = row[(base + at) / P], pd = row[(base + j) / P];
+            if (ps < 0 || ps >= p.n_pages || pd < 0 || pd >= p.n_pages) err.at(i, VB_PAGES_TABLE);
+            else if (p.refs[pd] != 1) err.at(i, VB_PAGES_SHARED);
+            else moves[e] = make_int2(ps * P + (base + at) % P, pd * P + (base + j) % P);
         }
-    __syncthreads();
-    if (err.key == INT_MAX)
-        for (int64_t e = threadIdx.x; e < (int64_t)n * ld; e += blockDim.x) {
-            const int i = (int)(e / ld), j = (int)(e % ld);
-            int2 mv = make_int2(-1, -1);
-            if (j < kept[i]) {
-                const int s = seqs[i], at = path[e], base = p.length[s] - drafted[i];
-                const int32_t *row = p.table + (int64_t)s * p.max_pages;
-                if (at < 0 || at >= drafted[i] || (j > 0 && path[e - 1] >= at)) err.at(i, VB_PAGES_PATH);
-                else if (at != j) {
-                    const int ps = row[(base + at) / P], pd = row[(base + j) / P];
-                    if (ps < 0 || ps >= p.n_pages || pd < 0 || pd >= p.n_pages) err.at(i, VB_PAGES_TABLE);
-                    else if (p.refs[pd] != 1) err.at(i, VB_PAGES_SHARED);
-                    mv = make_int2(ps * P + (base + at) % P, pd * P + (base + j) % P);
-                }
-            }
-            moves[e] = mv;
-        }
-    __syncthreads();
-    if (err.key != INT_MAX) {
-        if (threadIdx.x == 0) record(p, err.key);
+    }
+    if (__syncthreads_or(twice)) {
+        which_twice(n, seqs, &err);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) ws[0] = err.key == INT_MAX && !held ? n : 0;
+    if (err.key != INT_MAX || held) {
+        if (threadIdx.x == 0 && !held) record(p, err.key);
         return;
     }
     // pages past the new end
@@ -341,48 +395,49 @@ __global__ void __launch_bounds__(PG_PLAN) pages_keep_plan(vb_pages p, int n, co
         __syncwarp();
         if (lane == 0) p.length[s] = now;
     }
-    if (threadIdx.x == 0) ws[0] = n;
 }
 
-// grid (column blocks, request): a thread owns 16 bytes of every row of one
-// (layer, k or v, head) and walks the path in order.  A row goes to a place
-// at or before its own and later sources lie behind it, so a batch that is
-// loaded before it is stored never reads what it wrote.
+// A thread owns 16 bytes of every row of one (request, layer, k or v, head)
+// and walks the path in order.  A row goes to a place at or before its own and
+// later sources lie behind it, so a batch that is loaded before it is stored
+// never reads what it wrote.
 __global__ void __launch_bounds__(PG_COPY) pages_move_rows(vb_pages p, int ld, const int *ws) {
     constexpr int B = 8;
     pdl_trigger();
     pdl_wait();
-    if ((int)blockIdx.y >= ws[0]) return;
-    const int2 *mv = reinterpret_cast<const int2 *>(ws + 4) + (int64_t)blockIdx.y * ld;
-    const int row16 = p.head_dim / 8;
-    const int64_t col = (int64_t)blockIdx.x * PG_COPY + threadIdx.x;
-    if (col >= (int64_t)p.n_layers * 2 * p.n_kv_heads * row16) return;
-    const int c = (int)(col % row16), g = (int)(col / row16 % p.n_kv_heads);
-    const int lay = (int)(col / row16 / p.n_kv_heads);
-    uint4 *pool = static_cast<uint4 *>((lay & 1) ? p.v : p.k) +
-                  (int64_t)(lay >> 1) * p.n_pages * p.n_kv_heads * p.page_rows * row16;
-    auto at = [&](int r) {          // 16-byte unit of pool row r for this thread's head
-        const int pg = r / p.page_rows, sl = r % p.page_rows;
-        return (((int64_t)pg * p.n_kv_heads + g) * p.page_rows + sl) * row16 + c;
-    };
-    for (int j0 = 0; j0 < ld; j0 += B) {
-        uint4 x[B];
+    const int row16 = p.head_dim / 8, P = p.page_rows;
+    const int cols = p.n_layers * 2 * p.n_kv_heads * row16, blocks = (cols + PG_COPY - 1) / PG_COPY, n = ws[0];
+    for (int t = blockIdx.x; t < blocks * n; t += gridDim.x) {
+        const int i = t / blocks, col = (t - i * blocks) * PG_COPY + threadIdx.x;
+        if (col >= cols) continue;
+        const int2 *mv = reinterpret_cast<const int2 *>(ws + 4) + (int64_t)i * ld;
+        const int c = col % row16, h = col / row16 % p.n_kv_heads, lay = col / row16 / p.n_kv_heads;
+        uint4 *pool = static_cast<uint4 *>((lay & 1) ? p.v : p.k) +
+                      ((int64_t)(lay >> 1) * p.n_pages * p.n_kv_heads + h) * P * row16 + c;
+        auto at = [&](int r) { return ((int64_t)(r / P) * p.n_kv_heads * P + r % P) * row16; };
+        for (int j0 = 0; j0 < ld; j0 += B) {
+            uint4 x[B];
+            int2 m[B];
 #pragma unroll
-        for (int j = 0; j < B; j++)
-            if (j0 + j < ld && mv[j0 + j].x >= 0) x[j] = pool[at(mv[j0 + j].x)];
+            for (int j = 0; j < B; j++) m[j] = j0 + j < ld ? mv[j0 + j] : make_int2(-1, -1);
 #pragma unroll
-        for (int j = 0; j < B; j++)
-            if (j0 + j < ld && mv[j0 + j].x >= 0) pool[at(mv[j0 + j].y)] = x[j];
+            for (int j = 0; j < B; j++)
+                if (m[j].x >= 0) x[j] = pool[at(m[j].x)];
+#pragma unroll
+            for (int j = 0; j < B; j++)
+                if (m[j].x >= 0) pool[at(m[j].y)] = x[j];
+        }
     }
 }
 
 // ws: [0] live pages (0 after an error), [4 ..] the new number of each page,
 // then the old number of each new one.
 __global__ void __launch_bounds__(PG_PLAN) pages_compact_plan(vb_pages p, vb_pages to, int *ws) {
-    __shared__ int scan[33];
+    __shared__ int scan[2][32];
     __shared__ PageError err;
     pdl_trigger();
     pdl_wait();
+    int turn = 0;
     int *number = ws + 4, *live = ws + 4 + p.n_pages;
     if (threadIdx.x == 0) {
         err.key = INT_MAX;
@@ -402,7 +457,7 @@ __global__ void __launch_bounds__(PG_PLAN) pages_compact_plan(vb_pages p, vb_pag
         for (int j = 0; j < PG_SCAN; j++)
             if (q0 + j < p.n_pages && p.refs[q0 + j] > 0) used |= 1u << j;
         int here;
-        int k = total + block_scan(__popc(used), scan, here);
+        int k = total + block_scan(__popc(used), scan, turn++, here);
 #pragma unroll
         for (int j = 0; j < PG_SCAN; j++)
             if (q0 + j < p.n_pages) {
@@ -492,13 +547,18 @@ static int check_call(vb_ctx *ctx, const vb_pages *p, int n, const char *who, bo
     return VB_OK;
 }
 
+// CTAs for a call that may copy so many bytes: one for each 16 KB, four per SM at most.
+static unsigned share_out(const vb_ctx *ctx, int64_t bytes) {
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(4 * ctx->sm_count, bytes >> 14));
+}
+
 static size_t seq_bits(const vb_pages *p) { return (size_t)((p->n_seqs + 31) / 32) * 4; }
 
 int init_pages(vb_ctx *ctx) {
     VB_CHECK(ctx, cudaMalloc(&ctx->op_error, 256));
     VB_CHECK(ctx, cudaMemset(ctx->op_error, 0, 256));
     VB_CHECK(ctx, cudaFuncSetAttribute(pages_extend_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       2 * PG_MAX_SEQS * 4 + PG_MAX_SEQS / 8));
+                                       3 * PG_MAX_SEQS * 4 + PG_MAX_SEQS / 8));
     return VB_OK;
 }
 
@@ -521,13 +581,15 @@ extern "C" int vb_pages_extend(vb_ctx *ctx, const vb_pages *p, int n, const int3
     if (!ctx) return VB_ERR_INVALID_ARG;
     int rc = check_call(ctx, p, n, "vb_pages_extend", seqs && rows);
     if (rc || n == 0) return rc;
-    rc = arena_reserve(ctx, ctx->pages_ws, 16 + (size_t)n * sizeof(PageJob) + (size_t)p->n_pages * 4);
+    rc = arena_reserve(ctx, ctx->pages_ws, 16 + (size_t)n * sizeof(PageJob));
     if (rc) return rc;
     int *ws = static_cast<int *>(ctx->pages_ws.ptr);
-    VB_CHECK(ctx, pdl_launch(ctx, pages_extend_plan, dim3(1), dim3(PG_PLAN), (size_t)2 * n * 4 + seq_bits(p), *p, n,
-                             seqs, rows, ws));
+    VB_CHECK(ctx, pdl_launch(ctx, pages_extend_plan, dim3(1), dim3(PG_STEP), (size_t)3 * n * 4 + seq_bits(p), *p, n, seqs, rows,
+                             ws));
     VB_LAUNCH_CHECK(ctx, "pages_extend_plan");
-    VB_CHECK(ctx, pdl_launch(ctx, pages_copy_rows, dim3(2 * p->n_layers, n), dim3(PG_COPY), 0, *p,
+    // (as if every request left its page)
+    const int64_t bytes = (int64_t)n * 2 * p->n_layers * p->n_kv_heads * p->page_rows * p->head_dim * 2;
+    VB_CHECK(ctx, pdl_launch(ctx, pages_copy_rows, dim3(share_out(ctx, bytes)), dim3(PG_COPY), 0, *p,
                              static_cast<const int *>(ws)));
     VB_LAUNCH_CHECK(ctx, "pages_copy_rows");
     return VB_OK;
@@ -561,18 +623,19 @@ extern "C" int vb_pages_keep(vb_ctx *ctx, const vb_pages *p, int n, const int32_
     if (!ctx) return VB_ERR_INVALID_ARG;
     int rc = check_call(ctx, p, n, "vb_pages_keep", seqs && drafted && kept && (path || !ld_path));
     if (rc) return rc;
-    if (ld_path < 0 || (int64_t)n * ld_path > INT_MAX)
-        return set_error(ctx, VB_ERR_INVALID_ARG, "vb_pages_keep: bad path length");
+    const int64_t cols = (int64_t)p->n_layers * 2 * p->n_kv_heads * (p->head_dim / 8);
+    if (ld_path < 0 || (int64_t)n * ld_path > INT_MAX || cols > INT_MAX || (cols / PG_COPY + 1) * n > INT_MAX)
+        return set_error(ctx, VB_ERR_INVALID_ARG, "vb_pages_keep: path length or cache out of range");
     if (n == 0) return VB_OK;
     rc = arena_reserve(ctx, ctx->pages_ws, 16 + (size_t)n * ld_path * sizeof(int2));
     if (rc) return rc;
     int *ws = static_cast<int *>(ctx->pages_ws.ptr);
-    VB_CHECK(ctx, pdl_launch(ctx, pages_keep_plan, dim3(1), dim3(PG_PLAN), seq_bits(p), *p, n, seqs, drafted, kept,
-                             path, ld_path, ws));
+    VB_CHECK(ctx, pdl_launch(ctx, pages_keep_plan, dim3(1), dim3(PG_KEEP), seq_bits(p), *p, n, seqs, drafted, kept, path,
+                             ld_path, ws));
     VB_LAUNCH_CHECK(ctx, "pages_keep_plan");
-    const int64_t cols = (int64_t)p->n_layers * 2 * p->n_kv_heads * (p->head_dim / 8);
-    VB_CHECK(ctx, pdl_launch(ctx, pages_move_rows, dim3((unsigned)((cols + PG_COPY - 1) / PG_COPY), n), dim3(PG_COPY),
-                             0, *p, ld_path, static_cast<const int *>(ws)));
+    const int64_t bytes = (int64_t)n * 2 * p->n_layers * p->n_kv_heads * ld_path * p->head_dim * 2;
+    VB_CHECK(ctx, pdl_launch(ctx, pages_move_rows, dim3(share_out(ctx, bytes)), dim3(PG_COPY), 0, *p, ld_path,
+                             static_cast<const int *>(ws)));
     VB_LAUNCH_CHECK(ctx, "pages_move_rows");
     return VB_OK;
 }

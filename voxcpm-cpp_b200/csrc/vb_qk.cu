@@ -6,11 +6,12 @@
 // position's (cos, sin).  Everything is held in fp32 and each result rounded
 // once, to the output's type.
 //
-// Mapping: a group of LPH lanes (a power of two, at least head_dim / 8) owns
-// one head row.  A lane holds two pieces of four values whose pairs it
-// rotates itself -- i .. i+3 with i + rot/2 .. of the first half, or two
-// neighbouring pieces when pairs are adjacent -- so the only exchange is the
-// sum of squares over the group.  Rows of q, k and v are items of one grid.
+// Mapping: a group of LPH lanes (a power of two) owns head rows of one token.
+// A lane holds two pieces of V values whose pairs it rotates itself -- i ..
+// with i + rot/2 .. of the first half, or two neighbouring pieces when pairs
+// are adjacent -- so the only exchange is the sum of squares over the group.
+// V is 8 where the halves of the row allow it (a lane's piece is then 16 or 32
+// bytes), else 4.
 #include "vb_common.cuh"
 #include "vb_kernels.cuh"
 #include "vb_tc.cuh"
@@ -23,7 +24,9 @@ struct QKArgs {
     vb_qk_args a;
     vb_pages p;
     int store;              // rows go to the cache
-    int vec;                // pointers and strides allow 4-value accesses
+    int vec;                // pointers and strides allow 16-byte accesses
+    int vec_w;              // of the weights too
+    float inv_dim;          // 1 / head_dim
     int *err;
 };
 
@@ -45,194 +48,240 @@ struct Elem<__nv_bfloat16> {
     __device__ static __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
 };
 
-template <typename T>
-struct alignas(4 * sizeof(T)) Vec4 {
-    T x[4];
+// V values of a row, as they lie in memory.
+template <typename T, int V>
+struct Piece {
+    T x[V];
 };
 
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, bool vec, float (&v)[4]) {
+template <typename T, int V>
+__device__ __forceinline__ void load(const T *p, bool vec, Piece<T, V> &v) {
     if (vec) {
-        const Vec4<T> t = *reinterpret_cast<const Vec4<T> *>(p);
+        constexpr int N = V * sizeof(T) / 4;          // 32-bit words
+        uint32_t w[N];
+        if constexpr (N >= 4) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = Elem<T>::get(t.x[i]);
+            for (int i = 0; i < N; i += 4) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
+                w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+            }
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2 *>(p);
+            w[0] = q.x, w[1] = q.y;
+        }
+        memcpy(&v, w, sizeof(v));
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = Elem<T>::get(p[i]);
+        for (int i = 0; i < V; i++) v.x[i] = p[i];
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T *p, bool vec, const float (&v)[4]) {
+template <typename T, int V>
+__device__ __forceinline__ void store(T *p, bool vec, const float (&y)[V]) {
     if (vec) {
-        Vec4<T> t;
+        Piece<T, V> v;
 #pragma unroll
-        for (int i = 0; i < 4; i++) t.x[i] = Elem<T>::put(v[i]);
-        *reinterpret_cast<Vec4<T> *>(p) = t;
+        for (int i = 0; i < V; i++) v.x[i] = Elem<T>::put(y[i]);
+        constexpr int N = V * sizeof(T) / 4;
+        uint32_t w[N];
+        memcpy(w, &v, sizeof(v));
+        if constexpr (N >= 4) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4)
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint32_t *>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else {
+            *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = Elem<T>::put(v[i]);
+        for (int i = 0; i < V; i++) p[i] = Elem<T>::put(y[i]);
     }
 }
 
-template <typename T, int LPH>
-__global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const __grid_constant__ QKArgs g) {
+template <int V>
+__device__ __forceinline__ void load_floats(const float *p, bool vec, float (&y)[V]) {
+    Piece<float, V> v;
+    load(p, vec, v);
+#pragma unroll
+    for (int i = 0; i < V; i++) y[i] = v.x[i];
+}
+
+// A group takes ROWS head rows of one token, all their loads in flight
+// together: the token's place, its table row and the weights are fetched once
+// for them, and a thread has enough bytes on their way to keep HBM busy.
+template <int V>
+constexpr int QK_ROWS = 16 / V;
+
+template <typename T, int V, int LPH>
+__global__ void __launch_bounds__(QK_THREADS, 3) qk_norm_rope_kernel(const __grid_constant__ QKArgs g) {
+    constexpr int ROWS = QK_ROWS<V>;
     pdl_trigger();
     pdl_wait();
     const vb_qk_args &a = g.a;
     const int hd = a.head_dim, nq = a.n_heads, nk = a.n_kv_heads;
-    const int heads = nq + nk + (g.store ? nk : 0);
-    const int64_t item = ((int64_t)blockIdx.x * QK_THREADS + threadIdx.x) / LPH;
+    const int heads = nq + nk + (g.store ? nk : 0), chunks = (heads + ROWS - 1) / ROWS;
+    const unsigned item = (blockIdx.x * QK_THREADS + threadIdx.x) / LPH;
     const int lane = threadIdx.x % LPH;
     const unsigned group = LPH == 32 ? 0xffffffffu : ((1u << LPH) - 1u) << (threadIdx.x % 32 / LPH * LPH);
-    if (item >= (int64_t)a.n_tokens * heads) return;      // whole groups
-    const int t = (int)(item / heads), h = (int)(item % heads);
-    const bool is_q = h < nq, is_v = h >= nq + nk;
-    const int kvh = is_v ? h - nq - nk : h - nq;
-
-    // where the token goes; an invalid place or position skips the whole token
-    int pos = 0;
-    if (a.rope) {
-        pos = a.pos[t];
-        if (pos < 0 || pos >= a.rope_rows) {
-            if (lane == 0) {
-                atomicCAS(g.err, 0, VB_DEV_QK_POS);
-            }
-            pos = -1;
-        }
-    }
-    int64_t pool_row = -1;
-    bool bad = pos < 0;
-    if (g.store) {
-        const int s = a.seq[t], r = a.row[t];
-        if (s != -1) {
-            int page = -1;
-            if (s >= 0 && s < g.p.n_seqs && r >= 0 && r / g.p.page_rows < g.p.max_pages)
-                page = g.p.table[(int64_t)s * g.p.max_pages + r / g.p.page_rows];
-            if (page < 0 || page >= g.p.n_pages) {
-                if (lane == 0) atomicCAS(g.err, 0, VB_DEV_QK_ROW);
-                bad = true;
-            } else {
-                pool_row = (((int64_t)a.layer * g.p.n_pages + page) * nk) * g.p.page_rows + r % g.p.page_rows;
-            }
-        }
-    }
-    if (is_v && (pool_row < 0 || bad)) return;
-
-    const T *src = is_q ? static_cast<const T *>(a.q) + (int64_t)t * a.ldq + (int64_t)h * hd
-                        : static_cast<const T *>(is_v ? a.v : a.k) + (int64_t)t * (is_v ? a.ldv : a.ldk) +
-                              (int64_t)kvh * hd;
+    const int t = (int)(item / (unsigned)chunks), h0 = (int)(item - (unsigned)t * (unsigned)chunks) * ROWS;
+    if (t >= a.n_tokens) return;                          // whole groups
     // the lane's two pieces: i0 and i1, rotated with each other or passed on
-    const int rot = a.rope ? a.rot_dim : 0, c4 = 4 * lane;
-    const bool mine = lane < hd / 8;
+    const int rot = a.rope ? a.rot_dim : 0, c = V * lane;
+    const bool mine = lane < hd / (2 * V);
     int i0, i1;
     bool turn;
     if (a.adjacent) {
-        i0 = 2 * c4;
-        i1 = i0 + 4;
+        i0 = 2 * c;
+        i1 = i0 + V;
         turn = i0 < rot;
     } else {
-        turn = c4 < rot / 2;
-        i0 = turn ? c4 : rot + c4 - rot / 2;
+        turn = c < rot / 2;
+        i0 = turn ? c : rot + c - rot / 2;
         i1 = i0 + (turn ? rot / 2 : (hd - rot) / 2);
     }
-    float x0[4] = {}, x1[4] = {};
-    if (mine && !bad) {
-        load4(src + i0, g.vec, x0);
-        load4(src + i1, g.vec, x1);
+    // where the token goes, then the rows, then what hangs on the place: two
+    // round trips to memory in all
+    int pos = a.rope ? a.pos[t] : 0;
+    const int seq = g.store ? a.seq[t] : -1, row = g.store ? a.row[t] : 0;
+    Piece<T, V> x0[ROWS], x1[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const int h = h0 + r;
+        const T *src = h < nq        ? static_cast<const T *>(a.q) + (int64_t)t * a.ldq + h * hd
+                       : h < nq + nk ? static_cast<const T *>(a.k) + (int64_t)t * a.ldk + (h - nq) * hd
+                                     : static_cast<const T *>(a.v) + (int64_t)t * a.ldv + (h - nq - nk) * hd;
+        if (mine && h < heads) {
+            load(src + i0, g.vec, x0[r]);
+            load(src + i1, g.vec, x1[r]);
+        }
     }
-    if (!is_v) {
-        if (a.norm) {
+    // an invalid place or position skips the whole token
+    const bool off_table = a.rope && (pos < 0 || pos >= a.rope_rows);
+    if (off_table) pos = 0;
+    int page = 0;
+    const bool placed = seq >= 0 && seq < g.p.n_seqs && row >= 0 && row / g.p.page_rows < g.p.max_pages;
+    if (placed) page = g.p.table[(int64_t)seq * g.p.max_pages + row / g.p.page_rows];
+    float cs[2 * V];                                      // (cos, sin) of the lane's V pairs
+    if (turn && mine) load_floats(a.rope + (int64_t)pos * rot + (a.adjacent ? i0 : 2 * c), true, cs);
+    const bool no_row = g.store && seq != -1 && (!placed || page < 0 || page >= g.p.n_pages);
+    const bool bad = off_table || no_row;
+    if (bad && lane == 0) atomicCAS(g.err, 0, off_table ? VB_DEV_QK_POS : VB_DEV_QK_ROW);
+    int64_t pool_row = -1;
+    if (g.store && seq != -1 && !bad)
+        pool_row = (((int64_t)a.layer * g.p.n_pages + page) * nk) * g.p.page_rows + row % g.p.page_rows;
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const int h = h0 + r;
+        if (h >= heads) break;                            // for the whole group
+        const bool is_q = h < nq, is_v = h >= nq + nk;
+        const int kvh = is_v ? h - nq - nk : h - nq;
+        float y0[V], y1[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            y0[i] = mine ? Elem<T>::get(x0[r].x[i]) : 0.0f;
+            y1[i] = mine ? Elem<T>::get(x1[r].x[i]) : 0.0f;
+        }
+        if (!is_v && a.norm) {
             float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
+            for (int i = 0; i < V; i++) ss = fmaf(y0[i], y0[i], fmaf(y1[i], y1[i], ss));
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-            const float rs = rsqrtf(ss / (float)hd + a.eps);
+            const float rs = rsqrtf(ss * g.inv_dim + a.eps);
             const float *w = is_q ? a.q_weight : a.k_weight;
+            float w0[V], w1[V];
+            if (w && mine) {
+                load_floats(w + i0, g.vec_w, w0);
+                load_floats(w + i1, g.vec_w, w1);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x0[i] *= rs;
-                x1[i] *= rs;
-                if (w && mine) {
-                    x0[i] *= w[i0 + i];
-                    x1[i] *= w[i1 + i];
+            for (int i = 0; i < V; i++) {
+                y0[i] *= rs;
+                y1[i] *= rs;
+                if (w) {
+                    y0[i] *= w0[i];
+                    y1[i] *= w1[i];
                 }
             }
         }
-        if (turn && mine && !bad) {
-            const float *cs = a.rope + (int64_t)pos * rot;
+        if (!mine) continue;
+        if (!is_v && turn) {
             if (a.adjacent) {
-                const float4 u = *reinterpret_cast<const float4 *>(cs + i0);      // pairs i0/2, i0/2 + 1
-                const float4 v = *reinterpret_cast<const float4 *>(cs + i0 + 4);
-                const float cc[4] = {u.x, u.z, v.x, v.z}, sn[4] = {u.y, u.w, v.y, v.w};
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float p0 = x0[2 * i], q0 = x0[2 * i + 1], p1 = x1[2 * i], q1 = x1[2 * i + 1];
-                    x0[2 * i] = p0 * cc[i] - q0 * sn[i];
-                    x0[2 * i + 1] = p0 * sn[i] + q0 * cc[i];
-                    x1[2 * i] = p1 * cc[2 + i] - q1 * sn[2 + i];
-                    x1[2 * i + 1] = p1 * sn[2 + i] + q1 * cc[2 + i];
+                for (int i = 0; i < V / 2; i++) {
+                    const float p0 = y0[2 * i], q0 = y0[2 * i + 1], p1 = y1[2 * i], q1 = y1[2 * i + 1];
+                    const float c0 = cs[2 * i], s0 = cs[2 * i + 1], c1 = cs[V + 2 * i], s1 = cs[V + 2 * i + 1];
+                    y0[2 * i] = p0 * c0 - q0 * s0;
+                    y0[2 * i + 1] = p0 * s0 + q0 * c0;
+                    y1[2 * i] = p1 * c1 - q1 * s1;
+                    y1[2 * i + 1] = p1 * s1 + q1 * c1;
                 }
             } else {
-                const float4 u = *reinterpret_cast<const float4 *>(cs + 2 * c4);
-                const float4 v = *reinterpret_cast<const float4 *>(cs + 2 * c4 + 4);
-                const float cc[4] = {u.x, u.z, v.x, v.z}, sn[4] = {u.y, u.w, v.y, v.w};
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float p0 = x0[i], p1 = x1[i];
-                    x0[i] = p0 * cc[i] - p1 * sn[i];
-                    x1[i] = p0 * sn[i] + p1 * cc[i];
+                for (int i = 0; i < V; i++) {
+                    const float p0 = y0[i], p1 = y1[i];
+                    y0[i] = p0 * cs[2 * i] - p1 * cs[2 * i + 1];
+                    y1[i] = p0 * cs[2 * i + 1] + p1 * cs[2 * i];
                 }
             }
         }
-    }
-    if (!mine) return;
-    if (sizeof(T) == 4 && (a.flags & VB_OUT_BF16)) {
+        if (sizeof(T) == 4 && (a.flags & VB_OUT_BF16)) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x0[i] = bf16r(x0[i]);
-            x1[i] = bf16r(x1[i]);
+            for (int i = 0; i < V; i++) {
+                y0[i] = bf16r(y0[i]);
+                y1[i] = bf16r(y1[i]);
+            }
         }
-    }
-    if (bad) {
+        if (bad) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) x0[i] = x1[i] = 0.0f;
-    }
-    T *dst = is_q ? static_cast<T *>(a.q_out) + (int64_t)t * a.ldq_out + (int64_t)h * hd
-             : !is_v && a.k_out ? static_cast<T *>(a.k_out) + (int64_t)t * a.ldk_out + (int64_t)kvh * hd
-                                : nullptr;
-    if (dst) {
-        store4(dst + i0, g.vec, x0);
-        store4(dst + i1, g.vec, x1);
-    }
-    if (is_q || pool_row < 0 || bad) return;
-    const int64_t at = (pool_row + (int64_t)kvh * g.p.page_rows) * hd;
-    if (g.p.type == VB_TYPE_F16) {
-        __half *pool = static_cast<__half *>(is_v ? g.p.v : g.p.k) + at;
-        store4(pool + i0, true, x0);
-        store4(pool + i1, true, x1);
-    } else {
-        __nv_bfloat16 *pool = static_cast<__nv_bfloat16 *>(is_v ? g.p.v : g.p.k) + at;
-        store4(pool + i0, true, x0);
-        store4(pool + i1, true, x1);
+            for (int i = 0; i < V; i++) y0[i] = y1[i] = 0.0f;
+        }
+        T *dst = is_q               ? static_cast<T *>(a.q_out) + (int64_t)t * a.ldq_out + h * hd
+                 : !is_v && a.k_out ? static_cast<T *>(a.k_out) + (int64_t)t * a.ldk_out + kvh * hd
+                                    : nullptr;
+        if (dst) {
+            store(dst + i0, g.vec, y0);
+            store(dst + i1, g.vec, y1);
+        }
+        if (is_q || pool_row < 0) continue;
+        const int64_t at = (pool_row + (int64_t)kvh * g.p.page_rows) * hd;
+        if (g.p.type == VB_TYPE_F16) {
+            __half *pool = static_cast<__half *>(is_v ? g.p.v : g.p.k) + at;
+            store(pool + i0, true, y0);
+            store(pool + i1, true, y1);
+        } else {
+            __nv_bfloat16 *pool = static_cast<__nv_bfloat16 *>(is_v ? g.p.v : g.p.k) + at;
+            store(pool + i0, true, y0);
+            store(pool + i1, true, y1);
+        }
     }
 }
 
 int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who);
 
-template <typename T>
-static cudaError_t launch_qk(vb_ctx *ctx, const QKArgs &g) {
-    const int hd = g.a.head_dim;
-    const int64_t items = (int64_t)g.a.n_tokens * (g.a.n_heads + g.a.n_kv_heads * (g.store ? 2 : 1));
-    const int lph = hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
+template <typename T, int V>
+static cudaError_t launch_qk_v(vb_ctx *ctx, const QKArgs &g) {
+    const int rows = QK_ROWS<V>, heads = g.a.n_heads + g.a.n_kv_heads * (g.store ? 2 : 1);
+    const int64_t items = (int64_t)g.a.n_tokens * ((heads + rows - 1) / rows);
+    int lph = 1;
+    while (lph * 2 * V < g.a.head_dim) lph *= 2;
     const unsigned grid = (unsigned)((items * lph + QK_THREADS - 1) / QK_THREADS);
     switch (lph) {
-        case 4: return pdl_launch(ctx, qk_norm_rope_kernel<T, 4>, dim3(grid), dim3(QK_THREADS), 0, g);
-        case 8: return pdl_launch(ctx, qk_norm_rope_kernel<T, 8>, dim3(grid), dim3(QK_THREADS), 0, g);
-        case 16: return pdl_launch(ctx, qk_norm_rope_kernel<T, 16>, dim3(grid), dim3(QK_THREADS), 0, g);
-        default: return pdl_launch(ctx, qk_norm_rope_kernel<T, 32>, dim3(grid), dim3(QK_THREADS), 0, g);
+        case 1: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 1>, dim3(grid), dim3(QK_THREADS), 0, g);
+        case 2: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 2>, dim3(grid), dim3(QK_THREADS), 0, g);
+        case 4: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 4>, dim3(grid), dim3(QK_THREADS), 0, g);
+        case 8: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 8>, dim3(grid), dim3(QK_THREADS), 0, g);
+        case 16: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 16>, dim3(grid), dim3(QK_THREADS), 0, g);
+        default: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 32>, dim3(grid), dim3(QK_THREADS), 0, g);
     }
+}
+
+// Pieces of 8 values where both the turned and the passed part of a row split
+// into such pieces.
+template <typename T>
+static cudaError_t launch_qk(vb_ctx *ctx, const QKArgs &g) {
+    const int rot = g.a.rope ? g.a.rot_dim : 0;
+    return g.a.head_dim % 16 == 0 && rot % 16 == 0 ? launch_qk_v<T, 8>(ctx, g) : launch_qk_v<T, 4>(ctx, g);
 }
 
 }  // namespace vb
@@ -254,7 +303,7 @@ extern "C" int vb_qk_norm_rope(vb_ctx *ctx, const vb_qk_args *in) {
     if (a.norm && !(a.eps >= 0.0f)) return bad("negative eps");
     if ((a.flags & ~VB_OUT_BF16) || ((a.flags & VB_OUT_BF16) && a.type != VB_TYPE_F32)) return bad("unknown flags for this type");
     const int64_t qd = (int64_t)a.n_heads * a.head_dim, kd = (int64_t)a.n_kv_heads * a.head_dim;
-    if ((int64_t)a.n_tokens * (a.n_heads + 2 * (int64_t)a.n_kv_heads) * 32 / QK_THREADS >= INT32_MAX) return bad("too many rows");
+    if ((double)a.n_tokens * ((double)a.n_heads + 2.0 * a.n_kv_heads) * 32.0 >= 4294967295.0) return bad("too many rows");
     if (!a.ldq) a.ldq = qd;
     if (!a.ldk) a.ldk = kd;
     if (!a.ldv) a.ldv = kd;
@@ -279,7 +328,10 @@ extern "C" int vb_qk_norm_rope(vb_ctx *ctx, const vb_qk_args *in) {
     if (all % es || ((uintptr_t)a.pos | (uintptr_t)a.q_weight | (uintptr_t)a.k_weight | (uintptr_t)a.seq |
                      (uintptr_t)a.row) % 4 || (uintptr_t)a.rope % 16)
         return bad("misaligned pointer");
-    g.vec = all % (4 * es) == 0 && (a.ldq | a.ldk | a.ldv | a.ldq_out | a.ldk_out) % 4 == 0;
+    const int64_t lanes = 16 / (int64_t)es;
+    g.vec = all % 16 == 0 && (a.ldq | a.ldk | a.ldv | a.ldq_out | a.ldk_out) % lanes == 0;
+    g.vec_w = ((uintptr_t)a.q_weight | (uintptr_t)a.k_weight) % 16 == 0;
+    g.inv_dim = 1.0f / (float)a.head_dim;
     g.err = ctx->op_error;
     cudaError_t e = a.type == VB_TYPE_F32   ? launch_qk<float>(ctx, g)
                     : a.type == VB_TYPE_F16 ? launch_qk<__half>(ctx, g)

@@ -391,7 +391,7 @@ class Context:
         """Of the last drafted[i] rows of seqs[i] keep those at
         path[i][:kept[i]] (int32 [n][most])."""
         n = _count(seqs, drafted, kept)
-        if path.dim() != 2 or path.shape[0] != n or str(path.dtype) != "torch.int32" or not path.is_contiguous():
+        if path.dim() != 2 or path.shape[0] != n or not _is_int32(path) or not path.is_contiguous():
             raise ValueError("path: contiguous int32 [n][most]")
         self.check(self.L.vb_pages_keep(self.h, p.ref, n, seqs.data_ptr(), drafted.data_ptr(), kept.data_ptr(),
                                         path.data_ptr(), path.shape[1]))
@@ -419,13 +419,24 @@ class Context:
         self.check(self.L.vb_tree_attention(self.h, args.ref))
 
 
+_int32 = None
+
+
+def _is_int32(t):
+    global _int32
+    if _int32 is None:
+        import torch
+        _int32 = torch.int32
+    return t.dtype is _int32
+
+
 def _count(*arrays):
     """Length of device int32 vectors that belong together."""
-    n = arrays[0].shape[0]
+    shape = arrays[0].shape
     for a in arrays:
-        if a.dim() != 1 or a.shape[0] != n or str(a.dtype) != "torch.int32" or not (n < 2 or a.is_contiguous()):
+        if len(shape) != 1 or a.shape != shape or not _is_int32(a) or not a.is_contiguous():
             raise ValueError("contiguous int32 vectors of one length are wanted")
-    return n
+    return shape[0]
 
 
 def _type_of(t):
