@@ -10,15 +10,19 @@
 // A lane holds two pieces of V values whose pairs it rotates itself -- i ..
 // with i + rot/2 .. of the first half, or two neighbouring pieces when pairs
 // are adjacent -- so the only exchange is the sum of squares over the group.
-// V is 8 where the halves of the row allow it (a lane's piece is then 16 or 32
-// bytes), else 4.
+// V is what 16 bytes hold: 4 fp32 values, 8 of 16 bits (4 where the halves of
+// the row do not split into eights).  Longer pieces would leave gaps between
+// the lanes of a load.
 #include "vb_common.cuh"
 #include "vb_kernels.cuh"
 #include "vb_tc.cuh"
 
+#include <algorithm>
+
 namespace vb {
 
 constexpr int QK_THREADS = 256;
+constexpr int QK_WAVES = 2;
 
 struct QKArgs {
     vb_qk_args a;
@@ -27,6 +31,7 @@ struct QKArgs {
     int vec;                // pointers and strides allow 16-byte accesses
     int vec_w;              // of the weights too
     float inv_dim;          // 1 / head_dim
+    int per;                // head rows of a group
     int *err;
 };
 
@@ -98,39 +103,70 @@ __device__ __forceinline__ void store(T *p, bool vec, const float (&y)[V]) {
     }
 }
 
-template <int V>
-__device__ __forceinline__ void load_floats(const float *p, bool vec, float (&y)[V]) {
-    Piece<float, V> v;
-    load(p, vec, v);
-#pragma unroll
-    for (int i = 0; i < V; i++) y[i] = v.x[i];
+// Two fp32 values in a 64-bit register: the arithmetic below runs on pairs,
+// which halves its instructions.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+    f32x2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void split(f32x2 d, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f32x2 swapped(f32x2 d) {
+    float a, b;
+    split(d, a, b);
+    return pair(b, a);
 }
 
-// A group takes ROWS head rows of one token, all their loads in flight
-// together: the token's place, its table row and the weights are fetched once
-// for them, and a thread has enough bytes on their way to keep HBM busy.
-template <int V>
-constexpr int QK_ROWS = 16 / V;
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Piece<T, V> &x, f32x2 (&y)[V / 2]) {
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) y[i] = pair(Elem<T>::get(x.x[2 * i]), Elem<T>::get(x.x[2 * i + 1]));
+}
 
-template <typename T, int V, int LPH>
-__global__ void __launch_bounds__(QK_THREADS, 3) qk_norm_rope_kernel(const __grid_constant__ QKArgs g) {
-    constexpr int ROWS = QK_ROWS<V>;
+template <typename T, int V>
+__device__ __forceinline__ void store2(T *p, bool vec, const f32x2 (&y)[V]) {
+    float z[2 * V];
+#pragma unroll
+    for (int i = 0; i < V; i++) split(y[i], z[2 * i], z[2 * i + 1]);
+    store(p, vec, z);
+}
+
+// A group takes `per` head rows of one token (q heads, then k, then v), ROWS
+// of them at a time with the next ROWS on their way: the token's place, its
+// table row and the weights are fetched once for them, and a thread always has
+// bytes on their way.  Neighbouring groups take the same rows of neighbouring
+// tokens, so a warp's control flow is one.  A CTA of 256 threads needs about 80
+// registers a thread with pieces of 4 values and 120 with 8.
+constexpr int QK_ROWS = 2;
+
+template <typename T, int V, int LPH, bool ADJACENT>
+__global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kernel(const __grid_constant__ QKArgs g) {
+    constexpr int ROWS = QK_ROWS, H = V / 2;
     pdl_trigger();
     pdl_wait();
     const vb_qk_args &a = g.a;
     const int hd = a.head_dim, nq = a.n_heads, nk = a.n_kv_heads;
-    const int heads = nq + nk + (g.store ? nk : 0), chunks = (heads + ROWS - 1) / ROWS;
-    const unsigned item = (blockIdx.x * QK_THREADS + threadIdx.x) / LPH;
-    const int lane = threadIdx.x % LPH;
+    const int t = (int)((blockIdx.x * QK_THREADS + threadIdx.x) / LPH), lane = threadIdx.x % LPH;
     const unsigned group = LPH == 32 ? 0xffffffffu : ((1u << LPH) - 1u) << (threadIdx.x % 32 / LPH * LPH);
-    const int t = (int)(item / (unsigned)chunks), h0 = (int)(item - (unsigned)t * (unsigned)chunks) * ROWS;
     if (t >= a.n_tokens) return;                          // whole groups
+    const int h_lo = blockIdx.y * g.per, h_hi = min(h_lo + g.per, nq + nk + (g.store ? nk : 0));
     // the lane's two pieces: i0 and i1, rotated with each other or passed on
     const int rot = a.rope ? a.rot_dim : 0, c = V * lane;
     const bool mine = lane < hd / (2 * V);
     int i0, i1;
     bool turn;
-    if (a.adjacent) {
+    if (ADJACENT) {
         i0 = 2 * c;
         i1 = i0 + V;
         turn = i0 < rot;
@@ -143,145 +179,178 @@ __global__ void __launch_bounds__(QK_THREADS, 3) qk_norm_rope_kernel(const __gri
     // round trips to memory in all
     int pos = a.rope ? a.pos[t] : 0;
     const int seq = g.store ? a.seq[t] : -1, row = g.store ? a.row[t] : 0;
-    Piece<T, V> x0[ROWS], x1[ROWS];
+    auto fetch = [&](int h, Piece<T, V> (&u)[ROWS], Piece<T, V> (&v)[ROWS]) {
 #pragma unroll
-    for (int r = 0; r < ROWS; r++) {
-        const int h = h0 + r;
-        const T *src = h < nq        ? static_cast<const T *>(a.q) + (int64_t)t * a.ldq + h * hd
-                       : h < nq + nk ? static_cast<const T *>(a.k) + (int64_t)t * a.ldk + (h - nq) * hd
-                                     : static_cast<const T *>(a.v) + (int64_t)t * a.ldv + (h - nq - nk) * hd;
-        if (mine && h < heads) {
-            load(src + i0, g.vec, x0[r]);
-            load(src + i1, g.vec, x1[r]);
+        for (int r = 0; r < ROWS; r++, h++) {
+            const T *src = h < nq        ? static_cast<const T *>(a.q) + (int64_t)t * a.ldq + h * hd
+                           : h < nq + nk ? static_cast<const T *>(a.k) + (int64_t)t * a.ldk + (h - nq) * hd
+                                         : static_cast<const T *>(a.v) + (int64_t)t * a.ldv + (h - nq - nk) * hd;
+            if (mine && h < h_hi) {
+                load(src + i0, g.vec, u[r]);
+                load(src + i1, g.vec, v[r]);
+            }
         }
-    }
+    };
+    Piece<T, V> x0[ROWS], x1[ROWS];
+    fetch(h_lo, x0, x1);
     // an invalid place or position skips the whole token
     const bool off_table = a.rope && (pos < 0 || pos >= a.rope_rows);
     if (off_table) pos = 0;
     int page = 0;
     const bool placed = seq >= 0 && seq < g.p.n_seqs && row >= 0 && row / g.p.page_rows < g.p.max_pages;
     if (placed) page = g.p.table[(int64_t)seq * g.p.max_pages + row / g.p.page_rows];
-    float cs[2 * V];                                      // (cos, sin) of the lane's V pairs
-    if (turn && mine) load_floats(a.rope + (int64_t)pos * rot + (a.adjacent ? i0 : 2 * c), true, cs);
+    // A piece y turns to y * c + z * s: z is the other piece (and s negative for
+    // the first) or, where pairs are adjacent, y's own with each pair swapped.
+    f32x2 cs_c[ADJACENT ? V : H], cs_s[V], w0[H], w1[H];
+    if (turn && mine) {
+        Piece<float, 2 * V> cs;
+        load(a.rope + (int64_t)pos * rot + (ADJACENT ? i0 : 2 * c), true, cs);
+        if constexpr (ADJACENT) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                cs_c[i] = pair(cs.x[2 * i], cs.x[2 * i]);
+                cs_s[i] = pair(-cs.x[2 * i + 1], cs.x[2 * i + 1]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < H; i++) {
+                cs_c[i] = pair(cs.x[4 * i], cs.x[4 * i + 2]);
+                cs_s[i] = pair(-cs.x[4 * i + 1], -cs.x[4 * i + 3]);
+                cs_s[H + i] = pair(cs.x[4 * i + 1], cs.x[4 * i + 3]);
+            }
+        }
+    }
     const bool no_row = g.store && seq != -1 && (!placed || page < 0 || page >= g.p.n_pages);
     const bool bad = off_table || no_row;
     if (bad && lane == 0) atomicCAS(g.err, 0, off_table ? VB_DEV_QK_POS : VB_DEV_QK_ROW);
-    int64_t pool_row = -1;
-    if (g.store && seq != -1 && !bad)
-        pool_row = (((int64_t)a.layer * g.p.n_pages + page) * nk) * g.p.page_rows + row % g.p.page_rows;
+    const int64_t pool_head = (int64_t)g.p.page_rows * hd;
+    const bool keep = g.store && seq != -1 && !bad;
+    const int64_t at = keep ? ((int64_t)a.layer * g.p.n_pages + page) * nk * pool_head + (int64_t)(row % g.p.page_rows) * hd : 0;
+    auto weights = [&](const float *w) {                  // (ones where there are none)
+        Piece<float, V> u, v;
 #pragma unroll
-    for (int r = 0; r < ROWS; r++) {
-        const int h = h0 + r;
-        if (h >= heads) break;                            // for the whole group
-        const bool is_q = h < nq, is_v = h >= nq + nk;
-        const int kvh = is_v ? h - nq - nk : h - nq;
-        float y0[V], y1[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            y0[i] = mine ? Elem<T>::get(x0[r].x[i]) : 0.0f;
-            y1[i] = mine ? Elem<T>::get(x1[r].x[i]) : 0.0f;
+        for (int i = 0; i < V; i++) u.x[i] = v.x[i] = 1.0f;
+        if (w && mine) {
+            load(w + i0, g.vec_w, u);
+            load(w + i1, g.vec_w, v);
         }
-        if (!is_v && a.norm) {
-            float ss = 0.0f;
+        widen(u, w0);
+        widen(v, w1);
+    };
+    if (a.norm) weights(h_lo < nq ? a.q_weight : a.k_weight);
+    for (int h = h_lo; h < h_hi; h += ROWS) {
+        Piece<T, V> n0[ROWS], n1[ROWS];
+        fetch(h + ROWS, n0, n1);
 #pragma unroll
-            for (int i = 0; i < V; i++) ss = fmaf(y0[i], y0[i], fmaf(y1[i], y1[i], ss));
-#pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-            const float rs = rsqrtf(ss * g.inv_dim + a.eps);
-            const float *w = is_q ? a.q_weight : a.k_weight;
-            float w0[V], w1[V];
-            if (w && mine) {
-                load_floats(w + i0, g.vec_w, w0);
-                load_floats(w + i1, g.vec_w, w1);
+        for (int r = 0; r < ROWS; r++) {
+            const int hr = h + r;
+            if (hr >= h_hi) break;                            // for the whole warp
+            const bool is_q = hr < nq, is_v = hr >= nq + nk;
+            const int kvh = is_v ? hr - nq - nk : hr - nq;
+            if (hr == nq && hr > h_lo && a.norm) weights(a.k_weight);
+            f32x2 y0[H] = {}, y1[H] = {};
+            if (mine) {
+                widen(x0[r], y0);
+                widen(x1[r], y1);
             }
+            if (!is_v && a.norm) {
+                f32x2 sq = 0;
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                y0[i] *= rs;
-                y1[i] *= rs;
-                if (w) {
-                    y0[i] *= w0[i];
-                    y1[i] *= w1[i];
+                for (int i = 0; i < H; i++) sq = fma2(y0[i], y0[i], fma2(y1[i], y1[i], sq));
+                float ss, s2;
+                split(sq, ss, s2);
+                ss += s2;
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+                const float rs = rsqrtf(ss * g.inv_dim + a.eps);
+                const f32x2 rs2 = pair(rs, rs);
+#pragma unroll
+                for (int i = 0; i < H; i++) {
+                    y0[i] = mul2(y0[i], rs2);
+                    y1[i] = mul2(y1[i], rs2);
+                    y0[i] = mul2(y0[i], w0[i]);
+                    y1[i] = mul2(y1[i], w1[i]);
                 }
             }
-        }
-        if (!mine) continue;
-        if (!is_v && turn) {
-            if (a.adjacent) {
+            if (!mine) continue;
+            if (turn && !is_v) {
 #pragma unroll
-                for (int i = 0; i < V / 2; i++) {
-                    const float p0 = y0[2 * i], q0 = y0[2 * i + 1], p1 = y1[2 * i], q1 = y1[2 * i + 1];
-                    const float c0 = cs[2 * i], s0 = cs[2 * i + 1], c1 = cs[V + 2 * i], s1 = cs[V + 2 * i + 1];
-                    y0[2 * i] = p0 * c0 - q0 * s0;
-                    y0[2 * i + 1] = p0 * s0 + q0 * c0;
-                    y1[2 * i] = p1 * c1 - q1 * s1;
-                    y1[2 * i + 1] = p1 * s1 + q1 * c1;
+                for (int i = 0; i < H; i++) {
+                    const f32x2 p0 = y0[i], p1 = y1[i];
+                    y0[i] = fma2(p0, cs_c[i], mul2(ADJACENT ? swapped(p0) : p1, cs_s[i]));
+                    y1[i] = fma2(p1, cs_c[ADJACENT ? H + i : i], mul2(ADJACENT ? swapped(p1) : p0, cs_s[H + i]));
                 }
+            }
+            if (sizeof(T) == 4 && (a.flags & VB_OUT_BF16)) {
+#pragma unroll
+                for (int i = 0; i < H; i++) {
+                    float u, v;
+                    split(y0[i], u, v);
+                    y0[i] = pair(bf16r(u), bf16r(v));
+                    split(y1[i], u, v);
+                    y1[i] = pair(bf16r(u), bf16r(v));
+                }
+            }
+            if (bad) {
+#pragma unroll
+                for (int i = 0; i < H; i++) y0[i] = y1[i] = 0;
+            }
+            T *dst = is_q               ? static_cast<T *>(a.q_out) + (int64_t)t * a.ldq_out + hr * hd
+                     : !is_v && a.k_out ? static_cast<T *>(a.k_out) + (int64_t)t * a.ldk_out + kvh * hd
+                                        : nullptr;
+            if (dst) {
+                store2(dst + i0, g.vec, y0);
+                store2(dst + i1, g.vec, y1);
+            }
+            if (is_q || !keep) continue;
+            if (g.p.type == VB_TYPE_F16) {
+                __half *pool = static_cast<__half *>(is_v ? g.p.v : g.p.k) + at + kvh * pool_head;
+                store2(pool + i0, true, y0);
+                store2(pool + i1, true, y1);
             } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const float p0 = y0[i], p1 = y1[i];
-                    y0[i] = p0 * cs[2 * i] - p1 * cs[2 * i + 1];
-                    y1[i] = p0 * cs[2 * i + 1] + p1 * cs[2 * i];
-                }
+                __nv_bfloat16 *pool = static_cast<__nv_bfloat16 *>(is_v ? g.p.v : g.p.k) + at + kvh * pool_head;
+                store2(pool + i0, true, y0);
+                store2(pool + i1, true, y1);
             }
         }
-        if (sizeof(T) == 4 && (a.flags & VB_OUT_BF16)) {
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                y0[i] = bf16r(y0[i]);
-                y1[i] = bf16r(y1[i]);
-            }
-        }
-        if (bad) {
-#pragma unroll
-            for (int i = 0; i < V; i++) y0[i] = y1[i] = 0.0f;
-        }
-        T *dst = is_q               ? static_cast<T *>(a.q_out) + (int64_t)t * a.ldq_out + h * hd
-                 : !is_v && a.k_out ? static_cast<T *>(a.k_out) + (int64_t)t * a.ldk_out + kvh * hd
-                                    : nullptr;
-        if (dst) {
-            store(dst + i0, g.vec, y0);
-            store(dst + i1, g.vec, y1);
-        }
-        if (is_q || pool_row < 0) continue;
-        const int64_t at = (pool_row + (int64_t)kvh * g.p.page_rows) * hd;
-        if (g.p.type == VB_TYPE_F16) {
-            __half *pool = static_cast<__half *>(is_v ? g.p.v : g.p.k) + at;
-            store(pool + i0, true, y0);
-            store(pool + i1, true, y1);
-        } else {
-            __nv_bfloat16 *pool = static_cast<__nv_bfloat16 *>(is_v ? g.p.v : g.p.k) + at;
-            store(pool + i0, true, y0);
-            store(pool + i1, true, y1);
+        for (int r = 0; r < ROWS; r++) {
+            x0[r] = n0[r];
+            x1[r] = n1[r];
         }
     }
 }
 
 int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who);
 
-template <typename T, int V>
-static cudaError_t launch_qk_v(vb_ctx *ctx, const QKArgs &g) {
-    const int rows = QK_ROWS<V>, heads = g.a.n_heads + g.a.n_kv_heads * (g.store ? 2 : 1);
-    const int64_t items = (int64_t)g.a.n_tokens * ((heads + rows - 1) / rows);
+template <typename T, int V, bool ADJACENT>
+static cudaError_t launch_qk_v(vb_ctx *ctx, QKArgs &g) {
+    const int heads = g.a.n_heads + g.a.n_kv_heads * (g.store ? 2 : 1), rows = QK_ROWS;
     int lph = 1;
     while (lph * 2 * V < g.a.head_dim) lph *= 2;
-    const unsigned grid = (unsigned)((items * lph + QK_THREADS - 1) / QK_THREADS);
+    // as many rows to a group as leave QK_WAVES waves of threads: a token of few
+    // is spread over the SMs, one of many shares what it fetches once
+    const int64_t room = (int64_t)QK_WAVES * ctx->sm_count * 3 * QK_THREADS / lph;
+    int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((heads + rows - 1) / rows, room / std::max(1, g.a.n_tokens)));
+    g.per = (int)((heads + chunks - 1) / chunks + rows - 1) / rows * rows;
+    const dim3 grid((unsigned)(((int64_t)g.a.n_tokens * lph + QK_THREADS - 1) / QK_THREADS), (unsigned)((heads + g.per - 1) / g.per));
     switch (lph) {
-        case 1: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 1>, dim3(grid), dim3(QK_THREADS), 0, g);
-        case 2: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 2>, dim3(grid), dim3(QK_THREADS), 0, g);
-        case 4: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 4>, dim3(grid), dim3(QK_THREADS), 0, g);
-        case 8: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 8>, dim3(grid), dim3(QK_THREADS), 0, g);
-        case 16: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 16>, dim3(grid), dim3(QK_THREADS), 0, g);
-        default: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 32>, dim3(grid), dim3(QK_THREADS), 0, g);
+        case 1: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 1, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
+        case 2: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 2, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
+        case 4: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 4, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
+        case 8: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 8, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
+        case 16: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 16, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
+        default: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 32, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
     }
 }
 
-// Pieces of 8 values where both the turned and the passed part of a row split
-// into such pieces.
 template <typename T>
-static cudaError_t launch_qk(vb_ctx *ctx, const QKArgs &g) {
+static cudaError_t launch_qk(vb_ctx *ctx, QKArgs &g) {
     const int rot = g.a.rope ? g.a.rot_dim : 0;
-    return g.a.head_dim % 16 == 0 && rot % 16 == 0 ? launch_qk_v<T, 8>(ctx, g) : launch_qk_v<T, 4>(ctx, g);
+    if constexpr (sizeof(T) == 2)
+        if (g.a.head_dim % 16 == 0 && rot % 16 == 0)
+            return g.a.adjacent ? launch_qk_v<T, 8, true>(ctx, g) : launch_qk_v<T, 8, false>(ctx, g);
+    return g.a.adjacent ? launch_qk_v<T, 4, true>(ctx, g) : launch_qk_v<T, 4, false>(ctx, g);
 }
 
 }  // namespace vb
