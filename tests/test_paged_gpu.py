@@ -528,6 +528,14 @@ def test_tree_attention(ctx, type, lens, drafted, nh, nkv, hd, P, mask):
     check_tree(ctx, tree_case(ctx, type, lens, drafted, nh, nkv, hd, P, mask))
 
 
+@pytest.mark.parametrize("hd", [8, 64, 96, 128, 256])
+@pytest.mark.parametrize("drafted,nh,nkv", [(1, 1, 1), (4, 2, 2), (3, 1, 1), (1, 8, 2), (2, 4, 2), (1, 3, 1), (1, 10, 2), (5, 2, 2), (2, 4, 1),
+                                            (8, 1, 1), (1, 16, 2), (2, 6, 2), (7, 1, 1), (9, 1, 1), (3, 3, 1)])
+def test_tree_fp32_of_few_rows(ctx, drafted, nh, nkv, hd):
+    """Blocks of up to 4, 8 and 16 rows, within one CTA and across several."""
+    check_tree(ctx, tree_case(ctx, "f32", [drafted + 3, 2700, drafted], [drafted, drafted, drafted], nh, nkv, hd, 16, "any", seed=11))
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("lens,drafted,P", [([30000], [2], 64), ([9000, 20000], [1, 1], 16), ([25000, 100], [40, 3], 32)])
 def test_tree_many_tiles_for_each_cta(ctx, type, lens, drafted, P):

@@ -66,15 +66,23 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 // TYPE: the types; HDP: head_dim rounded up to 64, 128 or 256; R: 16-row
 // pieces per warp; WM: row groups of warps.  8 / WM warps share a row group
 // and split a tile's rows 16 each (with WM = 1 two sets of four take tiles
-// in turn) and merge at the item's end.
-template <int TYPE, int HDP, int R, int WM>
+// in turn) and merge at the item's end.  PK: with 4 or 8 rows a block the
+// 16-bit terms of an fp32 value lie under one another in the 16 rows of an
+// instruction (row t * PK + m: term t of row m), which then takes one product
+// or two in place of three; a row's scores and sums are added over its terms.
+template <int TYPE, int HDP, int R, int WM, int PK>
 __global__ void __launch_bounds__(TR_THREADS, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                           const __grid_constant__ TreeArgs g) {
-    constexpr int MT = 16 * R * WM;
+    constexpr bool PACKED = PK < 16;
+    static_assert(!PACKED || (TYPE == TR_F32 && R == 1 && WM == 1), "terms are packed for fp32 alone");
+    constexpr int MT = PACKED ? PK : 16 * R * WM;    // rows of a block
+    constexpr int H = PACKED ? 1 : 2;                // rows that a thread keeps of 16
     constexpr int KW = 8 / WM;                       // warps of a row group
     constexpr int SETS = WM == 1 ? 2 : 1;
     constexpr int QT = TYPE == TR_F32 ? 3 : 1;       // 16-bit terms of a query value: 3 bf16 hold an fp32 exactly
+    constexpr int NM = PK == 4 ? 1 : PK == 8 ? 2 : QT;                  // products that hold them
+    constexpr int QROWS = PACKED ? 16 * NM : QT * MT;
     constexpr int CB = HDP / 64;                     // 128-byte column blocks
     constexpr int NT = HDP / 8;                      // output tiles of 8 columns
     constexpr uint32_t TILE = TR_KT * 128;           // bytes of a column block
@@ -84,9 +92,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 
     extern __shared__ uint8_t raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    float *merge = reinterpret_cast<float *>(ring + (size_t)g.stages * STAGE);      // [4][16][MPITCH]
-    uint8_t *qs = reinterpret_cast<uint8_t *>(merge + 4 * 16 * MPITCH);             // [QT][MT][QPITCH]
-    float2 *ml = reinterpret_cast<float2 *>(qs + QT * MT * QPITCH);                 // [8][16 * R]
+    float *merge = reinterpret_cast<float *>(ring + (size_t)g.stages * STAGE);      // [4][8 * H][MPITCH]
+    uint8_t *qs = reinterpret_cast<uint8_t *>(merge + 4 * 8 * H * MPITCH);          // [QROWS][QPITCH]: term t of row m at t * MT + m
+    float2 *ml = reinterpret_cast<float2 *>(qs + QROWS * QPITCH);                   // [8][16 * R]
     __shared__ uint64_t full[TR_MAX_STAGES], empty[TR_MAX_STAGES];
     __shared__ TreeCut cut;
     __shared__ int abort_flag, not_finite;
@@ -209,7 +217,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 const int e = threadIdx.x + 256 * (i0 + i), m = e / (HDP / 4), d = e % (HDP / 4) * 4;
                 if (i0 + i >= N_Q || m >= MT) continue;
 #pragma unroll
-                for (int t = 0; t < QT; t++) {
+                for (int t = 0; t < (PK == 4 ? 4 : QT); t++) {      // four rows: the fourth term is 0 and fills the 16
                     if constexpr (TYPE == TR_F32) {
                         y[i] = make_uint2(pack2<TYPE>(x[i][0], x[i][1]), pack2<TYPE>(x[i][2], x[i][3]));
                         x[i][0] -= bf16_to_f((uint16_t)y[i].x);
@@ -223,19 +231,20 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         }
         consumer_sync(256);
 
-        float o[R][NT][4], m[R][2], l[R][2];
-        int tok[R][2];                                  // token of the thread's rows, -1: no such row
+        float o[R][NT][4], m[R][H], l[R][H];
+        int tok[R][H];                                  // token of the thread's rows, -1: no such row
 #pragma unroll
-        for (int r = 0; r < R; r++)
+        for (int r = 0; r < R; r++) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < H; h++) {
                 m[r][h] = -INFINITY;
                 l[r][h] = 0.0f;
-                const int mr = wm * 16 * R + 16 * r + quad + 8 * h;
+                const int mr = PACKED ? quad % PK : wm * 16 * R + 16 * r + quad + 8 * h;
                 tok[r][h] = mr < rows ? w.tok + mr / w.heads : -1;
-#pragma unroll
-                for (int t = 0; t < NT; t++) o[r][t][2 * h] = o[r][t][2 * h + 1] = 0.0f;
             }
+#pragma unroll
+            for (int t = 0; t < NT; t++) o[r][t][0] = o[r][t][1] = o[r][t][2] = o[r][t][3] = 0.0f;
+        }
         const uint32_t q_at = smem_u32(qs) +
                               (uint32_t)((wm * 16 * R + (lane & 7) + ((lane >> 3) & 1) * 8) * QPITCH + (lane >> 4) * 16);
         for (int x = 0; x < n_tiles; x++, it++) {
@@ -262,8 +271,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 for (int r = 0; r < R; r++) {
                     uint32_t qa[4];
 #pragma unroll
-                    for (int t = QT - 1; t > 0; t--) {
-                        ldsm4(qa, q_at + (uint32_t)((t * MT + 16 * r) * QPITCH + ks * 32));
+                    for (int t = NM - 1; t > 0; t--) {
+                        ldsm4(qa, q_at + (uint32_t)((t * (PACKED ? 16 : MT) + 16 * r) * QPITCH + ks * 32));
                         mma16816<TYPE>(lo[r][0], qa, kb[0], kb[1]);
                         mma16816<TYPE>(lo[r][1], qa, kb[2], kb[3]);
                     }
@@ -289,7 +298,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) c[r][t][e] += lo[r][t][e];
+                        for (int e = 0; e < 2 * H; e++) {
+                            if constexpr (PACKED) lo[r][t][e] += c[r][t][e + 2];
+                            c[r][t][e] += lo[r][t][e];
+                            if constexpr (PK == 4) c[r][t][e] += __shfl_xor_sync(0xffffffffu, c[r][t][e], 16);
+                        }
             }
             const int r0 = (w.tile + x) * TR_KT + slice;       // cache row of the warp's first column
             const bool edge = r0 + 16 > w.clear;               // not every row is seen by every token
@@ -298,14 +311,14 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) c[r][t][e] *= g.scale_log2;
+                    for (int e = 0; e < 2 * H; e++) c[r][t][e] *= g.scale_log2;
             if (edge) {
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
+                        for (int e = 0; e < 2 * H; e++) {
                             const int j = tok[r][e >> 1], d = r0 + 8 * t + 2 * ql + (e & 1) - w.q.base;
                             if (j < 0 || d + w.q.base >= w.visible || (d >= 0 && !tree_sees(g, w.q, j, d)))
                                 c[r][t][e] = -INFINITY;
@@ -329,12 +342,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 __syncwarp();
             }
             // running maximum and sum
-            float al[R][2];
+            float al[R][H];
             bool moved = false;
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < H; h++) {
                     float v = fmaxf(fmaxf(c[r][0][2 * h], c[r][0][2 * h + 1]), fmaxf(c[r][1][2 * h], c[r][1][2 * h + 1]));
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -368,13 +381,21 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
+                    for (int k = 0; k < 4; k += PACKED ? 2 : 1) {
                         const float x0 = c[r][k >> 1][2 * (k & 1)], x1 = c[r][k >> 1][2 * (k & 1) + 1];
                         pa[r][k] = pack2<TYPE>(x0, x1);
                         if constexpr (TYPE == TR_F32) {
                             const float y0 = x0 - bf16_to_f((uint16_t)pa[r][k]), y1 = x1 - bf16_to_f((uint16_t)(pa[r][k] >> 16));
                             pb[r][k] = pack2<TYPE>(y0, y1);
                             pc[r][k] = pack2<TYPE>(y0 - bf16_to_f((uint16_t)pb[r][k]), y1 - bf16_to_f((uint16_t)(pb[r][k] >> 16)));
+                        }
+                        if constexpr (PK == 4) {            // rows 0..3 | 4..7, 8..11 | 12..15
+                            pa[r][k + 1] = quad < 4 ? pc[r][k] : 0;
+                            pa[r][k] = quad < 4 ? pa[r][k] : pb[r][k];
+                        } else if constexpr (PK == 8) {     // rows 0..7, 8..15 of two products
+                            pa[r][k + 1] = pb[r][k];
+                            pb[r][k] = pc[r][k];
+                            pb[r][k + 1] = 0;
                         }
                     }
 #pragma unroll
@@ -389,16 +410,21 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                             // one rounded fp32 step: the tensor cores' own long sums
                             // lose more
                             float d0[4] = {}, d1[4] = {};
-                            mma16816<TYPE>(d0, pc[r], vb[0], vb[1]);
-                            mma16816<TYPE>(d1, pc[r], vb[2], vb[3]);
-                            mma16816<TYPE>(d0, pb[r], vb[0], vb[1]);
-                            mma16816<TYPE>(d1, pb[r], vb[2], vb[3]);
+                            if constexpr (NM > 2) {
+                                mma16816<TYPE>(d0, pc[r], vb[0], vb[1]);
+                                mma16816<TYPE>(d1, pc[r], vb[2], vb[3]);
+                            }
+                            if constexpr (NM > 1) {
+                                mma16816<TYPE>(d0, pb[r], vb[0], vb[1]);
+                                mma16816<TYPE>(d1, pb[r], vb[2], vb[3]);
+                            }
                             mma16816<TYPE>(d0, pa[r], vb[0], vb[1]);
                             mma16816<TYPE>(d1, pa[r], vb[2], vb[3]);
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                o[r][t][e] = fmaf(o[r][t][e], al[r][e >> 1], d0[e]);
-                                o[r][t + 1][e] = fmaf(o[r][t + 1][e], al[r][e >> 1], d1[e]);
+                                const float a = al[r][PACKED ? 0 : e >> 1];
+                                o[r][t][e] = fmaf(o[r][t][e], a, d0[e]);
+                                o[r][t + 1][e] = fmaf(o[r][t + 1][e], a, d1[e]);
                             }
                         } else {
                             mma16816<TYPE>(o[r][t], pa[r], vb[0], vb[1]);
@@ -412,11 +438,21 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             if (lane == 0) mbar_arrive(&empty[s]);
         }
 
+        if constexpr (PACKED) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float &x = o[0][t][e];
+                    x += o[0][t][e + 2];
+                    if constexpr (PK == 4) x += __shfl_xor_sync(0xffffffffu, x, 16);
+                }
+        }
         // ---- merge the row group's warps
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < H; h++) {
                 float &x = l[r][h];
                 x += __shfl_xor_sync(0xffffffffu, x, 1);
                 x += __shfl_xor_sync(0xffffffffu, x, 2);
@@ -427,7 +463,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < H; h++) {
                 float2 other[KW];
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -451,12 +487,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int half = KW / 2; half >= 1; half >>= 1) {
-                float *slot = merge + (size_t)((wm * (KW / 2) + kw % half) * 16) * MPITCH;
+                float *slot = merge + (size_t)((wm * (KW / 2) + kw % half) * 8 * H) * MPITCH;
                 if (kw >= half && kw < 2 * half) {
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++)
+                        for (int h = 0; h < H; h++)
                             *reinterpret_cast<float2 *>(slot + (quad + 8 * h) * MPITCH + 8 * t + 2 * ql) =
                                 make_float2(o[r][t][2 * h], o[r][t][2 * h + 1]);
                 }
@@ -465,7 +501,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
+                        for (int h = 0; h < H; h++) {
                             const float2 v = *reinterpret_cast<const float2 *>(slot + (quad + 8 * h) * MPITCH + 8 * t + 2 * ql);
                             o[r][t][2 * h] += v.x;
                             o[r][t][2 * h + 1] += v.y;
@@ -480,7 +516,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < H; h++) {
                     const int mr = wm * 16 * R + 16 * r + quad + 8 * h;
                     if (mr >= rows) continue;
                     if (whole) {
@@ -652,11 +688,11 @@ int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who);
 
 typedef void (*TreeKernel)(CUtensorMap, CUtensorMap, TreeArgs);
 
-template <int TYPE, int HDP, int R, int WM>
+template <int TYPE, int HDP, int R, int WM, int PK>
 static void tree_fit(TreeArgs &g, size_t &smem) {
-    constexpr int MT = 16 * R * WM, QT = TYPE == TR_F32 ? 3 : 1;
+    constexpr int QROWS = PK == 4 ? 16 : PK == 8 ? 32 : 16 * R * WM * (TYPE == TR_F32 ? 3 : 1), H = PK < 16 ? 1 : 2;
     constexpr size_t stage = (size_t)2 * TR_KT * HDP * 2;
-    constexpr size_t rest = (size_t)4 * 16 * (HDP + 4) * 4 + (size_t)QT * MT * (HDP * 2 + 16) + (size_t)8 * 16 * R * 8 + 1024;
+    constexpr size_t rest = (size_t)4 * 8 * H * (HDP + 4) * 4 + (size_t)QROWS * (HDP * 2 + 16) + (size_t)8 * 16 * R * 8 + 1024;
     static_assert(rest + 2 * stage <= TR_SMEM, "two stages must fit");
     g.stages = (int)std::min<size_t>(TR_MAX_STAGES, (TR_SMEM - rest) / stage);
     // two sets of warps take tiles in turn: an even ring gives each its own
@@ -712,12 +748,12 @@ int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g) {
     return VB_OK;
 }
 
-template <int TYPE, int HDP, int R, int WM>
+template <int TYPE, int HDP, int R, int WM, int PK = 16>
 static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     size_t smem;
-    tree_fit<TYPE, HDP, R, WM>(g, smem);
+    tree_fit<TYPE, HDP, R, WM, PK>(g, smem);
     const vb_pages &p = g.p;
-    int rc = tree_prepare(ctx, g, 16 * R * WM, 1, TR_KT, TR_OVER);
+    int rc = tree_prepare(ctx, g, PK < 16 ? PK : 16 * R * WM, 1, TR_KT, TR_OVER);
     if (rc) return rc;
     CUtensorMap tk, tv;
     const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;
@@ -726,7 +762,7 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     if (!make_map(&tk, static_cast<char *>(p.k) + layer, dt, 2, p.head_dim, rows, 64, box, true) ||
         !make_map(&tv, static_cast<char *>(p.v) + layer, dt, 2, p.head_dim, rows, 64, box, true))
         return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the cache refused");
-    VB_CHECK(ctx, pdl_launch(ctx, tree_attention_kernel<TYPE, HDP, R, WM>, dim3(ctx->sm_count), dim3(TR_THREADS), smem, tk,
+    VB_CHECK(ctx, pdl_launch(ctx, tree_attention_kernel<TYPE, HDP, R, WM, PK>, dim3(ctx->sm_count), dim3(TR_THREADS), smem, tk,
                              tv, g));
     VB_LAUNCH_CHECK(ctx, "tree_attention");
     return launch_tree_combine(ctx, g);
@@ -742,6 +778,10 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
 template <int TYPE, int HDP>
 static int launch_rows(vb_ctx *ctx, TreeArgs &g) {
     const int64_t rows = (int64_t)g.a.max_tokens * g.group;
+    if constexpr (TYPE == TR_F32) {
+        if (rows <= 4) return launch_tree<TYPE, HDP, 1, 1, 4>(ctx, g);
+        if (rows <= 8) return launch_tree<TYPE, HDP, 1, 1, 8>(ctx, g);
+    }
     if (rows <= 16) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);
     if constexpr (TYPE == TR_F32) {
         if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);      // more rows leave no room for two stages
@@ -759,18 +799,24 @@ static int launch_heads(vb_ctx *ctx, TreeArgs &g) {
     return hd <= 64 ? launch_rows<TYPE, 64>(ctx, g) : hd <= 128 ? launch_rows<TYPE, 128>(ctx, g) : launch_rows<TYPE, 256>(ctx, g);
 }
 
-template <int TYPE, int HDP, int R, int WM>
+template <int TYPE, int HDP, int R, int WM, int PK = 16>
 static cudaError_t allow_smem() {
-    return cudaFuncSetAttribute(tree_attention_kernel<TYPE, HDP, R, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
+    return cudaFuncSetAttribute(tree_attention_kernel<TYPE, HDP, R, WM, PK>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
 }
 
 int init_tree(vb_ctx *ctx) {
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 1, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 64, 2, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 64, 2, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 1, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 128, 2, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 128, 2, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 1, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_BF16, 64, 1, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_BF16, 128, 1, 1>()));
