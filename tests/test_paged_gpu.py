@@ -536,6 +536,13 @@ def test_tree_fp32_of_few_rows(ctx, drafted, nh, nkv, hd):
     check_tree(ctx, tree_case(ctx, "f32", [drafted + 3, 2700, drafted], [drafted, drafted, drafted], nh, nkv, hd, 16, "any", seed=11))
 
 
+@pytest.mark.parametrize("type,hd", [("f32", 64), ("f32", 128), ("f32", 256), ("bf16", 128), ("bf16", 256), ("f16", 256)])
+@pytest.mark.parametrize("drafted,nh,nkv", [(17, 1, 1), (4, 16, 2), (11, 6, 2), (8, 8, 1), (31, 4, 1), (65, 2, 1), (70, 16, 2), (3, 200, 1)])
+def test_tree_blocks_of_more_rows(ctx, type, hd, drafted, nh, nkv):
+    """Every size of a block of rows, filled and not."""
+    check_tree(ctx, tree_case(ctx, type, [drafted + 5, 1500, drafted], [drafted, drafted, drafted], nh, nkv, hd, 16, "any", seed=12))
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("lens,drafted,P", [([30000], [2], 64), ([9000, 20000], [1, 1], 16), ([25000, 100], [40, 3], 32)])
 def test_tree_many_tiles_for_each_cta(ctx, type, lens, drafted, P):

@@ -11,14 +11,20 @@
 // through a TMA ring in shared memory, the products through the tensor
 // cores.
 //
-// Work split: an item is (sequence, K/V head, block of MT rows), a unit one
+// Work split: an item is (sequence, K/V head, block of rows), a unit one
 // 64-row tile of an item's cache.  All units of a call form one line that is
 // cut evenly over the CTAs (one per SM), whatever the sequences' lengths, by
 // arithmetic that every CTA repeats from the device's own lengths.  A CTA's
 // first and last item may be shared with its neighbours: it leaves their
-// (max, sum, weighted sum) in its two slots of a workspace and
-// tree_combine_kernel adds the slots of an item in CTA order, so results do
-// not depend on timing.
+// (max, sum, weighted sum) in its two slots of a workspace and a join kernel
+// adds the slots of an item in CTA order, so results do not depend on timing.
+//
+// This file's kernel multiplies with mma.sync and serves blocks of up to 16
+// rows of any type, and what the tcgen05 kernel does not take (launch_rows).
+// With few rows the cache's bytes bound it: 524,288 rows of 2 x 2 heads of
+// 128 under one token of 16 heads take 97 us in bf16 and 103 us in fp32, the
+// next 262,144 rows 40 and 44 us of it (6.7 and 6.2 TB/s); the constant
+// 17 us are two launches, the cut, the first tiles' way and the join.
 #include "vb_common.cuh"
 #include "vb_kernels.cuh"
 #include "vb_tree.cuh"
@@ -38,13 +44,13 @@ constexpr int TR_SMEM = 226 * 1024;  // dynamic shared memory
 
 // ------------------------------------------------------------ mma helpers
 template <int TYPE>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
     if constexpr (TYPE == TR_F16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -63,23 +69,32 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "memory");
 }
 
-// TYPE: the types; HDP: head_dim rounded up to 64, 128 or 256; R: 16-row
-// pieces per warp; WM: row groups of warps.  8 / WM warps share a row group
-// and split a tile's rows 16 each (with WM = 1 two sets of four take tiles
-// in turn) and merge at the item's end.  PK: with 4 or 8 rows a block the
-// 16-bit terms of an fp32 value lie under one another in the 16 rows of an
-// instruction (row t * PK + m: term t of row m), which then takes one product
-// or two in place of three; a row's scores and sums are added over its terms.
-template <int TYPE, int HDP, int R, int WM, int PK>
+// Room for the queries, and after them for the merge of an item's warps.
+__host__ __device__ constexpr int tree_scratch(int hdp, int q_rows, int merge_rows) {
+    const int q = q_rows * (hdp * 2 + 16), merge = merge_rows * (hdp + 4) * 4;
+    return q > merge ? q : merge;
+}
+
+// TYPE: the types; HDP: head_dim rounded up to 64, 128 or 256; WM: groups of
+// warps with 16 rows each.  8 / WM warps share a group's rows, split a tile's
+// rows and merge at the item's end (with WM = 1 two sets of four warps take
+// tiles in turn).  PK: with 4 or 8 rows a block the 16-bit terms of an fp32
+// value lie under one another in the 16 rows of an instruction (row
+// t * PK + m: term t of row m), which then takes one product or two in place
+// of three; a row's scores and sums are added over its terms.  (64 sequences
+// of 8192 rows under one token of 16 heads over 2: 125 us with three
+// products, 111 us with two, of 82 us that reading the cache takes.)
+template <int TYPE, int HDP, int WM, int PK>
 __global__ void __launch_bounds__(TR_THREADS, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                           const __grid_constant__ TreeArgs g) {
     constexpr bool PACKED = PK < 16;
-    static_assert(!PACKED || (TYPE == TR_F32 && R == 1 && WM == 1), "terms are packed for fp32 alone");
-    constexpr int MT = PACKED ? PK : 16 * R * WM;    // rows of a block
+    static_assert(!PACKED || (TYPE == TR_F32 && WM == 1), "terms are packed for fp32 alone");
+    constexpr int MT = PACKED ? PK : 16 * WM;    // rows of a block
     constexpr int H = PACKED ? 1 : 2;                // rows that a thread keeps of 16
     constexpr int KW = 8 / WM;                       // warps of a row group
     constexpr int SETS = WM == 1 ? 2 : 1;
+    constexpr int NS = WM == 1 ? 1 : 4 / KW;         // 16-row slices of a tile per warp
     constexpr int QT = TYPE == TR_F32 ? 3 : 1;       // 16-bit terms of a query value: 3 bf16 hold an fp32 exactly
     constexpr int NM = PK == 4 ? 1 : PK == 8 ? 2 : QT;                  // products that hold them
     constexpr int QROWS = PACKED ? 16 * NM : QT * MT;
@@ -92,9 +107,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 
     extern __shared__ uint8_t raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    float *merge = reinterpret_cast<float *>(ring + (size_t)g.stages * STAGE);      // [4][8 * H][MPITCH]
-    uint8_t *qs = reinterpret_cast<uint8_t *>(merge + 4 * 8 * H * MPITCH);          // [QROWS][QPITCH]: term t of row m at t * MT + m
-    float2 *ml = reinterpret_cast<float2 *>(qs + QROWS * QPITCH);                   // [8][16 * R]
+    // the queries and the buffer of the merge share their room: an item's queries are done when its warps merge
+    uint8_t *qs = ring + (size_t)g.stages * STAGE;                                  // [QROWS][QPITCH]: term t of row m at t * MT + m
+    float *merge = reinterpret_cast<float *>(qs);                                   // [WM * KW / 2][8 * H][MPITCH]
+    constexpr int QS = tree_scratch(HDP, QROWS, WM * (KW / 2) * 8 * H);
+    float2 *ml = reinterpret_cast<float2 *>(qs + QS);                               // [8][16]
     __shared__ uint64_t full[TR_MAX_STAGES], empty[TR_MAX_STAGES];
     __shared__ TreeCut cut;
     __shared__ int abort_flag, not_finite;
@@ -173,7 +190,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     // ---------------------------------------------------------------- compute
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int wm = WM == 1 ? 0 : warp / KW, kw = warp % KW, set = SETS == 2 ? warp >> 2 : 0;
-    const int slice = (warp & 3) * 16;                 // this warp's 16 rows of a tile
+    const int slice = (WM == 1 ? warp & 3 : kw * NS) * 16;      // this warp's first row of a tile
     const int hd = g.p.head_dim;
     const int quad = lane >> 2, ql = lane & 3;
     int it = 0;
@@ -231,103 +248,97 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         }
         consumer_sync(256);
 
-        float o[R][NT][4], m[R][H], l[R][H];
-        int tok[R][H];                                  // token of the thread's rows, -1: no such row
+        float o[NT][4], m[H], l[H];
+        int tok[H];                                  // token of the thread's rows, -1: no such row
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-#pragma unroll
-            for (int h = 0; h < H; h++) {
-                m[r][h] = -INFINITY;
-                l[r][h] = 0.0f;
-                const int mr = PACKED ? quad % PK : wm * 16 * R + 16 * r + quad + 8 * h;
-                tok[r][h] = mr < rows ? w.tok + mr / w.heads : -1;
-            }
-#pragma unroll
-            for (int t = 0; t < NT; t++) o[r][t][0] = o[r][t][1] = o[r][t][2] = o[r][t][3] = 0.0f;
+        for (int h = 0; h < H; h++) {
+            m[h] = -INFINITY;
+            l[h] = 0.0f;
+            const int mr = PACKED ? quad % PK : wm * 16 + quad + 8 * h;
+            tok[h] = mr < rows ? w.tok + mr / w.heads : -1;
         }
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
         const uint32_t q_at = smem_u32(qs) +
-                              (uint32_t)((wm * 16 * R + (lane & 7) + ((lane >> 3) & 1) * 8) * QPITCH + (lane >> 4) * 16);
+                              (uint32_t)((wm * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * QPITCH + (lane >> 4) * 16);
         for (int x = 0; x < n_tiles; x++, it++) {
             if (SETS == 2 && (it & 1) != set) continue;
             const int s = it % g.stages;
             tree_wait_warp(&full[s], (uint32_t)(it / g.stages) & 1u, &abort_flag, g.err);
             const uint32_t kt = smem_u32(ring + (size_t)s * STAGE), vt = kt + CB * TILE;
-            // scores: 16 rows x 16 cache rows
-            float c[R][2][4], lo[R][2][4];
+            // scores: 16 rows x 16 cache rows for each r and slice
+            float c[2 * NS][4], lo[2 * NS][4];
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int t = 0; t < 2 * NS; t++)
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) c[r][t][e] = lo[r][t][e] = 0.0f;
+                for (int e = 0; e < 4; e++) c[t][e] = lo[t][e] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < HDP / 16; ks++) {
                 // fp32: the leading term of each step starts from zero and joins
                 // the sum in a rounded fp32 add, the small terms run along in `lo`
-                uint32_t kb[4];
-                ldsm4(kb, kt + (ks / 4) * TILE +
-                              sw128(slice + (lane & 7) + (lane >> 4) * 8, (ks % 4) * 2 + ((lane >> 3) & 1)));
+                uint32_t kb[NS][4];
 #pragma unroll
-                for (int r = 0; r < R; r++) {
-                    uint32_t qa[4];
+                for (int n = 0; n < NS; n++)
+                    ldsm4(kb[n], kt + (ks / 4) * TILE +
+                                     sw128(slice + 16 * n + (lane & 7) + (lane >> 4) * 8, (ks % 4) * 2 + ((lane >> 3) & 1)));
+                uint32_t qa[4];
 #pragma unroll
-                    for (int t = NM - 1; t > 0; t--) {
-                        ldsm4(qa, q_at + (uint32_t)((t * (PACKED ? 16 : MT) + 16 * r) * QPITCH + ks * 32));
-                        mma16816<TYPE>(lo[r][0], qa, kb[0], kb[1]);
-                        mma16816<TYPE>(lo[r][1], qa, kb[2], kb[3]);
+                for (int t = NM - 1; t > 0; t--) {
+                    ldsm4(qa, q_at + (uint32_t)(t * (PACKED ? 16 : MT) * QPITCH + ks * 32));
+#pragma unroll
+                    for (int n = 0; n < NS; n++) {
+                        mma16816<TYPE>(lo[2 * n], qa, kb[n][0], kb[n][1]);
+                        mma16816<TYPE>(lo[2 * n + 1], qa, kb[n][2], kb[n][3]);
                     }
-                    ldsm4(qa, q_at + (uint32_t)(16 * r * QPITCH + ks * 32));
+                }
+                ldsm4(qa, q_at + (uint32_t)(ks * 32));
+#pragma unroll
+                for (int n = 0; n < NS; n++) {
                     if constexpr (TYPE == TR_F32) {
                         float d0[4] = {}, d1[4] = {};
-                        mma16816<TYPE>(d0, qa, kb[0], kb[1]);
-                        mma16816<TYPE>(d1, qa, kb[2], kb[3]);
+                        mma16816<TYPE>(d0, qa, kb[n][0], kb[n][1]);
+                        mma16816<TYPE>(d1, qa, kb[n][2], kb[n][3]);
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            c[r][0][e] += d0[e];
-                            c[r][1][e] += d1[e];
+                            c[2 * n][e] += d0[e];
+                            c[2 * n + 1][e] += d1[e];
                         }
                     } else {
-                        mma16816<TYPE>(c[r][0], qa, kb[0], kb[1]);
-                        mma16816<TYPE>(c[r][1], qa, kb[2], kb[3]);
+                        mma16816<TYPE>(c[2 * n], qa, kb[n][0], kb[n][1]);
+                        mma16816<TYPE>(c[2 * n + 1], qa, kb[n][2], kb[n][3]);
                     }
                 }
             }
             if constexpr (TYPE == TR_F32) {
 #pragma unroll
-                for (int r = 0; r < R; r++)
+                for (int t = 0; t < 2 * NS; t++)
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int e = 0; e < 2 * H; e++) {
-                            if constexpr (PACKED) lo[r][t][e] += c[r][t][e + 2];
-                            c[r][t][e] += lo[r][t][e];
-                            if constexpr (PK == 4) c[r][t][e] += __shfl_xor_sync(0xffffffffu, c[r][t][e], 16);
-                        }
+                    for (int e = 0; e < 2 * H; e++) {
+                        if constexpr (PACKED) lo[t][e] += c[t][e + 2];
+                        c[t][e] += lo[t][e];
+                        if constexpr (PK == 4) c[t][e] += __shfl_xor_sync(0xffffffffu, c[t][e], 16);
+                    }
             }
             const int r0 = (w.tile + x) * TR_KT + slice;       // cache row of the warp's first column
-            const bool edge = r0 + 16 > w.clear;               // not every row is seen by every token
+            const bool edge = r0 + 16 * NS > w.clear;          // not every row is seen by every token
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int t = 0; t < 2 * NS; t++)
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int e = 0; e < 2 * H; e++) c[r][t][e] *= g.scale_log2;
+                for (int e = 0; e < 2 * H; e++) c[t][e] *= g.scale_log2;
             if (edge) {
 #pragma unroll
-                for (int r = 0; r < R; r++)
+                for (int t = 0; t < 2 * NS; t++)
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int e = 0; e < 2 * H; e++) {
-                            const int j = tok[r][e >> 1], d = r0 + 8 * t + 2 * ql + (e & 1) - w.q.base;
-                            if (j < 0 || d + w.q.base >= w.visible || (d >= 0 && !tree_sees(g, w.q, j, d)))
-                                c[r][t][e] = -INFINITY;
-                        }
+                    for (int e = 0; e < 2 * H; e++) {
+                        const int j = tok[e >> 1], d = r0 + 8 * t + 2 * ql + (e & 1) - w.q.base;
+                        if (j < 0 || d + w.q.base >= w.visible || (d >= 0 && !tree_sees(g, w.q, j, d)))
+                            c[t][e] = -INFINITY;
+                    }
                 // rows past the end may hold anything: they become zeros, as
                 // do draft values that are not finite
                 uint8_t *vg = ring + (size_t)s * STAGE + CB * TILE;
                 bool found = false;
-                for (int e = lane; e < 16 * CB * 8; e += 32) {
+                for (int e = lane; e < 16 * NS * CB * 8; e += 32) {
                     const int rr = e / (CB * 8), cc = e % (CB * 8);
                     uint4 *p = reinterpret_cast<uint4 *>(vg + (cc >> 3) * TILE + sw128(slice + rr, cc & 7));
                     if (r0 + rr >= w.visible) *p = make_uint4(0, 0, 0, 0);
@@ -342,94 +353,89 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 __syncwarp();
             }
             // running maximum and sum
-            float al[R][H];
+            float al[H];
             bool moved = false;
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int h = 0; h < H; h++) {
+                float v = fmaxf(c[0][2 * h], c[0][2 * h + 1]);
 #pragma unroll
-                for (int h = 0; h < H; h++) {
-                    float v = fmaxf(fmaxf(c[r][0][2 * h], c[r][0][2 * h + 1]), fmaxf(c[r][1][2 * h], c[r][1][2 * h + 1]));
-                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-                    const float mn = fmaxf(m[r][h], v), ms = mn == -INFINITY ? 0.0f : mn;
-                    al[r][h] = ex2(m[r][h] - ms);
-                    moved |= mn != m[r][h];
-                    m[r][h] = mn;
-                    float sum = 0.0f;
+                for (int t = 1; t < 2 * NS; t++) v = fmaxf(v, fmaxf(c[t][2 * h], c[t][2 * h + 1]));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+                const float mn = fmaxf(m[h], v), ms = mn == -INFINITY ? 0.0f : mn;
+                al[h] = ex2(m[h] - ms);
+                moved |= mn != m[h];
+                m[h] = mn;
+                float sum = 0.0f;
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
+                for (int t = 0; t < 2 * NS; t++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float &p = c[r][t][2 * h + e];
-                            p = ex2(p - ms);
-                            sum += p;
-                        }
-                    l[r][h] = fmaf(l[r][h], al[r][h], sum);
-                }
+                    for (int e = 0; e < 2; e++) {
+                        float &p = c[t][2 * h + e];
+                        p = ex2(p - ms);
+                        sum += p;
+                    }
+                l[h] = fmaf(l[h], al[h], sum);
+            }
             if constexpr (TYPE != TR_F32) {
                 if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                    for (int r = 0; r < R; r++)
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[r][t][e] *= al[r][e >> 1];
+                        for (int e = 0; e < 4; e++) o[t][e] *= al[e >> 1];
                 }
             }
             {
-                uint32_t pa[R][4], pb[R][4], pc[R][4];      // fp32: a weight in three bf16 terms
+                uint32_t pa[4 * NS], pb[4 * NS], pc[4 * NS];      // fp32: a weight in three bf16 terms
 #pragma unroll
-                for (int r = 0; r < R; r++)
-#pragma unroll
-                    for (int k = 0; k < 4; k += PACKED ? 2 : 1) {
-                        const float x0 = c[r][k >> 1][2 * (k & 1)], x1 = c[r][k >> 1][2 * (k & 1) + 1];
-                        pa[r][k] = pack2<TYPE>(x0, x1);
-                        if constexpr (TYPE == TR_F32) {
-                            const float y0 = x0 - bf16_to_f((uint16_t)pa[r][k]), y1 = x1 - bf16_to_f((uint16_t)(pa[r][k] >> 16));
-                            pb[r][k] = pack2<TYPE>(y0, y1);
-                            pc[r][k] = pack2<TYPE>(y0 - bf16_to_f((uint16_t)pb[r][k]), y1 - bf16_to_f((uint16_t)(pb[r][k] >> 16)));
-                        }
-                        if constexpr (PK == 4) {            // rows 0..3 | 4..7, 8..11 | 12..15
-                            pa[r][k + 1] = quad < 4 ? pc[r][k] : 0;
-                            pa[r][k] = quad < 4 ? pa[r][k] : pb[r][k];
-                        } else if constexpr (PK == 8) {     // rows 0..7, 8..15 of two products
-                            pa[r][k + 1] = pb[r][k];
-                            pb[r][k] = pc[r][k];
-                            pb[r][k + 1] = 0;
-                        }
+                for (int k = 0; k < 4 * NS; k += PACKED ? 2 : 1) {
+                    const float x0 = c[k >> 1][2 * (k & 1)], x1 = c[k >> 1][2 * (k & 1) + 1];
+                    pa[k] = pack2<TYPE>(x0, x1);
+                    if constexpr (TYPE == TR_F32) {
+                        const float y0 = x0 - bf16_to_f((uint16_t)pa[k]), y1 = x1 - bf16_to_f((uint16_t)(pa[k] >> 16));
+                        pb[k] = pack2<TYPE>(y0, y1);
+                        pc[k] = pack2<TYPE>(y0 - bf16_to_f((uint16_t)pb[k]), y1 - bf16_to_f((uint16_t)(pb[k] >> 16)));
                     }
+                    if constexpr (PK == 4) {            // rows 0..3 | 4..7, 8..11 | 12..15
+                        pa[k + 1] = quad < 4 ? pc[k] : 0;
+                        pa[k] = quad < 4 ? pa[k] : pb[k];
+                    } else if constexpr (PK == 8) {     // rows 0..7, 8..15 of two products
+                        pa[k + 1] = pb[k];
+                        pb[k] = pc[k];
+                        pb[k + 1] = 0;
+                    }
+                }
 #pragma unroll
-                for (int t = 0; t < NT; t += 2) {
-                    uint32_t vb[4];
-                    ldsm4_t(vb, vt + (t >> 3) * TILE +
-                                    sw128(slice + (lane & 7) + ((lane >> 3) & 1) * 8, (t & 7) + (lane >> 4)));
+                for (int t = 0; t < NT; t += 4) {
+                    // fp32: a tile's products start from zero and join the sum in
+                    // one rounded fp32 step: the tensor cores' own long sums lose
+                    // more.  Four sums at a time, so that none waits for its last.
+                    float d[4][4] = {};
 #pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        if constexpr (TYPE == TR_F32) {
-                            // a tile's products start from zero and join the sum in
-                            // one rounded fp32 step: the tensor cores' own long sums
-                            // lose more
-                            float d0[4] = {}, d1[4] = {};
-                            if constexpr (NM > 2) {
-                                mma16816<TYPE>(d0, pc[r], vb[0], vb[1]);
-                                mma16816<TYPE>(d1, pc[r], vb[2], vb[3]);
-                            }
-                            if constexpr (NM > 1) {
-                                mma16816<TYPE>(d0, pb[r], vb[0], vb[1]);
-                                mma16816<TYPE>(d1, pb[r], vb[2], vb[3]);
-                            }
-                            mma16816<TYPE>(d0, pa[r], vb[0], vb[1]);
-                            mma16816<TYPE>(d1, pa[r], vb[2], vb[3]);
+                    for (int n = 0; n < NS; n++) {
+                        uint32_t vb[2][4];
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const float a = al[r][PACKED ? 0 : e >> 1];
-                                o[r][t][e] = fmaf(o[r][t][e], a, d0[e]);
-                                o[r][t + 1][e] = fmaf(o[r][t + 1][e], a, d1[e]);
-                            }
-                        } else {
-                            mma16816<TYPE>(o[r][t], pa[r], vb[0], vb[1]);
-                            mma16816<TYPE>(o[r][t + 1], pa[r], vb[2], vb[3]);
+                        for (int u = 0; u < 2; u++)
+                            ldsm4_t(vb[u], vt + (t >> 3) * TILE + sw128(slice + 16 * n + (lane & 7) + ((lane >> 3) & 1) * 8,
+                                                                        (t & 7) + 2 * u + (lane >> 4)));
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            if constexpr (NM > 2) mma16816<TYPE>(d[u], pc + 4 * n, vb[u >> 1][2 * (u & 1)], vb[u >> 1][2 * (u & 1) + 1]);
                         }
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            if constexpr (NM > 1) mma16816<TYPE>(d[u], pb + 4 * n, vb[u >> 1][2 * (u & 1)], vb[u >> 1][2 * (u & 1) + 1]);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            mma16816<TYPE>(TYPE == TR_F32 ? d[u] : o[t + u], pa + 4 * n, vb[u >> 1][2 * (u & 1)],
+                                           vb[u >> 1][2 * (u & 1) + 1]);
+                    }
+                    if constexpr (TYPE == TR_F32) {
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[t + u][e] = fmaf(o[t + u][e], al[PACKED ? 0 : e >> 1], d[u][e]);
                     }
                 }
             }
@@ -443,122 +449,114 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float &x = o[0][t][e];
-                    x += o[0][t][e + 2];
+                    float &x = o[t][e];
+                    x += o[t][e + 2];
                     if constexpr (PK == 4) x += __shfl_xor_sync(0xffffffffu, x, 16);
                 }
         }
         // ---- merge the row group's warps
 #pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int h = 0; h < H; h++) {
-                float &x = l[r][h];
-                x += __shfl_xor_sync(0xffffffffu, x, 1);
-                x += __shfl_xor_sync(0xffffffffu, x, 2);
-                if (ql == 0) ml[warp * 16 * R + 16 * r + quad + 8 * h] = make_float2(m[r][h], x);
-            }
+        for (int h = 0; h < H; h++) {
+            float &x = l[h];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            if (ql == 0) ml[warp * 16 + quad + 8 * h] = make_float2(m[h], x);
+        }
         consumer_sync(256);
         const bool mend = not_finite != 0;
 #pragma unroll
-        for (int r = 0; r < R; r++)
+        for (int h = 0; h < H; h++) {
+            float2 other[KW];
+            float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int h = 0; h < H; h++) {
-                float2 other[KW];
-                float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KW; k++) {
-                    other[k] = ml[(wm * KW + k) * 16 * R + 16 * r + quad + 8 * h];
-                    top = fmaxf(top, other[k].x);
-                }
-                const float ms = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-                for (int k = 0; k < KW; k++) sum = fmaf(other[k].y, ex2(other[k].x - ms), sum);
-                const float f = ex2(m[r][h] - ms);
-                m[r][h] = top;
-                l[r][h] = sum;
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    o[r][t][2 * h] *= f;
-                    o[r][t][2 * h + 1] *= f;
-                }
+            for (int k = 0; k < KW; k++) {
+                other[k] = ml[(wm * KW + k) * 16 + quad + 8 * h];
+                top = fmaxf(top, other[k].x);
             }
+            const float ms = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-        for (int r = 0; r < R; r++)
+            for (int k = 0; k < KW; k++) sum = fmaf(other[k].y, ex2(other[k].x - ms), sum);
+            const float f = ex2(m[h] - ms);
+            m[h] = top;
+            l[h] = sum;
 #pragma unroll
-            for (int half = KW / 2; half >= 1; half >>= 1) {
-                float *slot = merge + (size_t)((wm * (KW / 2) + kw % half) * 8 * H) * MPITCH;
-                if (kw >= half && kw < 2 * half) {
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int h = 0; h < H; h++)
-                            *reinterpret_cast<float2 *>(slot + (quad + 8 * h) * MPITCH + 8 * t + 2 * ql) =
-                                make_float2(o[r][t][2 * h], o[r][t][2 * h + 1]);
-                }
-                consumer_sync(256);
-                if (kw < half) {
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int h = 0; h < H; h++) {
-                            const float2 v = *reinterpret_cast<const float2 *>(slot + (quad + 8 * h) * MPITCH + 8 * t + 2 * ql);
-                            o[r][t][2 * h] += v.x;
-                            o[r][t][2 * h + 1] += v.y;
-                        }
-                }
-                consumer_sync(256);
+            for (int t = 0; t < NT; t++) {
+                o[t][2 * h] *= f;
+                o[t][2 * h + 1] *= f;
             }
+        }
+#pragma unroll
+        for (int half = KW / 2; half >= 1; half >>= 1) {
+            float *slot = merge + (size_t)((wm * (KW / 2) + kw % half) * 8 * H) * MPITCH;
+            if (kw >= half && kw < 2 * half) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int h = 0; h < H; h++)
+                        *reinterpret_cast<float2 *>(slot + (quad + 8 * h) * MPITCH + 8 * t + 2 * ql) =
+                            make_float2(o[t][2 * h], o[t][2 * h + 1]);
+            }
+            consumer_sync(256);
+            if (kw < half) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
+                        const float2 v = *reinterpret_cast<const float2 *>(slot + (quad + 8 * h) * MPITCH + 8 * t + 2 * ql);
+                        o[t][2 * h] += v.x;
+                        o[t][2 * h + 1] += v.y;
+                    }
+            }
+            consumer_sync(256);
+        }
         if (threadIdx.x == 0) not_finite = 0;          // every warp has read it, and none sets it before the next barrier
         if (kw == 0) {
             float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * MT * (hd + 2);
             const int lo = max(w.clear, w.tile * TR_KT), hi = min(w.visible, (w.tile + n_tiles) * TR_KT);
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int h = 0; h < H; h++) {
+                const int mr = wm * 16 + quad + 8 * h;
+                if (mr >= rows) continue;
+                if (whole) {
+                    const int64_t at = tree_row(g, w.q.t0, w.tok, w.heads, w.head, 0, mr, g.a.ldo);
+                    const float inv = l[h] > 0.0f || l[h] != l[h] ? 1.0f / l[h] : 0.0f;
 #pragma unroll
-                for (int h = 0; h < H; h++) {
-                    const int mr = wm * 16 * R + 16 * r + quad + 8 * h;
-                    if (mr >= rows) continue;
-                    if (whole) {
-                        const int64_t at = tree_row(g, w.q.t0, w.tok, w.heads, w.head, 0, mr, g.a.ldo);
-                        const float inv = l[r][h] > 0.0f || l[r][h] != l[r][h] ? 1.0f / l[r][h] : 0.0f;
-#pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            if (8 * t >= hd) break;
-                            const float y0 = o[r][t][2 * h] * inv, y1 = o[r][t][2 * h + 1] * inv;
-                            const int64_t e = at + 8 * t + 2 * ql;
-                            if constexpr (TYPE == TR_F32) {
-                                float *dst = static_cast<float *>(g.a.out) + e;
-                                if (g.vec) *reinterpret_cast<float2 *>(dst) = make_float2(y0, y1);
-                                else dst[0] = y0, dst[1] = y1;
-                            } else {
-                                uint16_t *dst = static_cast<uint16_t *>(g.a.out) + e;
-                                const uint32_t y = pack2<TYPE>(y0, y1);
-                                if (g.vec) *reinterpret_cast<uint32_t *>(dst) = y;
-                                else dst[0] = (uint16_t)y, dst[1] = (uint16_t)(y >> 16);
-                            }
+                    for (int t = 0; t < NT; t++) {
+                        if (8 * t >= hd) break;
+                        const float y0 = o[t][2 * h] * inv, y1 = o[t][2 * h + 1] * inv;
+                        const int64_t e = at + 8 * t + 2 * ql;
+                        if constexpr (TYPE == TR_F32) {
+                            float *dst = static_cast<float *>(g.a.out) + e;
+                            if (g.vec) *reinterpret_cast<float2 *>(dst) = make_float2(y0, y1);
+                            else dst[0] = y0, dst[1] = y1;
+                        } else {
+                            uint16_t *dst = static_cast<uint16_t *>(g.a.out) + e;
+                            const uint32_t y = pack2<TYPE>(y0, y1);
+                            if (g.vec) *reinterpret_cast<uint32_t *>(dst) = y;
+                            else dst[0] = (uint16_t)y, dst[1] = (uint16_t)(y >> 16);
                         }
-                        __syncwarp(__activemask());
-                        if (mend && ql == 0)
-                            tree_not_finite<TYPE>(&g, w.q.t0, w.q.s, w.q.base, w.g, tok[r][h], lo, hi, 0, hd,
-                                                  static_cast<uint8_t *>(g.a.out) + at * (TYPE == TR_F32 ? 4 : 2), 1,
-                                                  TYPE == TR_F32);
-                    } else {
-                        if (ql == 0) {
-                            part[hd * MT + mr] = m[r][h];
-                            part[(hd + 1) * MT + mr] = l[r][h];
-                        }
-#pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            if (8 * t >= hd) break;
-                            part[(8 * t + 2 * ql) * MT + mr] = o[r][t][2 * h];
-                            part[(8 * t + 2 * ql + 1) * MT + mr] = o[r][t][2 * h + 1];
-                        }
-                        __syncwarp(__activemask());
-                        if (mend && ql == 0)
-                            tree_not_finite<TYPE>(&g, w.q.t0, w.q.s, w.q.base, w.g, tok[r][h], lo, hi, 0, hd, part + mr, MT, 1);
                     }
+                    __syncwarp(__activemask());
+                    if (mend && ql == 0)
+                        tree_not_finite<TYPE>(&g, w.q.t0, w.q.s, w.q.base, w.g, tok[h], lo, hi, 0, hd,
+                                              static_cast<uint8_t *>(g.a.out) + at * (TYPE == TR_F32 ? 4 : 2), 1,
+                                              TYPE == TR_F32);
+                } else {
+                    if (ql == 0) {
+                        part[hd * MT + mr] = m[h];
+                        part[(hd + 1) * MT + mr] = l[h];
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        if (8 * t >= hd) break;
+                        part[(8 * t + 2 * ql) * MT + mr] = o[t][2 * h];
+                        part[(8 * t + 2 * ql + 1) * MT + mr] = o[t][2 * h + 1];
+                    }
+                    __syncwarp(__activemask());
+                    if (mend && ql == 0)
+                        tree_not_finite<TYPE>(&g, w.q.t0, w.q.s, w.q.base, w.g, tok[h], lo, hi, 0, hd, part + mr, MT, 1);
                 }
+            }
         }
         if (threadIdx.x == 0) tree_describe(g, w, line, n_tiles, first_item);
         __syncwarp();
@@ -688,11 +686,11 @@ int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who);
 
 typedef void (*TreeKernel)(CUtensorMap, CUtensorMap, TreeArgs);
 
-template <int TYPE, int HDP, int R, int WM, int PK>
+template <int TYPE, int HDP, int WM, int PK>
 static void tree_fit(TreeArgs &g, size_t &smem) {
-    constexpr int QROWS = PK == 4 ? 16 : PK == 8 ? 32 : 16 * R * WM * (TYPE == TR_F32 ? 3 : 1), H = PK < 16 ? 1 : 2;
+    constexpr int QROWS = PK == 4 ? 16 : PK == 8 ? 32 : 16 * WM * (TYPE == TR_F32 ? 3 : 1), SLOTS = WM * (8 / WM / 2) * (PK < 16 ? 8 : 16);
     constexpr size_t stage = (size_t)2 * TR_KT * HDP * 2;
-    constexpr size_t rest = (size_t)4 * 8 * H * (HDP + 4) * 4 + (size_t)QROWS * (HDP * 2 + 16) + (size_t)8 * 16 * R * 8 + 1024;
+    constexpr size_t rest = tree_scratch(HDP, QROWS, SLOTS) + 8 * 16 * 8 + 1024;
     static_assert(rest + 2 * stage <= TR_SMEM, "two stages must fit");
     g.stages = (int)std::min<size_t>(TR_MAX_STAGES, (TR_SMEM - rest) / stage);
     // two sets of warps take tiles in turn: an even ring gives each its own
@@ -748,12 +746,12 @@ int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g) {
     return VB_OK;
 }
 
-template <int TYPE, int HDP, int R, int WM, int PK = 16>
+template <int TYPE, int HDP, int WM, int PK = 16>
 static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     size_t smem;
-    tree_fit<TYPE, HDP, R, WM, PK>(g, smem);
+    tree_fit<TYPE, HDP, WM, PK>(g, smem);
     const vb_pages &p = g.p;
-    int rc = tree_prepare(ctx, g, PK < 16 ? PK : 16 * R * WM, 1, TR_KT, TR_OVER);
+    int rc = tree_prepare(ctx, g, PK < 16 ? PK : 16 * WM, 1, TR_KT, TR_OVER);
     if (rc) return rc;
     CUtensorMap tk, tv;
     const int64_t rows = (int64_t)p.n_pages * p.n_kv_heads * p.page_rows, layer = (int64_t)g.a.layer * rows * p.head_dim * 2;
@@ -762,7 +760,7 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     if (!make_map(&tk, static_cast<char *>(p.k) + layer, dt, 2, p.head_dim, rows, 64, box, true) ||
         !make_map(&tv, static_cast<char *>(p.v) + layer, dt, 2, p.head_dim, rows, 64, box, true))
         return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the cache refused");
-    VB_CHECK(ctx, pdl_launch(ctx, tree_attention_kernel<TYPE, HDP, R, WM, PK>, dim3(ctx->sm_count), dim3(TR_THREADS), smem, tk,
+    VB_CHECK(ctx, pdl_launch(ctx, tree_attention_kernel<TYPE, HDP, WM, PK>, dim3(ctx->sm_count), dim3(TR_THREADS), smem, tk,
                              tv, g));
     VB_LAUNCH_CHECK(ctx, "tree_attention");
     return launch_tree_combine(ctx, g);
@@ -775,20 +773,32 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
 // delays the first result; heads above 128 values, whose sums and scores do
 // not fit its tensor memory; and fp32 queries, whose sums the tcgen05
 // accumulators hold less exactly.
+//
+// There more rows per block mean fewer readings of a tile and more work for
+// each; the warps then split rows rather than a tile, and each keeps its
+// operands for more products.  Measured at one sequence of 32,768 rows with
+// 2 heads (microseconds with blocks of 32 | 64 | 128 rows; "prompt": 4096
+// tokens over themselves):
+//   fp32, 128 values: 32 rows 29 | 33 | 49, 64 rows 38 | 35 | 50,
+//                     128 rows 60 | 52 | 56, 384 rows 144 | 123 | 123, prompt 943 | 681 | 614
+//   bf16, 256 values: 32 rows 41 | 45 | 56, 64 rows 51 | 53 | 62,
+//                     128 rows 71 | 69 | 78, 384 rows 141 | 121 | 135, prompt 1490 | 1084 | 915
+// fp32 heads of 256 values leave room for blocks of 32 and two stages only.
 template <int TYPE, int HDP>
 static int launch_rows(vb_ctx *ctx, TreeArgs &g) {
     const int64_t rows = (int64_t)g.a.max_tokens * g.group;
     if constexpr (TYPE == TR_F32) {
-        if (rows <= 4) return launch_tree<TYPE, HDP, 1, 1, 4>(ctx, g);
-        if (rows <= 8) return launch_tree<TYPE, HDP, 1, 1, 8>(ctx, g);
+        if (rows <= 4) return launch_tree<TYPE, HDP, 1, 4>(ctx, g);
+        if (rows <= 8) return launch_tree<TYPE, HDP, 1, 8>(ctx, g);
     }
-    if (rows <= 16) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);
+    if (rows <= 16) return launch_tree<TYPE, HDP, 1>(ctx, g);
     if constexpr (TYPE == TR_F32) {
-        if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 1, 1>(ctx, g);      // more rows leave no room for two stages
-        else if (rows <= 32) return launch_tree<TYPE, HDP, 2, 1>(ctx, g);
-        else return launch_tree<TYPE, HDP, 2, 2>(ctx, g);
+        if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 2>(ctx, g);      // more rows leave no room for two stages
+        else if (rows <= 32) return launch_tree<TYPE, HDP, 2>(ctx, g);
+        else if (rows <= 128) return launch_tree<TYPE, HDP, 4>(ctx, g);
+        else return launch_tree<TYPE, HDP, 8>(ctx, g);
     } else {
-        if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 1, 2>(ctx, g);      // more would not fit the registers
+        if constexpr (HDP == 256) return rows <= 64 ? launch_tree<TYPE, HDP, 2>(ctx, g) : rows <= 512 ? launch_tree<TYPE, HDP, 4>(ctx, g) : launch_tree<TYPE, HDP, 8>(ctx, g);
         else return launch_tree_tc(ctx, g);
     }
 }
@@ -799,33 +809,40 @@ static int launch_heads(vb_ctx *ctx, TreeArgs &g) {
     return hd <= 64 ? launch_rows<TYPE, 64>(ctx, g) : hd <= 128 ? launch_rows<TYPE, 128>(ctx, g) : launch_rows<TYPE, 256>(ctx, g);
 }
 
-template <int TYPE, int HDP, int R, int WM, int PK = 16>
+template <int TYPE, int HDP, int WM, int PK = 16>
 static cudaError_t allow_smem() {
-    return cudaFuncSetAttribute(tree_attention_kernel<TYPE, HDP, R, WM, PK>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
+    return cudaFuncSetAttribute(tree_attention_kernel<TYPE, HDP, WM, PK>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
 }
 
 int init_tree(vb_ctx *ctx) {
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 1, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 2, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 2, 2>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 1, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 2, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 2, 2>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 1, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 64, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 128, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1, 2>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 64, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 128, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 8>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 8>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 8>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 8>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 8>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 64, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 128, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 8>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 64, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 128, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 4>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 8>()));
     return init_tree_tc(ctx);
 }
 
