@@ -78,25 +78,28 @@ __host__ __device__ constexpr int tree_scratch(int hdp, int q_rows, int merge_ro
 // TYPE: the types; HDP: head_dim rounded up to 64, 128 or 256; WM: groups of
 // warps with 16 rows each.  8 / WM warps share a group's rows, split a tile's
 // rows and merge at the item's end (with WM = 1 two sets of four warps take
-// tiles in turn).  PK: with 4 or 8 rows a block the 16-bit terms of an fp32
-// value lie under one another in the 16 rows of an instruction (row
-// t * PK + m: term t of row m), which then takes one product or two in place
-// of three; a row's scores and sums are added over its terms.  (64 sequences
-// of 8192 rows under one token of 16 heads over 2: 125 us with three
-// products, 111 us with two, of 82 us that reading the cache takes.)
+// tiles in turn).  PK: rows of a block of 4 or 8.  A thread then keeps one row
+// in place of two (the other eight of an instruction's 16 count for nothing):
+// half the exponentials, merges and parts (bf16, 8 sequences of 4000 rows under
+// one token 20.4 -> 18.7 us).  The 16-bit terms of an fp32 value lie under one
+// another in the 16 rows (row t * PK + m: term t of row m), which takes one
+// product or two in place of three; a row's scores and sums are added over
+// its terms.  (64 sequences of 8192 rows under one token of 16 heads over 2:
+// 125 us with three products, 111 us with two, of 82 us that reading the
+// cache takes.)
 template <int TYPE, int HDP, int WM, int PK>
 __global__ void __launch_bounds__(TR_THREADS, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                           const __grid_constant__ TreeArgs g) {
     constexpr bool PACKED = PK < 16;
-    static_assert(!PACKED || (TYPE == TR_F32 && WM == 1), "terms are packed for fp32 alone");
+    static_assert(!PACKED || (WM == 1 && (PK == 8 || TYPE == TR_F32)), "only terms need four");
     constexpr int MT = PACKED ? PK : 16 * WM;    // rows of a block
     constexpr int H = PACKED ? 1 : 2;                // rows that a thread keeps of 16
     constexpr int KW = 8 / WM;                       // warps of a row group
     constexpr int SETS = WM == 1 ? 2 : 1;
     constexpr int NS = WM == 1 ? 1 : 4 / KW;         // 16-row slices of a tile per warp
     constexpr int QT = TYPE == TR_F32 ? 3 : 1;       // 16-bit terms of a query value: 3 bf16 hold an fp32 exactly
-    constexpr int NM = PK == 4 ? 1 : PK == 8 ? 2 : QT;                  // products that hold them
+    constexpr int NM = PK == 4 ? 1 : PK == 8 ? (QT + 1) / 2 : QT;                  // products that hold them
     constexpr int QROWS = PACKED ? 16 * NM : QT * MT;
     constexpr int CB = HDP / 64;                     // 128-byte column blocks
     constexpr int NT = HDP / 8;                      // output tiles of 8 columns
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[t][e] *= al[e >> 1];
+                        for (int e = 0; e < 4; e++) o[t][e] *= al[PACKED ? 0 : e >> 1];
                 }
             }
             {
@@ -399,6 +402,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     if constexpr (PK == 4) {            // rows 0..3 | 4..7, 8..11 | 12..15
                         pa[k + 1] = quad < 4 ? pc[k] : 0;
                         pa[k] = quad < 4 ? pa[k] : pb[k];
+                    } else if constexpr (PK == 8 && TYPE != TR_F32) {
+                        pa[k + 1] = 0;
                     } else if constexpr (PK == 8) {     // rows 0..7, 8..15 of two products
                         pa[k + 1] = pb[k];
                         pb[k] = pc[k];
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             if (lane == 0) mbar_arrive(&empty[s]);
         }
 
-        if constexpr (PACKED) {
+        if constexpr (PACKED && TYPE == TR_F32) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -688,7 +693,7 @@ typedef void (*TreeKernel)(CUtensorMap, CUtensorMap, TreeArgs);
 
 template <int TYPE, int HDP, int WM, int PK>
 static void tree_fit(TreeArgs &g, size_t &smem) {
-    constexpr int QROWS = PK == 4 ? 16 : PK == 8 ? 32 : 16 * WM * (TYPE == TR_F32 ? 3 : 1), SLOTS = WM * (8 / WM / 2) * (PK < 16 ? 8 : 16);
+    constexpr int QROWS = PK == 4 ? 16 : PK == 8 ? (TYPE == TR_F32 ? 32 : 16) : 16 * WM * (TYPE == TR_F32 ? 3 : 1), SLOTS = WM * (8 / WM / 2) * (PK < 16 ? 8 : 16);
     constexpr size_t stage = (size_t)2 * TR_KT * HDP * 2;
     constexpr size_t rest = tree_scratch(HDP, QROWS, SLOTS) + 8 * 16 * 8 + 1024;
     static_assert(rest + 2 * stage <= TR_SMEM, "two stages must fit");
@@ -789,8 +794,8 @@ static int launch_rows(vb_ctx *ctx, TreeArgs &g) {
     const int64_t rows = (int64_t)g.a.max_tokens * g.group;
     if constexpr (TYPE == TR_F32) {
         if (rows <= 4) return launch_tree<TYPE, HDP, 1, 4>(ctx, g);
-        if (rows <= 8) return launch_tree<TYPE, HDP, 1, 8>(ctx, g);
     }
+    if (rows <= 8) return launch_tree<TYPE, HDP, 1, 8>(ctx, g);
     if (rows <= 16) return launch_tree<TYPE, HDP, 1>(ctx, g);
     if constexpr (TYPE == TR_F32) {
         if constexpr (HDP == 256) return launch_tree<TYPE, HDP, 2>(ctx, g);      // more rows leave no room for two stages
@@ -831,14 +836,20 @@ int init_tree(vb_ctx *ctx) {
     VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_F32, 256, 2>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 64, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_BF16, 64, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 128, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_BF16, 128, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 2>()));
     VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 4>()));
     VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 8>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 64, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_F16, 64, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 128, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_F16, 128, 1>()));
+    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1, 8>()));
     VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1>()));
     VB_CHECK(ctx, (allow_smem<TR_F16, 256, 2>()));
     VB_CHECK(ctx, (allow_smem<TR_F16, 256, 4>()));
