@@ -543,6 +543,17 @@ def test_tree_blocks_of_more_rows(ctx, type, hd, drafted, nh, nkv):
     check_tree(ctx, tree_case(ctx, type, [drafted + 5, 1500, drafted], [drafted, drafted, drafted], nh, nkv, hd, 16, "any", seed=12))
 
 
+@pytest.mark.parametrize("type,hd", [("bf16", 128), ("f16", 96), ("bf16", 64)])
+@pytest.mark.parametrize("mask", ["any", "chain"])
+@pytest.mark.parametrize("lens,drafted", [
+    ([700, 40, 129, 1025, 2000, 385], [48, 16, 17, 33, 15, 1]), ([9000], [48]),
+    ([33 + 3 * i for i in range(60)], [(7 * i) % 33 for i in range(60)]), ([260, 300], [129, 40])])
+def test_tree_blocks_of_one_and_two_row_tiles(ctx, type, hd, mask, lens, drafted):
+    """Full blocks, blocks of one row tile and both of them after one another in a CTA; queries by TMA and by threads."""
+    check_tree(ctx, tree_case(ctx, type, lens, drafted, 16, 2, hd, 16, mask, seed=13))
+    check_tree(ctx, tree_case(ctx, type, lens, drafted, 16, 2, hd, 16, mask, seed=14, pad=3))
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("lens,drafted,P", [([30000], [2], 64), ([9000, 20000], [1, 1], 16), ([25000, 100], [40, 3], 32)])
 def test_tree_many_tiles_for_each_cta(ctx, type, lens, drafted, P):

@@ -17,8 +17,8 @@
 // by 2^8 (the weights stay far inside the 16-bit formats), so O is rarely
 // rescaled in tensor memory.
 //
-// Warps 0..7 softmax (warpgroup = stream), 8 loads (TMA, one box per page),
-// 9 issues the MMAs, 10 and 11 complete the warpgroup.
+// Warps 0..7 softmax (warpgroup = stream), 9 issues the MMAs, 8, 10 and 11
+// issue the copies (TMA, one box per page and column block).
 #include "vb_kernels.cuh"
 #include "vb_tree.cuh"
 
