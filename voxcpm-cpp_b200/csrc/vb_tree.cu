@@ -35,8 +35,10 @@ namespace vb {
 
 constexpr int TR_KT = 64;            // cache rows per tile
 constexpr int TR_MAX_STAGES = 8;
-constexpr int TR_OVER = 2;           // an item's start and end cost about as much as two of its tiles
-constexpr int TR_THREADS = 384;      // warps 0..7 compute, warp 8 loads
+// What an item's start and end cost, in tiles: with 2 | 4 | 6 the prompt of
+// 4096 fp32 tokens takes 614 | 590 | 611 us, 64 decode steps 104 | 104 | 105.
+constexpr int TR_OVER = 4;
+constexpr int TR_THREADS = 384;      // warps 0..7 compute, 8..11 load
 // Registers: the launch gives 168 a thread; the loading warpgroup goes down
 // to 56 and the two computing ones up to 224 (2 * 224 + 56 = 3 * 168), which
 // their sums need.
@@ -570,9 +572,22 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     }
 }
 
-// Joins the parts of items that several CTAs shared.  A task is 32 rows by
-// 16 columns of an item; a lane holds a row of it and adds up parts, several
-// of them on their way at once.
+// Joins the parts of items that several CTAs shared:
+//   o = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), m the largest m_c.
+// A task is 32 rows by 16 columns of an item; a lane holds a row of it and adds
+// up parts, several of them on their way at once.  The parts come out of L2:
+// bound by the launch and two or three trips there.
+//
+// Three forms, by the call's items (at most 148 CTAs, so few items have many
+// parts); microseconds of a whole call with 16 warps a task | 4 | 1:
+//   2 items (one token of 16 heads over 2, 4,000 rows)        14.8 | 22 | 54
+//   16 items (8 sequences of up to 25 tokens, 2000 rows)      33.2 | 23.8 | 30.9
+//   32 items (16 sequences of one token, 3000 rows)           24.6 | 22.3 | 24.7
+//   128 items (64 sequences of one token, 8192 rows)         118.7 | 103.7 | 103.8
+//   256 items (one prompt of 4096)                             -   | 138 | 98
+// (Joining in the attention kernel, by the last CTA to leave a part, saves the
+// launch but costs a fence, a ticket and one SM's reading: from 0.4 us less to
+// 15 us more.)
 constexpr int TC_COLS = 16;
 
 struct TreeTask {
@@ -721,7 +736,7 @@ int tree_prepare(vb_ctx *ctx, TreeArgs &g, int tile_rows, int tiles, int kt, int
     const int64_t most = ((int64_t)g.p.max_pages * g.p.page_rows + kt - 1) / kt + over;
     if ((double)items * (double)most >= 2147483647.0)
         return set_error(ctx, VB_ERR_INVALID_ARG, "vb_tree_attention: too many rows for one call");
-    g.by_item = items * 4 <= ctx->sm_count;      // four parts each, or more
+    g.by_item = items * 4 <= ctx->sm_count;      // four parts each, or more: the join's warps share them
     g.item_blocks = (int)blocks;
     const size_t parts = (size_t)2 * ctx->sm_count * g.mt * (g.p.head_dim + 2) * sizeof(float);
     int rc = arena_reserve(ctx, ctx->tree_ws, parts + (size_t)ctx->sm_count * sizeof(TreeShare));
@@ -786,7 +801,7 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
 // 2 heads (microseconds with blocks of 32 | 64 | 128 rows; "prompt": 4096
 // tokens over themselves):
 //   fp32, 128 values: 32 rows 29 | 33 | 49, 64 rows 38 | 35 | 50,
-//                     128 rows 60 | 52 | 56, 384 rows 144 | 123 | 123, prompt 943 | 681 | 614
+//                     128 rows 60 | 52 | 56, 384 rows 144 | 123 | 123, prompt 943 | 681 | 614 (590 with TR_OVER 4)
 //   bf16, 256 values: 32 rows 41 | 45 | 56, 64 rows 51 | 53 | 62,
 //                     128 rows 71 | 69 | 78, 384 rows 141 | 121 | 135, prompt 1490 | 1084 | 915
 // fp32 heads of 256 values leave room for blocks of 32 and two stages only.
