@@ -23,6 +23,7 @@
 #include "vb_tree.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vb {
 
@@ -542,30 +543,49 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     }
                     // One pass over the row in pieces of 32, the next on its way from
                     // tensor memory: the weights against the running maximum as it
-                    // stands, and the row's own maximum beside them.  They count if
-                    // that maximum is no further than 2^TT_SLACK above and there was
-                    // no NaN; else two passes, the maximum first.  (The weights wait
-                    // in registers: in tensor memory they would take the scores' place.)
+                    // stands (in an item's first tile that of the first piece), and the
+                    // row's own maximum beside them.  They count if that maximum is no
+                    // further than 2^TT_SLACK above and there was no NaN; else two
+                    // passes, the maximum first.  (The weights wait in registers: in
+                    // tensor memory they would take the scores' place.)
                     uint32_t a[32], b[32];
-                    bool done = !edge && x > 0;
-                    if (done) {
+                    bool done = false;
+                    auto one_pass = [&](auto is_masked) {
+                        constexpr bool masked = decltype(is_masked)::value;
+                        auto drop = [&](uint32_t (&v)[32], uint32_t out) {
+                            if constexpr (masked)
+#pragma unroll
+                                for (int c = 0; c < 32; c++)
+                                    if (out >> c & 1u) v[c] = 0xff800000u;
+                        };
+                        tmem_ld32_start(sc, a);
+                        tmem_ld32_wait(a);
+                        drop(a, gone[0]);
+                        if (x == 0) {                                    // no maximum yet: that of the first piece
+                            float u = -INFINITY, v = -INFINITY;
+#pragma unroll
+                            for (int c = 0; c < 16; c++) {
+                                float &z = c & 1 ? v : u;
+                                z = max3_nan(z, __uint_as_float(a[2 * c]), __uint_as_float(a[2 * c + 1]));
+                            }
+                            m = max3_nan(u, v, v) * g.scale_log2;
+                        }
                         const uint64_t off2 = pack_f32x2(-m, -m), scale2 = pack_f32x2(g.scale_log2, g.scale_log2);
                         uint32_t y[2][32];
                         uint64_t sum2 = 0;
                         float t0 = -INFINITY, t1 = -INFINITY;
-                        tmem_ld32_start(sc, a);
-                        tmem_ld32_wait(a);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             uint32_t (&now)[32] = k & 1 ? b : a;
                             if (k < 3) tmem_ld32_start(sc + 32 * (k + 1), k & 1 ? a : b);
+                            if (k > 0) drop(now, gone[k]);
 #pragma unroll
                             for (int c = 0; c < 16; c++) {
                                 float &z = c & 1 ? t1 : t0;
                                 z = max3_nan(z, __uint_as_float(now[2 * c]), __uint_as_float(now[2 * c + 1]));
                                 const uint64_t v = fma_f32x2(pack_b32x2(now[2 * c], now[2 * c + 1]), scale2, off2);
                                 float p0, p1;
-                                if (c % 16 < TT_POLY) exp2_pair(v, p0, p1);
+                                if (!masked && c % 16 < TT_POLY) exp2_pair(v, p0, p1);    // (which makes no 0 of -inf)
                                 else {
                                     unpack_f32x2(v, p0, p1);
                                     p0 = ex2(p0);
@@ -577,7 +597,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                             if (k < 3) tmem_ld32_wait(k & 1 ? a : b);
                         }
                         const float top = max3_nan(t0, t1, t1) * g.scale_log2;
-                        done = !__any_sync(0xffffffffu, !(top <= m + TT_SLACK) || m == -INFINITY);
+                        done = !__any_sync(0xffffffffu, j >= 0 && (!(top <= m + TT_SLACK) || m == -INFINITY));
                         if (done) {
                             tmem_st32(sc, y[0]);
                             tmem_st32(sc + 32, y[1]);
@@ -586,7 +606,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                             l += s0 + s1;
                             tmem_st_wait();
                         }
-                    }
+                    };
+                    if (edge) one_pass(std::true_type());
+                    else one_pass(std::false_type());
                     if (!done) {
                     float top = -INFINITY;
                     auto piece_max = [&](uint32_t (&x)[32], uint32_t out) {
