@@ -30,13 +30,14 @@ namespace vb {
 constexpr int TT_KT = 128;
 constexpr int TT_THREADS = 384;
 constexpr int TT_SLOTS = 12;
-// What an item's start and end (its first and last tiles take two passes) cost,
-// in tiles: with 0 | 2 | 4 | 6 the prompt of 4096 tokens takes 159 | 98 | 92 |
-// 95 us, 8 sequences of up to 25 drafted tokens 23 | 24 | 24 | 22.
-constexpr int TT_OVER = 4;
+// What an item's start and end cost, in tiles.  A prompt of 4096 tokens takes
+// with 3 | 4 89 | 89 us, four of them 282 | 287, 64 ragged drafts over 4000 rows
+// 60 | 62; while an item's first and last tiles still took two passes, that
+// prompt took 159 | 98 | 92 | 95 with 0 | 2 | 4 | 6.
+constexpr int TT_OVER = 3;
 constexpr int TT_SMEM = 225 * 1024;
 // Of 16 pairs of weights, those that the multiply-add pipe takes: 0 | 5 | 10
-// take 111 | 98 | 112 us of that prompt.
+// made that prompt 111 | 98 | 112 us (then with 2 tiles for an item's ends).
 constexpr int TT_POLY = 5;
 constexpr float TT_SLACK = 8.0f;     // log2 of how far a score may exceed the running maximum
 
