@@ -667,6 +667,47 @@ def test_tree_gives_the_same_bits_again(ctx, type, lens, drafted):
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
 
 
+@pytest.mark.parametrize("type,drafted", [("f32", 2), ("bf16", 1), ("bf16", 9), ("f16", 40)])
+def test_steps_replayed_from_a_graph(ctx, type, drafted):
+    """extend, attention and keep captured once: each replay finds the lengths of the one before, with the bits of direct calls."""
+    dtype = TYPES[type]
+    own = torch.cuda.Stream()
+    both = [new_cache(ctx, pages=60, P=16, hd=128, most=30, dtype=torch.bfloat16 if type == "f32" else dtype, seed=5) for _ in range(2)]
+    n = 2
+    seqs, rows, kept = ints([3, 1]), ints([drafted] * n), ints([1, min(drafted, 2)])
+    path, start = ints([[drafted - 1, 0], [0, drafted - 1]]), ints([0, drafted, 2 * drafted])
+    mask = ints(M.pack_mask(np.tile(M.tree_mask([j - 1 - (j > 2) for j in range(drafted)]), (n, 1)), -(-drafted // 32)))
+    q = torch.randn(n * drafted, 16 * 128, device="cuda").to(dtype)
+    got = [torch.zeros_like(q) for _ in both]
+    args = [vb.TreeArgs(q, c, 1, seqs, start, o, heads=16, max_tokens=drafted, mask=mask) for c, o in zip(both, got)]
+
+    def step(i):
+        ctx.pages_extend(both[i], seqs, rows)
+        ctx.tree_attention(args[i])
+        ctx.pages_keep(both[i], seqs, rows, kept, path)
+
+    for c in both:
+        ctx.pages_init(c)
+        ctx.pages_extend(c, seqs, ints([100, 37]))
+    torch.cuda.synchronize()
+    ctx.set_stream(own.cuda_stream)
+    step(0)
+    step(1)
+    ctx.sync()
+    ctx.graph_begin()
+    step(1)
+    g = ctx.graph_end()
+    for _ in range(4):
+        step(0)
+        ctx.graph_launch(g)
+        ctx.sync()
+        assert torch.equal(got[0], got[1]) and torch.equal(both[0].length, both[1].length) and bool(got[1].any())
+    ctx.graph_destroy(g)
+    ctx.set_stream(1)
+    assert both[0].length.tolist() == [0, 37 + 5 * min(drafted, 2), 0, 105, 0, 0]
+    assert ctx.device_status() == (0, 0) and all(ctx.pages_status(c)[0] == 0 for c in both)
+
+
 def test_tree_past_32_bit_offsets(ctx):
     """A layer whose rows lie past 2^31 elements of the pool."""
     nkv, P, hd, pages = 2, 64, 128, 70000
