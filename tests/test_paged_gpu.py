@@ -6,7 +6,7 @@ Tolerances.  Page calls move bits: equal.  Head norms and rotation: fp32
 arithmetic on a few values, 2^-20 relative to the row's largest value, plus
 half a unit of the output's type (2^-12 fp16, 2^-9 bf16).  Attention: with
 S = scale * max sum|q_i k_i|, a score is off by at most 2^-16 S (operands of
-the fp32 form are held in two bf16 terms, 2^-17 each; fp32 sums add less), a
+the fp32 form are held to 2^-17 or better; fp32 sums add less), a
 weight by twice that relatively; weights of the 16-bit forms are rounded to
 the cache's type (2^-8 bf16, 2^-11 fp16 bounds both the rounding and the
 output's), those of the fp32 form held to 2^-16: absolute error below
