@@ -792,3 +792,54 @@ def test_tree_empty_calls(ctx):
     t["args"].c.n = 0
     ctx.tree_attention(t["args"])
     assert ctx.device_status() == (0, 0)
+
+
+def test_captured_steps_outlive_larger_calls():
+    """Calls that need larger workspaces come between a step's capture and its replays."""
+    ctx, own = vb.Context(0), torch.cuda.Stream()                 # (a new context: its workspaces are still small)
+    ctx.set_stream(own.cuda_stream)
+    g0 = torch.Generator(device="cuda").manual_seed(3)
+    both = [new_cache(ctx, pages=60, P=16, hd=128, most=30, seed=5) for _ in range(2)]
+    seqs, one, path = ints([3, 1]), ints([1, 1]), ints([[0], [0]])
+    q = torch.randn(2, 16 * 128, generator=g0, device="cuda")
+    att, y = ([torch.zeros(n, 2048, device="cuda") for _ in both] for n in (2, 16))
+    args = [vb.TreeArgs(q, c, 1, seqs, ints([0, 1, 2]), o, heads=16, max_tokens=1) for c, o in zip(both, att)]
+    w = ctx.weight(vb.TYPE_F16, 2048, 2048, np.random.default_rng(0).standard_normal((2048, 2048)).astype(np.float16))
+    x = torch.randn(64, 2048, generator=g0, device="cuda")
+    prompt = tree_case(ctx, "bf16", [700], [700], 16, 2, 128, 16, "chain")
+    wide, to = (new_cache(ctx, 1, 200000, 1, 16, 8, 2, 8) for _ in range(2))
+    torch.cuda.synchronize()
+
+    def step(i):
+        ctx.pages_extend(both[i], seqs, one)
+        ctx.tree_attention(args[i])
+        ctx.pages_keep(both[i], seqs, one, one, path)
+        ctx.matmul(w, x, 16, y[i])
+
+    for c in both:
+        ctx.pages_init(c)
+        ctx.pages_extend(c, seqs, ints([100, 300]))
+    step(0)
+    step(1)
+    ctx.sync()
+    ctx.graph_begin()
+    step(1)
+    g = ctx.graph_end()
+    ctx.tree_attention(prompt["args"])
+    ctx.pages_compact(wide, to)
+    ctx.matmul(w, x, 64, torch.zeros(64, 2048, device="cuda"))
+    ctx.sync()
+    others = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(32)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        step(0)
+        ctx.graph_launch(g)
+        ctx.sync()
+        assert torch.equal(att[0], att[1]) and torch.equal(y[0], y[1]) and bool(att[1].any()) and bool(y[1].any())
+    assert all(bool(o.isnan().all()) for o in others)
+    ref, tol = tree_ref(prompt)
+    assert np.all(np.abs(prompt["out"].float().cpu().numpy() - ref) <= tol)
+    assert ctx.device_status() == (0, 0) and all(ctx.pages_status(c)[0] == 0 for c in both)
+    ctx.graph_destroy(g)
+    w.release()
+    ctx.close()

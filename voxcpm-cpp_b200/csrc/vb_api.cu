@@ -3,6 +3,7 @@
 #include "vb_common.cuh"
 #include "vb_kernels.cuh"
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -45,16 +46,26 @@ int arena_reserve(vb_ctx *ctx, Arena &ws, size_t bytes) {
     cudaStreamIsCapturing(ctx->stream, &cs);
     if (cs != cudaStreamCaptureStatusNone)
         return set_error(ctx, VB_ERR_BACKEND, "workspace must grow to %zu bytes during stream capture", bytes);
-    size_t want = bytes + bytes / 4 + (1u << 20);
-    if (ws.ptr) {
-        VB_CHECK(ctx, cudaStreamSynchronize(ctx->stream));
-        VB_CHECK(ctx, cudaFree(ws.ptr));
-        ws.ptr = nullptr;
-        ws.bytes = 0;
+    // twice the old block at least: all outgrown blocks together are no larger
+    // than the present one
+    const size_t want = std::max(bytes + bytes / 4 + (1u << 20), 2 * ws.bytes);
+    try {
+        ws.outgrown.reserve(ws.outgrown.size() + 1);
+    } catch (...) {
+        return set_error(ctx, VB_ERR_OOM, "workspace: out of host memory");
     }
-    VB_CHECK(ctx, cudaMalloc(&ws.ptr, want));
+    void *block = nullptr;
+    VB_CHECK(ctx, cudaMalloc(&block, want));
+    if (ws.ptr) ws.outgrown.push_back(ws.ptr);
+    ws.ptr = block;
     ws.bytes = want;
     return VB_OK;
+}
+
+void arena_free(Arena &ws) {
+    for (void *p : ws.outgrown) cudaFree(p);
+    cudaFree(ws.ptr);
+    ws = Arena();
 }
 
 // cos/sin table of ggml's NEOX rope_ext (freq_scale 1, ext_factor 0,
@@ -192,10 +203,7 @@ extern "C" void vb_destroy(vb_ctx *ctx) {
     cudaSetDevice(ctx->device);
     cudaStreamSynchronize(ctx->stream);
     for (auto &r : ctx->ropes) cudaFree(r.d_cs);
-    if (ctx->ws.ptr) cudaFree(ctx->ws.ptr);
-    if (ctx->attn_ws.ptr) cudaFree(ctx->attn_ws.ptr);
-    if (ctx->pages_ws.ptr) cudaFree(ctx->pages_ws.ptr);
-    if (ctx->tree_ws.ptr) cudaFree(ctx->tree_ws.ptr);
+    for (Arena *a : {&ctx->ws, &ctx->attn_ws, &ctx->pages_ws, &ctx->tree_ws}) arena_free(*a);
     if (ctx->op_error) cudaFree(ctx->op_error);
     gemm_free(ctx);
     if (ctx->own_stream_handle) cudaStreamDestroy(ctx->own_stream_handle);

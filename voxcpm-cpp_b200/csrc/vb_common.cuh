@@ -36,9 +36,12 @@ bool fault_injected(const char *what);
 // --------------------------------------------------------------- workspace
 // A growable device arena owned by the context.  Grows only outside of
 // stream capture; kernels address scratch through it.
+// Device scratch that grows.  A block that a call outgrew stays until the
+// arena goes: a captured graph may hold its address.
 struct Arena {
     void *ptr = nullptr;
     size_t bytes = 0;
+    std::vector<void *> outgrown;
 };
 
 struct RopeTable {
@@ -98,6 +101,7 @@ int set_error(vb_ctx *ctx, int code, const char *fmt, ...);
 int check_cuda(vb_ctx *ctx, cudaError_t e, const char *what);
 int check_launch(vb_ctx *ctx, const char *what);
 int arena_reserve(vb_ctx *ctx, Arena &a, size_t bytes);
+void arena_free(Arena &a);
 inline int ws_reserve(vb_ctx *ctx, size_t bytes) { return arena_reserve(ctx, ctx->ws, bytes); }
 const RopeTable *rope_table(vb_ctx *ctx, int head_dim, float theta, int use_factors, int need_pos);
 // The (cos, sin) table of positions 0..max_pos-1 on the host.

@@ -1187,8 +1187,8 @@ static GemmState *gemm_state(vb_ctx *ctx) {
 void gemm_free(vb_ctx *ctx) {
     GemmState *g = static_cast<GemmState *>(ctx->gemm);
     if (!g) return;
-    cudaFree(g->act.ptr);
-    cudaFree(g->part.ptr);
+    arena_free(g->act);
+    arena_free(g->part);
     cudaFree(g->cnt);
     cudaFree(g->err);
     delete g;

@@ -136,7 +136,7 @@ extern "C" void vb_gen_destroy(vb_ctx *ctx, vb_gen g) {
     weight_free(ctx, g->stop_w);
     weight_free(ctx, g->stop_hw);
     cudaFree(g->mem);
-    cudaFree(g->prompt.ptr);
+    vb::arena_free(g->prompt);
     cudaFreeHost(g->noise_host);
     cudaFreeHost(g->map_host);
     delete g;

@@ -845,7 +845,7 @@ static void dit_free(vb_ctx *ctx, vb_dit *d) {
     cudaFree(d->ones);
     cudaFree(d->cfg_hm);
     cudaFree(d->user_hm);
-    cudaFree(d->vel.ptr);
+    vb::arena_free(d->vel);
     lm_free(ctx, d->blocks);
     delete d;
 }
