@@ -843,3 +843,23 @@ def test_captured_steps_outlive_larger_calls():
     ctx.graph_destroy(g)
     w.release()
     ctx.close()
+
+
+@pytest.mark.parametrize("call", ["fork", "truncate"])
+def test_an_error_in_a_call_of_many_requests_changes_nothing(ctx, call):
+    """CTAs of a later wave start while the first record the error."""
+    n, most, half = 12000, 1024, 6000
+    c = new_cache(ctx, 1, 16, 1, 16, 8, n, most)
+    row = torch.arange(n, device="cuda", dtype=torch.int32) % 8
+    c.table[:, :3] = row[:, None]
+    c.length.fill_(40)
+    c.refs[:8] = 3 * n // 8
+    before = [x.clone() for x in (c.table, c.length, c.refs, c.k, c.v)]
+    seqs = np.arange(half)
+    for at in (half - 1, 0, half // 2):
+        a = seqs + half if call == "fork" else seqs.copy()
+        b = seqs.copy() if call == "fork" else np.zeros(half, int)
+        (a if call == "fork" else b)[at] = -1                     # a source out of range, a negative length
+        getattr(ctx, "pages_" + call)(c, ints(a), ints(b))
+        assert ctx.pages_status(c)[1:3] == (vb.PAGES_SEQ if call == "fork" else vb.PAGES_COUNT, at)
+        assert all(torch.equal(x, y) for x, y in zip((c.table, c.length, c.refs, c.k, c.v), before))

@@ -64,6 +64,11 @@ __device__ void record(const vb_pages &p, int key) {
     p.status[0] = key & 15;
 }
 
+// Whether an error waits to be read, for the CTA as a whole: in a call of many
+// CTAs the first may be recording the call's own while others start.  A CTA
+// that sees that one leaves; one that does not finds the error itself.
+__device__ bool any_error(const vb_pages &p) { return __syncthreads_or(threadIdx.x == 0 && p.status[0] != 0); }
+
 // Which requests came second for a sequence.
 __device__ void which_twice(int n, const int32_t *seqs, PageError *err) {
     for (int i = threadIdx.x; i < n; i += blockDim.x)
@@ -276,8 +281,7 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(vb_pages p, int n, cons
     pdl_wait();
     uint32_t *bits = reinterpret_cast<uint32_t *>(sm);
     if (threadIdx.x == 0) err.key = INT_MAX;
-    if (p.status[0]) return;
-    __syncthreads();
+    if (any_error(p)) return;
     check_seqs(p, n, dst, bits, &err);
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -308,8 +312,7 @@ __global__ void __launch_bounds__(256) pages_truncate_kernel(vb_pages p, int n, 
     pdl_wait();
     uint32_t *bits = reinterpret_cast<uint32_t *>(sm);
     if (threadIdx.x == 0) err.key = INT_MAX;
-    if (p.status[0]) return;
-    __syncthreads();
+    if (any_error(p)) return;
     check_seqs(p, n, seqs, bits, &err);
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += blockDim.x)
