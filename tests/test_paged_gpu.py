@@ -863,3 +863,35 @@ def test_an_error_in_a_call_of_many_requests_changes_nothing(ctx, call):
         getattr(ctx, "pages_" + call)(c, ints(a), ints(b))
         assert ctx.pages_status(c)[1:3] == (vb.PAGES_SEQ if call == "fork" else vb.PAGES_COUNT, at)
         assert all(torch.equal(x, y) for x, y in zip((c.table, c.length, c.refs, c.k, c.v), before))
+
+
+@pytest.mark.parametrize("type,hd,drafted,nh,nkv,before", [
+    ("f32", 64, 40, 8, 2, 300), ("f32", 128, 40, 8, 2, 20000), ("f32", 128, 20, 8, 2, 20000), ("f32", 128, 2, 8, 2, 9000),
+    ("f32", 256, 10, 8, 2, 9000), ("bf16", 256, 40, 32, 2, 300), ("f16", 256, 40, 32, 2, 20000), ("bf16", 256, 40, 8, 2, 9000),
+    ("bf16", 128, 40, 16, 2, 20000), ("f16", 64, 12, 16, 2, 9000), ("bf16", 128, 1, 16, 2, 9000)])
+def test_tree_seen_infinities_show_in_every_form(ctx, type, hd, drafted, nh, nkv, before):
+    """Every size of a block, held by one CTA and by several; calls one after another give the same."""
+    t = tree_case(ctx, type, [before + drafted, drafted + 9], [drafted, drafted], nh, nkv, hd, 16, "any" if drafted > 1 else "tree", seed=15)
+    bad = [(0, 0, 3), (0, drafted - 1, hd - 1), (1, drafted // 2, 0)]       # sequence, draft row, column
+    for value in (float("inf"), float("nan")):
+        for i, r, col in bad:
+            at = t["lens"][i] - drafted + r
+            t["c"].v[1, t["table"][t["seqs"][i], at // 16], :, at % 16, col] = value
+        got = []
+        for _ in range(3):
+            ctx.tree_attention(t["args"])
+            torch.cuda.synchronize()
+            got.append(t["out"].float().cpu().numpy().reshape(2, drafted, nh, hd))
+        assert ctx.device_status() == (0, 0)
+        want = np.zeros((2, drafted, hd), bool)
+        for i, r, col in bad:
+            want[i, :, col] |= t["seen"][i][:, t["lens"][i] - drafted + r]
+        for x in got:
+            assert np.array_equal(~np.isfinite(x), np.broadcast_to(want[:, :, None], x.shape))
+            assert np.array_equal(np.isnan(x), ~np.isfinite(x) & np.isnan(value))
+    for i, r, col in bad:
+        at = t["lens"][i] - drafted + r
+        t["c"].v[1, t["table"][t["seqs"][i], at // 16], :, at % 16, col] = 0.0
+    ref, tol = tree_ref(t)
+    ok = np.abs(got[-1].reshape(ref.shape) - ref) <= tol
+    assert np.all(ok | np.broadcast_to(want[:, :, None], got[0].shape).reshape(ref.shape))

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     float2 *ml = reinterpret_cast<float2 *>(qs + QS);                               // [8][16]
     __shared__ uint64_t full[TR_MAX_STAGES], empty[TR_MAX_STAGES];
     __shared__ TreeCut cut;
-    __shared__ int abort_flag, not_finite;
+    __shared__ int abort_flag, not_finite;           // last item (by its number in this CTA) with a draft value that was not finite
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         }
         mbar_fence_init();
         abort_flag = 0;
-        not_finite = 0;
+        not_finite = -1;
     }
     pdl_trigger();
     pdl_wait();
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     const int slice = (WM == 1 ? warp & 3 : kw * NS) * 16;      // this warp's first row of a tile
     const int hd = g.p.head_dim;
     const int quad = lane >> 2, ql = lane & 3;
-    int it = 0;
+    int it = 0, item = 0;
     bool first_item = true;
     while (w.left > 0) {
         const int n_tiles = tree_take(g, w);
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         found |= here;
                     }
                 }
-                if (found) not_finite = 1;
+                if (found) not_finite = item;
                 __syncwarp();
             }
             // running maximum and sum
@@ -470,7 +470,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             if (ql == 0) ml[warp * 16 + quad + 8 * h] = make_float2(m[h], x);
         }
         consumer_sync(256);
-        const bool mend = not_finite != 0;
+        // (no warp marks the next item before the barrier behind its queries, which
+        // every warp reaches after this)
+        const bool mend = *(volatile int *)&not_finite == item;
 #pragma unroll
         for (int h = 0; h < H; h++) {
             float2 other[KW];
@@ -516,7 +518,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             }
             consumer_sync(256);
         }
-        if (threadIdx.x == 0) not_finite = 0;          // every warp has read it, and none sets it before the next barrier
         if (kw == 0) {
             float *part = g.part + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * MT * (hd + 2);
             const int lo = max(w.clear, w.tile * TR_KT), hi = min(w.visible, (w.tile + n_tiles) * TR_KT);
@@ -568,6 +569,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         if (threadIdx.x == 0) tree_describe(g, w, line, n_tiles, first_item);
         __syncwarp();
         first_item = false;
+        item++;
         if (w.left > 0) tree_next(g, w);
     }
 }
