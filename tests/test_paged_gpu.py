@@ -895,3 +895,16 @@ def test_tree_seen_infinities_show_in_every_form(ctx, type, hd, drafted, nh, nkv
     ref, tol = tree_ref(t)
     ok = np.abs(got[-1].reshape(ref.shape) - ref) <= tol
     assert np.all(ok | np.broadcast_to(want[:, :, None], got[0].shape).reshape(ref.shape))
+
+
+@pytest.mark.parametrize("type,drafted", [("f32", 1), ("bf16", 1), ("f16", 12), ("f32", 30), ("bf16", 48)])
+@pytest.mark.parametrize("hd,P", [(64, 64), (64, 128), (64, 1024), (128, 128), (128, 1024)])
+def test_tree_tiles_of_few_boxes(ctx, type, drafted, hd, P):
+    """Tiles whose copies leave some of the loading warps without one, many of them in a row: whole pages, and sequences of a
+    few rows, after one another."""
+    long = tree_case(ctx, type, [40000 + drafted], [drafted], 2, 1, hd, P, seed=16, layers=1)
+    short = tree_case(ctx, type, [drafted + i % 30 for i in range(400)], [drafted] * 400, 2, 1, hd, P, seed=17, layers=1)
+    for t in (long, short):
+        for _ in range(4):
+            ctx.tree_attention(t["args"])
+        check_tree(ctx, t)

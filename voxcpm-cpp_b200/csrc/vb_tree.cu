@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < TR_MAX_STAGES; s++) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], 4);
             mbar_init(&empty[s], WM == 1 ? 4 : 8);
         }
         mbar_fence_init();
@@ -144,8 +144,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         // ------------------------------------------------------------ loads
         // Four warps issue a tile's copies (a box per page, column block and
         // K or V; with pages of 16 rows 16 of them, more than one warp can
-        // issue in the time of a tile).  Every warp waits for every stage, so
-        // that none meets a barrier two fills ahead.
+        // issue in the time of a tile).  Every warp waits for every stage and
+        // arrives at every fill, whether or not it has a box in it: a fill is over
+        // only when all four have come by, so that none can fall behind, or run
+        // ahead, to where a parity names another phase than its own.
         const int P = g.p.page_rows, box = min(P, TR_KT), me = warp - 8;
         int it = 0;
         while (w.left > 0) {
@@ -172,8 +174,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 tree_wait_warp(&empty[s], ((uint32_t)(it / g.stages) & 1u) ^ 1u, &abort_flag, g.err);
                 // after a wait that ran out no barrier is touched any more
                 const bool go = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag, 0) == 0;
-                if (go && me == 0 && lane == 0) {
-                    if (nbox) mbar_arrive_expect_tx(&full[s], (uint32_t)nbox * box * 128 * 2 * CB);
+                if (go && lane == 0) {
+                    if (me == 0 && nbox) mbar_arrive_expect_tx(&full[s], (uint32_t)nbox * box * 128 * 2 * CB);
                     else mbar_arrive(&full[s]);
                 }
                 if (go && k < nbox)

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < TT_SLOTS; s++) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], 3);
             mbar_init(&empty[s], 1);
         }
         mbar_init(&q_full, g.q_tma ? 1 : 8);
@@ -284,8 +284,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             // -------------------------------------------------------- loads
             // Three warps issue a tile's copies (a box per page and column
             // block: 16 of them with pages of 16 rows, more than one warp can
-            // issue in the time of a tile).  Every warp waits for every slot, so
-            // that none meets a barrier two fills ahead.
+            // issue in the time of a tile).  Every warp waits for every slot and
+            // arrives at every fill, whether or not it has a box in it: a fill is
+            // over only when all three have come by, so that none can fall behind, or
+            // run ahead, to where a parity names another phase than its own.
             const int P = g.p.page_rows, box = min(P, TT_KT), me = warp == 8 ? 0 : warp - 9;
             const int u = 3 * lane + me, k = u / CB, c = u % CB;         // box and column block of the lane's copy
             int slot = 0, item = 0;
@@ -336,8 +338,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     const int y1 = e + 1 < 2 * n ? place(e + 1, nbox1, is_v1) : 0;
                     tree_wait_warp(&empty[slot], phase, &abort_flag, g.err);
                     const bool go = going();
-                    if (go && me == 0 && lane == 0) {
-                        if (nbox) mbar_arrive_expect_tx(&full[slot], (uint32_t)nbox * box * 128 * CB);
+                    if (go && lane == 0) {
+                        if (me == 0 && nbox) mbar_arrive_expect_tx(&full[slot], (uint32_t)nbox * box * 128 * CB);
                         else mbar_arrive(&full[slot]);
                     }
                     if (go && k < nbox)
