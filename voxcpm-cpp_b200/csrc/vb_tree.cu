@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < TR_MAX_STAGES; s++) {
-            mbar_init(&full[s], 4);
+            mbar_init(&full[s], 1);
             mbar_init(&empty[s], WM == 1 ? 4 : 8);
         }
         mbar_fence_init();
@@ -142,19 +142,23 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         // ------------------------------------------------------------ loads
-        // Four warps issue a tile's copies (a box per page, column block and
-        // K or V; with pages of 16 rows 16 of them, more than one warp can
-        // issue in the time of a tile).  Every warp waits for every stage and
-        // arrives at every fill, whether or not it has a box in it: a fill is over
-        // only when all four have come by, so that none can fall behind, or run
-        // ahead, to where a parity names another phase than its own.
+        // Four warps (two for one column block) issue a tile's copies: a box per
+        // page, column block and K or V; with pages of 16 rows 16 of them, more
+        // than one warp can issue in the time of a tile.  Every warp has a box in
+        // every tile (a tile without rows takes the pool's first, which count for
+        // nothing), so no fill is over before all have come by, and none can fall
+        // behind, or run ahead, to where a parity names another phase than its own.
+        // (With an arrival of every warp for that 64 sequences of 8192 rows take
+        // 106 us, with a box of every warp 98.)
+        constexpr int LW = CB == 1 ? 2 : 4;
         const int P = g.p.page_rows, box = min(P, TR_KT), me = warp - 8;
+        if (me >= LW) return;
         int it = 0;
         while (w.left > 0) {
             const int n_tiles = tree_take(g, w);
             const int32_t *row = g.p.table + (int64_t)w.q.s * g.p.max_pages;
             // unit u of a tile: K or V, box u / 2 / CB, column block u / 2 % CB
-            const int u = 4 * lane + me, k = u / 2 / CB, c = u / 2 % CB;
+            const int u = LW * lane + me, k = u / 2 / CB, c = u / 2 % CB;
             auto place = [&](int x) {                   // row of the pool that the lane's box starts at
                 const int r = (w.tile + x) * TR_KT + k * box;
                 if (r >= w.visible || k * box >= TR_KT) return 0;
@@ -169,15 +173,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             for (int x = 0; x < n_tiles; x++, it++) {
                 const int y1 = x + 1 < n_tiles ? place(x + 1) : 0;
                 const int have = min(TR_KT, w.visible - (w.tile + x) * TR_KT);        // rows of the tile that count
-                const int nbox = have <= 0 ? 0 : (have + box - 1) / box;
+                const int nbox = max(1, (have + box - 1) / box);
                 const int s = it % g.stages;
                 tree_wait_warp(&empty[s], ((uint32_t)(it / g.stages) & 1u) ^ 1u, &abort_flag, g.err);
                 // after a wait that ran out no barrier is touched any more
                 const bool go = __shfl_sync(0xffffffffu, *(volatile int *)&abort_flag, 0) == 0;
-                if (go && lane == 0) {
-                    if (me == 0 && nbox) mbar_arrive_expect_tx(&full[s], (uint32_t)nbox * box * 128 * 2 * CB);
-                    else mbar_arrive(&full[s]);
-                }
+                if (go && me == 0 && lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)nbox * box * 128 * 2 * CB);
                 if (go && k < nbox)
                     tma_load_2d(ring + (size_t)s * STAGE + ((u & 1) * CB + c) * TILE + k * box * 128, u & 1 ? &tv : &tk, 64 * c, y,
                                 &full[s]);
