@@ -566,8 +566,9 @@ typedef struct {
 
 /* Errors of the page calls.  They are found on the device: the call that
  * meets one changes nothing and records it with the lowest request index it
- * was found at, and later page calls on the cache change nothing either
- * until vb_pages_status has read it. */
+ * was found at, and later calls on the cache change nothing either until
+ * vb_pages_status has read it: page calls leave it as it is, vb_qk_norm_rope
+ * stores nothing and vb_tree_attention gives zeros (both report it, VB_DEV_*). */
 enum {
     VB_PAGES_SEQ = 1,     /* sequence out of range, or in two requests of one call */
     VB_PAGES_COUNT = 2,   /* negative count, drafted > length, kept > drafted */
@@ -618,8 +619,8 @@ int vb_pages_status(vb_ctx *ctx, const vb_pages *p, int *error, int *request, in
  * after VB_DEV_TREE_PAGE its rows are of no use). */
 enum {
     VB_DEV_QK_POS = 21,   /* position outside the rotation table */
-    VB_DEV_QK_ROW = 22,   /* sequence or row outside the cache, or no page there */
-    VB_DEV_TREE_SEQ = 31, /* sequence, start or length outside the bounds of the call */
+    VB_DEV_QK_ROW = 22,   /* a row that the sequence does not hold (vb_pages_extend), no page there, or an unread page error */
+    VB_DEV_TREE_SEQ = 31, /* sequence, start or length outside the bounds of the call, or an unread page error */
     VB_DEV_TREE_PAGE = 32, /* a table entry names no page of the pool */
     VB_DEV_TREE_WAIT = 33 /* a wait inside the kernel ran out (its waits are bounded) */
 };
@@ -653,7 +654,8 @@ typedef struct {
     void *q_out, *k_out;            /* may alias q and k; k_out may be NULL */
     int64_t ldq_out, ldk_out;
     const vb_pages *pages;          /* or NULL: k and v are not stored */
-    const int32_t *seq, *row;       /* device [n_tokens]: where token t is stored; seq -1: nowhere.  No row twice. */
+    const int32_t *seq, *row;       /* device [n_tokens]: where token t is stored; seq -1: nowhere.  No row twice.
+                                     * A row that forked sequences share is one row: what is stored shows in all. */
 } vb_qk_args;
 int vb_qk_norm_rope(vb_ctx *ctx, const vb_qk_args *a);
 

@@ -908,3 +908,65 @@ def test_tree_tiles_of_few_boxes(ctx, type, drafted, hd, P):
         for _ in range(4):
             ctx.tree_attention(t["args"])
         check_tree(ctx, t)
+
+
+def step_args(c, seq, place, nh=4, seed=0):
+    """(norm and store, attention) of one sequence's tokens at `place`."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kv, hd, n = c.k.shape[2], c.k.shape[4], len(place)
+    qkv = torch.randn(n, (nh + 2 * kv) * hd, generator=g, device="cuda")
+    q, out = torch.full((n, nh * hd), 7.0, device="cuda"), torch.full((n, nh * hd), 7.0, device="cuda")
+    store = vb.QKArgs(qkv[:, :nh * hd], qkv[:, nh * hd:(nh + kv) * hd], qkv[:, (nh + kv) * hd:], heads=nh, kv_heads=kv,
+                      head_dim=hd, q_out=q, pages=c, layer=1, seq=ints([seq] * n), row=ints(place))
+    return store, vb.TreeArgs(q, c, 1, ints([seq]), ints([0, n]), out, heads=nh, max_tokens=n), qkv, q, out
+
+
+def test_a_step_after_a_failed_extend_writes_nowhere(ctx):
+    """A fork cut back into a shared page cannot be extended: its rows do not land on its parent's."""
+    c = new_cache(ctx, pages=5, most=4)
+    m = M.PoolModel(rows_of(c), 6, 4)
+    for f, a in (("extend", ([0], [40])), ("fork", ([0], [1])), ("truncate", ([1], [35])), ("extend", ([2], [32]))):
+        getattr(ctx, "pages_" + f)(c, *(ints(x) for x in a))
+        getattr(m, f)(*a)
+    ctx.pages_extend(c, ints([1]), ints([2]))                     # wants a page of its own, and there is none
+    store, attend, qkv, q, out = step_args(c, 1, [35, 36])
+    ctx.qk_norm_rope(store)
+    assert ctx.device_status() == (vb.VB_ERR_BACKEND, vb.DEV_QK_ROW)
+    ctx.tree_attention(attend)
+    assert ctx.device_status() == (vb.VB_ERR_BACKEND, vb.DEV_TREE_SEQ)
+    assert not q.any() and not out.any()
+    assert_state(c, m)
+    # the error is read and the rows are still not held
+    assert ctx.pages_status(c)[:3] == (vb.VB_ERR_BACKEND, vb.PAGES_FULL, 0)
+    ctx.qk_norm_rope(store)
+    assert ctx.device_status() == (vb.VB_ERR_BACKEND, vb.DEV_QK_ROW)
+    assert_state(c, m)
+    # with a page free the same step goes through, on a copy of the shared one
+    for f, a in (("truncate", ([2], [0])), ("extend", ([1], [2]))):
+        getattr(ctx, "pages_" + f)(c, *(ints(x) for x in a))
+        getattr(m, f)(*a)
+    ctx.qk_norm_rope(store)
+    ctx.tree_attention(attend)
+    assert ctx.device_status() == (0, 0) and bool(out.any())
+    kv = qkv[:, 4 * 64:].bfloat16().view(torch.int16).cpu().numpy().reshape(2, 2, 2, 64)
+    for t, row in enumerate((35, 36)):
+        m.data[1, :, m.table[1, row // 16], :, row % 16] = kv[t]
+    assert m.table[1, 2] != m.table[0, 2]
+    assert_state(c, m)
+
+
+def test_rows_are_stored_while_they_are_held(ctx):
+    """Rows at and past a sequence's length are skipped, whatever its page holds; shared ones that it holds are stored."""
+    c = new_cache(ctx)
+    ctx.pages_extend(c, ints([0]), ints([21]))
+    ctx.pages_fork(c, ints([0]), ints([1]))
+    ctx.pages_truncate(c, ints([0]), ints([20]))
+    store, _, qkv, q, _ = step_args(c, 0, [18, 19, 20, 31])
+    before = rows_of(c)
+    ctx.qk_norm_rope(store)
+    assert ctx.device_status() == (vb.VB_ERR_BACKEND, vb.DEV_QK_ROW)
+    assert torch.equal(q[:2], qkv[:2, :4 * 64]) and not q[2:].any()
+    kv = qkv[:, 4 * 64:].bfloat16().view(torch.int16).cpu().numpy().reshape(4, 2, 2, 64)
+    page = int(c.table[1, 1])
+    before[1, :, page, :, 2], before[1, :, page, :, 3] = kv[0], kv[1]
+    assert np.array_equal(rows_of(c), before)

@@ -187,6 +187,9 @@ __global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kerne
     // round trips to memory in all
     int pos = a.rope ? a.pos[t] : 0;
     const int seq = g.store ? a.seq[t] : -1, row = g.store ? a.row[t] : 0;
+    // an error of a page call that nobody has read: rows may not be where the
+    // caller takes them to be, so nothing is stored
+    const bool unread = g.store && g.p.status[0] != 0;
     auto fetch = [&](int h, Piece<T, V> (&u)[ROWS], Piece<T, V> (&v)[ROWS]) {
 #pragma unroll
         for (int r = 0; r < ROWS; r++, h++) {
@@ -204,9 +207,12 @@ __global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kerne
     // an invalid place or position skips the whole token
     const bool off_table = a.rope && (pos < 0 || pos >= a.rope_rows);
     if (off_table) pos = 0;
-    int page = 0;
+    int page = 0, held = 0;                               // rows that the sequence holds
     const bool placed = seq >= 0 && seq < g.p.n_seqs && row >= 0 && row / g.p.page_rows < g.p.max_pages;
-    if (placed) page = g.p.table[(int64_t)seq * g.p.max_pages + row / g.p.page_rows];
+    if (placed) {
+        page = g.p.table[(int64_t)seq * g.p.max_pages + row / g.p.page_rows];
+        held = g.p.length[seq];
+    }
     // A piece y turns to y * c + z * s: z is the other piece (and s negative for
     // the first) or, where pairs are adjacent, y's own with each pair swapped.
     f32x2 cs_c[ADJACENT ? V : H], cs_s[V], w0[H], w1[H];
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kerne
             }
         }
     }
-    const bool no_row = g.store && seq != -1 && (!placed || page < 0 || page >= g.p.n_pages);
+    const bool no_row = g.store && seq != -1 && (unread || !placed || row >= held || page < 0 || page >= g.p.n_pages);
     const bool bad = off_table || no_row;
     if (bad && lane == 0) atomicCAS(g.err, 0, off_table ? VB_DEV_QK_POS : VB_DEV_QK_ROW);
     const int64_t pool_head = (int64_t)g.p.page_rows * hd;

@@ -33,7 +33,8 @@ struct TreeArgs {
 };
 
 // Sequence i of the call.  T = 0: no rows of q (or none that can be named);
-// bad: its tokens get zeros.
+// bad: its tokens get zeros.  So do all while an error of a page call waits to
+// be read: the newest rows are then not those of the call's tokens.
 struct TreeSeq {
     int t0, T, s, len, base, bad;
 };
@@ -54,7 +55,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &g, int i) {
     }
     q.len = q.s >= 0 && q.s < g.p.n_seqs ? g.p.length[q.s] : -1;
     q.base = q.len - q.T;
-    if (q.base < 0 || (int64_t)q.len > (int64_t)g.p.max_pages * g.p.page_rows ||
+    if (g.p.status[0] != 0 || q.base < 0 || (int64_t)q.len > (int64_t)g.p.max_pages * g.p.page_rows ||
         (a.mask && q.T > 32 * (int64_t)a.mask_words)) {
         q.bad = 1;
         q.len = q.base = 0;
