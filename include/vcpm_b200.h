@@ -572,7 +572,7 @@ typedef struct {
 enum {
     VB_PAGES_SEQ = 1,     /* sequence out of range, or in two requests of one call */
     VB_PAGES_COUNT = 2,   /* negative count, drafted > length, kept > drafted */
-    VB_PAGES_LONG = 3,    /* more than max_pages * page_rows rows */
+    VB_PAGES_LONG = 3,    /* more than max_pages * page_rows rows, or a length that is no number of rows */
     VB_PAGES_FULL = 4,    /* not enough free pages */
     VB_PAGES_SHARED = 5,  /* keep would move rows of a page that another sequence names */
     VB_PAGES_PATH = 6,    /* path not rising, or outside the draft */

@@ -970,3 +970,17 @@ def test_rows_are_stored_while_they_are_held(ctx):
     page = int(c.table[1, 1])
     before[1, :, page, :, 2], before[1, :, page, :, 3] = kv[0], kv[1]
     assert np.array_equal(rows_of(c), before)
+
+
+@pytest.mark.parametrize("length", [-5, -40, -2 ** 31, 65, 2 ** 31 - 1])
+@pytest.mark.parametrize("call,args", [("extend", ([2], [1])), ("extend", ([0], [0])), ("keep", ([2], [3], [2], [[1, 2]])),
+                                       ("keep", ([0], [0], [0], [[0]]))])
+def test_a_broken_length_is_reported(ctx, call, args, length):
+    """A length that is no number of rows leads nowhere outside the table."""
+    c, m = start_state(ctx)                                       # 4 pages of 16 rows for a sequence
+    seq = args[0][0]
+    c.length[seq] = length
+    m.length[seq] = length
+    getattr(ctx, "pages_" + call)(c, *(ints(x) for x in args))
+    assert ctx.pages_status(c)[:3] == (vb.VB_ERR_BACKEND, vb.PAGES_LONG, 0)
+    assert_state(c, m)

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(PG_STEP) pages_extend_plan(vb_pages p, int n, 
         twice |= atomicOr(&bits[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u;
         length[i] = len;
         if (r < 0) err.at(i, VB_PAGES_COUNT);
-        else if ((int64_t)len + r > (int64_t)p.max_pages * P) err.at(i, VB_PAGES_LONG);
+        else if (len < 0 || (int64_t)len + r > (int64_t)p.max_pages * P) err.at(i, VB_PAGES_LONG);
         else if (r > 0 && len % P) {
             const int pg = p.table[(int64_t)s * p.max_pages + len / P];
             if (pg < 0 || pg >= p.n_pages) err.at(i, VB_PAGES_TABLE);
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(PG_KEEP) pages_keep_plan(vb_pages p, int n, co
     __shared__ PageError err;
     uint32_t *bits = reinterpret_cast<uint32_t *>(sm);
     int2 *moves = reinterpret_cast<int2 *>(ws + 4);
-    const int P = p.page_rows;
+    const int P = p.page_rows, most = p.max_pages * P;
     if (threadIdx.x == 0) err.key = INT_MAX;
     for (int i = threadIdx.x; i < (p.n_seqs + 31) / 32; i += blockDim.x) bits[i] = 0;
     pdl_trigger();
@@ -357,7 +357,9 @@ __global__ void __launch_bounds__(PG_KEEP) pages_keep_plan(vb_pages p, int n, co
             continue;
         }
         twice |= atomicOr(&bits[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u;
-        if (d < 0 || k < 0 || k > d || k > ld || d > p.length[s]) err.at(i, VB_PAGES_COUNT);
+        const int len = p.length[s];
+        if (len < 0 || len > most) err.at(i, VB_PAGES_LONG);
+        else if (d < 0 || k < 0 || k > d || k > ld || d > len) err.at(i, VB_PAGES_COUNT);
     }
     // the paths, of requests that are in order themselves; by the other warps
     // first, while those above wait for their lengths
@@ -366,8 +368,8 @@ __global__ void __launch_bounds__(PG_KEEP) pages_keep_plan(vb_pages p, int n, co
         const int i = e / ld, j = e - i * ld, s = seqs[i], d = drafted[i], at = path[e], prev = j ? path[e - 1] : -1;
         moves[e] = make_int2(-1, -1);
         if (j >= kept[i] || s < 0 || s >= p.n_seqs) continue;
-        const int base = p.length[s] - d;
-        if (d < 0 || kept[i] > d || base < 0) continue;
+        const int len = p.length[s], base = len - d;
+        if (d < 0 || kept[i] > d || len < 0 || len > most || base < 0) continue;
         const int32_t *row = p.table + (int64_t)s * p.max_pages;
         if (at < 0 || at >= d || prev >= at) err.at(i, VB_PAGES_PATH);
         else if (at != j) {
