@@ -667,7 +667,9 @@ int vb_qk_norm_rope(vb_ctx *ctx, const vb_qk_args *a);
  * drafted tokens names its ancestors and itself.  Without a mask they are a
  * chain: token j sees 0 .. j, so one token is a decode step and many are a
  * prompt.  A token that sees nothing gives zeros; what lies in rows that it
- * does not see never reaches its result. */
+ * does not see never reaches its result.  A score of plus infinity or NaN
+ * makes its result NaN (with F32 queries an infinite key that it sees may,
+ * whatever the sign). */
 typedef struct {
     int type;                       /* of q and out: VB_TYPE_F32 (cache BF16), or the cache's type */
     int layer;

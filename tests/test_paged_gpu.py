@@ -984,3 +984,42 @@ def test_a_broken_length_is_reported(ctx, call, args, length):
     getattr(ctx, "pages_" + call)(c, *(ints(x) for x in args))
     assert ctx.pages_status(c)[:3] == (vb.VB_ERR_BACKEND, vb.PAGES_LONG, 0)
     assert_state(c, m)
+
+
+@pytest.mark.parametrize("type,drafted,nh", [("f32", 1, 2), ("f32", 40, 8), ("bf16", 1, 2), ("bf16", 12, 16), ("bf16", 40, 16),
+                                             ("f16", 40, 16), ("f16", 12, 16)])
+@pytest.mark.parametrize("row", [0, 4, 20, 70, 130, 5003])
+def test_tree_infinite_scores_show(ctx, type, drafted, nh, row):
+    """An infinite score leaves no weight that can be named: NaN, wherever its row lies in the cache and however it is cut.  A
+    row whose score is minus infinity has no weight (fp32 queries: their terms' products with it cancel to NaN)."""
+    t = tree_case(ctx, type, [9000 + drafted], [drafted], nh, 1, 128, 16, "tree", seed=18)
+    t["q"][:, 5::128] = t["q"][:, 5::128].abs() + 1               # each head's value 5 is positive
+    page, at = t["table"][t["seqs"][0], row // 16], row % 16
+    t["c"].k[1, page, 0, at, 5] = float("inf")
+    ctx.tree_attention(t["args"])
+    assert ctx.device_status() == (0, 0)
+    assert bool(t["out"].isnan().all())
+    if type == "f32":
+        return
+    t["c"].k[1, page, 0, at, 5] = float("-inf")
+    ctx.tree_attention(t["args"])
+    t["c"].k[1, page, 0, at] = 0
+    t["seen"][0][:, row] = False
+    ref, tol = tree_ref(t)
+    got = t["out"].float().cpu().numpy()
+    assert np.all(np.abs(got - ref) <= tol)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,row", [(128, 0), (128, 4), (128, 20), (64, 9), (64, 40)])
+def test_tree_infinite_scores_show_in_whole_items(ctx, type, hd, row):
+    """The same in items that a CTA holds alone, after a tile that every token sees."""
+    n, drafted = 600, 20
+    t = tree_case(ctx, type, [128 + drafted] * n, [drafted] * n, 16, 1, hd, 16, "tree", seed=19)
+    t["q"][:, 5::hd] = t["q"][:, 5::hd].abs() + 1
+    with_inf = np.arange(n) % 3 == 1
+    t["c"].k[1, t["table"][t["seqs"][with_inf], row // 16], 0, row % 16, 5] = float("inf")
+    ctx.tree_attention(t["args"])
+    assert ctx.device_status() == (0, 0)
+    nan = t["out"].isnan().cpu().numpy().reshape(n, -1)
+    assert nan[with_inf].all() and not nan[~with_inf].any()

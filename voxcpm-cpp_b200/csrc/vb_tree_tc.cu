@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                     // tensor memory: the weights against the running maximum as it
                     // stands (in an item's first tile that of the first piece), and the
                     // row's own maximum beside them.  They count if that maximum is no
-                    // further than 2^TT_SLACK above and there was no NaN; else two
+                    // further than 2^TT_SLACK above and there was no NaN and no infinite
+                    // score (whose NaN exp2_pair would not keep); else two
                     // passes, the maximum first.  (The weights wait in registers: in
                     // tensor memory they would take the scores' place.)
                     uint32_t a[32], b[32];
@@ -606,7 +607,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
                             if (k < 3) tmem_ld32_wait(k & 1 ? a : b);
                         }
                         const float top = max3_nan(t0, t1, t1) * g.scale_log2;
-                        done = !__any_sync(0xffffffffu, j >= 0 && (!(top <= m + TT_SLACK) || m == -INFINITY));
+                        done = !__any_sync(0xffffffffu, j >= 0 && (!(top <= m + TT_SLACK) || m == -INFINITY || top == INFINITY));
                         if (done) {
                             tmem_st32(sc, y[0]);
                             tmem_st32(sc + 32, y[1]);
