@@ -1023,3 +1023,17 @@ def test_tree_infinite_scores_show_in_whole_items(ctx, type, hd, row):
     assert ctx.device_status() == (0, 0)
     nan = t["out"].isnan().cpu().numpy().reshape(n, -1)
     assert nan[with_inf].all() and not nan[~with_inf].any()
+
+
+@pytest.mark.parametrize("pool", ["bf16", "f16"])
+def test_qk_rounds_cache_rows_once(ctx, pool):
+    """Results rounded to bf16 beside a cache of another type: its rows come from the unrounded values."""
+    args, out, kout, c, v, (rq, rk), (seq, row) = qk_case(ctx, "f32", 40, 4, 2, 64, flags=vb.OUT_BF16, pool=TYPES[pool])
+    plain = qk_case(ctx, "f32", 40, 4, 2, 64, pool=TYPES[pool])
+    ctx.qk_norm_rope(args)
+    ctx.qk_norm_rope(plain[0])
+    torch.cuda.synchronize()
+    assert torch.equal(out, plain[1].bfloat16().float()) and torch.equal(kout, plain[2].bfloat16().float())
+    page = c.table.long().cpu()[seq, row // 16]
+    k_rows, v_rows = (x[1].cpu()[page, :, row % 16].reshape(40, -1) for x in (c.k, c.v))
+    assert torch.equal(k_rows, plain[2].cpu().to(TYPES[pool])) and torch.equal(v_rows, v.cpu().to(TYPES[pool]))

@@ -158,7 +158,8 @@ __device__ __forceinline__ void store2(T *p, bool vec, const f32x2 (&y)[V]) {
 // 7.4 | 9.2.
 constexpr int QK_ROWS = 2;
 
-template <typename T, int V, int LPH, bool ADJACENT>
+// ROUND: VB_OUT_BF16.
+template <typename T, int V, int LPH, bool ADJACENT, bool ROUND>
 __global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kernel(const __grid_constant__ QKArgs g) {
     constexpr int ROWS = QK_ROWS, H = V / 2;
     pdl_trigger();
@@ -295,7 +296,20 @@ __global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kerne
                     y1[i] = fma2(p1, cs_c[ADJACENT ? H + i : i], mul2(ADJACENT ? swapped(p1) : p0, cs_s[H + i]));
                 }
             }
-            if (sizeof(T) == 4 && (a.flags & VB_OUT_BF16)) {
+            auto keep_row = [&]() {
+                if (is_q || !keep) return;
+                if (g.p.type == VB_TYPE_F16) {
+                    __half *pool = static_cast<__half *>(is_v ? g.p.v : g.p.k) + at + kvh * pool_head;
+                    store2(pool + i0, true, y0);
+                    store2(pool + i1, true, y1);
+                } else {
+                    __nv_bfloat16 *pool = static_cast<__nv_bfloat16 *>(is_v ? g.p.v : g.p.k) + at + kvh * pool_head;
+                    store2(pool + i0, true, y0);
+                    store2(pool + i1, true, y1);
+                }
+            };
+            if constexpr (ROUND) {
+                keep_row();                                   // before: a row of the cache is rounded once, to its type
 #pragma unroll
                 for (int i = 0; i < H; i++) {
                     float u, v;
@@ -316,16 +330,7 @@ __global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kerne
                 store2(dst + i0, g.vec, y0);
                 store2(dst + i1, g.vec, y1);
             }
-            if (is_q || !keep) continue;
-            if (g.p.type == VB_TYPE_F16) {
-                __half *pool = static_cast<__half *>(is_v ? g.p.v : g.p.k) + at + kvh * pool_head;
-                store2(pool + i0, true, y0);
-                store2(pool + i1, true, y1);
-            } else {
-                __nv_bfloat16 *pool = static_cast<__nv_bfloat16 *>(is_v ? g.p.v : g.p.k) + at + kvh * pool_head;
-                store2(pool + i0, true, y0);
-                store2(pool + i1, true, y1);
-            }
+            if constexpr (!ROUND) keep_row();
         }
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kerne
 
 int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who);
 
-template <typename T, int V, bool ADJACENT>
+template <typename T, int V, bool ADJACENT, bool ROUND = false>
 static cudaError_t launch_qk_v(vb_ctx *ctx, QKArgs &g) {
     const int heads = g.a.n_heads + g.a.n_kv_heads * (g.store ? 2 : 1), rows = QK_ROWS;
     int lph = 1;
@@ -349,12 +354,12 @@ static cudaError_t launch_qk_v(vb_ctx *ctx, QKArgs &g) {
     g.per = (int)((heads + chunks - 1) / chunks + rows - 1) / rows * rows;
     const dim3 grid((unsigned)(((int64_t)g.a.n_tokens * lph + QK_THREADS - 1) / QK_THREADS), (unsigned)((heads + g.per - 1) / g.per));
     switch (lph) {
-        case 1: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 1, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
-        case 2: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 2, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
-        case 4: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 4, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
-        case 8: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 8, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
-        case 16: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 16, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
-        default: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 32, ADJACENT>, grid, dim3(QK_THREADS), 0, g);
+        case 1: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 1, ADJACENT, ROUND>, grid, dim3(QK_THREADS), 0, g);
+        case 2: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 2, ADJACENT, ROUND>, grid, dim3(QK_THREADS), 0, g);
+        case 4: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 4, ADJACENT, ROUND>, grid, dim3(QK_THREADS), 0, g);
+        case 8: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 8, ADJACENT, ROUND>, grid, dim3(QK_THREADS), 0, g);
+        case 16: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 16, ADJACENT, ROUND>, grid, dim3(QK_THREADS), 0, g);
+        default: return pdl_launch(ctx, qk_norm_rope_kernel<T, V, 32, ADJACENT, ROUND>, grid, dim3(QK_THREADS), 0, g);
     }
 }
 
@@ -364,6 +369,9 @@ static cudaError_t launch_qk(vb_ctx *ctx, QKArgs &g) {
     if constexpr (sizeof(T) == 2)
         if (g.a.head_dim % 16 == 0 && rot % 16 == 0)
             return g.a.adjacent ? launch_qk_v<T, 8, true>(ctx, g) : launch_qk_v<T, 8, false>(ctx, g);
+    if constexpr (sizeof(T) == 4)
+        if (g.a.flags & VB_OUT_BF16)
+            return g.a.adjacent ? launch_qk_v<T, 4, true, true>(ctx, g) : launch_qk_v<T, 4, false, true>(ctx, g);
     return g.a.adjacent ? launch_qk_v<T, 4, true>(ctx, g) : launch_qk_v<T, 4, false>(ctx, g);
 }
 
