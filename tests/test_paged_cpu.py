@@ -65,3 +65,13 @@ def test_pool_model_shares_and_copies():
     assert m.refs.tolist() == [2, 1, 1, 0] and np.array_equal(m.data[:, :, 2, :, :4], m.data[:, :, 1, :, :4])
     m.truncate([0], [0])
     assert m.refs.tolist() == [1, 0, 1, 0]
+
+
+def test_broadcast_rows_are_refused():
+    """A row stride of 0 means packed rows to the library: a broadcast tensor would be read past its end."""
+    torch = pytest.importorskip("torch")
+    for t in (torch.zeros(1, 16).expand(3, 16), torch.zeros(64).as_strided((3, 16), (8, 1))):
+        with pytest.raises(ValueError, match="rows of their own"):
+            vb._rows(t, 16, "q")
+    for t, ld in ((torch.zeros(3, 20)[:, :16], 20), (torch.zeros(1, 16).expand(1, 16), 16), (torch.zeros(3, 16), 16)):
+        assert vb._rows(t, 16, "q") == (t.data_ptr(), ld)

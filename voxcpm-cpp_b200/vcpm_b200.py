@@ -447,9 +447,10 @@ def _type_of(t):
 
 
 def _rows(t, width, what):
-    """(address, row stride) of a [rows][width] tensor whose rows are dense."""
-    if t.dim() != 2 or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: [tokens][{width}] with dense rows is wanted")
+    """(address, row stride) of a [rows][width] tensor whose rows are dense and
+    apart (the rows of a broadcast tensor are one)."""
+    if t.dim() != 2 or t.shape[1] != width or (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
+        raise ValueError(f"{what}: [tokens][{width}] with dense rows of their own is wanted")
     return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
 
 
