@@ -75,3 +75,18 @@ def test_broadcast_rows_are_refused():
             vb._rows(t, 16, "q")
     for t, ld in ((torch.zeros(3, 20)[:, :16], 20), (torch.zeros(1, 16).expand(1, 16), 16), (torch.zeros(3, 16), 16)):
         assert vb._rows(t, 16, "q") == (t.data_ptr(), ld)
+
+
+def test_host_tensors_are_refused():
+    """Their addresses would fault on the device."""
+    torch = pytest.importorskip("torch")
+    new = lambda *s, dtype=torch.int32: torch.zeros(s, dtype=dtype)  # noqa: E731
+    q, k = new(3, 16, dtype=torch.float32), new(3, 8, dtype=torch.float32)
+    with pytest.raises(ValueError, match="CUDA"):
+        vb.Pages(new(1, 2, 1, 16, 8, dtype=torch.bfloat16), new(1, 2, 1, 16, 8, dtype=torch.bfloat16), new(1, 2), new(1), new(2), new(4))
+    with pytest.raises(ValueError, match="CUDA"):
+        vb.QKArgs(q, k, k, heads=2, kv_heads=1, head_dim=8, q_out=q)
+    with pytest.raises(ValueError, match="CUDA"):
+        vb._count(new(2), new(2))
+    with pytest.raises(ValueError, match="pos"):
+        vb.QKArgs(q, k, k, heads=2, kv_heads=1, head_dim=8, q_out=q, rope=new(4, 8, dtype=torch.float32))

@@ -391,8 +391,8 @@ class Context:
         """Of the last drafted[i] rows of seqs[i] keep those at
         path[i][:kept[i]] (int32 [n][most])."""
         n = _count(seqs, drafted, kept)
-        if path.dim() != 2 or path.shape[0] != n or not _is_int32(path) or not path.is_contiguous():
-            raise ValueError("path: contiguous int32 [n][most]")
+        if path.dim() != 2 or path.shape[0] != n or not _is_int32(path) or not path.is_contiguous() or not path.is_cuda:
+            raise ValueError("path: contiguous int32 [n][most] in CUDA memory")
         self.check(self.L.vb_pages_keep(self.h, p.ref, n, seqs.data_ptr(), drafted.data_ptr(), kept.data_ptr(),
                                         path.data_ptr(), path.shape[1]))
 
@@ -434,8 +434,8 @@ def _count(*arrays):
     """Length of device int32 vectors that belong together."""
     shape = arrays[0].shape
     for a in arrays:
-        if len(shape) != 1 or a.shape != shape or not _is_int32(a) or not a.is_contiguous():
-            raise ValueError("contiguous int32 vectors of one length are wanted")
+        if len(shape) != 1 or a.shape != shape or not _is_int32(a) or not a.is_contiguous() or not a.is_cuda:
+            raise ValueError("contiguous int32 CUDA vectors of one length are wanted")
     return shape[0]
 
 
@@ -454,8 +454,15 @@ def _rows(t, width, what):
     return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
 
 
+def _on_device(*tensors):
+    """The kernels read what the records name: host memory is refused here."""
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise ValueError("CUDA tensors are wanted")
+
+
 def _vector(t, n, what):
-    if t.shape != (n,) or str(t.dtype) != "torch.int32" or not (n < 2 or t.is_contiguous()):
+    if t is None or t.shape != (n,) or str(t.dtype) != "torch.int32" or not (n < 2 or t.is_contiguous()):
         raise ValueError(f"{what}: contiguous int32 [{n}] is wanted")
     return t.data_ptr()
 
@@ -475,6 +482,7 @@ class Pages:
         for t in (k, v, table, length, refs, status):
             if not t.is_contiguous():
                 raise ValueError("the cache's tensors are contiguous")
+        _on_device(k, v, table, length, refs, status)
         for t in (table, length, refs, status):
             if str(t.dtype) != "torch.int32":
                 raise ValueError("table, length, refs and status are int32")
@@ -531,6 +539,7 @@ class QKArgs:
             c.pages, c.seq, c.row = C.addressof(pages.c), _vector(seq, n, "seq"), _vector(row, n, "row")
         self.c, self.ref = c, C.byref(c)
         self._keep = (q, k, v, q_out, k_out, rope, pos, q_weight, k_weight, pages, seq, row)
+        _on_device(q, k, v, q_out, k_out, rope, pos, q_weight, k_weight, seq, row)
 
 
 class TreeArgs:
@@ -553,6 +562,7 @@ class TreeArgs:
             c.mask, c.mask_words = mask.data_ptr(), mask.shape[1]
         self.c, self.ref = c, C.byref(c)
         self._keep = (q, pages, seqs, start, out, mask)
+        _on_device(q, seqs, start, out, mask)
 
 
 def rope_table(rot_dim, theta, longrope, n_pos):
