@@ -98,3 +98,21 @@ def test_refusals(ctx):
     with pytest.raises(vb.VBError):
         lm.check()
     lm.close()
+
+
+def test_a_check_says_what_came_since_the_last(ctx):
+    """A failed step, a check that raises, then a step that fits: the next check passes."""
+    ref = Refs(O.TYPE_F16, 1)
+    cfg = vb.LMConfig(H, NH, NKV, HD, F, LAYERS, 1e-5, 10000.0, 1, 0.0, O.TYPE_F16)
+    lm = PL.PagedLM(ctx, cfg, ref.layers, ref.fn, seqs=2, pages=2, page_rows=16, most_rows=32)
+    a, b = rows(20), rows(16)
+    lm.step(torch.from_numpy(a).cuda(), [0], [20])
+    lm.step(torch.from_numpy(b).cuda(), [1], [16])            # no page is left
+    with pytest.raises(vb.VBError, match="pages: error 4 in request 0; device error"):
+        lm.check()
+    assert lm.check() == 0
+    lm.truncate([0], [0])
+    got = lm.step(torch.from_numpy(b).cuda(), [1], [16]).cpu().numpy()
+    assert lm.check() == 1
+    S.assert_envelope(got, *ref.last([b]))
+    lm.close()

@@ -140,12 +140,13 @@ class PagedLM:
 
     def check(self):
         """Raises if a call since the last check met a full pool or bad numbers."""
+        # both are read, and so cleared, first: a step behind a failed page call
+        # records errors of its own
         rc, error, request, free = self.ctx.pages_status(self.cache)
-        if rc:
-            raise vb.VBError(rc, f"pages: error {error} in request {request}")
-        rc, code = self.ctx.device_status()
-        if rc:
-            raise vb.VBError(rc, f"device error {code}")
+        device_rc, code = self.ctx.device_status()
+        if rc or device_rc:
+            said = ([f"pages: error {error} in request {request}"] if rc else []) + ([f"device error {code}"] if device_rc else [])
+            raise vb.VBError(rc or device_rc, "; ".join(said))
         return free
 
     def close(self):
