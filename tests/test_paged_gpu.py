@@ -1037,3 +1037,20 @@ def test_qk_rounds_cache_rows_once(ctx, pool):
     page = c.table.long().cpu()[seq, row // 16]
     k_rows, v_rows = (x[1].cpu()[page, :, row % 16].reshape(40, -1) for x in (c.k, c.v))
     assert torch.equal(k_rows, plain[2].cpu().to(TYPES[pool])) and torch.equal(v_rows, v.cpu().to(TYPES[pool]))
+
+
+def test_every_error_is_reported_once(ctx):
+    """The report clears the word before what the next call records."""
+    bad, good = (tree_case(ctx, "f32", [20], [4], 4, 2, 64, 16) for _ in range(2))
+    bad["args"]._keep[2][0] = 99
+    own = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ctx.set_stream(own.cuda_stream)
+    for _ in range(100):
+        ctx.tree_attention(bad["args"])
+        assert ctx.device_status() == (vb.VB_ERR_BACKEND, vb.DEV_TREE_SEQ)
+        ctx.tree_attention(bad["args"])
+        assert ctx.device_status() == (vb.VB_ERR_BACKEND, vb.DEV_TREE_SEQ)
+        ctx.tree_attention(good["args"])
+        assert ctx.device_status() == (0, 0)
+    ctx.set_stream(1)

@@ -204,7 +204,6 @@ extern "C" void vb_destroy(vb_ctx *ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (auto &r : ctx->ropes) cudaFree(r.d_cs);
     for (Arena *a : {&ctx->ws, &ctx->attn_ws, &ctx->pages_ws, &ctx->tree_ws}) arena_free(*a);
-    if (ctx->op_error) cudaFree(ctx->op_error);
     gemm_free(ctx);
     if (ctx->own_stream_handle) cudaStreamDestroy(ctx->own_stream_handle);
     delete ctx;
@@ -216,14 +215,16 @@ extern "C" const char *vb_last_error(const vb_ctx *ctx) {
 
 extern "C" int vb_device_status(vb_ctx *ctx, int *device_error) {
     if (!ctx || !device_error) return VB_ERR_INVALID_ARG;
-    int rc = gemm_device_error(ctx, device_error);
+    int code[2];
+    int rc = device_errors(ctx, code);
+    *device_error = code[0];
     if (rc) return rc;
-    if (*device_error) return set_error(ctx, VB_ERR_BACKEND, "mat-mul kernel reported error %d", *device_error);
-    VB_CHECK(ctx, cudaStreamSynchronize(ctx->stream));
-    VB_CHECK(ctx, cudaMemcpy(device_error, ctx->op_error, sizeof(int), cudaMemcpyDeviceToHost));
-    if (*device_error) {
-        VB_CHECK(ctx, cudaMemset(ctx->op_error, 0, sizeof(int)));
-        return set_error(ctx, VB_ERR_BACKEND, "paged-cache operator reported error %d", *device_error);
+    if (code[0]) return set_error(ctx, VB_ERR_BACKEND, "mat-mul kernel reported error %d", code[0]);
+    *device_error = code[1];
+    if (code[1]) {
+        // in stream order: before what the next calls record
+        VB_CHECK(ctx, cudaMemsetAsync(ctx->op_error, 0, sizeof(int), ctx->stream));
+        return set_error(ctx, VB_ERR_BACKEND, "paged-cache operator reported error %d", code[1]);
     }
     return VB_OK;
 }

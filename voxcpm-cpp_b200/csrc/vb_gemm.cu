@@ -1161,7 +1161,7 @@ struct GemmState {
     Arena act;                  // activation operands
     Arena part;                 // split partials
     unsigned *cnt = nullptr;    // tile counters
-    int *err = nullptr;
+    int *err = nullptr;         // two words: the mat-mul kernels' and the paged-cache operators'
     bool init = false;
     ActMaps cache[8];           // most recent activation descriptors
     int next = 0;
@@ -1173,7 +1173,7 @@ static GemmState *gemm_state(vb_ctx *ctx) {
     g = new GemmState();
     if (cudaMalloc(&g->cnt, 65536 * sizeof(unsigned)) != cudaSuccess ||
         cudaMemset(g->cnt, 0, 65536 * sizeof(unsigned)) != cudaSuccess ||
-        cudaMalloc(&g->err, sizeof(int)) != cudaSuccess || cudaMemset(g->err, 0, sizeof(int)) != cudaSuccess) {
+        cudaMalloc(&g->err, 2 * sizeof(int)) != cudaSuccess || cudaMemset(g->err, 0, 2 * sizeof(int)) != cudaSuccess) {
         cudaFree(g->cnt);
         cudaFree(g->err);
         delete g;
@@ -1181,6 +1181,7 @@ static GemmState *gemm_state(vb_ctx *ctx) {
     }
     g->init = true;
     ctx->gemm = g;
+    ctx->op_error = g->err + 1;
     return g;
 }
 
@@ -1193,6 +1194,7 @@ void gemm_free(vb_ctx *ctx) {
     cudaFree(g->err);
     delete g;
     ctx->gemm = nullptr;
+    ctx->op_error = nullptr;
 }
 
 int init_gemm(vb_ctx *ctx) {
@@ -1674,12 +1676,12 @@ int *gemm_error_word(vb_ctx *ctx) {
     return gs ? gs->err : nullptr;
 }
 
-int gemm_device_error(vb_ctx *ctx, int *code) {
+int device_errors(vb_ctx *ctx, int (&code)[2]) {
     GemmState *gs = static_cast<GemmState *>(ctx->gemm);
-    *code = 0;
+    code[0] = code[1] = 0;
     if (!gs) return VB_OK;
     VB_CHECK(ctx, cudaStreamSynchronize(ctx->stream));
-    VB_CHECK(ctx, cudaMemcpy(code, gs->err, sizeof(int), cudaMemcpyDeviceToHost));
+    VB_CHECK(ctx, cudaMemcpy(code, gs->err, sizeof(code), cudaMemcpyDeviceToHost));
     return VB_OK;
 }
 

@@ -56,7 +56,9 @@ bool matmul_uses_gemm(vb_ctx *ctx, vb_weight w, int64_t M);
 // caller checks matmul_uses_gemm first.
 int launch_matmul_pro(vb_ctx *ctx, vb_weight w, const float *x, int64_t M, int64_t ldx, const GemmPro &pro,
                       const MatmulOut &out);
-int gemm_device_error(vb_ctx *ctx, int *code);
+// Waits for the stream and reads the device error words: the mat-mul kernels',
+// the paged-cache operators'.
+int device_errors(vb_ctx *ctx, int (&code)[2]);
 // The context's device error word of the mat-mul kernels (created on first
 // use): a bounded wait that runs out records its code there.
 int *gemm_error_word(vb_ctx *ctx);

@@ -561,8 +561,6 @@ static unsigned share_out(const vb_ctx *ctx, int64_t bytes) {
 static size_t seq_bits(const vb_pages *p) { return (size_t)((p->n_seqs + 31) / 32) * 4; }
 
 int init_pages(vb_ctx *ctx) {
-    VB_CHECK(ctx, cudaMalloc(&ctx->op_error, 256));
-    VB_CHECK(ctx, cudaMemset(ctx->op_error, 0, 256));
     VB_CHECK(ctx, cudaFuncSetAttribute(pages_extend_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        3 * PG_MAX_SEQS * 4 + PG_MAX_SEQS / 8));
     return VB_OK;
