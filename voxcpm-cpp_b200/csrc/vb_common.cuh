@@ -90,6 +90,7 @@ struct vb_ctx {
     void *gemm = nullptr;               // tensor-core path state (vb_gemm.cu)
     vb::Arena pages_ws;                 // paged cache: lists a plan kernel leaves for the copy kernel
     vb::Arena tree_ws;                  // drafted-token attention: partial results of split rows
+    std::vector<const void *> tree_kernels;   // and its kernels that may take the shared memory they ask for
     int *op_error = nullptr;            // device error word of the paged-cache operators (VB_DEV_*; vb_gemm.cu owns it)
     void *attn_noalloc = nullptr;       // device address of vb_attention_noalloc's fixed scratch on this device
     long long dep_wait_limit = 0;       // streaming kernel: cycles of a wait on other CTAs (0 = default)

@@ -11,7 +11,6 @@ int init_model_kernels(vb_ctx *ctx);
 int init_stream(vb_ctx *ctx);
 int init_gemm(vb_ctx *ctx);
 int init_pages(vb_ctx *ctx);
-int init_tree(vb_ctx *ctx);
 
 int init_kernels(vb_ctx *ctx) {
     if (init_gemv(ctx)) return VB_ERR_BACKEND;
@@ -20,7 +19,6 @@ int init_kernels(vb_ctx *ctx) {
     if (init_model_kernels(ctx)) return VB_ERR_BACKEND;
     if (init_gemm(ctx)) return VB_ERR_BACKEND;
     if (init_pages(ctx)) return VB_ERR_BACKEND;
-    if (init_tree(ctx)) return VB_ERR_BACKEND;
     return VB_OK;
 }
 }  // namespace vb

@@ -785,6 +785,8 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
     if (!make_map(&tk, static_cast<char *>(p.k) + layer, dt, 2, p.head_dim, rows, 64, box, true) ||
         !make_map(&tv, static_cast<char *>(p.v) + layer, dt, 2, p.head_dim, rows, 64, box, true))
         return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the cache refused");
+    rc = tree_allow(ctx, reinterpret_cast<const void *>(tree_attention_kernel<TYPE, HDP, WM, PK>), TR_SMEM);
+    if (rc) return rc;
     VB_CHECK(ctx, pdl_launch(ctx, tree_attention_kernel<TYPE, HDP, WM, PK>, dim3(ctx->sm_count), dim3(TR_THREADS), smem, tk,
                              tv, g));
     VB_LAUNCH_CHECK(ctx, "tree_attention");
@@ -835,47 +837,18 @@ static int launch_heads(vb_ctx *ctx, TreeArgs &g) {
     return hd <= 64 ? launch_rows<TYPE, 64>(ctx, g) : hd <= 128 ? launch_rows<TYPE, 128>(ctx, g) : launch_rows<TYPE, 256>(ctx, g);
 }
 
-template <int TYPE, int HDP, int WM, int PK = 16>
-static cudaError_t allow_smem() {
-    return cudaFuncSetAttribute(tree_attention_kernel<TYPE, HDP, WM, PK>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
-}
-
-int init_tree(vb_ctx *ctx) {
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 2>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 64, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 2>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 128, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F32, 256, 2>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 64, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 64, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 128, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 128, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 2>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_BF16, 256, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 64, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 64, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 128, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 128, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1, 8>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 1>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 2>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 4>()));
-    VB_CHECK(ctx, (allow_smem<TR_F16, 256, 8>()));
-    return init_tree_tc(ctx);
+// A kernel's leave to take so much dynamic shared memory, asked for once, when
+// it first runs: asking loads it, which took a context's creation 18 ms for all
+// of this operator's.
+int tree_allow(vb_ctx *ctx, const void *kernel, int bytes) {
+    for (const void *k : ctx->tree_kernels)
+        if (k == kernel) return VB_OK;
+    VB_CHECK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    try {
+        ctx->tree_kernels.push_back(kernel);
+    } catch (...) {                                   // asked for again next time
+    }
+    return VB_OK;
 }
 
 }  // namespace vb

@@ -425,7 +425,7 @@ __device__ __forceinline__ void tree_store8(const TreeArgs &g, int64_t at, const
 }
 
 int launch_tree_tc(vb_ctx *ctx, TreeArgs &g);
-int init_tree_tc(vb_ctx *ctx);
+int tree_allow(vb_ctx *ctx, const void *kernel, int bytes);
 int tree_prepare(vb_ctx *ctx, TreeArgs &g, int tile_rows, int tiles, int kt, int over);
 int launch_tree_combine(vb_ctx *ctx, const TreeArgs &g);
 

@@ -812,6 +812,8 @@ static int launch_tc(vb_ctx *ctx, TreeArgs &g) {
     else if (!make_map_3d(&tq, g.a.q, dt, p.head_dim, g.a.n_heads, g.a.n_tokens, (int64_t)p.head_dim * 2, g.a.ldq * 2, 64, g.group,
                           g.tile_tokens))
         return set_error(ctx, VB_ERR_BACKEND, "vb_tree_attention: tensor map of the queries refused");
+    rc = tree_allow(ctx, reinterpret_cast<const void *>(tree_tc_kernel<TYPE, HDP, PAIR>), TT_SMEM);
+    if (rc) return rc;
     VB_CHECK(ctx, pdl_launch(ctx, tree_tc_kernel<TYPE, HDP, PAIR>, dim3(ctx->sm_count), dim3(TT_THREADS), smem, tk, tv, tq, g));
     VB_LAUNCH_CHECK(ctx, "tree_tc");
     return launch_tree_combine(ctx, g);
@@ -826,23 +828,6 @@ int launch_tree_tc(vb_ctx *ctx, TreeArgs &g) {
     if (g.a.type == VB_TYPE_F16)
         return g.p.head_dim <= 64 ? launch_tc_rows<TR_F16, 64>(ctx, g) : launch_tc_rows<TR_F16, 128>(ctx, g);
     return g.p.head_dim <= 64 ? launch_tc_rows<TR_BF16, 64>(ctx, g) : launch_tc_rows<TR_BF16, 128>(ctx, g);
-}
-
-template <int TYPE, int HDP, bool PAIR>
-static cudaError_t allow_tc() {
-    return cudaFuncSetAttribute(tree_tc_kernel<TYPE, HDP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TT_SMEM);
-}
-
-int init_tree_tc(vb_ctx *ctx) {
-    VB_CHECK(ctx, (allow_tc<TR_BF16, 64, false>()));
-    VB_CHECK(ctx, (allow_tc<TR_BF16, 64, true>()));
-    VB_CHECK(ctx, (allow_tc<TR_BF16, 128, false>()));
-    VB_CHECK(ctx, (allow_tc<TR_BF16, 128, true>()));
-    VB_CHECK(ctx, (allow_tc<TR_F16, 64, false>()));
-    VB_CHECK(ctx, (allow_tc<TR_F16, 64, true>()));
-    VB_CHECK(ctx, (allow_tc<TR_F16, 128, false>()));
-    VB_CHECK(ctx, (allow_tc<TR_F16, 128, true>()));
-    return VB_OK;
 }
 
 }  // namespace vb
