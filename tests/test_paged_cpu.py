@@ -3,6 +3,7 @@ the header's layout, null arguments are refused without a device, and the
 rotation table is the one that the oracle rotates with."""
 import ctypes as C
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -90,3 +91,13 @@ def test_host_tensors_are_refused():
         vb._count(new(2), new(2))
     with pytest.raises(ValueError, match="pos"):
         vb.QKArgs(q, k, k, heads=2, kv_heads=1, head_dim=8, q_out=q, rope=new(4, 8, dtype=torch.float32))
+
+
+def test_the_cubic_of_the_powers():
+    """2^f on [-1/2, 1/2] by the polynomial of the tcgen05 attention kernel: its stated relative error holds."""
+    src = open(os.path.join(ROOT, "voxcpm-cpp_b200", "csrc", "vb_tree_tc.cu")).read()
+    body = src[src.index("void exp2_pair"):]
+    coef = [float(x) for x in re.findall(r"pack_f32x2\((0\.\d+)f, \1f\)", body[:body.index("\n}\n")])]
+    assert len(coef) == 4                                         # cubic first
+    f = np.linspace(-0.5, 0.5, 200001)
+    assert np.max(np.abs(np.polyval(coef, f) / np.exp2(f) - 1)) < 7.6e-5

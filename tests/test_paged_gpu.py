@@ -1054,3 +1054,54 @@ def test_every_error_is_reported_once(ctx):
         ctx.tree_attention(good["args"])
         assert ctx.device_status() == (0, 0)
     ctx.set_stream(1)
+
+
+def terms_case(ctx, T, group, hd, rows):
+    """fp32 queries over `rows` rows of zeros before a draft that no token sees; row r of the cache: put(r, k, v)."""
+    t = tree_case(ctx, "f32", [rows + T], [T], group, 1, hd, 16, "any", seed=20)
+    t["args"]._keep[5].zero_()
+    t["args"].c.scale = 1.0
+    t["c"].k[1], t["c"].v[1] = 0, 0
+    t["q"].zero_()
+
+    def put(r, k, v):
+        at = (1, int(t["table"][t["seqs"][0], r // 16]), 0, r % 16)
+        t["c"].k[at][:2] = torch.tensor(k, device="cuda")
+        t["c"].v[at] = v
+    return t, put
+
+
+FP32_FORMS = [(1, 2, 64), (2, 2, 128), (1, 4, 256), (2, 3, 64), (1, 8, 128), (4, 2, 256), (1, 12, 64), (2, 8, 128), (1, 16, 256),
+              (3, 8, 64), (3, 8, 128), (3, 8, 256), (10, 8, 64), (10, 8, 128), (20, 8, 64), (20, 8, 128), (20, 8, 256)]
+
+
+@pytest.mark.parametrize("T,group,hd", FP32_FORMS)
+def test_tree_fp32_queries_keep_their_third_term(ctx, T, group, hd):
+    """Two rows whose scores differ by what a query value's third bf16 term adds.
+
+    Scores of 46 (in powers of two): their products and the sum of the terms are exact here, the scale's product is rounded to
+    2^-19, so the difference of two scores is off by 2^-18, its weight's logarithm by 2^-18 ln 2 and the result by half of that,
+    1.3e-6; the power and the sums add less than 5e-7.  Without the term the result is 0 in place of 6.1e-5."""
+    t, put = terms_case(ctx, T, group, hd, 2)
+    put(0, (1.0, 0.0), 1.0)
+    put(1, (0.0, 1.0), -1.0)
+    t["q"][:, 0::hd], t["q"][:, 1::hd] = 32 * (1 + 2.0 ** -9 + 2.0 ** -18), 32 * (1 + 2.0 ** -9)
+    ctx.tree_attention(t["args"])
+    assert ctx.device_status() == (0, 0)
+    assert np.all(np.abs(t["out"].cpu().numpy().astype(np.float64) - np.tanh(16 * 2.0 ** -18)) <= 1.8e-6)
+
+
+@pytest.mark.parametrize("T,group,hd", FP32_FORMS)
+def test_tree_fp32_weights_keep_their_third_term(ctx, T, group, hd):
+    """32 rows of one weight, of which three bf16 terms are 1/2, 2^-10 and 2^-19, beside a row of weight 1.
+
+    result = 32 p / (1 + 32 p): an error of p itself shrinks to a 17th, the sums of 33 values and the division round a few
+    times to 2^-24: 1e-6 holds them.  Without the third term the result is off by 2^-18 of it, 3.6e-6."""
+    t, put = terms_case(ctx, T, group, hd, 33)
+    for r in range(33):
+        put(r, (float(r == 16), 0.0), float(r != 16))
+    p = 0.5 * (1 + 2.0 ** -9 + 2.0 ** -18)
+    t["q"][:, 0::hd] = -np.log(p)
+    ctx.tree_attention(t["args"])
+    assert ctx.device_status() == (0, 0)
+    assert np.all(np.abs(t["out"].cpu().numpy().astype(np.float64) - 32 * p / (1 + 32 * p)) <= 1e-6)
