@@ -298,7 +298,11 @@ __global__ void __launch_bounds__(QK_THREADS, V == 8 ? 2 : 3) qk_norm_rope_kerne
             }
             auto keep_row = [&]() {
                 if (is_q || !keep) return;
-                if (g.p.type == VB_TYPE_F16) {
+                if constexpr (sizeof(T) == 2) {               // of the cache's type
+                    uint16_t *pool = static_cast<uint16_t *>(is_v ? g.p.v : g.p.k) + at + kvh * pool_head;
+                    store2(reinterpret_cast<T *>(pool) + i0, true, y0);
+                    store2(reinterpret_cast<T *>(pool) + i1, true, y1);
+                } else if (g.p.type == VB_TYPE_F16) {
                     __half *pool = static_cast<__half *>(is_v ? g.p.v : g.p.k) + at + kvh * pool_head;
                     store2(pool + i0, true, y0);
                     store2(pool + i1, true, y1);
