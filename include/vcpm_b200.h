@@ -669,13 +669,15 @@ int vb_qk_norm_rope(vb_ctx *ctx, const vb_qk_args *a);
  * prompt.  A token that sees nothing gives zeros; what lies in rows that it
  * does not see never reaches its result.  A score of plus infinity or NaN
  * makes its result NaN (with F32 queries an infinite key that it sees may,
- * whatever the sign). */
+ * whatever the sign).  A call is refused when the tiles of n sequences of
+ * max_pages pages, times n_kv_heads and the blocks of max_tokens, could pass
+ * 2^31: max_pages is best kept near the longest sequence. */
 typedef struct {
     int type;                       /* of q and out: VB_TYPE_F32 (cache BF16), or the cache's type */
     int layer;
     int n;                          /* sequences in the call */
     int n_tokens;                   /* rows of q and out */
-    int max_tokens;                 /* at least the most tokens of one sequence */
+    int max_tokens;                 /* at least the most tokens of one sequence; picks the kernel's form */
     int n_heads;                    /* a multiple of the cache's n_kv_heads */
     int mask_words;                 /* 32-bit words of a mask row */
     float scale;                    /* 0 = 1/sqrt(head_dim) */

@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(PG_PLAN) pages_compact_plan(vb_pages p, vb_pag
 
 // Page contents (a unit: the K or V of one page of one layer, contiguous)
 // and the table, over all CTAs.  Bound by HBM: 1000 pages of 64 rows in 28
-// layers of 2 heads (3.76 GB read and written) take 569 us, the copy rate.
+// layers of 2 heads (3.76 GB read and written) take 569 to 574 us, the copy rate.
 __global__ void __launch_bounds__(PG_COPY) pages_compact_copy(vb_pages p, vb_pages to, const int *ws) {
     constexpr int B = 4;
     pdl_trigger();

@@ -23,7 +23,7 @@ namespace vb {
 
 constexpr int QK_THREADS = 256;
 // Waves of threads that a call is spread over: with 1 | 2 | 8 of them 12,800
-// tokens take 44.9 | 45.0 | 47.5 us in fp32 and 37.2 | 33.0 | 38.6 in bf16.
+// tokens take 45.1 | 45.1 | 47.6 us in fp32 and 38.7 | 34.6 | 40.9 in bf16.
 constexpr int QK_WAVES = 2;
 
 struct QKArgs {
@@ -152,10 +152,11 @@ __device__ __forceinline__ void store2(T *p, bool vec, const f32x2 (&y)[V]) {
 // registers a thread with pieces of 4 values and 120 with 8.
 //
 // Bound by HBM where tokens are many: 12,800 tokens of 16 + 2 heads of 128 take
-// 45.0 us in fp32 (249 MB, 85 % of the copy rate) and 33.0 in bf16; one token
-// is a launch and two trips to memory.  With 1 | 2 | 4 rows at a time the two
-// take 55.6 | 45.0 | 59.3 and 37.5 | 33.0 | 57.4 us, 1024 tokens of bf16 8.6 |
-// 7.4 | 9.2.
+// 45 to 46 us in fp32 (249 MB, 84 % of the copy rate) and 35 in bf16 (131 MB, 20
+// us at that rate), which its instructions bound as well: with pieces of 4
+// values, twice as many, it takes 55.  One token is a launch and two trips to
+// memory.  With 1 | 2 | 4 rows at a time the two take 52.2 | 45.1 | 53.0 and
+// 38.4 | 34.6 | 51.8 us.
 constexpr int QK_ROWS = 2;
 
 // ROUND: VB_OUT_BF16.

@@ -22,9 +22,9 @@
 // This file's kernel multiplies with mma.sync and serves blocks of up to 16
 // rows of any type, and what the tcgen05 kernel does not take (launch_rows).
 // With few rows the cache's bytes bound it: 524,288 rows of 2 x 2 heads of
-// 128 under one token of 16 heads take 97 us in bf16 and 103 us in fp32, the
-// next 262,144 rows 40 and 44 us of it (6.7 and 6.2 TB/s); the constant
-// 17 us are two launches, the cut, the first tiles' way and the join.
+// 128 under one token of 16 heads take 95 us in bf16 and in fp32, the second
+// 262,144 rows 39 us of it (6.9 TB/s); the constant 17 us are two launches,
+// the cut, the first tiles' way and the join.
 #include "vb_common.cuh"
 #include "vb_kernels.cuh"
 #include "vb_tree.cuh"
@@ -36,7 +36,7 @@ namespace vb {
 constexpr int TR_KT = 64;            // cache rows per tile
 constexpr int TR_MAX_STAGES = 8;
 // What an item's start and end cost, in tiles: with 2 | 4 | 6 the prompt of
-// 4096 fp32 tokens takes 614 | 590 | 611 us, 64 decode steps 104 | 104 | 105.
+// 4096 fp32 tokens takes 607 | 566 | 588 us, 64 decode steps 98 | 97 | 97.
 constexpr int TR_OVER = 4;
 constexpr int TR_THREADS = 384;      // warps 0..7 compute, 8..11 load
 // Registers: the launch gives 168 a thread; the loading warpgroup goes down
@@ -83,12 +83,12 @@ __host__ __device__ constexpr int tree_scratch(int hdp, int q_rows, int merge_ro
 // tiles in turn).  PK: rows of a block of 4 or 8.  A thread then keeps one row
 // in place of two (the other eight of an instruction's 16 count for nothing):
 // half the exponentials, merges and parts (bf16, 8 sequences of 4000 rows under
-// one token 20.4 -> 18.7 us).  The 16-bit terms of an fp32 value lie under one
+// one token took 20.4 us without and 18.7 with it; 17.5 since its loads changed).  The 16-bit terms of an fp32 value lie under one
 // another in the 16 rows (row t * PK + m: term t of row m), which takes one
 // product or two in place of three; a row's scores and sums are added over
-// its terms.  (64 sequences of 8192 rows under one token of 16 heads over 2:
-// 125 us with three products, 111 us with two, of 82 us that reading the
-// cache takes.)
+// its terms.  (64 sequences of 8192 rows under one token of 16 heads over 2 took
+// 125 us with three products and 111 us with two; 98 to 107 since the loads
+// changed, of 82 us that reading the cache takes.)
 template <int TYPE, int HDP, int WM, int PK>
 __global__ void __launch_bounds__(TR_THREADS, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -585,10 +585,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 //
 // Three forms, by the call's items (at most 148 CTAs, so few items have many
 // parts); microseconds of a whole call with 16 warps a task | 4 | 1:
-//   2 items (one token of 16 heads over 2, 4,000 rows)        14.8 | 22 | 54
-//   16 items (8 sequences of up to 25 tokens, 2000 rows)      33.2 | 23.8 | 30.9
-//   32 items (16 sequences of one token, 3000 rows)           24.6 | 22.3 | 24.7
-//   128 items (64 sequences of one token, 8192 rows)         118.7 | 103.7 | 103.8
+//   2 items (one token of 16 heads over 2, 4,000 rows)        14.5 | 22 | 53
+//   16 items (8 sequences of up to 25 tokens, 2000 rows)      32.1 | 22.4 | 29.4
+//   32 items (16 sequences of one token, 3000 rows)           23.6 | 21.2 | 23.4
+//   128 items (64 sequences of one token, 8192 rows)         112.4 | 97.2 | 97.7
 //   256 items (one prompt of 4096)                             -   | 138 | 98
 // (Joining in the attention kernel, by the last CTA to leave a part, saves the
 // launch but costs a fence, a ticket and one SM's reading: from 0.4 us less to
@@ -796,9 +796,9 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
 // Which kernel and how many rows per block.  16-bit queries of more than 16
 // rows go to the tcgen05 kernel (vb_tree_tc.cu), whose tile of 128 rows costs
 // the tensor cores less than reading the cache costs the memory, however few
-// of its rows exist (8 sequences of 32,768 rows, 32 rows of queries: 58 us
-// there, 67 us here; 64 rows 58 | 86).  What is left: up to 16 rows, where padding to 128 only
-// delays the first result; heads above 128 values, whose sums and scores do
+// of its rows exist (8 sequences of 32,768 rows, 32 rows of queries: 64 us
+// there, 67 us here; 64 rows 64 | 82; pages of 16 rows).  What is left: up to
+// 16 rows, where padding to 128 only delays the first result; heads above 128 values, whose sums and scores do
 // not fit its tensor memory; and fp32 queries, whose sums the tcgen05
 // accumulators hold less exactly.
 //
@@ -807,10 +807,10 @@ static int launch_tree(vb_ctx *ctx, TreeArgs &g) {
 // operands for more products.  Measured at one sequence of 32,768 rows with
 // 2 heads (microseconds with blocks of 32 | 64 | 128 rows; "prompt": 4096
 // tokens over themselves):
-//   fp32, 128 values: 32 rows 29 | 33 | 49, 64 rows 38 | 35 | 50,
-//                     128 rows 60 | 52 | 56, 384 rows 144 | 123 | 123, prompt 943 | 681 | 614 (590 with TR_OVER 4)
-//   bf16, 256 values: 32 rows 41 | 45 | 56, 64 rows 51 | 53 | 62,
-//                     128 rows 71 | 69 | 78, 384 rows 141 | 121 | 135, prompt 1490 | 1084 | 915
+//   fp32, 128 values: 32 rows 27 | 33 | 48, 64 rows 36 | 34 | 49,
+//                     128 rows 59 | 49 | 52, 384 rows 144 | 123 | 115, prompt 787 | 635 | 567
+//   bf16, 256 values: 32 rows 34 | 38 | 51, 64 rows 46 | 44 | 55,
+//                     128 rows 66 | 66 | 66, 384 rows 136 | 121 | 132, prompt 1153 | 863 | 730
 // fp32 heads of 256 values leave room for blocks of 32 and two stages only.
 template <int TYPE, int HDP>
 static int launch_rows(vb_ctx *ctx, TreeArgs &g) {

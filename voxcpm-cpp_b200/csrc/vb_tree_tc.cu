@@ -18,10 +18,11 @@
 // rescaled in tensor memory.
 //
 // Bound by the tensor cores with the exponentials beside them where rows are
-// many (four prompts of 4096 tokens, 16 heads over 2 of 128 values: 284 us, 967
-// TFLOP/s of the 1647 that a large matrix product reaches), by the cache's
+// many (four prompts of 4096 tokens, 16 heads over 2 of 128 values: 282 to 289 us, 950
+// to 975 TFLOP/s of the 1647 that a large matrix product reaches), by the cache's
 // bytes and the first and last tiles below that (262,144 rows under 32 tokens
-// 79 us, of which reading takes 41 and the products alone 42).
+// 79 to 81 us, of which reading takes 41 and the products alone 42).  In a block
+// of two row tiles whose second has no rows that one's products are issued too.
 //
 // Warps 0..7 softmax (warpgroup = stream), 9 issues the MMAs, 8, 10 and 11
 // issue the copies (TMA, one box per page and column block).
@@ -36,8 +37,8 @@ namespace vb {
 constexpr int TT_KT = 128;
 constexpr int TT_THREADS = 384;
 constexpr int TT_SLOTS = 12;
-// What an item's start and end cost, in tiles.  A prompt of 4096 tokens takes
-// with 3 | 4 89 | 89 us, four of them 282 | 287, 64 ragged drafts over 4000 rows
+// What an item's start and end cost, in tiles.  A prompt of 4096 tokens (89 to 97
+// us over several GPUs) took on one of them with 3 | 4 89 | 89 us, four of them 282 | 287, 64 ragged drafts over 4000 rows
 // 60 | 62; while an item's first and last tiles still took two passes, that
 // prompt took 159 | 98 | 92 | 95 with 0 | 2 | 4 | 6.
 constexpr int TT_OVER = 3;

@@ -23,7 +23,7 @@ TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
 QRULE_X86, QRULE_REF = 0, 1
 OUT_BF16 = 1
 PAGES_SEQ, PAGES_COUNT, PAGES_LONG, PAGES_FULL, PAGES_SHARED, PAGES_PATH, PAGES_TABLE = 1, 2, 3, 4, 5, 6, 7
-DEV_QK_POS, DEV_QK_ROW, DEV_TREE_SEQ, DEV_TREE_PAGE = 21, 22, 31, 32
+DEV_QK_POS, DEV_QK_ROW, DEV_TREE_SEQ, DEV_TREE_PAGE, DEV_TREE_WAIT = 21, 22, 31, 32, 33
 GEN_LM_HIDDEN, GEN_LAST_LM_HIDDEN, GEN_RESIDUAL_HIDDEN, GEN_PREV_PATCH = 0, 1, 2, 3
 
 _lib = None
