@@ -331,3 +331,41 @@ def test_generation_step_replays_from_a_graph(ctx):
     ga.close()
     gb.close()
     m.close()
+
+
+def test_generation_step_replays_after_larger_calls():
+    """Between a step's capture and its replay other calls grow the rotary tables and the workspaces."""
+    ctx = vb.Context(0)
+    m = Model(ctx, O.TYPE_F16)
+    parts = m.device_parts()
+    B, T, seed = 2, 6, 77
+    embeds = dev(O.bf16_round(S.normal((8, 24, H), 0.5)))
+    ga, gb = vb.Gen(ctx, parts, B, 32), vb.Gen(ctx, parts, B, 32)
+    first, places = embeds[:B, :T].contiguous(), torch.arange(4, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    for g in (ga, gb):
+        g.prefill(T, first)
+        g.step(seed, zeros((B, PATCH, FEAT)), zeros((B, 2)))
+    pa, sa = zeros((B, PATCH, FEAT)), zeros((B, 2))
+    ga.step(seed, pa, sa)
+    pb, sb = zeros((B, PATCH, FEAT)), zeros((B, 2))
+    ctx.sync()
+    ctx.graph_begin()
+    gb.step(seed, pb, sb)
+    graph = ctx.graph_end()
+    more = vb.Gen(ctx, parts, 8, 2048)
+    more.prefill(24, embeds)
+    more.step(seed, zeros((8, PATCH, FEAT)), zeros((8, 2)))
+    q = zeros((4, 128))
+    for hd in (64, 128):
+        ctx.rope_neox(q, hd, 1, 4, places, 10000.0)
+    ctx.sync()
+    ctx.graph_launch(graph)
+    ctx.sync()
+    assert np.array_equal(pa.cpu().numpy(), pb.cpu().numpy())
+    assert np.array_equal(sa.cpu().numpy(), sb.cpu().numpy())
+    ctx.graph_destroy(graph)
+    for g in (ga, gb, more):
+        g.close()
+    m.close()
+    ctx.close()

@@ -276,3 +276,40 @@ def test_cfm_solve_replays_from_a_graph(ctx):
         assert np.array_equal(host(x), want)
     ctx.graph_destroy(g)
     gpu.close()
+
+
+def test_cfm_solves_replay_after_larger_ones(ctx):
+    """Solves of other sizes come between a solve's capture and its replays: with guidance (the branch table is one of each size)
+    and without."""
+    fresh = vb.Context(0)
+    gpu, _ = build_dit(fresh, O.TYPE_Q8_0)
+    d = DIT
+    mu = dev(S.normal((9, 2 * d["hidden"])))
+    cond = dev(O.bf16_round(S.normal((9, d["patch"], d["feat"]))))
+    x0 = dev(np.stack([O.cfm_noise(5, i, d["patch"] * d["feat"]).reshape(d["patch"], d["feat"]) for i in range(9)]))
+    want, graphs = [], []
+    x = x0[:3].clone()
+    for cfg_value in (2.0, 1.0):
+        x.copy_(x0[:3])
+        torch.cuda.synchronize()
+        gpu.cfm_solve(3, mu, cond, x, 4, cfg_value)
+        fresh.sync()
+        want.append(host(x))
+        fresh.graph_begin()
+        gpu.cfm_solve(3, mu, cond, x, 4, cfg_value)
+        graphs.append(fresh.graph_end())
+    for n in (5, 9, 2):
+        y = x0[:n].clone()
+        torch.cuda.synchronize()
+        for cfg_value in (2.0, 1.0):
+            gpu.cfm_solve(n, mu, cond, y, 4, cfg_value)
+        fresh.sync()
+    for g, w in zip(graphs, want):
+        x.copy_(x0[:3])
+        torch.cuda.synchronize()
+        fresh.graph_launch(g)
+        fresh.sync()
+        assert np.array_equal(host(x), w)
+        fresh.graph_destroy(g)
+    gpu.close()
+    fresh.close()

@@ -112,16 +112,7 @@ const RopeTable *rope_table(vb_ctx *ctx, int head_dim, float theta, int use_fact
         set_error(ctx, VB_ERR_BACKEND, "rope table upload failed");
         return nullptr;
     }
-    // drop smaller tables of the same kind
-    for (size_t i = 0; i < ctx->ropes.size(); i++) {
-        auto &r = ctx->ropes[i];
-        if (r.head_dim == head_dim && r.theta == theta && r.use_factors == use_factors) {
-            cudaStreamSynchronize(ctx->stream);
-            cudaFree(r.d_cs);
-            ctx->ropes.erase(ctx->ropes.begin() + (long)i);
-            break;
-        }
-    }
+    // smaller tables of the same kind stay: captured graphs may read them
     ctx->ropes.push_back(t);
     return &ctx->ropes.back();
 }

@@ -827,8 +827,8 @@ struct vb_dit {
     std::map<int, int32_t *> seg_tables;        // items -> [4][items * (3 + 2P)]
     int *ones = nullptr;                        // [ones_n] all 1
     int ones_n = 0;
-    int *cfg_hm = nullptr;                      // [2 * cfg_n]: n ones then n zeros
-    int cfg_n = 0, cfg_cap = 0;
+    std::map<int, int *> cfg_hm;                // n -> [2 * n]: n ones then n zeros
+    std::vector<void *> outgrown;               // smaller `ones` and `user_hm`: captured graphs may read them
     int *user_hm = nullptr;                     // caller's has_mu, [user_cap]
     int user_cap = 0;
     vb::Arena vel;                              // velocities [items][patch * feat]
@@ -843,8 +843,9 @@ static void dit_free(vb_ctx *ctx, vb_dit *d) {
     for (auto &e : d->sin_rows) cudaFree(e.second);
     for (auto &e : d->seg_tables) cudaFree(e.second);
     cudaFree(d->ones);
-    cudaFree(d->cfg_hm);
     cudaFree(d->user_hm);
+    for (auto &e : d->cfg_hm) cudaFree(e.second);
+    for (void *p : d->outgrown) cudaFree(p);
     vb::arena_free(d->vel);
     lm_free(ctx, d->blocks);
     delete d;
@@ -995,10 +996,7 @@ static const int *dit_ones(vb_ctx *ctx, vb_dit *d, int n, int *rc) {
     std::vector<int> ones((size_t)n, 1);
     void *dev = nullptr;
     if ((*rc = device_table(ctx, &dev, ones.data(), (size_t)n * 4, "LocDiT has_mu table"))) return nullptr;
-    if (d->ones) {
-        cudaStreamSynchronize(ctx->stream);
-        cudaFree(d->ones);
-    }
+    if (d->ones) d->outgrown.push_back(d->ones);
     d->ones = (int *)dev;
     d->ones_n = n;
     return d->ones;
@@ -1141,11 +1139,10 @@ extern "C" int vb_dit_forward(vb_ctx *ctx, vb_dit *d, int n, const float *x, con
         // the caller may reuse its array when this returns
         if (d->user_cap < n) {
             if (capturing(ctx)) return set_error(ctx, VB_ERR_BACKEND, "vb_dit_forward: has_mu buffer grows during capture");
-            VB_CHECK(ctx, cudaStreamSynchronize(ctx->stream));
-            cudaFree(d->user_hm);
-            d->user_hm = nullptr;
-            d->user_cap = 0;
-            VB_CHECK(ctx, cudaMalloc(&d->user_hm, (size_t)n * 4));
+            int *grown = nullptr;
+            VB_CHECK(ctx, cudaMalloc(&grown, (size_t)n * 4));
+            if (d->user_hm) d->outgrown.push_back(d->user_hm);
+            d->user_hm = grown;
             d->user_cap = n;
         }
         VB_CHECK(ctx, cudaMemcpyAsync(d->user_hm, has_mu, (size_t)n * 4, cudaMemcpyHostToDevice, ctx->stream));
@@ -1170,22 +1167,15 @@ extern "C" int vb_cfm_solve(vb_ctx *ctx, vb_dit *d, int n, const float *mu, cons
     float *vel = (float *)d->vel.ptr;
     const int *hm = nullptr;
     if (use_cfg) {
-        if (d->cfg_n != n) {
-            if (capturing(ctx)) return set_error(ctx, VB_ERR_BACKEND, "vb_cfm_solve: branch table changes during capture");
+        auto it = d->cfg_hm.find(n);
+        if (it == d->cfg_hm.end()) {
             std::vector<int> hmh((size_t)items, 0);
             for (int i = 0; i < n; i++) hmh[i] = 1;
-            if (d->cfg_cap < items) {
-                VB_CHECK(ctx, cudaStreamSynchronize(ctx->stream));
-                cudaFree(d->cfg_hm);
-                d->cfg_hm = nullptr;
-                d->cfg_cap = 0;
-                VB_CHECK(ctx, cudaMalloc(&d->cfg_hm, (size_t)items * 4));
-                d->cfg_cap = items;
-            }
-            VB_CHECK(ctx, cudaMemcpyAsync(d->cfg_hm, hmh.data(), (size_t)items * 4, cudaMemcpyHostToDevice, ctx->stream));
-            d->cfg_n = n;
+            void *dev = nullptr;
+            if ((rc = device_table(ctx, &dev, hmh.data(), (size_t)items * 4, "vb_cfm_solve branch table"))) return rc;
+            it = d->cfg_hm.emplace(n, static_cast<int *>(dev)).first;
         }
-        hm = d->cfg_hm;
+        hm = it->second;
     } else if (mu) {
         if (!(hm = dit_ones(ctx, d, items, &rc))) return rc;
     }
