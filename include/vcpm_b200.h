@@ -553,7 +553,8 @@ size_t vb_vae_stream_state_bytes(vb_vae_stream s);       /* device bytes of the 
  * cache, like all calls of one context, are ordered by the caller when they
  * go to different streams.
  * page_rows: a power of two, 16 to 1024; head_dim: a multiple of 8, at most
- * 256; n_seqs at most 16384; every pointer 16-byte aligned. */
+ * 256; n_seqs at most 16384; max_pages * page_rows below 2^31 - 1024; every
+ * pointer 16-byte aligned. */
 typedef struct {
     void *k, *v;          /* [n_layers][n_pages][n_kv_heads][page_rows][head_dim] of `type` */
     int32_t *table;       /* [n_seqs][max_pages], -1 past a sequence's end */

@@ -1105,3 +1105,14 @@ def test_tree_fp32_weights_keep_their_third_term(ctx, T, group, hd):
     ctx.tree_attention(t["args"])
     assert ctx.device_status() == (0, 0)
     assert np.all(np.abs(t["out"].cpu().numpy().astype(np.float64) - 32 * p / (1 + 32 * p)) <= 1e-6)
+
+
+@pytest.mark.parametrize("rows,pages", [(16, 2 ** 27 - 1), (16, 2 ** 27 - 64), (1024, 2 ** 21 - 1)])
+def test_sequences_of_2_to_the_31_rows_are_refused(ctx, rows, pages):
+    """A length rounded up to pages or tiles stays a 32-bit number."""
+    c = new_cache(ctx)
+    c.c.page_rows, c.c.max_pages, c.c.n_pages = rows, pages, 1
+    for call in (lambda: ctx.pages_extend(c, ints([0]), ints([1])), lambda: ctx.pages_truncate(c, ints([0]), ints([0]))):
+        with pytest.raises(vb.VBError) as e:
+            call()
+        assert e.value.code == vb.VB_ERR_INVALID_ARG and "too large" in ctx.last_error()

@@ -536,8 +536,9 @@ int check_pages(vb_ctx *ctx, const vb_pages *p, const char *who) {
         return set_error(ctx, VB_ERR_INVALID_ARG, "%s: page_rows must be a power of two, 16 to 1024", who);
     if (p->head_dim < 8 || p->head_dim > 256 || p->head_dim % 8)
         return set_error(ctx, VB_ERR_INVALID_ARG, "%s: head_dim must be a multiple of 8, at most 256", who);
-    // row numbers of one layer, and rows of one sequence, are 32-bit
-    if ((int64_t)p->n_pages * p->n_kv_heads * p->page_rows > INT_MAX || (int64_t)p->max_pages * p->page_rows > INT_MAX)
+    // row numbers of one layer, and rows of one sequence, are 32-bit; a length
+    // is rounded up to pages of up to 1024 rows and to tiles of 128
+    if ((int64_t)p->n_pages * p->n_kv_heads * p->page_rows > INT_MAX || (int64_t)p->max_pages * p->page_rows > INT_MAX - 1024)
         return set_error(ctx, VB_ERR_INVALID_ARG, "%s: cache too large", who);
     if (((uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->table | (uintptr_t)p->length | (uintptr_t)p->refs |
          (uintptr_t)p->status) & 15)
